@@ -6,7 +6,7 @@
 #include <cstdarg>
 #include <cstdio>
 
-#include "moe_common.h"
+#include "low_rank.h"
 
 namespace moe {
 
@@ -40,6 +40,24 @@ int launch_gateup_swiglu_gathered(const uint16_t*, const int32_t*, int64_t, cons
 int launch_dispatch_rows(const int32_t*, int32_t*, int32_t*, int32_t*, int32_t*, int32_t*, const int32_t*, int32_t*,
                          int64_t, int64_t, int, int, int, int64_t, hipStream_t);
 void set_gemm_workgroup_limit(int);
+int64_t router_loss_scratch_bytes(int64_t, int64_t);
+int launch_router_loss(const float*, const float*, const int32_t*, const uint8_t*, float*, int32_t*, float*, int64_t, int,
+                       int, hipStream_t);
+int launch_router_logits_grad(const float*, const float*, const int32_t*, const uint8_t*, const int32_t*, const float*,
+                              const float*, float*, float*, float*, int64_t, int, int, hipStream_t);
+int64_t route_backward_scratch_bytes(int64_t, int64_t, int64_t);
+int launch_route_backward(const uint16_t*, const float*, const float*, const float*, const int32_t*, const uint8_t*,
+                          const int32_t*, const float*, const float*, const uint16_t*, uint16_t*, float*, float*, char*,
+                          int64_t, int64_t, int, int, hipStream_t);
+int launch_combine_grad(const void*, const void*, int, const int32_t*, const float*, const int32_t*, const int32_t*,
+                        void*, float*, int64_t, int64_t, int, int, int64_t, hipStream_t);
+int launch_adapter_group(const int32_t*, void*, int64_t, int, hipStream_t);
+int64_t low_rank_scratch_bytes(int64_t, int64_t, int64_t, int64_t, int64_t, bool);
+int launch_low_rank_add(const uint16_t*, const uint16_t*, const uint16_t*, const float*, const void*, const uint16_t*,
+                        uint16_t*, float*, char*, int64_t, int64_t, int64_t, int, int, hipStream_t);
+int launch_low_rank_backward(const uint16_t*, const uint16_t*, const uint16_t*, const uint16_t*, const float*,
+                             const void*, const float*, const uint16_t*, uint16_t*, void*, void*, bool, char*, int64_t,
+                             int64_t, int64_t, int, int, hipStream_t);
 
 static thread_local char g_last_error[512] = "";
 
@@ -575,6 +593,231 @@ int moe_set_gemm_workgroups(int64_t workgroups) {
                 "workgroups must be in [0, INT_MAX]");
     set_gemm_workgroup_limit(static_cast<int>(workgroups));
     return MOE_OK;
+}
+
+// -- training: the router's losses and gradients ------------------------------
+
+static int check_router_grad(const float* logits, const float* bias, const int32_t* ids, int64_t tokens, int64_t experts,
+                             int64_t topk) {
+    MOE_REQUIRE(tokens >= 0, MOE_ERR_INVALID_ARGUMENT, "tokens must be >= 0");
+    MOE_REQUIRE(experts >= 1 && experts <= kMaxExperts, MOE_ERR_UNSUPPORTED, "routing supports 1..64 experts");
+    MOE_REQUIRE(topk >= 1 && topk <= kMaxTopk, MOE_ERR_UNSUPPORTED, "topk must be in 1..8");
+    MOE_REQUIRE(tokens <= INT_MAX / experts && tokens <= INT_MAX / topk, MOE_ERR_CAPACITY,
+                "tokens*experts and tokens*topk must fit int32");
+    MOE_REQUIRE(tokens == 0 || (logits && ids), MOE_ERR_INVALID_ARGUMENT, "null pointer");
+    MOE_REQUIRE(aligned_to(logits, 4) && aligned_to(bias, 4) && aligned_to(ids, 4), MOE_ERR_INVALID_ARGUMENT,
+                "pointers must be aligned to their element size");
+    return MOE_OK;
+}
+
+int64_t moe_router_loss_scratch_bytes(int64_t tokens, int64_t experts) {
+    if (tokens < 0 || experts < 1 || experts > kMaxExperts) return -1;
+    return router_loss_scratch_bytes(tokens, experts);
+}
+
+int moe_router_loss(const float* logits, const float* bias, const int32_t* ids, const uint8_t* mask, float* losses,
+                    int32_t* stats, void* scratch, int64_t scratch_bytes, int64_t tokens, int64_t experts, int64_t topk,
+                    void* stream) {
+    const int rc = check_router_grad(logits, bias, ids, tokens, experts, topk);
+    if (rc != MOE_OK) return rc;
+    MOE_REQUIRE(losses && stats, MOE_ERR_INVALID_ARGUMENT, "null pointer");
+    const int64_t need = router_loss_scratch_bytes(tokens, experts);
+    MOE_REQUIRE(scratch && scratch_bytes >= need, MOE_ERR_WORKSPACE, "loss scratch needs %lld bytes, got %lld",
+                (long long)need, (long long)scratch_bytes);
+    MOE_REQUIRE(aligned_to(losses, 4) && aligned_to(stats, 4) && aligned_to(scratch, 4), MOE_ERR_INVALID_ARGUMENT,
+                "pointers must be aligned to their element size");
+    return launch_router_loss(logits, bias, ids, mask, losses, stats, static_cast<float*>(scratch), tokens,
+                              (int)experts, (int)topk, static_cast<hipStream_t>(stream));
+}
+
+static int check_router_grad_inputs(const int32_t* stats, const float* grad_losses, const float* grad_weights) {
+    MOE_REQUIRE(!grad_losses || stats, MOE_ERR_INVALID_ARGUMENT, "grad_losses needs the forward's stats");
+    MOE_REQUIRE(aligned_to(stats, 4) && aligned_to(grad_losses, 4) && aligned_to(grad_weights, 4),
+                MOE_ERR_INVALID_ARGUMENT, "pointers must be aligned to their element size");
+    return MOE_OK;
+}
+
+int moe_router_logits_backward(const float* logits, const float* bias, const int32_t* ids, const uint8_t* mask,
+                               const int32_t* stats, const float* grad_losses, const float* grad_weights,
+                               float* grad_logits, int64_t tokens, int64_t experts, int64_t topk, void* stream) {
+    int rc = check_router_grad(logits, bias, ids, tokens, experts, topk);
+    if (rc == MOE_OK) rc = check_router_grad_inputs(stats, grad_losses, grad_weights);
+    if (rc != MOE_OK) return rc;
+    if (tokens == 0) return MOE_OK;
+    MOE_REQUIRE(grad_logits, MOE_ERR_INVALID_ARGUMENT, "null pointer");
+    MOE_REQUIRE(aligned_to(grad_logits, 4), MOE_ERR_INVALID_ARGUMENT, "pointers must be aligned to their element size");
+    return launch_router_logits_grad(logits, bias, ids, mask, stats, grad_losses, grad_weights, grad_logits, nullptr,
+                                     nullptr, tokens, (int)experts, (int)topk, static_cast<hipStream_t>(stream));
+}
+
+int64_t moe_route_backward_scratch_bytes(int64_t tokens, int64_t hidden, int64_t experts) {
+    if (tokens < 0 || tokens > kMaxAdapterTokens || experts < 1 || experts > kMaxExperts || hidden < 8 ||
+        hidden % 8 != 0 || hidden > kMaxLowRankWidth)
+        return -1;
+    return route_backward_scratch_bytes(tokens, hidden, experts);
+}
+
+int moe_route_backward(const void* x, const float* router_w, const float* logits, const float* bias, const int32_t* ids,
+                       const uint8_t* mask, const int32_t* stats, const float* grad_losses, const float* grad_weights,
+                       const void* grad_x_base, void* grad_x, float* grad_router_w, float* grad_bias, void* scratch,
+                       int64_t scratch_bytes, int64_t tokens, int64_t hidden, int64_t experts, int64_t topk,
+                       void* stream) {
+    int rc = check_router_grad(logits, bias, ids, tokens, experts, topk);
+    if (rc == MOE_OK) rc = check_router_grad_inputs(stats, grad_losses, grad_weights);
+    if (rc != MOE_OK) return rc;
+    MOE_REQUIRE(hidden >= 8 && hidden % 8 == 0 && hidden <= kMaxLowRankWidth, MOE_ERR_UNSUPPORTED,
+                "route backward needs hidden a positive multiple of 8 up to %lld", (long long)kMaxLowRankWidth);
+    MOE_REQUIRE(tokens >= 1 && tokens <= kMaxAdapterTokens, MOE_ERR_CAPACITY, "route backward takes 1..%lld tokens",
+                (long long)kMaxAdapterTokens);
+    MOE_REQUIRE((!grad_x || router_w) && (!grad_router_w || x), MOE_ERR_INVALID_ARGUMENT, "null pointer");
+    const int64_t need = route_backward_scratch_bytes(tokens, hidden, experts);
+    MOE_REQUIRE(scratch && scratch_bytes >= need, MOE_ERR_WORKSPACE, "route backward scratch needs %lld bytes, got %lld",
+                (long long)need, (long long)scratch_bytes);
+    MOE_REQUIRE(aligned_to(x, 16) && aligned_to(router_w, 16) && aligned_to(grad_x_base, 16) && aligned_to(grad_x, 16) &&
+                    aligned_to(grad_router_w, 16) && aligned_to(scratch, 16),
+                MOE_ERR_INVALID_ARGUMENT, "x, router weights, their gradients and scratch must be 16-byte aligned");
+    MOE_REQUIRE(aligned_to(grad_bias, 4), MOE_ERR_INVALID_ARGUMENT, "pointers must be aligned to their element size");
+    return launch_route_backward(static_cast<const uint16_t*>(x), router_w, logits, bias, ids, mask, stats, grad_losses,
+                                 grad_weights, static_cast<const uint16_t*>(grad_x_base), static_cast<uint16_t*>(grad_x),
+                                 grad_router_w, grad_bias, static_cast<char*>(scratch), tokens, hidden, (int)experts,
+                                 (int)topk, static_cast<hipStream_t>(stream));
+}
+
+// -- training: the transport's gradients --------------------------------------
+
+int moe_combine_backward(const void* grad_output, const void* expert_output, int dtype, const int32_t* inverse,
+                         const float* weights, const int32_t* counts, const int32_t* offsets, void* grad_expert_output,
+                         float* grad_weights, int64_t tokens, int64_t hidden, int64_t experts, int64_t topk,
+                         int64_t packed_rows, void* stream) {
+    MOE_REQUIRE(valid_dtype(dtype), MOE_ERR_INVALID_ARGUMENT, "only FP32, FP16 and BF16 are supported");
+    MOE_REQUIRE(topk >= 1 && topk <= kMaxTopk, MOE_ERR_UNSUPPORTED, "topk must be in 1..8");
+    MOE_REQUIRE(experts >= 1 && experts <= kMaxExperts, MOE_ERR_UNSUPPORTED, "supports 1..64 experts");
+    MOE_REQUIRE(tokens >= 0 && hidden > 0, MOE_ERR_INVALID_ARGUMENT, "invalid shape");
+    MOE_REQUIRE(tokens * topk <= INT_MAX && hidden <= INT_MAX && packed_rows <= INT_MAX, MOE_ERR_CAPACITY,
+                "shape exceeds int32 indexing capacity");
+    MOE_REQUIRE(packed_rows >= tokens * topk, MOE_ERR_INVALID_ARGUMENT, "packed rows hold fewer than the assignments");
+    if (packed_rows == 0) return MOE_OK;
+    MOE_REQUIRE(counts && offsets && grad_expert_output, MOE_ERR_INVALID_ARGUMENT, "null pointer");
+    MOE_REQUIRE(tokens == 0 || (grad_output && expert_output && inverse && weights && grad_weights),
+                MOE_ERR_INVALID_ARGUMENT, "null pointer");
+    const uintptr_t elem = static_cast<uintptr_t>(dtype_size(dtype));
+    MOE_REQUIRE(aligned_to(grad_output, elem) && aligned_to(expert_output, elem) && aligned_to(grad_expert_output, elem),
+                MOE_ERR_INVALID_ARGUMENT, "rows must be aligned to their element size");
+    MOE_REQUIRE(aligned_to(inverse, 4) && aligned_to(weights, 4) && aligned_to(counts, 4) && aligned_to(offsets, 4) &&
+                    aligned_to(grad_weights, 4),
+                MOE_ERR_INVALID_ARGUMENT, "index and weight buffers must be 4-byte aligned");
+    return launch_combine_grad(grad_output, expert_output, dtype, inverse, weights, counts, offsets, grad_expert_output,
+                               grad_weights, tokens, hidden, (int)topk, (int)experts, packed_rows,
+                               static_cast<hipStream_t>(stream));
+}
+
+int moe_dispatch_backward(const void* grad_packed, int dtype, const int32_t* inverse, void* grad_x, int64_t tokens,
+                          int64_t hidden, int64_t topk, int64_t packed_rows, void* stream) {
+    MOE_REQUIRE(valid_dtype(dtype), MOE_ERR_INVALID_ARGUMENT, "only FP32, FP16 and BF16 are supported");
+    MOE_REQUIRE(topk >= 1 && topk <= kMaxTopk, MOE_ERR_UNSUPPORTED, "topk must be in 1..8");
+    MOE_REQUIRE(tokens >= 0 && hidden > 0, MOE_ERR_INVALID_ARGUMENT, "invalid shape");
+    MOE_REQUIRE(tokens * topk <= INT_MAX && hidden <= INT_MAX && packed_rows <= INT_MAX, MOE_ERR_CAPACITY,
+                "shape exceeds int32 indexing capacity");
+    MOE_REQUIRE(packed_rows >= tokens * topk, MOE_ERR_INVALID_ARGUMENT, "packed rows hold fewer than the assignments");
+    if (tokens == 0) return MOE_OK;
+    MOE_REQUIRE(grad_packed && inverse && grad_x, MOE_ERR_INVALID_ARGUMENT, "null pointer");
+    const uintptr_t elem = static_cast<uintptr_t>(dtype_size(dtype));
+    MOE_REQUIRE(aligned_to(grad_packed, elem) && aligned_to(grad_x, elem) && aligned_to(inverse, 4),
+                MOE_ERR_INVALID_ARGUMENT, "rows must be aligned to their element size, inverse to 4 bytes");
+    return launch_combine(grad_packed, dtype, inverse, nullptr, grad_x, tokens, hidden, (int)topk, packed_rows,
+                          static_cast<hipStream_t>(stream));
+}
+
+// -- low-rank adapters --------------------------------------------------------
+
+int64_t moe_adapter_table_bytes(int64_t tokens, int64_t adapters) {
+    if (tokens < 0 || tokens > kMaxAdapterTokens || adapters < 1 || adapters > kMaxAdapters) return -1;
+    return table_layout(tokens, adapters).ints * 4;
+}
+
+static int check_adapter_table(const void* table, int64_t table_bytes, int64_t tokens, int64_t adapters) {
+    MOE_REQUIRE(adapters >= 1 && adapters <= kMaxAdapters, MOE_ERR_UNSUPPORTED, "supports 1..%d adapters", kMaxAdapters);
+    MOE_REQUIRE(tokens >= 0, MOE_ERR_INVALID_ARGUMENT, "tokens must be >= 0");
+    MOE_REQUIRE(tokens <= kMaxAdapterTokens, MOE_ERR_CAPACITY, "takes up to %lld tokens", (long long)kMaxAdapterTokens);
+    const int64_t need = table_layout(tokens, adapters).ints * 4;
+    MOE_REQUIRE(table && table_bytes >= need, MOE_ERR_WORKSPACE, "adapter table needs %lld bytes, got %lld",
+                (long long)need, (long long)table_bytes);
+    MOE_REQUIRE(aligned_to(table, 16), MOE_ERR_INVALID_ARGUMENT, "adapter table must be 16-byte aligned");
+    return MOE_OK;
+}
+
+int moe_adapter_group(const int32_t* ids, void* table, int64_t table_bytes, int64_t tokens, int64_t adapters,
+                      void* stream) {
+    const int rc = check_adapter_table(table, table_bytes, tokens, adapters);
+    if (rc != MOE_OK) return rc;
+    MOE_REQUIRE(tokens == 0 || ids, MOE_ERR_INVALID_ARGUMENT, "null pointer");
+    MOE_REQUIRE(aligned_to(ids, 4), MOE_ERR_INVALID_ARGUMENT, "adapter ids must be 4-byte aligned");
+    return launch_adapter_group(ids, table, tokens, (int)adapters, static_cast<hipStream_t>(stream));
+}
+
+static bool valid_low_rank_width(int64_t n) { return n >= 8 && n % 8 == 0 && n <= kMaxLowRankWidth; }
+
+int64_t moe_low_rank_scratch_bytes(int64_t tokens, int64_t hidden, int64_t width, int64_t rank, int64_t adapters,
+                                   int backward) {
+    if (tokens < 0 || tokens > kMaxAdapterTokens || adapters < 1 || adapters > kMaxAdapters ||
+        !valid_low_rank_width(hidden) || !valid_low_rank_width(width) || rank < 1 || rank > kMaxRank)
+        return -1;
+    return low_rank_scratch_bytes(tokens, hidden, width, rank, adapters, backward != 0);
+}
+
+static int check_low_rank(const void* table, int64_t table_bytes, const void* scratch, int64_t scratch_bytes,
+                          int64_t tokens, int64_t hidden, int64_t width, int64_t rank, int64_t adapters, bool backward) {
+    const int rc = check_adapter_table(table, table_bytes, tokens, adapters);
+    if (rc != MOE_OK) return rc;
+    MOE_REQUIRE(valid_low_rank_width(hidden) && valid_low_rank_width(width), MOE_ERR_UNSUPPORTED,
+                "low-rank widths must be multiples of 8 up to %lld", (long long)kMaxLowRankWidth);
+    MOE_REQUIRE(rank >= 1 && rank <= kMaxRank, MOE_ERR_UNSUPPORTED, "rank must be in 1..%d", kMaxRank);
+    const int64_t need = low_rank_scratch_bytes(tokens, hidden, width, rank, adapters, backward);
+    MOE_REQUIRE((scratch || need == 0) && scratch_bytes >= need, MOE_ERR_WORKSPACE,
+                "low-rank scratch needs %lld bytes, got %lld", (long long)need, (long long)scratch_bytes);
+    MOE_REQUIRE(aligned_to(scratch, 16), MOE_ERR_INVALID_ARGUMENT, "scratch must be 16-byte aligned");
+    return MOE_OK;
+}
+
+int moe_low_rank_add(const void* x, const void* down, const void* up, const float* scales, const void* table,
+                     int64_t table_bytes, const void* base, void* output, float* hidden_out, void* scratch,
+                     int64_t scratch_bytes, int64_t tokens, int64_t hidden, int64_t width, int64_t rank,
+                     int64_t adapters, void* stream) {
+    const int rc = check_low_rank(table, table_bytes, scratch, scratch_bytes, tokens, hidden, width, rank, adapters,
+                                  false);
+    if (rc != MOE_OK || tokens == 0) return rc;
+    MOE_REQUIRE(x && down && up && output, MOE_ERR_INVALID_ARGUMENT, "null pointer");
+    MOE_REQUIRE(aligned_to(x, 16) && aligned_to(down, 16) && aligned_to(up, 16) && aligned_to(base, 16) &&
+                    aligned_to(output, 16) && aligned_to(scales, 4) && aligned_to(hidden_out, 4),
+                MOE_ERR_INVALID_ARGUMENT, "rows and adapters must be 16-byte aligned");
+    return launch_low_rank_add(static_cast<const uint16_t*>(x), static_cast<const uint16_t*>(down),
+                               static_cast<const uint16_t*>(up), scales, table, static_cast<const uint16_t*>(base),
+                               static_cast<uint16_t*>(output), hidden_out, static_cast<char*>(scratch), tokens, hidden,
+                               width, (int)rank, (int)adapters, static_cast<hipStream_t>(stream));
+}
+
+int moe_low_rank_backward(const void* grad_output, const void* x, const void* down, const void* up, const float* scales,
+                          const void* table, int64_t table_bytes, const float* hidden_in, const void* grad_x_base,
+                          void* grad_x, void* grad_down, void* grad_up, int grad_dtype, void* scratch,
+                          int64_t scratch_bytes, int64_t tokens, int64_t hidden, int64_t width, int64_t rank,
+                          int64_t adapters, void* stream) {
+    const int rc = check_low_rank(table, table_bytes, scratch, scratch_bytes, tokens, hidden, width, rank, adapters, true);
+    if (rc != MOE_OK) return rc;
+    MOE_REQUIRE(grad_dtype == MOE_DTYPE_F32 || grad_dtype == MOE_DTYPE_BF16, MOE_ERR_INVALID_ARGUMENT,
+                "adapter gradients are FP32 or BF16");
+    if (tokens > 0) {
+        MOE_REQUIRE(grad_output && x && down && up, MOE_ERR_INVALID_ARGUMENT, "null pointer");
+        MOE_REQUIRE(!grad_up || hidden_in, MOE_ERR_INVALID_ARGUMENT, "grad_up needs the forward's hidden");
+    }
+    MOE_REQUIRE(aligned_to(grad_output, 16) && aligned_to(x, 16) && aligned_to(down, 16) && aligned_to(up, 16) &&
+                    aligned_to(grad_x_base, 16) && aligned_to(grad_x, 16) && aligned_to(grad_down, 16) &&
+                    aligned_to(grad_up, 16) && aligned_to(scales, 4) && aligned_to(hidden_in, 4),
+                MOE_ERR_INVALID_ARGUMENT, "rows and adapters must be 16-byte aligned");
+    return launch_low_rank_backward(
+        static_cast<const uint16_t*>(grad_output), static_cast<const uint16_t*>(x), static_cast<const uint16_t*>(down),
+        static_cast<const uint16_t*>(up), scales, table, hidden_in, static_cast<const uint16_t*>(grad_x_base),
+        static_cast<uint16_t*>(grad_x), grad_down, grad_up, grad_dtype == MOE_DTYPE_BF16, static_cast<char*>(scratch),
+        tokens, hidden, width, (int)rank, (int)adapters, static_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"

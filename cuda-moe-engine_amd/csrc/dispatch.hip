@@ -366,8 +366,9 @@ __global__ __launch_bounds__(kPackThreads) void pack_kernel(
 // 4096 tokens, top-2: fewer waves fit a CU). As in pack_kernel,
 // the last vector of a row that is no multiple of VE overlaps the one before.
 // ---------------------------------------------------------------------------
-// WHOLE: every vector is VE elements of its own at a VE-aligned address.
-template <int DT, int VE, int VECS, bool WHOLE>
+// WHOLE: every vector is VE elements of its own at a VE-aligned address. UNIT: every
+// weight is 1 (the dispatch's gradient; weights is not read).
+template <int DT, int VE, int VECS, bool WHOLE, bool UNIT>
 __global__ __launch_bounds__(256) void combine_kernel(
     const typename Elem<DT>::T* __restrict__ y, const int32_t* __restrict__ inverse,
     const float* __restrict__ weights, typename Elem<DT>::T* __restrict__ out, int64_t tokens,
@@ -412,7 +413,7 @@ __global__ __launch_bounds__(256) void combine_kernel(
                 const int row = inverse[pa];
                 ok[kk] = row >= 0 && row < rows;
                 if (ok[kk]) {
-                    w[kk] = weights[pa];
+                    w[kk] = UNIT ? 1.0f : weights[pa];
                     const T* src = y + static_cast<int64_t>(row) * hidden;
 #pragma unroll
                     for (int u = 0; u < VECS; ++u)
@@ -659,8 +660,8 @@ static int launch_pack(const void* x, int dtype, const int32_t* ids, int32_t* co
     return check_launch("pack_kernel");
 }
 
-template <int DT, int VE>
-static void launch_combine_t(const void* y, const int32_t* inverse, const float* weights,
+template <int DT, int VE, bool UNIT>
+static void launch_combine_u(const void* y, const int32_t* inverse, const float* weights,
                              void* out, int64_t tokens, int64_t hidden, int topk, int64_t rows,
                              hipStream_t stream) {
     using T = typename Elem<DT>::T;
@@ -676,7 +677,7 @@ static void launch_combine_t(const void* y, const int32_t* inverse, const float*
         const int64_t groups = ((hidden + VE - 1) / VE + VECS - 1) / VECS;
         const int64_t threads = tokens * groups;
         const dim3 grid(static_cast<unsigned>((threads + 255) / 256));
-        hipLaunchKernelGGL((combine_kernel<DT, VE, VECS, WHOLE>), grid, dim3(256), 0, stream,
+        hipLaunchKernelGGL((combine_kernel<DT, VE, VECS, WHOLE, UNIT>), grid, dim3(256), 0, stream,
                            static_cast<const T*>(y), inverse, weights, static_cast<T*>(out), tokens,
                            hidden, topk, rows);
     };
@@ -691,6 +692,18 @@ static void launch_combine_t(const void* y, const int32_t* inverse, const float*
     else
         vecs(std::false_type{});
 }
+
+template <int DT, int VE>
+static void launch_combine_t(const void* y, const int32_t* inverse, const float* weights,
+                             void* out, int64_t tokens, int64_t hidden, int topk, int64_t rows,
+                             hipStream_t stream) {
+    if (weights)
+        launch_combine_u<DT, VE, false>(y, inverse, weights, out, tokens, hidden, topk, rows, stream);
+    else
+        launch_combine_u<DT, VE, true>(y, inverse, weights, out, tokens, hidden, topk, rows, stream);
+}
+
+// weights == nullptr: every weight is 1.
 
 int launch_combine(const void* y, int dtype, const int32_t* inverse, const float* weights,
                    void* out, int64_t tokens, int64_t hidden, int topk, int64_t rows,

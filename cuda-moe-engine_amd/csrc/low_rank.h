@@ -1,0 +1,107 @@
+// Row grouping by adapter and the three products of low-rank adapters (contract,
+// spread, outer), shared by low_rank.hip and router_grad.hip.
+#pragma once
+
+#include "moe_common.h"
+
+namespace moe {
+
+constexpr int kMaxAdapters = 4096;
+constexpr int kMaxRank = 128;
+constexpr int64_t kMaxAdapterTokens = 1 << 24;
+constexpr int64_t kMaxLowRankWidth = 1 << 20;
+constexpr int kTileRows = 64;     // rows of one adapter per tile (contract, spread)
+constexpr int kSpreadCols = 512;  // columns per workgroup of spread: 128 per wave
+constexpr int kOuterCols = 128;   // columns per workgroup of outer
+
+// Where the parts of an adapter table lie, in int32 from its start:
+//   head         [4]     tiles, splits, 0, 0
+//   order        [T]     rows sorted by adapter (stable); rows of no adapter last
+//   starts       [N + 2] first sorted row of each adapter, of the rows of none, T
+//   split_start  [N + 1] first split of each adapter
+//   tiles        [tile_bound]  {adapter (-1: none), first sorted row, rows <= kTileRows, 0}
+//   splits       [split_bound] {adapter, first sorted row, rows <= split_rows, adapter's splits}
+struct TableLayout {
+    int64_t order, starts, split_start, tiles, splits, ints;
+    int tile_bound, split_bound, split_rows;
+};
+
+// Rows per split of the outer product: a split's partial result is written and read
+// back once (4 * rank * width bytes twice), so few of them, but enough workgroups
+// (splits * width / 128) to fill the card: about 16 splits of a batch.
+inline int outer_split_rows(int64_t tokens) {
+    int rows = 128;
+    while (rows < 1024 && rows * 16 < tokens) rows <<= 1;
+    return rows;
+}
+
+inline TableLayout table_layout(int64_t tokens, int64_t adapters) {
+    TableLayout t{};
+    const auto up4 = [](int64_t n) { return (n + 3) / 4 * 4; };
+    t.split_rows = outer_split_rows(tokens);
+    // Each group has at most one partial tile (split).
+    t.tile_bound = static_cast<int>(tokens / kTileRows + (adapters + 1 < tokens ? adapters + 1 : tokens));
+    t.split_bound = static_cast<int>(tokens / t.split_rows + (adapters < tokens ? adapters : tokens));
+    t.order = 4;
+    t.starts = t.order + up4(tokens);
+    t.split_start = t.starts + up4(adapters + 2);
+    t.tiles = t.split_start + up4(adapters + 1);
+    t.splits = t.tiles + 4 * static_cast<int64_t>(t.tile_bound);
+    t.ints = t.splits + 4 * static_cast<int64_t>(t.split_bound);
+    return t;
+}
+
+// Device view of a table. A null order stands for one group of all rows in order.
+struct Groups {
+    const int32_t* head = nullptr;
+    const int32_t* order = nullptr;
+    const int32_t* split_start = nullptr;
+    const int4* tiles = nullptr;
+    const int4* splits = nullptr;
+    int tile_bound = 0, split_bound = 0, split_rows = 0;
+};
+
+inline Groups groups_of(const void* table, int64_t tokens, int64_t adapters) {
+    const TableLayout t = table_layout(tokens, adapters);
+    const int32_t* base = static_cast<const int32_t*>(table);
+    Groups g;
+    g.head = base;
+    g.order = base + t.order;
+    g.split_start = base + t.split_start;
+    g.tiles = reinterpret_cast<const int4*>(base + t.tiles);
+    g.splits = reinterpret_cast<const int4*>(base + t.splits);
+    g.tile_bound = t.tile_bound;
+    g.split_bound = t.split_bound;
+    g.split_rows = t.split_rows;
+    return g;
+}
+
+inline Groups one_group(int64_t tokens) {
+    Groups g;
+    g.split_rows = outer_split_rows(tokens);
+    g.tile_bound = static_cast<int>((tokens + kTileRows - 1) / kTileRows);
+    g.split_bound = static_cast<int>((tokens + g.split_rows - 1) / g.split_rows);
+    return g;
+}
+
+// K slices of contract for this shape; partials holds that many [tokens, rank] sums.
+int contract_slices(int tile_bound, int64_t k);
+
+// partials[s][i][c] = sum over slice s of x[order[i]][k] * w[adapter][c][k]; rows of no
+// adapter are not written.
+int launch_contract(const uint16_t* x, const uint16_t* w, const Groups& g, float* partials, int slices, int64_t tokens,
+                    int64_t k, int rank, hipStream_t stream);
+
+// out[order[i]][j] = base[order[i]][j] + scale * sum_c h[i][c] * w[adapter][c][j], h the sum
+// of `slices` partials; rows of no adapter: out = base. base may be null (0) or out.
+// w is bf16, or fp32 for w32. h_out (may be null) receives h.
+int launch_spread(const float* partials, int slices, const void* w, bool w32, const float* scales, const Groups& g,
+                  const uint16_t* base, uint16_t* out, float* h_out, int64_t tokens, int64_t width, int rank,
+                  hipStream_t stream);
+
+// out[a][c][j] = scale_a * sum over a's rows of h[i][c] * x[order[i]][j], fp32 or bf16;
+// 0 for an adapter without rows. partials: split_bound * rank * width fp32.
+int launch_outer(const float* h, const uint16_t* x, const float* scales, const Groups& g, float* partials, void* out,
+                 bool out_bf16, int64_t tokens, int64_t width, int rank, int adapters, hipStream_t stream);
+
+}  // namespace moe

@@ -64,6 +64,19 @@ _SIGNATURES = {
                                                    + [_c_void_p] * 2 + [_i64] * 4 + [_c_void_p]),
     "moe_block_forward": (_int, [_c_void_p] * 4),
     "moe_set_gemm_workgroups": (_int, [_i64]),
+    "moe_router_loss_scratch_bytes": (_i64, [_i64, _i64]),
+    "moe_router_loss": (_int, [_c_void_p] * 7 + [_i64] * 4 + [_c_void_p]),
+    "moe_router_logits_backward": (_int, [_c_void_p] * 8 + [_i64] * 3 + [_c_void_p]),
+    "moe_route_backward_scratch_bytes": (_i64, [_i64] * 3),
+    "moe_route_backward": (_int, [_c_void_p] * 14 + [_i64] * 5 + [_c_void_p]),
+    "moe_combine_backward": (_int, [_c_void_p, _c_void_p, _int] + [_c_void_p] * 6 + [_i64] * 5 + [_c_void_p]),
+    "moe_dispatch_backward": (_int, [_c_void_p, _int, _c_void_p, _c_void_p] + [_i64] * 4 + [_c_void_p]),
+    "moe_adapter_table_bytes": (_i64, [_i64, _i64]),
+    "moe_adapter_group": (_int, [_c_void_p, _c_void_p] + [_i64] * 3 + [_c_void_p]),
+    "moe_low_rank_scratch_bytes": (_i64, [_i64] * 5 + [_int]),
+    "moe_low_rank_add": (_int, [_c_void_p] * 5 + [_i64] + [_c_void_p] * 4 + [_i64] * 6 + [_c_void_p]),
+    "moe_low_rank_backward": (_int, [_c_void_p] * 6 + [_i64] + [_c_void_p] * 5 + [_int, _c_void_p] + [_i64] * 6
+                              + [_c_void_p]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)

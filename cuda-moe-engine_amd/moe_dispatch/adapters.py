@@ -1,0 +1,179 @@
+"""Low-rank adapters of many requests at once, beside a shared or grouped projection.
+
+A batch's rows belong to requests with adapters of their own: row t with adapter a gets
+
+    output[t] = base[t] + scales[a] * up[a]^T (down[a] x[t]),
+
+``base`` the shared projection's output (``experts.grouped_linear``, or any other product);
+rows without an adapter keep it. ``down`` is [N, r, H] and ``up`` [N, r, O], both
+rank-major, so that the forward and the gradients are the same kernels; an adapter stored
+as [O, r] is transposed once when it is loaded, one of a lower rank padded with zero rows.
+
+``AdapterGroups`` sorts a batch's rows by adapter once a step; every projection of every
+layer of that step then takes the same groups. ``low_rank_add`` serves prefill batches
+and single tokens alike; ``low_rank_backward`` gives x's and the adapters' gradients. Rows
+packed by expert (``ops.dispatch``) are grouped the same way, with each packed row's
+expert, or expert and adapter, as its id. No counterpart in the reference.
+
+Checks, streams and errors are those of ``moe_dispatch.training``.
+"""
+
+from dataclasses import dataclass
+
+import torch
+
+from ._extension import DTYPE_CODES, current_stream_handle, get_extension
+from .training import _ptr, on_device, refuse_autograd, require_tensor, scratch_for
+
+MAX_ADAPTERS = 4096
+MAX_RANK = 128
+MAX_ROWS = 2**24
+MAX_WIDTH = 2**20
+
+
+class AdapterGroups:
+    """The rows of one batch sorted by adapter, on the device.
+
+    ``assign(ids)`` groups the rows by their int32 adapter ids [T]; an id outside
+    [0, adapters) means no adapter. The groups hold until the next ``assign``. One object
+    serves one sequential stream of calls; a graph that captured its calls needs it kept.
+    """
+
+    def __init__(self, tokens, adapters, *, device="cuda", extension=None):
+        if not isinstance(tokens, int) or not 0 <= tokens <= MAX_ROWS:
+            raise ValueError("tokens must be an integer in 0..2^24")
+        if not isinstance(adapters, int) or not 1 <= adapters <= MAX_ADAPTERS:
+            raise ValueError("adapters must be an integer in 1..4096")
+        device = torch.device(device)
+        if device.type != "cuda" or not torch.cuda.is_available():
+            raise RuntimeError("AdapterGroups requires an AMD GPU")
+        if device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        self.tokens, self.adapters, self.device = tokens, adapters, device
+        self.extension = extension if extension is not None else get_extension()
+        self.assignment = 0  # how many times assign ran: what a kept hidden belongs to
+        nbytes = self.extension.lib.moe_adapter_table_bytes(tokens, adapters)
+        self.table = torch.empty(nbytes // 4, dtype=torch.int32, device=device)
+
+    def assign(self, ids):
+        require_tensor(ids, "ids", (self.tokens,), torch.int32, self.device)
+        lib = self.extension.lib
+        with on_device(self.device):
+            lib.check(lib.moe_adapter_group(ids.data_ptr(), self.table.data_ptr(), self.table.numel() * 4, self.tokens,
+                                            self.adapters, current_stream_handle(self.device.index)), "assign")
+        self.assignment += 1
+
+    @property
+    def order(self):
+        """The rows in sorted order, int32 [T] (a view): by adapter, each one's rows in
+        batch order, rows of no adapter last."""
+        return self.table[4:4 + self.tokens]
+
+
+@dataclass(frozen=True)
+class LowRankHidden:
+    """``down[a] x`` of one ``low_rank_add``, fp32 [T, r] in the groups' row order, for its
+    ``low_rank_backward`` on the same assignment."""
+
+    values: torch.Tensor
+    groups: AdapterGroups
+    assignment: int
+
+
+def _check_width(n, name):
+    if n < 8 or n % 8 or n > MAX_WIDTH:
+        raise ValueError(f"{name} must be a multiple of 8 up to 2^20")
+
+
+def _check_operands(x, down, up, groups, scales):
+    if not isinstance(groups, AdapterGroups):
+        raise TypeError("groups must be AdapterGroups")
+    if groups.assignment == 0:
+        raise RuntimeError("AdapterGroups.assign has not grouped any rows yet")
+    device = groups.device
+    tokens, adapters = groups.tokens, groups.adapters
+    require_tensor(x, "x", (tokens, None), torch.bfloat16, device)
+    hidden = x.shape[1]
+    require_tensor(down, "down", (adapters, None, hidden), torch.bfloat16, device)
+    rank = down.shape[1]
+    require_tensor(up, "up", (adapters, rank, None), torch.bfloat16, device)
+    width = up.shape[2]
+    _check_width(hidden, "hidden")
+    _check_width(width, "width")
+    if not 1 <= rank <= MAX_RANK:
+        raise ValueError("rank must be in 1..128")
+    if scales is not None:
+        require_tensor(scales, "scales", (adapters,), torch.float32, device)
+    return tokens, adapters, hidden, width, rank, device
+
+
+def _overlaps(a, b):
+    return a.numel() > 0 and b.numel() > 0 and a.data_ptr() < b.data_ptr() + b.numel() * b.element_size() and (
+        b.data_ptr() < a.data_ptr() + a.numel() * a.element_size())
+
+
+def low_rank_add(base, x, down, up, groups, *, scales=None, output=None, return_hidden=False):
+    """``base`` plus each row's adapter: bf16 [T, O], rounded once from fp32.
+
+    ``base`` bf16 [T, O] (None: 0), x bf16 [T, H], ``scales`` fp32 [N] (None: 1). H and O are
+    multiples of 8, r is 1..128. ``output``: where the result goes, ``base`` itself included
+    (in place); a new tensor when None. With ``return_hidden`` the result is
+    ``(output, hidden)``, ``hidden`` for ``low_rank_backward``.
+    """
+    tokens, adapters, hidden, width, rank, device = _check_operands(x, down, up, groups, scales)
+    if base is not None:
+        require_tensor(base, "base", (tokens, width), torch.bfloat16, device)
+    if output is not None:
+        require_tensor(output, "output", (tokens, width), torch.bfloat16, device)
+        if any(_overlaps(output, t) for t in (x, down, up)) or (
+                base is not None and output.data_ptr() != base.data_ptr() and _overlaps(output, base)):
+            raise ValueError("output may be base itself, but must not overlap another operand")
+    refuse_autograd(base, x, down, up, scales, output)
+    lib = groups.extension.lib
+    with on_device(device):
+        if output is None:
+            output = torch.empty((tokens, width), dtype=torch.bfloat16, device=device)
+        kept = torch.empty((tokens, rank), dtype=torch.float32, device=device) if return_hidden else None
+        scratch = scratch_for(lib.moe_low_rank_scratch_bytes(tokens, hidden, width, rank, adapters, 0), device)
+        lib.check(lib.moe_low_rank_add(
+            x.data_ptr(), down.data_ptr(), up.data_ptr(), _ptr(scales), groups.table.data_ptr(),
+            groups.table.numel() * 4, _ptr(base), output.data_ptr(), _ptr(kept), scratch.data_ptr(), scratch.numel(),
+            tokens, hidden, width, rank, adapters, current_stream_handle(device.index)), "low_rank_add")
+    return (output, LowRankHidden(kept, groups, groups.assignment)) if return_hidden else output
+
+
+def low_rank_backward(grad_output, x, down, up, groups, *, scales=None, hidden, grad_x=None,
+                      grad_dtype=torch.float32):
+    """Gradients of ``low_rank_add``: ``(grad_x, grad_down, grad_up)``; base's is ``grad_output``.
+
+    ``hidden`` is what the forward returned with ``return_hidden``, on the groups' current
+    assignment. ``grad_x`` bf16 [T, H] is x's gradient along its other paths (the shared
+    projection): the result is the sum, rounded once. grad_down and grad_up are
+    ``grad_dtype`` (fp32, or bf16 rounded once), zero for adapters without rows. scales get
+    no gradient.
+    """
+    tokens, adapters, h, width, rank, device = _check_operands(x, down, up, groups, scales)
+    require_tensor(grad_output, "grad_output", (tokens, width), torch.bfloat16, device)
+    if not isinstance(hidden, LowRankHidden):
+        raise TypeError("hidden must be what low_rank_add returned with return_hidden")
+    if hidden.groups is not groups or hidden.assignment != groups.assignment:
+        raise RuntimeError("hidden belongs to another assignment of these groups")
+    require_tensor(hidden.values, "hidden", (tokens, rank), torch.float32, device)
+    if grad_x is not None:
+        require_tensor(grad_x, "grad_x", (tokens, h), torch.bfloat16, device)
+    if grad_dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError("grad_dtype must be float32 or bfloat16")
+    refuse_autograd(grad_output, x, down, up, scales, grad_x)
+    lib = groups.extension.lib
+    with on_device(device):
+        out_x = torch.empty_like(x)
+        grad_down = torch.empty(down.shape, dtype=grad_dtype, device=device)
+        grad_up = torch.empty(up.shape, dtype=grad_dtype, device=device)
+        scratch = scratch_for(lib.moe_low_rank_scratch_bytes(tokens, h, width, rank, adapters, 1), device)
+        lib.check(lib.moe_low_rank_backward(
+            grad_output.data_ptr(), x.data_ptr(), down.data_ptr(), up.data_ptr(), _ptr(scales),
+            groups.table.data_ptr(), groups.table.numel() * 4, hidden.values.data_ptr(), _ptr(grad_x),
+            out_x.data_ptr(), grad_down.data_ptr(), grad_up.data_ptr(), DTYPE_CODES[grad_dtype], scratch.data_ptr(),
+            scratch.numel(), tokens, h, width, rank, adapters, current_stream_handle(device.index)),
+            "low_rank_backward")
+    return out_x, grad_down, grad_up

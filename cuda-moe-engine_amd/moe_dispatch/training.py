@@ -1,0 +1,254 @@
+"""The router's training losses, and the gradients of the router and the transport.
+
+The forward path's kernels (``MoEBlock.route``, ``ops.dispatch``, ``ops.combine``) record
+no autograd graph. These operators are their training side, on the kernels of
+``libmoe_hip.so``, as plain calls on tensors:
+
+* ``router_loss``: balance loss, z loss and per-expert counts of a routed batch;
+* ``route_logits_backward``: the gradient of the logits, from the losses' and the
+  routing weights' gradients;
+* ``route_backward``: that, and behind it the gradients of x, router weight and bias;
+* ``combine_backward`` and ``dispatch_backward``: the transport's gradients.
+
+``moe_dispatch.autograd`` wraps them for ``loss.backward()``. Nothing here has a
+counterpart in the reference, which is forward-only.
+
+Each call checks its tensors on the host (``ValueError`` for shapes, devices and layouts,
+``TypeError`` for dtypes, ``RuntimeError`` without a GPU), launches on the current stream
+of the tensors' device and does not synchronise. Results are new tensors. Every sum has
+one order: results do not vary from call to call.
+"""
+
+from contextlib import nullcontext
+from dataclasses import dataclass
+
+import torch
+
+from ._extension import DTYPE_CODES, current_stream_handle, get_extension
+from .workspace import MAX_EXPERTS, MAX_TOPK
+
+
+def on_device(device):
+    """Makes ``device`` current where it is not: streams and launches go by the current device."""
+    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def require_tensor(t, name, shape, dtype, device=None):
+    """The checks every operand shares; ``dtype`` may be a tuple of the dtypes allowed."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor")
+    if t.dtype != dtype and not (isinstance(dtype, tuple) and t.dtype in dtype):
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.dim() != len(shape) or any(want is not None and have != want for have, want in zip(t.shape, shape)):
+        raise ValueError(f"{name}: expected shape {['any' if n is None else n for n in shape]}, got {list(t.shape)}")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} must be on {device}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
+def refuse_autograd(*tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError("this operator records no autograd graph: detach its inputs, call it under no_grad, "
+                         "or use moe_dispatch.autograd")
+
+
+def require_gpu(t):
+    if not t.is_cuda:
+        raise RuntimeError("training operators require an AMD GPU")
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def scratch_for(nbytes, device):
+    return torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
+
+
+@dataclass(frozen=True)
+class RouterLoss:
+    """``losses`` fp32 [2] (balance, z) and ``stats`` int32 [E + 1] (per-expert counts of the
+    valid tokens' assignments, then the number of valid tokens)."""
+
+    losses: torch.Tensor
+    stats: torch.Tensor
+
+    @property
+    def balance(self):
+        return self.losses[0]
+
+    @property
+    def z(self):
+        return self.losses[1]
+
+    @property
+    def counts(self):
+        return self.stats[:-1]
+
+
+def _check_routed(logits, expert_ids, bias, mask):
+    require_tensor(logits, "logits", (None, None), torch.float32)
+    tokens, experts = logits.shape
+    if not 1 <= experts <= MAX_EXPERTS:
+        raise ValueError("logits must have 1..64 experts")
+    require_tensor(expert_ids, "expert_ids", (tokens, None), torch.int32, logits.device)
+    if not 1 <= expert_ids.shape[1] <= MAX_TOPK:
+        raise ValueError("topk must be in 1..8")
+    if tokens * max(experts, expert_ids.shape[1]) > 2**31 - 1:
+        raise ValueError("tokens*experts and tokens*topk must fit int32")
+    if bias is not None:
+        require_tensor(bias, "bias", (experts,), torch.float32, logits.device)
+    if mask is not None:
+        require_tensor(mask, "mask", (tokens,), torch.bool, logits.device)
+    return tokens, experts, expert_ids.shape[1]
+
+
+def router_loss(logits, expert_ids, bias=None, *, mask=None):
+    """Balance loss, z loss and per-expert counts of a routed batch.
+
+    ``logits`` fp32 [T, E] (without the bias), ``expert_ids`` int32 [T, K] as the router
+    chose them on ``logits + bias``, ``mask`` bool [T] false for padding tokens. With p the
+    softmax of ``logits + bias``, N the valid tokens and c_e their assignments to expert e:
+
+    * balance = E * sum_e (c_e / (N K)) * mean_t p_te, 1 where both are uniform;
+    * z = mean_t (log sum_e exp(logits + bias)_te)^2.
+
+    Both are 0 without valid tokens. Ids out of range count nowhere. Logits may be -inf (a
+    token of none but -inf adds nothing to the losses); +inf or NaN ones of a valid token
+    show in the losses.
+    """
+    tokens, experts, topk = _check_routed(logits, expert_ids, bias, mask)
+    require_gpu(logits)
+    refuse_autograd(logits, bias)
+    lib = get_extension().lib
+    device = logits.device
+    with on_device(device):
+        # Losses and stats are parts of one buffer, one allocation.
+        buffer = torch.empty(experts + 3, dtype=torch.float32, device=device)
+        losses, stats = buffer[:2], buffer[2:].view(torch.int32)
+        scratch = scratch_for(lib.moe_router_loss_scratch_bytes(tokens, experts), device)
+        lib.check(lib.moe_router_loss(
+            _ptr(logits), _ptr(bias), _ptr(expert_ids), _ptr(mask), _ptr(losses), _ptr(stats), _ptr(scratch),
+            scratch.numel(), tokens, experts, topk, current_stream_handle(device.index)), "router_loss")
+    return RouterLoss(losses, stats)
+
+
+def _check_gradients(logits, expert_ids, loss, grad_losses, grad_weights):
+    if grad_losses is not None:
+        require_tensor(grad_losses, "grad_losses", (2,), torch.float32, logits.device)
+        if not isinstance(loss, RouterLoss):
+            raise TypeError("grad_losses needs the forward's RouterLoss as loss")
+        require_tensor(loss.stats, "loss.stats", (logits.shape[1] + 1,), torch.int32, logits.device)
+    if grad_weights is not None:
+        require_tensor(grad_weights, "grad_weights", tuple(expert_ids.shape), torch.float32, logits.device)
+
+
+def route_logits_backward(logits, expert_ids, bias=None, *, mask=None, loss=None, grad_losses=None, grad_weights=None):
+    """The gradient of the logits, fp32 [T, E].
+
+    ``grad_losses`` fp32 [2]: the gradients of ``loss.balance`` and ``loss.z``, with ``loss``
+    the ``router_loss`` of the same logits, ids, bias and mask. ``grad_weights`` fp32 [T, K]:
+    the routing weights' gradient. Either may be None (0). The routing weights are the
+    softmax of the chosen logits (K = 1: the constant 1, without a gradient); the counts in
+    the balance loss are constants. Masked tokens get 0.
+    """
+    tokens, experts, topk = _check_routed(logits, expert_ids, bias, mask)
+    _check_gradients(logits, expert_ids, loss, grad_losses, grad_weights)
+    require_gpu(logits)
+    refuse_autograd(logits, bias, grad_losses, grad_weights)
+    lib = get_extension().lib
+    device = logits.device
+    with on_device(device):
+        grad_logits = torch.empty_like(logits)
+        lib.check(lib.moe_router_logits_backward(
+            _ptr(logits), _ptr(bias), _ptr(expert_ids), _ptr(mask), _ptr(loss.stats) if loss is not None else None,
+            _ptr(grad_losses), _ptr(grad_weights), _ptr(grad_logits), tokens, experts, topk,
+            current_stream_handle(device.index)), "route_logits_backward")
+    return grad_logits
+
+
+def route_backward(x, router_weight, logits, expert_ids, bias=None, *, mask=None, loss=None, grad_losses=None,
+                   grad_weights=None, grad_x=None):
+    """Gradients of x, router weight and bias: ``(grad_x, grad_router_weight, grad_bias)``.
+
+    x bf16 [T, H] and router_weight fp32 [E, H] are the router's inputs (H a multiple of 8),
+    the rest is ``route_logits_backward``'s. ``grad_x`` bf16 [T, H] is x's gradient along its
+    other paths: the result is the sum, rounded once. grad_router_weight [E, H] and grad_bias
+    [E] are fp32.
+    """
+    tokens, experts, topk = _check_routed(logits, expert_ids, bias, mask)
+    _check_gradients(logits, expert_ids, loss, grad_losses, grad_weights)
+    device = logits.device
+    require_tensor(x, "x", (tokens, None), torch.bfloat16, device)
+    hidden = x.shape[1]
+    if hidden < 8 or hidden % 8 or hidden > 2**20:
+        raise ValueError("hidden must be a multiple of 8 up to 2^20")
+    require_tensor(router_weight, "router_weight", (experts, hidden), torch.float32, device)
+    if grad_x is not None:
+        require_tensor(grad_x, "grad_x", (tokens, hidden), torch.bfloat16, device)
+    require_gpu(x)
+    refuse_autograd(x, router_weight, logits, bias, grad_losses, grad_weights, grad_x)
+    lib = get_extension().lib
+    with on_device(device):
+        if tokens == 0:
+            return torch.empty_like(x), torch.zeros_like(router_weight), torch.zeros(experts, device=device)
+        out_x = torch.empty_like(x)
+        grad_router_weight = torch.empty_like(router_weight)
+        grad_bias = torch.empty(experts, dtype=torch.float32, device=device)
+        need = lib.moe_route_backward_scratch_bytes(tokens, hidden, experts)
+        if need < 0:
+            raise ValueError("route_backward takes up to 2^24 tokens")
+        scratch = scratch_for(need, device)
+        lib.check(lib.moe_route_backward(
+            _ptr(x), _ptr(router_weight), _ptr(logits), _ptr(bias), _ptr(expert_ids), _ptr(mask),
+            _ptr(loss.stats) if loss is not None else None, _ptr(grad_losses), _ptr(grad_weights), _ptr(grad_x),
+            _ptr(out_x), _ptr(grad_router_weight), _ptr(grad_bias), _ptr(scratch), scratch.numel(), tokens, hidden,
+            experts, topk, current_stream_handle(device.index)), "route_backward")
+    return out_x, grad_router_weight, grad_bias
+
+
+def _check_batch(batch):
+    workspace = batch.workspace
+    tokens, hidden, experts, topk = workspace.shape
+    return workspace, tokens, hidden, experts, topk
+
+
+def combine_backward(grad_output, expert_output, batch, weights):
+    """Gradients of ``combine(expert_output, batch, weights)``: ``(grad_expert_output, grad_weights)``.
+
+    ``batch`` is the ``PackedTokens`` of the dispatch, its workspace not dispatched again
+    since. grad_expert_output has the packed rows' shape and dtype; rows that hold no
+    assignment (padding) are zero. grad_weights is fp32 [T, K].
+    """
+    workspace, tokens, hidden, experts, topk = _check_batch(batch)
+    device = workspace.device
+    require_tensor(grad_output, "grad_output", (tokens, hidden), workspace.dtype, device)
+    require_tensor(expert_output, "expert_output", tuple(batch.packed.shape), workspace.dtype, device)
+    require_tensor(weights, "weights", (tokens, topk), torch.float32, device)
+    refuse_autograd(grad_output, expert_output, weights)
+    lib = get_extension().lib
+    with on_device(device):
+        grad_expert = torch.empty_like(expert_output)
+        grad_weights = torch.empty_like(weights)
+        lib.check(lib.moe_combine_backward(
+            _ptr(grad_output), _ptr(expert_output), DTYPE_CODES[workspace.dtype], _ptr(batch.inverse), _ptr(weights),
+            _ptr(batch.counts), _ptr(batch.offsets), _ptr(grad_expert), _ptr(grad_weights), tokens, hidden, experts,
+            topk, expert_output.shape[0], current_stream_handle(device.index)), "combine_backward")
+    return grad_expert, grad_weights
+
+
+def dispatch_backward(grad_packed, batch):
+    """Gradient of ``dispatch(x, ...)``: [T, H], each token's K packed rows' gradients summed
+    in fp32 in k order and rounded once."""
+    workspace, tokens, hidden, _, topk = _check_batch(batch)
+    device = workspace.device
+    require_tensor(grad_packed, "grad_packed", tuple(batch.packed.shape), workspace.dtype, device)
+    refuse_autograd(grad_packed)
+    lib = get_extension().lib
+    with on_device(device):
+        grad_x = torch.empty((tokens, hidden), dtype=workspace.dtype, device=device)
+        lib.check(lib.moe_dispatch_backward(
+            _ptr(grad_packed), DTYPE_CODES[workspace.dtype], _ptr(batch.inverse), _ptr(grad_x), tokens, hidden, topk,
+            grad_packed.shape[0], current_stream_handle(device.index)), "dispatch_backward")
+    return grad_x

@@ -399,6 +399,132 @@ int moe_block_forward(const moe_block_args* args, const void* x, const float* ro
  */
 int moe_set_gemm_workgroups(int64_t workgroups);
 
+/*
+ * ---------------------------------------------------------------------------
+ * Training and adapters. None of what follows has a counterpart in the
+ * reference (it is forward-only and has no adapters).
+ * ---------------------------------------------------------------------------
+ */
+
+/* Bytes of scratch moe_router_loss needs for (T, E); -1 for invalid sizes. */
+int64_t moe_router_loss_scratch_bytes(int64_t tokens, int64_t experts);
+
+/*
+ * The router's auxiliary losses and per-expert counts. v = logits + bias (bias may
+ * be NULL), p = softmax(v), N the tokens whose mask byte is non-zero (mask NULL: all),
+ * c_e the valid tokens' assignments to e:
+ *   losses[0] = E * sum_e (c_e / (N K)) * (sum_t p_te / N)    (balance)
+ *   losses[1] = sum_t (log sum_e exp v_te)^2 / N              (z)
+ *   stats[e] = c_e, stats[E] = N   (int32 [E + 1])
+ * N = 0: both losses are 0. Ids out of range count nowhere. Masked tokens are not read
+ * further. Logits below +inf; a token whose logits are all -inf adds nothing to either
+ * loss; a +inf or NaN logit of a valid token makes the losses NaN or infinite.
+ * Sums are fp32 in a fixed order. Limits: 1 <= E <= 64, 1 <= K <= 8.
+ */
+int moe_router_loss(const float* logits, const float* bias, const int32_t* ids, const uint8_t* mask, float* losses,
+                    int32_t* stats, void* scratch, int64_t scratch_bytes, int64_t tokens, int64_t experts,
+                    int64_t topk, void* stream);
+
+/*
+ * The gradient of the logits, grad_logits [T, E] fp32, from the losses' gradients
+ * (grad_losses, 2 fp32 on the device, with moe_router_loss's stats for the same logits,
+ * ids and mask) and the routing weights' (grad_weights [T, K]); either may be NULL (0).
+ * The routing weights are the softmax of the chosen logits, as the router computes them;
+ * the counts have no gradient. Masked tokens and ids out of range: 0.
+ */
+int moe_router_logits_backward(const float* logits, const float* bias, const int32_t* ids, const uint8_t* mask,
+                               const int32_t* stats, const float* grad_losses, const float* grad_weights,
+                               float* grad_logits, int64_t tokens, int64_t experts, int64_t topk, void* stream);
+
+/* Bytes of scratch moe_route_backward needs for (T, H, E); -1 for invalid sizes. */
+int64_t moe_route_backward_scratch_bytes(int64_t tokens, int64_t hidden, int64_t experts);
+
+/*
+ * moe_router_logits_backward and the router projection's gradients behind it, with
+ * dv the logits' gradient and x bf16 [T, H]:
+ *   grad_x = round_bf16(grad_x_base + dv . router_w)   (grad_x_base bf16 [T, H], NULL: 0;
+ *            it may be grad_x itself)
+ *   grad_router_w = dv^T . x  (fp32 [E, H]),  grad_bias = sum_t dv  (fp32 [E])
+ * Any of the three may be NULL. Products of dv and x are exact and accumulate in fp32;
+ * dv and router_w enter grad_x as two bf16 parts each (16 bits). Requires hidden % 8 == 0
+ * and 16-byte aligned rows.
+ */
+int moe_route_backward(const void* x, const float* router_w, const float* logits, const float* bias,
+                       const int32_t* ids, const uint8_t* mask, const int32_t* stats, const float* grad_losses,
+                       const float* grad_weights, const void* grad_x_base, void* grad_x, float* grad_router_w,
+                       float* grad_bias, void* scratch, int64_t scratch_bytes, int64_t tokens, int64_t hidden,
+                       int64_t experts, int64_t topk, void* stream);
+
+/*
+ * Gradients of moe_combine: for every assignment with a row in range
+ *   grad_expert_output[inverse[t,k]] = round(weights[t,k] * grad_output[t])
+ *   grad_weights[t,k] = sum_j grad_output[t,j] * expert_output[inverse[t,k],j]  (fp32)
+ * and 0 weight gradients for the others. counts and offsets as the dispatch wrote them:
+ * every packed row that holds no assignment (the padding rows and the rows from offsets[E] on)
+ * is set to zero.
+ */
+int moe_combine_backward(const void* grad_output, const void* expert_output, int dtype, const int32_t* inverse,
+                         const float* weights, const int32_t* counts, const int32_t* offsets,
+                         void* grad_expert_output, float* grad_weights, int64_t tokens, int64_t hidden,
+                         int64_t experts, int64_t topk, int64_t packed_rows, void* stream);
+
+/* Gradient of moe_dispatch: grad_x[t] = round(sum_k grad_packed[inverse[t,k]]), the sum in
+ * fp32 in k order (moe_combine with weights of 1). */
+int moe_dispatch_backward(const void* grad_packed, int dtype, const int32_t* inverse, void* grad_x, int64_t tokens,
+                          int64_t hidden, int64_t topk, int64_t packed_rows, void* stream);
+
+/* Bytes of the table moe_adapter_group writes for (T, N); -1 for invalid sizes. */
+int64_t moe_adapter_table_bytes(int64_t tokens, int64_t adapters);
+
+/*
+ * Sorts the rows of a batch by adapter: ids [T] int32, an id outside [0, N) being a row
+ * of no adapter. The table (16-byte aligned, moe_adapter_table_bytes(T, N) bytes) serves
+ * every low-rank call of the same T and N until it is written again; calls that read
+ * it must not overlap with one that writes it. The order is stable, so results do not
+ * vary from call to call. Limits: 1 <= N <= 4096, T <= 2^24.
+ */
+int moe_adapter_group(const int32_t* ids, void* table, int64_t table_bytes, int64_t tokens, int64_t adapters,
+                      void* stream);
+
+/* Bytes of scratch moe_low_rank_add (backward == 0) or moe_low_rank_backward needs; -1 for
+ * invalid sizes. */
+int64_t moe_low_rank_scratch_bytes(int64_t tokens, int64_t hidden, int64_t width, int64_t rank, int64_t adapters,
+                                   int backward);
+
+/*
+ * Low-rank adapters of many requests beside a shared projection, a the row's adapter:
+ *   output[t] = round_bf16(base[t] + scales[a] * up[a]^T . (down[a] . x[t]))
+ *   output[t] = base[t] for a row of no adapter
+ * x [T, hidden], base and output [T, width], down [N, rank, hidden], up [N, rank, width]
+ * (both rank-major: an up matrix stored [width, rank] is transposed once), all bf16;
+ * scales fp32 [N] (NULL: 1). base may be NULL (0) or output itself; output must not
+ * overlap x. down . x is summed in fp32, written to hidden_out (fp32 [T, rank], in the
+ * table's row order, unscaled, 0 for a row of no adapter) unless that is NULL, and enters
+ * the second product as two bf16 parts (16 bits). An adapter of lower rank is padded with zero rows.
+ * Limits: hidden and width multiples of 8 up to 2^20, 1 <= rank <= 128; rows 16-byte aligned.
+ */
+int moe_low_rank_add(const void* x, const void* down, const void* up, const float* scales, const void* table,
+                     int64_t table_bytes, const void* base, void* output, float* hidden_out, void* scratch,
+                     int64_t scratch_bytes, int64_t tokens, int64_t hidden, int64_t width, int64_t rank,
+                     int64_t adapters, void* stream);
+
+/*
+ * Gradients of moe_low_rank_add, g = grad_output [T, width] bf16 (base's own gradient is g):
+ *   dh[t] = scales[a] * up[a] . g[t]
+ *   grad_x[t] = round_bf16(grad_x_base[t] + down[a]^T . dh[t])  (grad_x_base NULL: 0, or grad_x)
+ *   grad_down[a] = sum of dh[t] x[t]^T,  grad_up[a] = scales[a] * sum of h[t] g[t]^T over a's rows
+ * hidden_in is the forward's hidden_out on the same table (needed for grad_up). Any of the
+ * three gradients may be NULL. grad_down and grad_up are [N, rank, hidden] and
+ * [N, rank, width] of grad_dtype (FP32, or BF16 rounded once from the fp32 sums), zero for
+ * an adapter without rows; their products are exact and accumulate in fp32 in row order.
+ * grad_x must not overlap x or grad_output.
+ */
+int moe_low_rank_backward(const void* grad_output, const void* x, const void* down, const void* up,
+                          const float* scales, const void* table, int64_t table_bytes, const float* hidden_in,
+                          const void* grad_x_base, void* grad_x, void* grad_down, void* grad_up, int grad_dtype,
+                          void* scratch, int64_t scratch_bytes, int64_t tokens, int64_t hidden, int64_t width,
+                          int64_t rank, int64_t adapters, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
