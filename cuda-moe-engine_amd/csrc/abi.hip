@@ -44,7 +44,7 @@ int64_t router_loss_scratch_bytes(int64_t, int64_t);
 int launch_router_loss(const float*, const float*, const int32_t*, const uint8_t*, float*, int32_t*, float*, int64_t, int,
                        int, hipStream_t);
 int launch_router_logits_grad(const float*, const float*, const int32_t*, const uint8_t*, const int32_t*, const float*,
-                              const float*, float*, float*, float*, int64_t, int, int, hipStream_t);
+                              const float*, float*, ColumnSums*, int64_t, int, int, hipStream_t);
 int64_t route_backward_scratch_bytes(int64_t, int64_t, int64_t);
 int launch_route_backward(const uint16_t*, const float*, const float*, const float*, const int32_t*, const uint8_t*,
                           const int32_t*, const float*, const float*, const uint16_t*, uint16_t*, float*, float*, char*,
@@ -622,7 +622,7 @@ int moe_router_loss(const float* logits, const float* bias, const int32_t* ids, 
     if (rc != MOE_OK) return rc;
     MOE_REQUIRE(losses && stats, MOE_ERR_INVALID_ARGUMENT, "null pointer");
     const int64_t need = router_loss_scratch_bytes(tokens, experts);
-    MOE_REQUIRE(scratch && scratch_bytes >= need, MOE_ERR_WORKSPACE, "loss scratch needs %lld bytes, got %lld",
+    MOE_REQUIRE((scratch || need == 0) && scratch_bytes >= need, MOE_ERR_WORKSPACE, "loss scratch needs %lld bytes, got %lld",
                 (long long)need, (long long)scratch_bytes);
     MOE_REQUIRE(aligned_to(losses, 4) && aligned_to(stats, 4) && aligned_to(scratch, 4), MOE_ERR_INVALID_ARGUMENT,
                 "pointers must be aligned to their element size");
@@ -647,7 +647,7 @@ int moe_router_logits_backward(const float* logits, const float* bias, const int
     MOE_REQUIRE(grad_logits, MOE_ERR_INVALID_ARGUMENT, "null pointer");
     MOE_REQUIRE(aligned_to(grad_logits, 4), MOE_ERR_INVALID_ARGUMENT, "pointers must be aligned to their element size");
     return launch_router_logits_grad(logits, bias, ids, mask, stats, grad_losses, grad_weights, grad_logits, nullptr,
-                                     nullptr, tokens, (int)experts, (int)topk, static_cast<hipStream_t>(stream));
+                                     tokens, (int)experts, (int)topk, static_cast<hipStream_t>(stream));
 }
 
 int64_t moe_route_backward_scratch_bytes(int64_t tokens, int64_t hidden, int64_t experts) {

@@ -8,10 +8,9 @@ namespace moe {
 
 constexpr int kMaxAdapters = 4096;
 constexpr int kMaxRank = 128;
-constexpr int64_t kMaxAdapterTokens = 1 << 24;
+constexpr int64_t kMaxAdapterTokens = 1 << 21;  // tiles and adapters within a grid's 65535
 constexpr int64_t kMaxLowRankWidth = 1 << 20;
 constexpr int kTileRows = 64;     // rows of one adapter per tile (contract, spread)
-constexpr int kSpreadCols = 512;  // columns per workgroup of spread: 128 per wave
 constexpr int kOuterCols = 128;   // columns per workgroup of outer
 
 // Where the parts of an adapter table lie, in int32 from its start:
@@ -28,10 +27,10 @@ struct TableLayout {
 
 // Rows per split of the outer product: a split's partial result is written and read
 // back once (4 * rank * width bytes twice), so few of them, but enough workgroups
-// (splits * width / 128) to fill the card: about 16 splits of a batch.
+// (splits * width / 128) to fill the card: about 8 splits of a batch.
 inline int outer_split_rows(int64_t tokens) {
     int rows = 128;
-    while (rows < 1024 && rows * 16 < tokens) rows <<= 1;
+    while (rows < 1024 && rows * 8 < tokens) rows <<= 1;
     return rows;
 }
 
@@ -76,12 +75,43 @@ inline Groups groups_of(const void* table, int64_t tokens, int64_t adapters) {
     return g;
 }
 
-inline Groups one_group(int64_t tokens) {
+// The splits of one group may follow the width too: about 512 workgroups.
+inline Groups one_group(int64_t tokens, int64_t width) {
     Groups g;
-    g.split_rows = outer_split_rows(tokens);
+    const int64_t columns = (width + kOuterCols - 1) / kOuterCols;
+    g.split_rows = 128;
+    while (g.split_rows < 1024 && tokens * columns > static_cast<int64_t>(g.split_rows) * 512) g.split_rows <<= 1;
     g.tile_bound = static_cast<int>((tokens + kTileRows - 1) / kTileRows);
     g.split_bound = static_cast<int>((tokens + g.split_rows - 1) / g.split_rows);
     return g;
+}
+
+// out[c] = sum over rows of part[row][c], c < columns <= 64; nothing when rows is 0.
+struct ColumnSums {
+    const float* part = nullptr;
+    float* out = nullptr;
+    int rows = 0, columns = 0;
+};
+
+// By one block of 256 threads: thread (quarter, column) takes every fourth row, sixteen of
+// them in flight, and the quarters are added in order.
+__device__ __forceinline__ void sum_columns(const ColumnSums& c) {
+    constexpr int U = 16;
+    __shared__ float quarter[4][64];
+    const int column = threadIdx.x & 63, q = threadIdx.x >> 6;
+    float f = 0.0f;
+    if (column < c.columns)
+        for (int r0 = q; r0 < c.rows; r0 += 4 * U) {
+            float v[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) v[u] = r0 + 4 * u < c.rows ? c.part[(r0 + 4 * u) * c.columns + column] : 0.0f;
+#pragma unroll
+            for (int u = 0; u < U; ++u) f += v[u];
+        }
+    quarter[q][column] = f;
+    __syncthreads();
+    if (threadIdx.x < static_cast<unsigned>(c.columns))
+        c.out[column] = (quarter[0][column] + quarter[1][column]) + (quarter[2][column] + quarter[3][column]);
 }
 
 // K slices of contract for this shape; partials holds that many [tokens, rank] sums.
@@ -101,7 +131,17 @@ int launch_spread(const float* partials, int slices, const void* w, bool w32, co
 
 // out[a][c][j] = scale_a * sum over a's rows of h[i][c] * x[order[i]][j], fp32 or bf16;
 // 0 for an adapter without rows. partials: split_bound * rank * width fp32.
-int launch_outer(const float* h, const uint16_t* x, const float* scales, const Groups& g, float* partials, void* out,
-                 bool out_bf16, int64_t tokens, int64_t width, int rank, int adapters, hipStream_t stream);
+struct OuterJob {
+    const float* h = nullptr;
+    const uint16_t* x = nullptr;
+    float* partials = nullptr;
+    void* out = nullptr;
+    int64_t width = 0;  // 0: no job
+};
+
+// One or two such products on the same groups. `extra` sums ride on the launch that adds
+// the splits up (one group: only where it has several).
+int launch_outer(const OuterJob& first, const OuterJob& second, const float* scales, const Groups& g, bool out_bf16,
+                 int64_t tokens, int rank, int adapters, hipStream_t stream, ColumnSums extra = {});
 
 }  // namespace moe

@@ -183,114 +183,167 @@ int launch_adapter_group(const int32_t* ids, void* table, int64_t tokens, int ad
 
 // ---------------------------------------------------------------------------
 // contract: h[i][c] = sum_k x[i][k] w[c][k].
-// A workgroup takes a tile of up to 64 rows of one adapter and a slice of k, its four
-// waves a quarter of the slice each. Both operands lie along k as the MFMA reads them
-// (lane l: row l % 16, 8 k from 8 (l / 16)); k is permuted inside 64 so that a lane
-// reads 32 bytes and a step whole 128-byte lines. Rows past the tile and ranks past r
-// are read from the last one and not stored (an output depends on its own row and rank
-// alone). The waves' sums meet in LDS, the slices' in the consumer, in slice order.
+// A workgroup takes a tile of up to 64 rows of one adapter and a slice of k. A wave takes
+// 16 rows and the slice, or for r > 32, where w's lines are the more, 32 rows and half of
+// it; with fewer rows in the tile more waves share them and split the slice. Eight lanes load a 128-byte line of a row, D
+// steps of 64 k ahead, and the wave turns the step over in LDS of its own into the MFMA's
+// operands (lane l: row l % 16, 8 k from 8 (l / 16); k is permuted inside 64). Loaded as
+// operands, neighbouring lanes hold different rows and each 16 bytes is a line of its own
+// to the L1: T=4096, H=4096, r=16 and 64 took 17.2 and 38.6 us, 12.1 and 16.8 now.
+// Rows past the tile and ranks past r are read from the last one and not stored (an output
+// depends on its own row and rank alone). Waves on one row meet in LDS, slices in the
+// consumer, both in order.
 // ---------------------------------------------------------------------------
-template <int MF, int NR>
-struct ContractStep {
-    u32x4_t x[MF][2], w[NR][2];
+// 16 rows of 64 k: lane i loads piece i % 8 (8 k) of rows i / 8 and i / 8 + 8.
+struct LineRows {
+    const uint16_t* row[2];
+};
+struct Lines {
+    u32x4_t v[2];
 };
 
-template <int MF, int NR>
-__device__ __forceinline__ void contract_load(ContractStep<MF, NR>& s, const uint16_t* const (&xr)[MF],
-                                              const uint16_t* const (&wr)[NR], int kk, int k) {
+__device__ __forceinline__ void load_lines(Lines& s, const LineRows& r, int at, int k) {
     const u32x4_t zero = {0, 0, 0, 0};
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int at = kk + 8 * h;
-        if (at < k) {
-#pragma unroll
-            for (int m = 0; m < MF; ++m) s.x[m][h] = load16(xr[m] + at);
-#pragma unroll
-            for (int n = 0; n < NR; ++n) s.w[n][h] = load16(wr[n] + at);
-        } else {
-#pragma unroll
-            for (int m = 0; m < MF; ++m) s.x[m][h] = zero;
-#pragma unroll
-            for (int n = 0; n < NR; ++n) s.w[n][h] = zero;
-        }
-    }
+    for (int h = 0; h < 2; ++h) s.v[h] = at < k ? load16(r.row[h] + at) : zero;
 }
 
-template <int MF, int NR>
-__device__ __forceinline__ void contract_tile(const uint16_t* __restrict__ x, const uint16_t* __restrict__ w,
-                                              const int32_t* order, int first, int rows, float* __restrict__ part,
-                                              int k, int rank, int kb, int ke, float* lds) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int l = lane & 15, g = lane >> 4;
-    const uint16_t* xr[MF];
-    const uint16_t* wr[NR];
-#pragma unroll
-    for (int m = 0; m < MF; ++m)
-        xr[m] = x + static_cast<int64_t>(order[first + min(16 * m + l, rows - 1)]) * k;
-#pragma unroll
-    for (int n = 0; n < NR; ++n) wr[n] = w + static_cast<int64_t>(min(16 * n + l, rank - 1)) * k;
-    f32x4_t acc[MF][NR];
-#pragma unroll
-    for (int m = 0; m < MF; ++m)
-#pragma unroll
-        for (int n = 0; n < NR; ++n) acc[m][n] = f32x4_t{0, 0, 0, 0};
-    if (kb < ke) {
-        ContractStep<MF, NR> cur, next;
-        contract_load<MF, NR>(cur, xr, wr, kb + 16 * g, k);
-        for (int k0 = kb; k0 < ke; k0 += 64) {
-            if (k0 + 64 < ke) contract_load<MF, NR>(next, xr, wr, k0 + 64 + 16 * g, k);
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int m = 0; m < MF; ++m)
-#pragma unroll
-                    for (int n = 0; n < NR; ++n) acc[m][n] = mfma(cur.x[m][h], cur.w[n][h], acc[m][n]);
-            cur = next;
-        }
-    }
-    // One 16-row fragment at a time: [wave][row][rank] in LDS, summed in wave order.
-    constexpr int C = 16 * NR;
-#pragma unroll
-    for (int m = 0; m < MF; ++m) {
-        if (m > 0) __syncthreads();
-#pragma unroll
-        for (int n = 0; n < NR; ++n)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) lds[(wave * 16 + 4 * g + q) * C + 16 * n + l] = acc[m][n][q];
-        __syncthreads();
-        for (int i = threadIdx.x; i < 16 * C; i += 256) {
-            const int row = 16 * m + i / C, c = i % C;
-            if (row < rows && c < rank)
-                part[static_cast<int64_t>(first + row) * rank + c] =
-                    ((lds[i] + lds[i + 16 * C]) + lds[i + 32 * C]) + lds[i + 48 * C];
-        }
-    }
+// A wave's 2 KiB: piece p of row r lies at slot p ^ (r % 8) of its 128 bytes, so that the
+// operands' 16 rows fall on different banks.
+__device__ __forceinline__ void put_lines(uint16_t* lds, const Lines& s, int lane) {
+    const int row = lane / 8, slot = (lane % 8) ^ row;
+    *reinterpret_cast<u32x4_t*>(lds + row * 64 + slot * 8) = s.v[0];
+    *reinterpret_cast<u32x4_t*>(lds + (row + 8) * 64 + slot * 8) = s.v[1];
+}
+__device__ __forceinline__ u32x4_t get_operand(const uint16_t* lds, int l, int g, int h) {
+    return *reinterpret_cast<const u32x4_t*>(lds + l * 64 + (((2 * g + h) ^ (l & 7)) * 8));
 }
 
-template <int NR>
+// Orders a wave's LDS accesses: what its lanes wrote before is there for all of them after.
+// (A wave's LDS operations complete in order; this keeps the compiler from moving them.)
+__device__ __forceinline__ void wave_lds_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// NR: 16-rank fragments. F: 16-row fragments a wave.
+template <int NR, int F>
 __global__ __launch_bounds__(256) void contract_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict__ w,
                                                        Groups gr, float* __restrict__ partials, int64_t tokens, int k,
                                                        int rank, int span) {
-    __shared__ float lds[4 * 16 * 16 * NR];
-    if (static_cast<int>(blockIdx.x) >= gr.head[0]) return;
+    constexpr int D = NR <= 2 ? 6 : NR == 4 ? 3 : 2;  // steps in flight
+    constexpr int C = 16 * NR;
+    constexpr int kWaveHalfs = 1024 * (F + NR);  // x's fragments and w's
+    __shared__ __attribute__((aligned(16))) uint16_t lines[4 * kWaveHalfs];
     const int4 tile = gr.tiles[blockIdx.x];
-    if (tile.x < 0) return;
-    const int kb = blockIdx.y * span + static_cast<int>(threadIdx.x >> 6) * (span / 4);
-    const int ke = min(kb + span / 4, k);
-    const uint16_t* wa = w + static_cast<int64_t>(tile.x) * rank * k;
-    float* part = partials + static_cast<int64_t>(blockIdx.y) * tokens * rank;
-    if (tile.z > 32)
-        contract_tile<4, NR>(x, wa, gr.order, tile.y, tile.z, part, k, rank, kb, ke, lds);
-    else if (tile.z > 16)
-        contract_tile<2, NR>(x, wa, gr.order, tile.y, tile.z, part, k, rank, kb, ke, lds);
-    else
-        contract_tile<1, NR>(x, wa, gr.order, tile.y, tile.z, part, k, rank, kb, ke, lds);
+    if (static_cast<int>(blockIdx.x) >= gr.head[0] || tile.x < 0) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int l = lane & 15, g = lane >> 4;
+    const int first = tile.y, rows = tile.z;
+    // Waves on the same rows, this wave's rows and its part of the slice.
+    const int kw = rows > 32 ? F : rows > 16 ? 2 * F : 4;
+    const int m = wave / kw, kpart = wave % kw;
+    const bool two = F == 2 && rows - 32 * m > 16;
+    const int kb = blockIdx.y * span + kpart * (span / kw);
+    const int ke = 16 * F * m < rows ? min(kb + span / kw, k) : 0;
+    f32x4_t acc[F][NR];
+#pragma unroll
+    for (int f = 0; f < F; ++f)
+#pragma unroll
+        for (int n = 0; n < NR; ++n) acc[f][n] = f32x4_t{0, 0, 0, 0};
+    if (kb < ke) {
+        LineRows xr[F], wr[NR];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int r = lane / 8 + 8 * h;
+#pragma unroll
+            for (int f = 0; f < F; ++f)
+                xr[f].row[h] = x + static_cast<int64_t>(gr.order[first + min(16 * (F * m + f) + r, rows - 1)]) * k;
+#pragma unroll
+            for (int n = 0; n < NR; ++n)
+                wr[n].row[h] = w + (static_cast<int64_t>(tile.x) * rank + min(16 * n + r, rank - 1)) * k;
+        }
+        struct Step {
+            Lines x[F], w[NR];
+        };
+        Step ring[D];
+        const auto fetch = [&](Step& s, int k0) {
+            const int at = k0 + 8 * (lane % 8);
+            load_lines(s.x[0], xr[0], at, k);
+            if (two) load_lines(s.x[F - 1], xr[F - 1], at, k);
+#pragma unroll
+            for (int n = 0; n < NR; ++n) load_lines(s.w[n], wr[n], at, k);
+        };
+        uint16_t* mine = lines + wave * kWaveHalfs;
+#pragma unroll
+        for (int d = 0; d < D; ++d)
+            if (kb + 64 * d < ke) fetch(ring[d], kb + 64 * d);
+        for (int k0 = kb; k0 < ke; k0 += 64 * D)
+#pragma unroll
+            for (int d = 0; d < D; ++d)
+                if (k0 + 64 * d < ke) {
+                    put_lines(mine, ring[d].x[0], lane);
+                    if (two) put_lines(mine + 1024, ring[d].x[F - 1], lane);
+#pragma unroll
+                    for (int n = 0; n < NR; ++n) put_lines(mine + 1024 * (F + n), ring[d].w[n], lane);
+                    wave_lds_order();
+                    const int ahead = k0 + 64 * (d + D);
+                    if (ahead < ke) fetch(ring[d], ahead);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const u32x4_t a = get_operand(mine, l, g, h);
+                        u32x4_t b[NR];
+#pragma unroll
+                        for (int n = 0; n < NR; ++n) {
+                            b[n] = get_operand(mine + 1024 * (F + n), l, g, h);
+                            acc[0][n] = mfma(a, b[n], acc[0][n]);
+                        }
+                        if (two) {
+                            const u32x4_t a1 = get_operand(mine + 1024, l, g, h);
+#pragma unroll
+                            for (int n = 0; n < NR; ++n) acc[F - 1][n] = mfma(a1, b[n], acc[F - 1][n]);
+                        }
+                    }
+                    wave_lds_order();
+                }
+    }
+    // The other waves of the rows pass their sums to the first, a fragment at a time
+    // through the same LDS.
+    float* lds = reinterpret_cast<float*>(lines);
+    float* part = partials + (static_cast<int64_t>(blockIdx.y) * tokens + first + 16 * F * m) * rank;
+#pragma unroll
+    for (int f = 0; f < F; ++f) {
+        if (kw > 1) __syncthreads();
+        if (kpart > 0) {
+            float* dst = lds + (m * (kw - 1) + kpart - 1) * 16 * C;
+#pragma unroll
+            for (int n = 0; n < NR; ++n)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) dst[(4 * g + q) * C + 16 * n + l] = acc[f][n][q];
+        }
+        if (kw > 1) __syncthreads();
+        if (kpart > 0) continue;
+        for (int p = 1; p < kw; ++p) {
+            const float* src = lds + (m * (kw - 1) + p - 1) * 16 * C;
+#pragma unroll
+            for (int n = 0; n < NR; ++n)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) acc[f][n][q] += src[(4 * g + q) * C + 16 * n + l];
+        }
+#pragma unroll
+        for (int n = 0; n < NR; ++n)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int r = 16 * f + 4 * g + q;
+                if (16 * F * m + r < rows && 16 * n + l < rank) part[r * rank + 16 * n + l] = acc[f][n][q];
+            }
+    }
 }
 
 int contract_slices(int tile_bound, int64_t k) {
     const int64_t most = (k + 255) / 256;
     int64_t s = 1;
-    while (s < 16 && s * 2 <= most && s * 2 * tile_bound <= 1024) s <<= 1;
+    while (s < 16 && s * 2 <= most && s * 2 * tile_bound <= 512) s <<= 1;
     return static_cast<int>(s);
 }
 
@@ -302,26 +355,27 @@ int launch_contract(const uint16_t* x, const uint16_t* w, const Groups& g, float
         hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, x, w, g, partials, tokens, static_cast<int>(k), rank, span);
         return check_launch("contract_kernel");
     };
-    if (rank <= 16) return run(contract_kernel<1>);
-    if (rank <= 32) return run(contract_kernel<2>);
-    if (rank <= 64) return run(contract_kernel<4>);
-    return run(contract_kernel<8>);
+    if (rank <= 16) return run(contract_kernel<1, 1>);
+    if (rank <= 32) return run(contract_kernel<2, 1>);
+    if (rank <= 64) return run(contract_kernel<4, 2>);
+    return run(contract_kernel<8, 2>);
 }
 
 // ---------------------------------------------------------------------------
 // spread: out[i][j] = base[i][j] + s sum_c h[i][c] w[c][j].
-// A workgroup takes a tile of up to 64 rows and 512 columns, a wave 128 of them. w lies
-// across the MFMA's k (the ranks), so a lane loads 16 bytes of 8 rank rows and transposes
-// the 8 x 8 block in registers (32 v_perm_b32); MFMA i then covers columns n0 + 8 l + i,
+// A workgroup takes a tile of up to 64 rows and 512 columns (256), a wave 128 of them. w
+// lies across the MFMA's k (the ranks), so a lane loads 8 (4) columns of 8 rank rows and
+// transposes the block in registers (v_perm_b32); MFMA i then covers columns n0 + 8 l + i,
 // and a lane ends with 8 neighbouring columns of a row: base and out move 16 bytes a lane.
 // h enters as two bf16 parts (rest below 2^-16 of it, under the result's own rounding to
 // bf16): for r <= 16 side by side in one MFMA's 32 k, else as two MFMAs on one w.
 // ---------------------------------------------------------------------------
-// The 8 x 8 block of 16-bit values v[j] (row j, two columns a dword) as B operands:
+// The 8 x N block of 16-bit values v[j] (row j, two columns a dword) as B operands:
 // column i of all rows.
-__device__ __forceinline__ void transpose8(const u32x4_t (&v)[8], u32x4_t (&b)[8]) {
+template <int N, typename V>
+__device__ __forceinline__ void transpose8(const V (&v)[8], u32x4_t (&b)[N]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < N; ++i)
 #pragma unroll
         for (int p = 0; p < 4; ++p)
             b[i][p] = __builtin_amdgcn_perm(v[2 * p + 1][i / 2], v[2 * p][i / 2], (i & 1) ? 0x07060302u : 0x05040100u);
@@ -329,139 +383,199 @@ __device__ __forceinline__ void transpose8(const u32x4_t (&v)[8], u32x4_t (&b)[8
 
 // NK: 32-rank chunks. HALF (r <= 16): one chunk whose k 0-15 are h's first parts and
 // 16-31 the rests, w's rows twice. W32: w is fp32, taken as two bf16 parts as well
-// (the product of the two rests, below 2^-32 of the term, is left out).
-template <int NK, bool HALF, bool W32>
+// (the product of the two rests, below 2^-32 of the term, is left out). A workgroup takes
+// `fragments` 16-row fragments of a tile, blockIdx.z the first: 4, or 1 where whole tiles
+// would leave CUs idle. base's rows are on their way one fragment ahead.
+// COLS: columns a lane, 8, or 4 where w's operands for 8 would leave a SIMD one wave
+// (r > 32, fp32 w).
+template <int NK, bool HALF, bool W32, int COLS>
 __global__ __launch_bounds__(256) void spread_kernel(const float* __restrict__ partials, int slices, const void* wv,
                                                      const float* __restrict__ scales, Groups gr, const uint16_t* base,
                                                      uint16_t* out, float* __restrict__ h_out, int64_t tokens,
-                                                     int64_t width, int rank) {
+                                                     int64_t width, int rank, int fragments) {
     constexpr int KP = 32 * NK + 8;  // 16-byte rows, off the banks' period
+    constexpr int C = HALF ? 16 : 32 * NK;
     __shared__ __attribute__((aligned(16))) uint16_t hi[kTileRows * KP];
     __shared__ __attribute__((aligned(16))) uint16_t lo[HALF ? 8 : kTileRows * KP];
-    __shared__ int32_t row_of[kTileRows];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int l = lane & 15, g = lane >> 4;
     int adapter = 0, first = blockIdx.x * kTileRows, rows;
     if (gr.order) {
-        if (static_cast<int>(blockIdx.x) >= gr.head[0]) return;
         const int4 tile = gr.tiles[blockIdx.x];
+        if (static_cast<int>(blockIdx.x) >= gr.head[0]) return;
         adapter = tile.x;
         first = tile.y;
         rows = tile.z;
     } else {
         rows = static_cast<int>(min(static_cast<int64_t>(kTileRows), tokens - first));
     }
-    if (tid < rows) row_of[tid] = gr.order ? gr.order[first + tid] : first + tid;
-    const int64_t col = static_cast<int64_t>(blockIdx.y) * kSpreadCols + wave * 128 + 8 * l;
+    first += 16 * fragments * blockIdx.z;
+    rows = min(rows - static_cast<int>(16 * fragments * blockIdx.z), 16 * fragments);
+    if (rows <= 0) return;
+    const int64_t col = static_cast<int64_t>(blockIdx.y) * (64 * COLS) + (wave * 16 + l) * COLS;
     const bool inside = col < width;
-    const u32x4_t zero = {0, 0, 0, 0};
+    typedef uint32_t cols_t __attribute__((ext_vector_type(COLS / 2)));  // 16-bit columns
+    typedef float wide_t __attribute__((ext_vector_type(COLS)));
+    const cols_t zero = {};
+    // This lane's rows of a fragment, 16 m + 4 g + q, and what base has there.
+    int64_t at[4];
+    cols_t old[4];
+    const auto fetch = [&](int m) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int r = first + min(16 * m + 4 * g + q, rows - 1);
+            at[q] = (gr.order ? gr.order[r] : r) * width + col;
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) old[q] = base && inside ? *reinterpret_cast<const cols_t*>(base + at[q]) : zero;
+    };
+    if (out) fetch(0);
     if (adapter < 0) {  // no adapter: h is 0, the base as it is
         if (h_out && blockIdx.y == 0)
             for (int i = tid; i < rows * rank; i += 256) h_out[static_cast<int64_t>(first) * rank + i] = 0.0f;
-        if (base == out || !out) return;
-        __syncthreads();
-        if (inside)
-            for (int r = g; r < rows; r += 4) {
-                const int64_t at = row_of[r] * width + col;
-                *reinterpret_cast<u32x4_t*>(out + at) = base ? load16(base + at) : zero;
-            }
+        if (base == out || !out || !inside) return;
+        for (int m = 0; 16 * m < rows; ++m) {
+            if (m > 0) fetch(m);
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (16 * m + 4 * g + q < rows) *reinterpret_cast<cols_t*>(out + at[q]) = old[q];
+        }
         return;
     }
-    // h: the slices' sums as bf16 parts; zero past the rank and past the rows.
-    for (int i = tid; i < kTileRows * (HALF ? 16 : 32 * NK); i += 256) {
-        const int row = i / (HALF ? 16 : 32 * NK), c = i % (HALF ? 16 : 32 * NK);
-        float h = 0.0f;
-        if (row < rows && c < rank) {
-            const int64_t at = static_cast<int64_t>(first + row) * rank + c;
-            for (int s = 0; s < slices; ++s) h += partials[static_cast<int64_t>(s) * tokens * rank + at];
-            if (h_out && blockIdx.y == 0) h_out[at] = h;
+    u32x4_t b[NK][COLS], b2[W32 ? NK : 1][COLS];
+    cols_t raw[W32 ? 1 : NK][8];
+    wide_t raw32[W32 ? NK : 1][8];
+    const int64_t skip = static_cast<int64_t>(adapter) * rank * width;
+    const uint16_t* wa = static_cast<const uint16_t*>(wv) + skip;
+    const float* wf = static_cast<const float*>(wv) + skip;
+#pragma unroll
+    for (int n = 0; n < NK; ++n)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int c = HALF ? (8 * g + j) & 15 : 32 * n + 8 * g + j;
+            // A scalar base and a 32-bit offset (rank * width is below 2^28).
+            const uint32_t from = static_cast<uint32_t>(c) * static_cast<uint32_t>(width) + static_cast<uint32_t>(col);
+            const bool held = inside && c < rank;
+            if constexpr (W32) {
+                raw32[n][j] = held ? *reinterpret_cast<const wide_t*>(wf + from) : wide_t{};
+            } else {
+                raw[n][j] = held ? *reinterpret_cast<const cols_t*>(wa + from) : zero;
+            }
         }
-        const uint16_t a = f32_to_bf16(h);
-        const uint16_t b = f32_to_bf16(bf16_rest(h, a));
-        hi[row * KP + c] = a;
-        if (HALF)
-            hi[row * KP + 16 + c] = b;
-        else
-            lo[row * KP + c] = b;
+    // h: the slices' sums as bf16 parts; zero past the rank and past the rows, up to a
+    // whole fragment. A thread takes four ranks of a row, up to eight slices in flight.
+    constexpr int Q = C / 4;
+    const int filled = (rows + 15) / 16 * 16 * Q;
+    const int64_t slice = tokens * rank;
+    const auto stage = [&](auto count) {
+        constexpr int S = decltype(count)::value;
+        using V = Unaligned<float, 4>;
+#pragma unroll 1
+        for (int i = tid; i < filled; i += 256) {
+            const int row = i / Q, c = i % Q * 4;
+            const uint32_t from = static_cast<uint32_t>(first + row) * rank + c;  // below 2^28
+            float h[4] = {0, 0, 0, 0};
+#pragma unroll 1
+            for (int s0 = 0; s0 < slices; s0 += S) {
+                V part[S];
+#pragma unroll
+                for (int s = 0; s < S; ++s) {
+                    part[s] = V{{0, 0, 0, 0}};
+                    if (row < rows) {
+                        const float* src = partials + (s0 + s) * slice + from;
+                        if (c + 4 <= rank) {
+                            part[s] = *reinterpret_cast<const V*>(src);
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 3; ++j)
+                                if (c + j < rank) part[s].v[j] = src[j];
+                        }
+                    }
+                }
+#pragma unroll
+                for (int s = 0; s < S; ++s)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) h[j] += part[s].v[j];
+            }
+            uint16_t a[4], rest[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (h_out && blockIdx.y == 0 && row < rows && c + j < rank) h_out[from + j] = h[j];
+                a[j] = f32_to_bf16(h[j]);
+                rest[j] = f32_to_bf16(bf16_rest(h[j], a[j]));
+            }
+            const auto two = [](uint16_t x, uint16_t y) { return x | static_cast<uint32_t>(y) << 16; };
+            uint16_t* other = HALF ? hi + row * KP + 16 + c : lo + row * KP + c;
+            *reinterpret_cast<uint2*>(hi + row * KP + c) = make_uint2(two(a[0], a[1]), two(a[2], a[3]));
+            *reinterpret_cast<uint2*>(other) = make_uint2(two(rest[0], rest[1]), two(rest[2], rest[3]));
+        }
+    };
+    if constexpr (W32)  // the router's gradient is one
+        stage(std::integral_constant<int, 1>{});
+    else switch (slices) {
+        case 1: stage(std::integral_constant<int, 1>{}); break;
+        case 2: stage(std::integral_constant<int, 2>{}); break;
+        case 4: stage(std::integral_constant<int, 4>{}); break;
+        default: stage(std::integral_constant<int, 8>{}); break;
     }
-    // w's operands.
-    u32x4_t b[NK][8], b2[W32 ? NK : 1][8];
+    if (!out) return;
 #pragma unroll
     for (int n = 0; n < NK; ++n) {
-        if (W32) {
-            const float* w = static_cast<const float*>(wv);
-            f32x4_t v[8][2];
+        if constexpr (W32) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int c = HALF ? (8 * g + j) & 15 : 32 * n + 8 * g + j;
-                v[j][0] = v[j][1] = f32x4_t{0, 0, 0, 0};
-                if (inside && c < rank) {
-                    const float* src = w + static_cast<int64_t>(c) * width + col;
-                    v[j][0] = *reinterpret_cast<const f32x4_t*>(src);
-                    v[j][1] = *reinterpret_cast<const f32x4_t*>(src + 4);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
+            for (int i = 0; i < COLS; ++i)
 #pragma unroll
                 for (int p = 0; p < 4; ++p) {
-                    const float f0 = v[2 * p][i / 4][i % 4], f1 = v[2 * p + 1][i / 4][i % 4];
+                    const float f0 = raw32[n][2 * p][i], f1 = raw32[n][2 * p + 1][i];
                     b[n][i][p] = pack_bf16x2(f0, f1);
                     b2[n][i][p] = pack_bf16x2(bf16_rest(f0, b[n][i][p]), bf16_rest(f1, b[n][i][p] >> 16));
                 }
         } else {
-            const uint16_t* w = static_cast<const uint16_t*>(wv) + static_cast<int64_t>(adapter) * rank * width;
-            u32x4_t v[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int c = HALF ? (8 * g + j) & 15 : 32 * n + 8 * g + j;
-                v[j] = inside && c < rank ? load16(w + static_cast<int64_t>(c) * width + col) : zero;
-            }
-            transpose8(v, b[n]);
+            transpose8(raw[n], b[n]);
         }
     }
-    if (!out) return;
     const float scale = scales ? scales[adapter] : 1.0f;
     __syncthreads();
 #pragma unroll 1
-    for (int m = 0; m < (rows + 15) / 16; ++m) {
-        u32x4_t old[4];
+    for (int m = 0; 16 * m < rows; ++m) {
+        int64_t now[4];
+        cols_t there[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            const int r = 16 * m + 4 * g + q;
-            old[q] = base && inside && r < rows ? load16(base + row_of[r] * width + col) : zero;
+            now[q] = at[q];
+            there[q] = old[q];
         }
-        f32x4_t acc[8];
+        if (16 * (m + 1) < rows) fetch(m + 1);
+        f32x4_t acc[COLS];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) acc[i] = f32x4_t{0, 0, 0, 0};
+        for (int i = 0; i < COLS; ++i) acc[i] = f32x4_t{0, 0, 0, 0};
 #pragma unroll
         for (int n = 0; n < NK; ++n) {
-            const int at = (16 * m + l) * KP + 32 * n + 8 * g;
-            const u32x4_t a = *reinterpret_cast<const u32x4_t*>(hi + at);
+            const int from = (16 * m + l) * KP + 32 * n + 8 * g;
+            const u32x4_t a = *reinterpret_cast<const u32x4_t*>(hi + from);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) acc[i] = mfma(a, b[n][i], acc[i]);
+            for (int i = 0; i < COLS; ++i) acc[i] = mfma(a, b[n][i], acc[i]);
             if (!HALF) {
-                const u32x4_t a2 = *reinterpret_cast<const u32x4_t*>(lo + at);
+                const u32x4_t a2 = *reinterpret_cast<const u32x4_t*>(lo + from);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) acc[i] = mfma(a2, b[n][i], acc[i]);
+                for (int i = 0; i < COLS; ++i) acc[i] = mfma(a2, b[n][i], acc[i]);
             }
             if (W32) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) acc[i] = mfma(a, b2[n][i], acc[i]);
+                for (int i = 0; i < COLS; ++i) acc[i] = mfma(a, b2[n][i], acc[i]);
             }
         }
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            const int r = 16 * m + 4 * g + q;
-            if (!inside || r >= rows) continue;
-            u32x4_t o;
+            if (!inside || 16 * m + 4 * g + q >= rows) continue;
+            cols_t o;
 #pragma unroll
-            for (int d = 0; d < 4; ++d) {
-                const float b0 = bf16_to_f32(static_cast<uint16_t>(old[q][d]));
-                const float b1 = bf16_to_f32(static_cast<uint16_t>(old[q][d] >> 16));
+            for (int d = 0; d < COLS / 2; ++d) {
+                const float b0 = bf16_to_f32(static_cast<uint16_t>(there[q][d]));
+                const float b1 = bf16_to_f32(static_cast<uint16_t>(there[q][d] >> 16));
                 o[d] = pack_bf16x2(b0 + scale * acc[2 * d][q], b1 + scale * acc[2 * d + 1][q]);
             }
-            *reinterpret_cast<u32x4_t*>(out + row_of[r] * width + col) = o;
+            *reinterpret_cast<cols_t*>(out + now[q]) = o;
         }
     }
 }
@@ -469,22 +583,23 @@ __global__ __launch_bounds__(256) void spread_kernel(const float* __restrict__ p
 int launch_spread(const float* partials, int slices, const void* w, bool w32, const float* scales, const Groups& g,
                   const uint16_t* base, uint16_t* out, float* h_out, int64_t tokens, int64_t width, int rank,
                   hipStream_t stream) {
-    const unsigned columns = static_cast<unsigned>((width + kSpreadCols - 1) / kSpreadCols);
-    const dim3 grid(g.tile_bound, out ? columns : 1);  // without out: h_out alone
-    const auto run = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, partials, slices, w, scales, g, base, out, h_out, tokens,
-                           width, rank);
+    const auto run = [&](auto kernel, int cols) {
+        // Without out: h_out alone.
+        const unsigned columns = out ? static_cast<unsigned>((width + 64 * cols - 1) / (64 * cols)) : 1;
+        const int fragments = static_cast<int64_t>(g.tile_bound) * columns > 256 ? 4 : 1;
+        hipLaunchKernelGGL(kernel, dim3(g.tile_bound, columns, 4 / fragments), dim3(256), 0, stream, partials, slices, w,
+                           scales, g, base, out, h_out, tokens, width, rank, fragments);
         return check_launch("spread_kernel");
     };
     if (w32) {  // the router: at most 64 experts
-        if (rank <= 16) return run(spread_kernel<1, true, true>);
-        if (rank <= 32) return run(spread_kernel<1, false, true>);
-        return run(spread_kernel<2, false, true>);
+        if (rank <= 16) return run(spread_kernel<1, true, true, 8>, 8);
+        if (rank <= 32) return run(spread_kernel<1, false, true, 8>, 8);
+        return run(spread_kernel<2, false, true, 4>, 4);
     }
-    if (rank <= 16) return run(spread_kernel<1, true, false>);
-    if (rank <= 32) return run(spread_kernel<1, false, false>);
-    if (rank <= 64) return run(spread_kernel<2, false, false>);
-    return run(spread_kernel<4, false, false>);
+    if (rank <= 16) return run(spread_kernel<1, true, false, 8>, 8);
+    if (rank <= 32) return run(spread_kernel<1, false, false, 8>, 8);
+    if (rank <= 64) return run(spread_kernel<2, false, false, 4>, 4);
+    return run(spread_kernel<4, false, false, 4>, 4);
 }
 
 // ---------------------------------------------------------------------------
@@ -496,31 +611,37 @@ int launch_spread(const float* partials, int slices, const void* w, bool w32, co
 // an adapter of one split is done, of more its partial sums are added in split order.
 // ---------------------------------------------------------------------------
 template <bool BF16>
-__device__ __forceinline__ void store8(void* out, int64_t at, const float (&v)[8]) {
-    if (BF16) {
-        u32x4_t o;
-#pragma unroll
-        for (int d = 0; d < 4; ++d) o[d] = pack_bf16x2(v[2 * d], v[2 * d + 1]);
-        *reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(out) + at) = o;
-    } else {
-        float* p = static_cast<float*>(out) + at;
-        *reinterpret_cast<f32x4_t*>(p) = f32x4_t{v[0], v[1], v[2], v[3]};
-        *reinterpret_cast<f32x4_t*>(p + 4) = f32x4_t{v[4], v[5], v[6], v[7]};
-    }
+__device__ __forceinline__ void store4(void* out, int64_t at, f32x4_t v) {
+    if (BF16)
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + at) =
+            make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+    else
+        *reinterpret_cast<f32x4_t*>(static_cast<float*>(out) + at) = v;
 }
 
-template <int NR, bool BF16>
-__global__ __launch_bounds__(256) void outer_kernel(const float* __restrict__ h, const uint16_t* __restrict__ x,
-                                                    const float* __restrict__ scales, Groups gr,
-                                                    float* __restrict__ partials, void* __restrict__ out,
-                                                    int64_t tokens, int64_t width, int rank) {
-    __shared__ __attribute__((aligned(16))) float lds[4 * 16 * 128];
+// A wave holds NR 16-rank fragments; RG of the W waves share the ranks (r <= 16 NR RG)
+// and W / RG the rows. Rows of the step after are in flight while one is computed.
+// A launch does up to two products on the same groups (an adapter's two gradients).
+struct OuterJobs {
+    OuterJob job[2];
+    int columns[2];  // column parts of each; the grid has both
+};
+
+template <int NR, int RG, int W, bool BF16>
+__global__ __launch_bounds__(64 * W) void outer_kernel(OuterJobs jobs, const float* __restrict__ scales, Groups gr,
+                                                              int64_t tokens, int rank) {
+    constexpr int TG = W / RG;
+    __shared__ __attribute__((aligned(16))) float lds[W * 16 * 128];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int l = lane & 15, g = lane >> 4;
+    const bool second = static_cast<int>(blockIdx.y) >= jobs.columns[0];
+    const OuterJob job = jobs.job[second];
+    const int part_column = blockIdx.y - (second ? jobs.columns[0] : 0);
+    const int64_t width = job.width;
     int adapter = 0, first = blockIdx.x * gr.split_rows, rows, parts = gr.split_bound;
     if (gr.order) {
-        if (static_cast<int>(blockIdx.x) >= gr.head[1]) return;
         const int4 split = gr.splits[blockIdx.x];
+        if (static_cast<int>(blockIdx.x) >= gr.head[1]) return;
         adapter = split.x;
         first = split.y;
         rows = split.z;
@@ -528,40 +649,49 @@ __global__ __launch_bounds__(256) void outer_kernel(const float* __restrict__ h,
     } else {
         rows = static_cast<int>(min(static_cast<int64_t>(gr.split_rows), tokens - first));
     }
-    const int64_t col = static_cast<int64_t>(blockIdx.y) * kOuterCols + 8 * l;
+    const int64_t col = static_cast<int64_t>(part_column) * kOuterCols + 8 * l;
     const bool inside = col < width;
-    const int c0 = blockIdx.z * 16 * NR;
+    const int c0 = wave % RG * 16 * NR;
     const u32x4_t zero = {0, 0, 0, 0};
     f32x4_t acc[NR][8];
 #pragma unroll
     for (int n = 0; n < NR; ++n)
 #pragma unroll
         for (int i = 0; i < 8; ++i) acc[n][i] = f32x4_t{0, 0, 0, 0};
-    for (int t0 = 32 * wave; t0 < rows; t0 += 128) {
+    struct Step {
         u32x4_t v[8];
-        float hv[NR][8];
+        float h[NR][8];
+    };
+    const auto fetch = [&](Step& s, int t0) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const int i = t0 + 8 * g + j;
-            v[j] = zero;
+            s.v[j] = zero;
             if (i < rows && inside) {
                 const int64_t row = gr.order ? gr.order[first + i] : first + i;
-                v[j] = load16(x + row * width + col);
+                s.v[j] = load16(job.x + row * width + col);
             }
 #pragma unroll
             for (int n = 0; n < NR; ++n) {
                 const int c = c0 + 16 * n + l;
-                hv[n][j] = i < rows && c < rank ? h[static_cast<int64_t>(first + i) * rank + c] : 0.0f;
+                s.h[n][j] = i < rows && c < rank ? job.h[static_cast<int64_t>(first + i) * rank + c] : 0.0f;
             }
         }
+    };
+    Step next;
+    int t0 = 32 * (wave / RG);
+    if (t0 < rows) fetch(next, t0);
+    for (; t0 < rows; t0 += 32 * TG) {
+        const Step cur = next;
+        if (t0 + 32 * TG < rows) fetch(next, t0 + 32 * TG);
         u32x4_t b[8];
-        transpose8(v, b);
+        transpose8(cur.v, b);
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
             u32x4_t a0, a1, a2;
 #pragma unroll
             for (int p = 0; p < 4; ++p) {
-                float f0 = hv[n][2 * p], f1 = hv[n][2 * p + 1];
+                float f0 = cur.h[n][2 * p], f1 = cur.h[n][2 * p + 1];
                 a0[p] = pack_bf16x2(f0, f1);
                 f0 = bf16_rest(f0, a0[p]);
                 f1 = bf16_rest(f1, a0[p] >> 16);
@@ -577,6 +707,8 @@ __global__ __launch_bounds__(256) void outer_kernel(const float* __restrict__ h,
         }
     }
     const float scale = scales ? scales[adapter] : 1.0f;
+    // One fragment of every wave at a time: [wave][rank][column] in LDS, the row groups
+    // summed in order; a thread takes four columns.
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
         if (n > 0) __syncthreads();
@@ -587,68 +719,86 @@ __global__ __launch_bounds__(256) void outer_kernel(const float* __restrict__ h,
             *reinterpret_cast<f32x4_t*>(dst + 4) = f32x4_t{acc[n][4][q], acc[n][5][q], acc[n][6][q], acc[n][7][q]};
         }
         __syncthreads();
-        const int c = c0 + 16 * n + tid / 16;
-        const int64_t j = static_cast<int64_t>(blockIdx.y) * kOuterCols + 8 * (tid & 15);
-        if (c < rank && j < width) {
-            float v[8];
-            const float* src = lds + (tid / 16) * 128 + 8 * (tid & 15);
+        const int64_t j = static_cast<int64_t>(part_column) * kOuterCols + 4 * (tid & 31);
+        // 2 W rows of 128 columns a turn.
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                v[i] = scale * (((src[i] + src[i + 2048]) + src[i + 4096]) + src[i + 6144]);
+        for (int r0 = 0; r0 < 16 * RG; r0 += 2 * W) {
+            const int r = r0 + tid / 32, rg = r / 16;
+            const int c = (rg * NR + n) * 16 + r % 16;
+            if (r >= 16 * RG || c >= rank || j >= width) continue;
+            const float* src = lds + r * 128 + 4 * (tid & 31);
+            f32x4_t sum = *reinterpret_cast<const f32x4_t*>(src);
+#pragma unroll
+            for (int t = 1; t < TG; ++t) sum += *reinterpret_cast<const f32x4_t*>(src + t * RG * 2048);
+            sum *= scale;
             if (parts == 1)
-                store8<BF16>(out, (static_cast<int64_t>(adapter) * rank + c) * width + j, v);
+                store4<BF16>(job.out, (static_cast<int64_t>(adapter) * rank + c) * width + j, sum);
             else
-                store8<false>(partials, (static_cast<int64_t>(blockIdx.x) * rank + c) * width + j, v);
+                store4<false>(job.partials, (static_cast<int64_t>(blockIdx.x) * rank + c) * width + j, sum);
         }
     }
 }
 
 // An adapter's partial sums in split order, or zeros for one without rows.
 template <bool BF16>
-__global__ __launch_bounds__(256) void outer_sum_kernel(const float* __restrict__ partials, Groups gr,
-                                                        void* __restrict__ out, int64_t elements) {
+__global__ __launch_bounds__(256) void outer_sum_kernel(OuterJobs jobs, Groups gr, int rank, ColumnSums extra) {
     const int a = blockIdx.y;
+    const int64_t blocks0 = (jobs.job[0].width * rank + 1023) / 1024;
+    const int64_t blocks1 = (jobs.job[1].width * rank + 1023) / 1024;
+    if (static_cast<int64_t>(blockIdx.x) >= blocks0 + blocks1) {
+        sum_columns(extra);
+        return;
+    }
+    const bool second = static_cast<int64_t>(blockIdx.x) >= blocks0;
+    const OuterJob job = jobs.job[second];
+    const int64_t elements = job.width * rank;
     const int s0 = gr.order ? gr.split_start[a] : 0;
     const int s1 = gr.order ? gr.split_start[a + 1] : gr.split_bound;
     if (s1 - s0 == 1) return;
-    const int64_t at = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 8;
+    const int64_t at = ((static_cast<int64_t>(blockIdx.x) - (second ? blocks0 : 0)) * 256 + threadIdx.x) * 4;
     if (at >= elements) return;
-    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    for (int s = s0; s < s1; ++s) {
-        const float* p = partials + static_cast<int64_t>(s) * elements + at;
-        const f32x4_t lo = *reinterpret_cast<const f32x4_t*>(p), hi = *reinterpret_cast<const f32x4_t*>(p + 4);
+    f32x4_t sum = {0, 0, 0, 0};
+    constexpr int U = 8;  // splits in flight
+    for (int s = s0; s < s1; s += U) {
+        f32x4_t v[U];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[i] += lo[i];
-            v[4 + i] += hi[i];
-        }
+        for (int u = 0; u < U; ++u)
+            v[u] = *reinterpret_cast<const f32x4_t*>(job.partials + static_cast<int64_t>(min(s + u, s1 - 1)) * elements + at);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (s + u < s1) sum += v[u];
     }
-    store8<BF16>(out, a * elements + at, v);
+    store4<BF16>(job.out, a * elements + at, sum);
 }
 
-int launch_outer(const float* h, const uint16_t* x, const float* scales, const Groups& g, float* partials, void* out,
-                 bool out_bf16, int64_t tokens, int64_t width, int rank, int adapters, hipStream_t stream) {
-    const int nr = rank <= 16 ? 1 : rank <= 32 ? 2 : 4;
-    const dim3 grid(g.split_bound, static_cast<unsigned>((width + kOuterCols - 1) / kOuterCols),
-                    (rank + 16 * nr - 1) / (16 * nr));
-    const auto run = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, h, x, scales, g, partials, out, tokens, width, rank);
+int launch_outer(const OuterJob& first, const OuterJob& second, const float* scales, const Groups& g, bool out_bf16,
+                 int64_t tokens, int rank, int adapters, hipStream_t stream, ColumnSums extra) {
+    OuterJobs jobs;
+    jobs.job[0] = first;
+    jobs.job[1] = second;
+    for (int i = 0; i < 2; ++i) jobs.columns[i] = static_cast<int>((jobs.job[i].width + kOuterCols - 1) / kOuterCols);
+    const dim3 grid(g.split_bound, jobs.columns[0] + jobs.columns[1]);
+    const auto run = [&](auto kernel, int waves) {
+        hipLaunchKernelGGL(kernel, grid, dim3(64 * waves), 0, stream, jobs, scales, g, tokens, rank);
         return check_launch("outer_kernel");
     };
+    const auto by_rank = [&](auto bf16) {
+        constexpr bool B = decltype(bf16)::value;
+        if (rank <= 16) return run(outer_kernel<1, 1, 4, B>, 4);
+        if (rank <= 32) return run(outer_kernel<2, 1, 4, B>, 4);
+        if (rank <= 64) return run(outer_kernel<2, 2, 8, B>, 8);
+        return run(outer_kernel<2, 4, 8, B>, 8);
+    };
     int rc = MOE_OK;
-    if (g.split_bound == 0)
-        rc = MOE_OK;  // no rows: zeros, below
-    else if (out_bf16)
-        rc = nr == 1 ? run(outer_kernel<1, true>) : nr == 2 ? run(outer_kernel<2, true>) : run(outer_kernel<4, true>);
-    else
-        rc = nr == 1 ? run(outer_kernel<1, false>) : nr == 2 ? run(outer_kernel<2, false>) : run(outer_kernel<4, false>);
+    if (g.split_bound > 0) rc = out_bf16 ? by_rank(std::true_type{}) : by_rank(std::false_type{});
     if (rc != MOE_OK || (!g.order && g.split_bound == 1)) return rc;
-    const int64_t elements = rank * width;
-    const dim3 sum_grid(static_cast<unsigned>((elements + 2047) / 2048), adapters);
+    // One more block for the extra sums (of the router, whose rows are one group).
+    const int64_t blocks = (first.width * rank + 1023) / 1024 + (second.width * rank + 1023) / 1024 + (extra.rows > 0);
+    const dim3 sum_grid(static_cast<unsigned>(blocks), adapters);
     if (out_bf16)
-        hipLaunchKernelGGL(outer_sum_kernel<true>, sum_grid, dim3(256), 0, stream, partials, g, out, elements);
+        hipLaunchKernelGGL(outer_sum_kernel<true>, sum_grid, dim3(256), 0, stream, jobs, g, rank, extra);
     else
-        hipLaunchKernelGGL(outer_sum_kernel<false>, sum_grid, dim3(256), 0, stream, partials, g, out, elements);
+        hipLaunchKernelGGL(outer_sum_kernel<false>, sum_grid, dim3(256), 0, stream, jobs, g, rank, extra);
     return check_launch("outer_sum_kernel");
 }
 
@@ -657,14 +807,14 @@ int launch_outer(const float* h, const uint16_t* x, const float* scales, const G
 // ---------------------------------------------------------------------------
 static int64_t up16(int64_t bytes) { return (bytes + 15) / 16 * 16; }
 
-// Forward: contract's partial sums. Backward: those of dh, dh itself, outer's partial sums.
+// Forward: contract's partial sums. Backward: those of dh, dh itself, the two products' partial sums.
 int64_t low_rank_scratch_bytes(int64_t tokens, int64_t hidden, int64_t width, int64_t rank, int64_t adapters,
                                bool backward) {
     const TableLayout t = table_layout(tokens, adapters);
     const int64_t row = tokens * rank * 4;
     if (!backward) return contract_slices(t.tile_bound, hidden) * row;
     return up16(contract_slices(t.tile_bound, width) * row) + up16(row) +
-           static_cast<int64_t>(t.split_bound) * rank * std::max(hidden, width) * 4;
+           static_cast<int64_t>(t.split_bound) * rank * (hidden + width) * 4;
 }
 
 int launch_low_rank_add(const uint16_t* x, const uint16_t* down, const uint16_t* up, const float* scales,
@@ -697,11 +847,13 @@ int launch_low_rank_backward(const uint16_t* grad_output, const uint16_t* x, con
             rc = launch_spread(dh_parts, slices, down, false, scales, g, grad_x_base, grad_x, dh, tokens, hidden, rank,
                                stream);
     }
-    if (rc == MOE_OK && grad_down)
-        rc = launch_outer(dh, x, scales, g, partials, grad_down, grad_bf16, tokens, hidden, rank, adapters, stream);
-    if (rc == MOE_OK && grad_up)
-        rc = launch_outer(hidden_in, grad_output, scales, g, partials, grad_up, grad_bf16, tokens, width, rank, adapters,
-                          stream);
+    if (rc == MOE_OK && (grad_down || grad_up)) {
+        OuterJob jobs[2];
+        if (grad_down) jobs[0] = {dh, x, partials, grad_down, hidden};
+        if (grad_up)
+            jobs[1] = {hidden_in, grad_output, partials + g.split_bound * rank * hidden, grad_up, width};
+        rc = launch_outer(jobs[0], jobs[1], scales, g, grad_bf16, tokens, rank, adapters, stream);
+    }
     return rc;
 }
 

@@ -18,16 +18,16 @@ expert, or expert and adapter, as its id. No counterpart in the reference.
 Checks, streams and errors are those of ``moe_dispatch.training``.
 """
 
-from dataclasses import dataclass
+from typing import NamedTuple
 
 import torch
 
 from ._extension import DTYPE_CODES, current_stream_handle, get_extension
-from .training import _ptr, on_device, refuse_autograd, require_tensor, scratch_for
+from .training import _ptr, on_device, refuse_autograd, require_tensor, scratch_bytes, shape_of
 
 MAX_ADAPTERS = 4096
 MAX_RANK = 128
-MAX_ROWS = 2**24
+MAX_ROWS = 2**21
 MAX_WIDTH = 2**20
 
 
@@ -41,7 +41,7 @@ class AdapterGroups:
 
     def __init__(self, tokens, adapters, *, device="cuda", extension=None):
         if not isinstance(tokens, int) or not 0 <= tokens <= MAX_ROWS:
-            raise ValueError("tokens must be an integer in 0..2^24")
+            raise ValueError("tokens must be an integer in 0..2^21")
         if not isinstance(adapters, int) or not 1 <= adapters <= MAX_ADAPTERS:
             raise ValueError("adapters must be an integer in 1..4096")
         device = torch.device(device)
@@ -54,12 +54,13 @@ class AdapterGroups:
         self.assignment = 0  # how many times assign ran: what a kept hidden belongs to
         nbytes = self.extension.lib.moe_adapter_table_bytes(tokens, adapters)
         self.table = torch.empty(nbytes // 4, dtype=torch.int32, device=device)
+        self.table_bytes = nbytes
 
     def assign(self, ids):
         require_tensor(ids, "ids", (self.tokens,), torch.int32, self.device)
         lib = self.extension.lib
         with on_device(self.device):
-            lib.check(lib.moe_adapter_group(ids.data_ptr(), self.table.data_ptr(), self.table.numel() * 4, self.tokens,
+            lib.check(lib.moe_adapter_group(ids.data_ptr(), self.table.data_ptr(), self.table_bytes, self.tokens,
                                             self.adapters, current_stream_handle(self.device.index)), "assign")
         self.assignment += 1
 
@@ -70,8 +71,7 @@ class AdapterGroups:
         return self.table[4:4 + self.tokens]
 
 
-@dataclass(frozen=True)
-class LowRankHidden:
+class LowRankHidden(NamedTuple):
     """``down[a] x`` of one ``low_rank_add``, fp32 [T, r] in the groups' row order, for its
     ``low_rank_backward`` on the same assignment."""
 
@@ -92,12 +92,12 @@ def _check_operands(x, down, up, groups, scales):
         raise RuntimeError("AdapterGroups.assign has not grouped any rows yet")
     device = groups.device
     tokens, adapters = groups.tokens, groups.adapters
-    require_tensor(x, "x", (tokens, None), torch.bfloat16, device)
-    hidden = x.shape[1]
-    require_tensor(down, "down", (adapters, None, hidden), torch.bfloat16, device)
-    rank = down.shape[1]
-    require_tensor(up, "up", (adapters, rank, None), torch.bfloat16, device)
-    width = up.shape[2]
+    hidden = shape_of(x, "x", 2)[1]
+    require_tensor(x, "x", (tokens, hidden), torch.bfloat16, device)
+    rank = shape_of(down, "down", 3)[1]
+    require_tensor(down, "down", (adapters, rank, hidden), torch.bfloat16, device)
+    width = shape_of(up, "up", 3)[2]
+    require_tensor(up, "up", (adapters, rank, width), torch.bfloat16, device)
     _check_width(hidden, "hidden")
     _check_width(width, "width")
     if not 1 <= rank <= MAX_RANK:
@@ -132,13 +132,14 @@ def low_rank_add(base, x, down, up, groups, *, scales=None, output=None, return_
     lib = groups.extension.lib
     with on_device(device):
         if output is None:
-            output = torch.empty((tokens, width), dtype=torch.bfloat16, device=device)
-        kept = torch.empty((tokens, rank), dtype=torch.float32, device=device) if return_hidden else None
-        scratch = scratch_for(lib.moe_low_rank_scratch_bytes(tokens, hidden, width, rank, adapters, 0), device)
+            output = x.new_empty((tokens, width))
+        kept = x.new_empty((tokens, rank), dtype=torch.float32) if return_hidden else None
+        need = scratch_bytes("moe_low_rank_scratch_bytes", tokens, hidden, width, rank, adapters, 0)
+        scratch = x.new_empty(need // 2)
         lib.check(lib.moe_low_rank_add(
             x.data_ptr(), down.data_ptr(), up.data_ptr(), _ptr(scales), groups.table.data_ptr(),
-            groups.table.numel() * 4, _ptr(base), output.data_ptr(), _ptr(kept), scratch.data_ptr(), scratch.numel(),
-            tokens, hidden, width, rank, adapters, current_stream_handle(device.index)), "low_rank_add")
+            groups.table_bytes, _ptr(base), output.data_ptr(), _ptr(kept), scratch.data_ptr(), need, tokens,
+            hidden, width, rank, adapters, current_stream_handle(device.index)), "low_rank_add")
     return (output, LowRankHidden(kept, groups, groups.assignment)) if return_hidden else output
 
 
@@ -167,13 +168,14 @@ def low_rank_backward(grad_output, x, down, up, groups, *, scales=None, hidden, 
     lib = groups.extension.lib
     with on_device(device):
         out_x = torch.empty_like(x)
-        grad_down = torch.empty(down.shape, dtype=grad_dtype, device=device)
-        grad_up = torch.empty(up.shape, dtype=grad_dtype, device=device)
-        scratch = scratch_for(lib.moe_low_rank_scratch_bytes(tokens, h, width, rank, adapters, 1), device)
+        grad_down = torch.empty_like(down, dtype=grad_dtype)
+        grad_up = torch.empty_like(up, dtype=grad_dtype)
+        need = scratch_bytes("moe_low_rank_scratch_bytes", tokens, h, width, rank, adapters, 1)
+        scratch = x.new_empty(need // 2)
         lib.check(lib.moe_low_rank_backward(
             grad_output.data_ptr(), x.data_ptr(), down.data_ptr(), up.data_ptr(), _ptr(scales),
-            groups.table.data_ptr(), groups.table.numel() * 4, hidden.values.data_ptr(), _ptr(grad_x),
+            groups.table.data_ptr(), groups.table_bytes, hidden.values.data_ptr(), _ptr(grad_x),
             out_x.data_ptr(), grad_down.data_ptr(), grad_up.data_ptr(), DTYPE_CODES[grad_dtype], scratch.data_ptr(),
-            scratch.numel(), tokens, h, width, rank, adapters, current_stream_handle(device.index)),
+            need, tokens, h, width, rank, adapters, current_stream_handle(device.index)),
             "low_rank_backward")
     return out_x, grad_down, grad_up

@@ -20,37 +20,54 @@ one order: results do not vary from call to call.
 """
 
 from contextlib import nullcontext
-from dataclasses import dataclass
+from functools import lru_cache
+from typing import NamedTuple
 
 import torch
 
 from ._extension import DTYPE_CODES, current_stream_handle, get_extension
 from .workspace import MAX_EXPERTS, MAX_TOPK
 
+_CURRENT = nullcontext()
+
 
 def on_device(device):
     """Makes ``device`` current where it is not: streams and launches go by the current device."""
-    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _CURRENT if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
-def require_tensor(t, name, shape, dtype, device=None):
-    """The checks every operand shares; ``dtype`` may be a tuple of the dtypes allowed."""
+def require_tensor(t, name, shape, dtype, device):
+    """The checks every operand shares. A call on small tensors is host work first: the
+    passing case is a few comparisons, and only a failing one finds out what to say."""
+    if (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.device == device
+            and t.is_contiguous()):
+        return
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor")
-    if t.dtype != dtype and not (isinstance(dtype, tuple) and t.dtype in dtype):
+    if t.dtype is not dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.dim() != len(shape) or any(want is not None and have != want for have, want in zip(t.shape, shape)):
-        raise ValueError(f"{name}: expected shape {['any' if n is None else n for n in shape]}, got {list(t.shape)}")
-    if device is not None and t.device != device:
+    if t.shape != shape:
+        raise ValueError(f"{name}: expected shape {list(shape)}, got {list(t.shape)}")
+    if t.device != device:
         raise ValueError(f"{name} must be on {device}")
-    if not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous")
+    raise ValueError(f"{name} must be contiguous")
+
+
+def shape_of(t, name, dims):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor")
+    shape = t.shape
+    if len(shape) != dims:
+        raise ValueError(f"{name}: expected {dims} dimensions, got shape {list(shape)}")
+    return shape
 
 
 def refuse_autograd(*tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError("this operator records no autograd graph: detach its inputs, call it under no_grad, "
-                         "or use moe_dispatch.autograd")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError("this operator records no autograd graph: detach its inputs, call it under no_grad, "
+                                 "or use moe_dispatch.autograd")
 
 
 def require_gpu(t):
@@ -62,12 +79,13 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def scratch_for(nbytes, device):
-    return torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
+@lru_cache(maxsize=1024)
+def scratch_bytes(name, *sizes):
+    """What one of the library's ``*_scratch_bytes`` functions says (-1 for sizes it refuses)."""
+    return getattr(get_extension().lib, name)(*sizes)
 
 
-@dataclass(frozen=True)
-class RouterLoss:
+class RouterLoss(NamedTuple):
     """``losses`` fp32 [2] (balance, z) and ``stats`` int32 [E + 1] (per-expert counts of the
     valid tokens' assignments, then the number of valid tokens)."""
 
@@ -88,20 +106,22 @@ class RouterLoss:
 
 
 def _check_routed(logits, expert_ids, bias, mask):
-    require_tensor(logits, "logits", (None, None), torch.float32)
-    tokens, experts = logits.shape
+    tokens, experts = shape_of(logits, "logits", 2)
+    device = logits.device
+    require_tensor(logits, "logits", (tokens, experts), torch.float32, device)
     if not 1 <= experts <= MAX_EXPERTS:
         raise ValueError("logits must have 1..64 experts")
-    require_tensor(expert_ids, "expert_ids", (tokens, None), torch.int32, logits.device)
-    if not 1 <= expert_ids.shape[1] <= MAX_TOPK:
+    topk = shape_of(expert_ids, "expert_ids", 2)[1]
+    require_tensor(expert_ids, "expert_ids", (tokens, topk), torch.int32, device)
+    if not 1 <= topk <= MAX_TOPK:
         raise ValueError("topk must be in 1..8")
-    if tokens * max(experts, expert_ids.shape[1]) > 2**31 - 1:
+    if tokens * max(experts, topk) > 2**31 - 1:
         raise ValueError("tokens*experts and tokens*topk must fit int32")
     if bias is not None:
-        require_tensor(bias, "bias", (experts,), torch.float32, logits.device)
+        require_tensor(bias, "bias", (experts,), torch.float32, device)
     if mask is not None:
-        require_tensor(mask, "mask", (tokens,), torch.bool, logits.device)
-    return tokens, experts, expert_ids.shape[1]
+        require_tensor(mask, "mask", (tokens,), torch.bool, device)
+    return tokens, experts, topk, device
 
 
 def router_loss(logits, expert_ids, bias=None, *, mask=None):
@@ -118,19 +138,18 @@ def router_loss(logits, expert_ids, bias=None, *, mask=None):
     token of none but -inf adds nothing to the losses); +inf or NaN ones of a valid token
     show in the losses.
     """
-    tokens, experts, topk = _check_routed(logits, expert_ids, bias, mask)
+    tokens, experts, topk, device = _check_routed(logits, expert_ids, bias, mask)
     require_gpu(logits)
     refuse_autograd(logits, bias)
     lib = get_extension().lib
-    device = logits.device
     with on_device(device):
-        # Losses and stats are parts of one buffer, one allocation.
-        buffer = torch.empty(experts + 3, dtype=torch.float32, device=device)
-        losses, stats = buffer[:2], buffer[2:].view(torch.int32)
-        scratch = scratch_for(lib.moe_router_loss_scratch_bytes(tokens, experts), device)
+        losses = logits.new_empty(2)
+        stats = expert_ids.new_empty(experts + 1)
+        need = scratch_bytes("moe_router_loss_scratch_bytes", tokens, experts)
+        scratch = logits.new_empty(need // 4) if need else None
         lib.check(lib.moe_router_loss(
-            _ptr(logits), _ptr(bias), _ptr(expert_ids), _ptr(mask), _ptr(losses), _ptr(stats), _ptr(scratch),
-            scratch.numel(), tokens, experts, topk, current_stream_handle(device.index)), "router_loss")
+            logits.data_ptr(), _ptr(bias), expert_ids.data_ptr(), _ptr(mask), losses.data_ptr(), stats.data_ptr(),
+            _ptr(scratch), need, tokens, experts, topk, current_stream_handle(device.index)), "router_loss")
     return RouterLoss(losses, stats)
 
 
@@ -141,7 +160,7 @@ def _check_gradients(logits, expert_ids, loss, grad_losses, grad_weights):
             raise TypeError("grad_losses needs the forward's RouterLoss as loss")
         require_tensor(loss.stats, "loss.stats", (logits.shape[1] + 1,), torch.int32, logits.device)
     if grad_weights is not None:
-        require_tensor(grad_weights, "grad_weights", tuple(expert_ids.shape), torch.float32, logits.device)
+        require_tensor(grad_weights, "grad_weights", expert_ids.shape, torch.float32, logits.device)
 
 
 def route_logits_backward(logits, expert_ids, bias=None, *, mask=None, loss=None, grad_losses=None, grad_weights=None):
@@ -153,17 +172,17 @@ def route_logits_backward(logits, expert_ids, bias=None, *, mask=None, loss=None
     softmax of the chosen logits (K = 1: the constant 1, without a gradient); the counts in
     the balance loss are constants. Masked tokens get 0.
     """
-    tokens, experts, topk = _check_routed(logits, expert_ids, bias, mask)
+    tokens, experts, topk, device = _check_routed(logits, expert_ids, bias, mask)
     _check_gradients(logits, expert_ids, loss, grad_losses, grad_weights)
     require_gpu(logits)
     refuse_autograd(logits, bias, grad_losses, grad_weights)
     lib = get_extension().lib
-    device = logits.device
     with on_device(device):
         grad_logits = torch.empty_like(logits)
         lib.check(lib.moe_router_logits_backward(
-            _ptr(logits), _ptr(bias), _ptr(expert_ids), _ptr(mask), _ptr(loss.stats) if loss is not None else None,
-            _ptr(grad_losses), _ptr(grad_weights), _ptr(grad_logits), tokens, experts, topk,
+            logits.data_ptr(), _ptr(bias), expert_ids.data_ptr(), _ptr(mask),
+            loss.stats.data_ptr() if loss is not None else None, _ptr(grad_losses), _ptr(grad_weights),
+            grad_logits.data_ptr(), tokens, experts, topk,
             current_stream_handle(device.index)), "route_logits_backward")
     return grad_logits
 
@@ -177,11 +196,10 @@ def route_backward(x, router_weight, logits, expert_ids, bias=None, *, mask=None
     other paths: the result is the sum, rounded once. grad_router_weight [E, H] and grad_bias
     [E] are fp32.
     """
-    tokens, experts, topk = _check_routed(logits, expert_ids, bias, mask)
+    tokens, experts, topk, device = _check_routed(logits, expert_ids, bias, mask)
     _check_gradients(logits, expert_ids, loss, grad_losses, grad_weights)
-    device = logits.device
-    require_tensor(x, "x", (tokens, None), torch.bfloat16, device)
-    hidden = x.shape[1]
+    hidden = shape_of(x, "x", 2)[1]
+    require_tensor(x, "x", (tokens, hidden), torch.bfloat16, device)
     if hidden < 8 or hidden % 8 or hidden > 2**20:
         raise ValueError("hidden must be a multiple of 8 up to 2^20")
     require_tensor(router_weight, "router_weight", (experts, hidden), torch.float32, device)
@@ -195,23 +213,17 @@ def route_backward(x, router_weight, logits, expert_ids, bias=None, *, mask=None
             return torch.empty_like(x), torch.zeros_like(router_weight), torch.zeros(experts, device=device)
         out_x = torch.empty_like(x)
         grad_router_weight = torch.empty_like(router_weight)
-        grad_bias = torch.empty(experts, dtype=torch.float32, device=device)
-        need = lib.moe_route_backward_scratch_bytes(tokens, hidden, experts)
+        grad_bias = logits.new_empty(experts)
+        need = scratch_bytes("moe_route_backward_scratch_bytes", tokens, hidden, experts)
         if need < 0:
-            raise ValueError("route_backward takes up to 2^24 tokens")
-        scratch = scratch_for(need, device)
+            raise ValueError("route_backward takes up to 2^21 tokens")
+        scratch = logits.new_empty(need // 4)
         lib.check(lib.moe_route_backward(
-            _ptr(x), _ptr(router_weight), _ptr(logits), _ptr(bias), _ptr(expert_ids), _ptr(mask),
-            _ptr(loss.stats) if loss is not None else None, _ptr(grad_losses), _ptr(grad_weights), _ptr(grad_x),
-            _ptr(out_x), _ptr(grad_router_weight), _ptr(grad_bias), _ptr(scratch), scratch.numel(), tokens, hidden,
-            experts, topk, current_stream_handle(device.index)), "route_backward")
+            x.data_ptr(), router_weight.data_ptr(), logits.data_ptr(), _ptr(bias), expert_ids.data_ptr(), _ptr(mask),
+            loss.stats.data_ptr() if loss is not None else None, _ptr(grad_losses), _ptr(grad_weights), _ptr(grad_x),
+            out_x.data_ptr(), grad_router_weight.data_ptr(), grad_bias.data_ptr(), scratch.data_ptr(), need, tokens,
+            hidden, experts, topk, current_stream_handle(device.index)), "route_backward")
     return out_x, grad_router_weight, grad_bias
-
-
-def _check_batch(batch):
-    workspace = batch.workspace
-    tokens, hidden, experts, topk = workspace.shape
-    return workspace, tokens, hidden, experts, topk
 
 
 def combine_backward(grad_output, expert_output, batch, weights):
@@ -221,10 +233,12 @@ def combine_backward(grad_output, expert_output, batch, weights):
     since. grad_expert_output has the packed rows' shape and dtype; rows that hold no
     assignment (padding) are zero. grad_weights is fp32 [T, K].
     """
-    workspace, tokens, hidden, experts, topk = _check_batch(batch)
-    device = workspace.device
-    require_tensor(grad_output, "grad_output", (tokens, hidden), workspace.dtype, device)
-    require_tensor(expert_output, "expert_output", tuple(batch.packed.shape), workspace.dtype, device)
+    workspace = batch.workspace
+    tokens, hidden, experts, topk = workspace.shape
+    dtype, device = workspace.dtype, workspace.device
+    packed = batch.packed.shape
+    require_tensor(grad_output, "grad_output", (tokens, hidden), dtype, device)
+    require_tensor(expert_output, "expert_output", packed, dtype, device)
     require_tensor(weights, "weights", (tokens, topk), torch.float32, device)
     refuse_autograd(grad_output, expert_output, weights)
     lib = get_extension().lib
@@ -232,23 +246,26 @@ def combine_backward(grad_output, expert_output, batch, weights):
         grad_expert = torch.empty_like(expert_output)
         grad_weights = torch.empty_like(weights)
         lib.check(lib.moe_combine_backward(
-            _ptr(grad_output), _ptr(expert_output), DTYPE_CODES[workspace.dtype], _ptr(batch.inverse), _ptr(weights),
-            _ptr(batch.counts), _ptr(batch.offsets), _ptr(grad_expert), _ptr(grad_weights), tokens, hidden, experts,
-            topk, expert_output.shape[0], current_stream_handle(device.index)), "combine_backward")
+            grad_output.data_ptr(), expert_output.data_ptr(), DTYPE_CODES[dtype], batch.inverse.data_ptr(),
+            weights.data_ptr(), batch.counts.data_ptr(), batch.offsets.data_ptr(), grad_expert.data_ptr(),
+            grad_weights.data_ptr(), tokens, hidden, experts, topk, packed[0], current_stream_handle(device.index)),
+            "combine_backward")
     return grad_expert, grad_weights
 
 
 def dispatch_backward(grad_packed, batch):
     """Gradient of ``dispatch(x, ...)``: [T, H], each token's K packed rows' gradients summed
     in fp32 in k order and rounded once."""
-    workspace, tokens, hidden, _, topk = _check_batch(batch)
-    device = workspace.device
-    require_tensor(grad_packed, "grad_packed", tuple(batch.packed.shape), workspace.dtype, device)
+    workspace = batch.workspace
+    tokens, hidden, _, topk = workspace.shape
+    dtype, device = workspace.dtype, workspace.device
+    packed = batch.packed.shape
+    require_tensor(grad_packed, "grad_packed", packed, dtype, device)
     refuse_autograd(grad_packed)
     lib = get_extension().lib
     with on_device(device):
-        grad_x = torch.empty((tokens, hidden), dtype=workspace.dtype, device=device)
+        grad_x = grad_packed.new_empty((tokens, hidden))
         lib.check(lib.moe_dispatch_backward(
-            _ptr(grad_packed), DTYPE_CODES[workspace.dtype], _ptr(batch.inverse), _ptr(grad_x), tokens, hidden, topk,
-            grad_packed.shape[0], current_stream_handle(device.index)), "dispatch_backward")
+            grad_packed.data_ptr(), DTYPE_CODES[dtype], batch.inverse.data_ptr(), grad_x.data_ptr(), tokens, hidden,
+            topk, packed[0], current_stream_handle(device.index)), "dispatch_backward")
     return grad_x

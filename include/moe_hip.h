@@ -406,7 +406,7 @@ int moe_set_gemm_workgroups(int64_t workgroups);
  * ---------------------------------------------------------------------------
  */
 
-/* Bytes of scratch moe_router_loss needs for (T, E); -1 for invalid sizes. */
+/* Bytes of scratch moe_router_loss needs for (T, E) (0: none); -1 for invalid sizes. */
 int64_t moe_router_loss_scratch_bytes(int64_t tokens, int64_t experts);
 
 /*
@@ -481,7 +481,7 @@ int64_t moe_adapter_table_bytes(int64_t tokens, int64_t adapters);
  * of no adapter. The table (16-byte aligned, moe_adapter_table_bytes(T, N) bytes) serves
  * every low-rank call of the same T and N until it is written again; calls that read
  * it must not overlap with one that writes it. The order is stable, so results do not
- * vary from call to call. Limits: 1 <= N <= 4096, T <= 2^24.
+ * vary from call to call. Limits: 1 <= N <= 4096, T <= 2^21.
  */
 int moe_adapter_group(const int32_t* ids, void* table, int64_t table_bytes, int64_t tokens, int64_t adapters,
                       void* stream);

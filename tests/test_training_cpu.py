@@ -101,7 +101,7 @@ def test_transport_gradients_refuse_bad_tensors():
 def _groups(tokens=4, adapters=3, assigned=True):
     groups = object.__new__(AdapterGroups)
     groups.tokens, groups.adapters, groups.device = tokens, adapters, torch.device("cpu")
-    groups.assignment = int(assigned)
+    groups.assignment, groups.table_bytes = int(assigned), 0
     return groups
 
 
@@ -113,7 +113,7 @@ def _operands(tokens=4, hidden=64, width=32, rank=8, adapters=3):
 
 
 def test_groups_refuse_bad_sizes():
-    for tokens, adapters in ((-1, 2), (2**24 + 1, 2), (4.0, 2), (4, 0), (4, 4097)):
+    for tokens, adapters in ((-1, 2), (2**21 + 1, 2), (4.0, 2), (4, 0), (4, 4097)):
         with pytest.raises(ValueError):
             AdapterGroups(tokens, adapters)
     with pytest.raises(RuntimeError):
@@ -193,7 +193,10 @@ def test_c_entries_check_their_arguments_without_launching():
     assert lib.moe_router_loss(A, A, A, None, A, A, A, big, 4, 8, 9, None) == 2
     assert lib.moe_router_loss(None, A, A, None, A, A, A, big, 4, 8, 2, None) == 1
     assert lib.moe_router_loss(A, A, A, None, None, A, A, big, 4, 8, 2, None) == 1
-    assert lib.moe_router_loss(A, A, A, None, A, A, A, 0, 4, 8, 2, None) == 4
+    assert lib.moe_router_loss_scratch_bytes(128, 8) == 0  # one block
+    need = lib.moe_router_loss_scratch_bytes(8192, 64)
+    assert lib.moe_router_loss(A, A, A, None, A, A, A, need - 1, 8192, 64, 2, None) == 4
+    assert lib.moe_router_loss(A, A, A, None, A, A, None, need, 8192, 64, 2, None) == 4
     assert lib.moe_router_loss(A, A, A, None, A, A, A, big, 1 << 29, 8, 2, None) == 3
     # logits, bias, ids, mask, stats, grad_losses, grad_weights, grad_logits, T, E, K
     assert lib.moe_router_logits_backward(A, A, A, None, None, A, A, A, 4, 8, 2, None) == 1
