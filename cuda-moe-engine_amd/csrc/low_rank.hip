@@ -603,6 +603,225 @@ int launch_spread(const float* partials, int slices, const void* w, bool w32, co
 }
 
 // ---------------------------------------------------------------------------
+// contract and spread in one launch, for small batches: decoding steps are launch and
+// latency. A workgroup takes 16 rows of a tile and up to 1024 columns a turn; its eight
+// waves split all of k, add up in LDS, and each spread 128 columns. Every column part
+// computes h again, from w in the L2, so that nothing is handed over between workgroups.
+// The sums' order is k's over eight waves: results differ from the two launches' in fp32
+// rounding.
+// ---------------------------------------------------------------------------
+constexpr int kFusedWaves = 8;
+constexpr int kFusedCols = kFusedWaves * 128;
+
+template <int NR>
+__global__ __launch_bounds__(64 * kFusedWaves) void fused_kernel(
+    const uint16_t* __restrict__ x, const uint16_t* __restrict__ down, const uint16_t* __restrict__ up,
+    const float* __restrict__ scales, Groups gr, const uint16_t* base, uint16_t* out, float* __restrict__ h_out, int k,
+    int64_t width, int rank, int turns) {
+    constexpr bool HALF = NR == 1;
+    constexpr int NK = 1, C = 16 * NR, KP = 32 * NK + 8;
+    constexpr int D = 4;
+    constexpr int kStepHalfs = 1024 * (1 + NR), kWaveHalfs = 2 * kStepHalfs;  // two steps' lines a wave
+    __shared__ __attribute__((aligned(16))) uint16_t lines[kFusedWaves * kWaveHalfs];
+    __shared__ __attribute__((aligned(16))) uint16_t hi[16 * KP];
+    __shared__ __attribute__((aligned(16))) uint16_t lo[HALF ? 8 : 16 * KP];
+    const int4 tile = gr.tiles[blockIdx.x / 4];
+    if (static_cast<int>(blockIdx.x / 4) >= gr.head[0]) return;
+    const int skip = 16 * (blockIdx.x % 4);
+    const int adapter = tile.x, first = tile.y + skip, rows = min(tile.z - skip, 16);
+    if (rows <= 0) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int l = lane & 15, g = lane >> 4;
+    int64_t row_at[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) row_at[q] = gr.order[first + min(4 * g + q, rows - 1)] * width;
+    int64_t col = static_cast<int64_t>(blockIdx.y) * turns * kFusedCols + wave * 128 + 8 * l;
+    const u32x4_t zero = {0, 0, 0, 0};
+    if (adapter < 0) {  // no adapter: h is 0, the base as it is
+        if (h_out && blockIdx.y == 0)
+            for (int i = tid; i < rows * rank; i += 64 * kFusedWaves) h_out[static_cast<int64_t>(first) * rank + i] = 0.0f;
+        if (base == out) return;
+        for (int turn = 0; turn < turns && col < width; ++turn, col += kFusedCols)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (4 * g + q < rows)
+                    *reinterpret_cast<u32x4_t*>(out + row_at[q] + col) = base ? load16(base + row_at[q] + col) : zero;
+        return;
+    }
+    // The first turn's rows of up and base are on their way while h is made.
+    const uint16_t* wa = up + static_cast<int64_t>(adapter) * rank * width;
+    u32x4_t raw[NK][8], old[4];
+    const auto fetch = [&] {
+        const bool inside = col < width;
+#pragma unroll
+        for (int n = 0; n < NK; ++n)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int c = HALF ? (8 * g + j) & 15 : 32 * n + 8 * g + j;
+                const uint32_t from = static_cast<uint32_t>(c) * static_cast<uint32_t>(width) + static_cast<uint32_t>(col);
+                raw[n][j] = inside && c < rank ? load16(wa + from) : zero;
+            }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) old[q] = base && inside ? load16(base + row_at[q] + col) : zero;
+    };
+    fetch();
+    f32x4_t acc[NR];
+#pragma unroll
+    for (int n = 0; n < NR; ++n) acc[n] = f32x4_t{0, 0, 0, 0};
+    uint16_t* mine = lines + wave * kWaveHalfs;
+    {
+        // A wave's share of k: whole steps of 64.
+        const int steps = (k + 63) / 64, share = (steps + kFusedWaves - 1) / kFusedWaves * 64;
+        const int kb = wave * share, ke = min(kb + share, k);
+        LineRows xr, wr[NR];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int r = lane / 8 + 8 * h;
+            xr.row[h] = x + static_cast<int64_t>(gr.order[first + min(r, rows - 1)]) * k;
+#pragma unroll
+            for (int n = 0; n < NR; ++n)
+                wr[n].row[h] = down + (static_cast<int64_t>(adapter) * rank + min(16 * n + r, rank - 1)) * k;
+        }
+        struct Step {
+            Lines x, w[NR];
+        };
+        Step ring[D];
+        const auto load = [&](Step& s, int k0) {
+            const int at = k0 + 8 * (lane % 8);
+            load_lines(s.x, xr, at, k);
+#pragma unroll
+            for (int n = 0; n < NR; ++n) load_lines(s.w[n], wr[n], at, k);
+        };
+#pragma unroll
+        for (int d = 0; d < D; ++d)
+            if (kb + 64 * d < ke) load(ring[d], kb + 64 * d);
+        const auto put = [&](const Step& s, int parity) {
+            uint16_t* to = mine + parity * kStepHalfs;
+            put_lines(to, s.x, lane);
+#pragma unroll
+            for (int n = 0; n < NR; ++n) put_lines(to + 1024 * (1 + n), s.w[n], lane);
+        };
+        // A step's lines are in LDS before the one before it is read.
+        if (kb < ke) put(ring[0], 0);
+        for (int k0 = kb; k0 < ke; k0 += 64 * D)
+#pragma unroll
+            for (int d = 0; d < D; ++d)
+                if (k0 + 64 * d < ke) {
+                    const int ahead = k0 + 64 * (d + D);
+                    if (ahead < ke) load(ring[d], ahead);
+                    wave_lds_order();
+                    if (k0 + 64 * (d + 1) < ke) put(ring[(d + 1) % D], (d + 1) % 2);
+                    const uint16_t* from = mine + d % 2 * kStepHalfs;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const u32x4_t a = get_operand(from, l, g, h);
+#pragma unroll
+                        for (int n = 0; n < NR; ++n) acc[n] = mfma(a, get_operand(from + 1024 * (1 + n), l, g, h), acc[n]);
+                    }
+                    wave_lds_order();
+                }
+    }
+    // The waves' sums, each in its own lines, added in wave order.
+    float* sums = reinterpret_cast<float*>(mine);
+#pragma unroll
+    for (int n = 0; n < NR; ++n)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) sums[(4 * g + q) * C + 16 * n + l] = acc[n][q];
+    __syncthreads();
+    for (int i = tid; i < 16 * (HALF ? 16 : 32 * NK); i += 64 * kFusedWaves) {
+        const int row = i / C, c = i % C;
+        float h = 0.0f;
+        if (row < rows && c < rank) {
+#pragma unroll
+            for (int p = 0; p < kFusedWaves; ++p) h += reinterpret_cast<const float*>(lines + p * kWaveHalfs)[i];
+            if (h_out && blockIdx.y == 0) h_out[static_cast<int64_t>(first + row) * rank + c] = h;
+        }
+        const uint16_t a = f32_to_bf16(h), rest = f32_to_bf16(bf16_rest(h, a));
+        hi[row * KP + c] = a;
+        if (HALF)
+            hi[row * KP + 16 + c] = rest;
+        else
+            lo[row * KP + c] = rest;
+    }
+    __syncthreads();
+    const float scale = scales ? scales[adapter] : 1.0f;
+    for (int turn = 0; turn < turns; ++turn) {
+        u32x4_t b[NK][8], there[4];
+#pragma unroll
+        for (int n = 0; n < NK; ++n) transpose8(raw[n], b[n]);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) there[q] = old[q];
+        const int64_t now = col;
+        col += kFusedCols;
+        if (turn + 1 < turns) fetch();
+        f32x4_t sum[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum[i] = f32x4_t{0, 0, 0, 0};
+#pragma unroll
+        for (int n = 0; n < NK; ++n) {
+            const int from = l * KP + 32 * n + 8 * g;
+            const u32x4_t a = *reinterpret_cast<const u32x4_t*>(hi + from);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum[i] = mfma(a, b[n][i], sum[i]);
+            if (!HALF) {
+                const u32x4_t a2 = *reinterpret_cast<const u32x4_t*>(lo + from);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sum[i] = mfma(a2, b[n][i], sum[i]);
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            if (now >= width || 4 * g + q >= rows) continue;
+            u32x4_t o;
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+                const float b0 = bf16_to_f32(static_cast<uint16_t>(there[q][d]));
+                const float b1 = bf16_to_f32(static_cast<uint16_t>(there[q][d] >> 16));
+                o[d] = pack_bf16x2(b0 + scale * sum[2 * d][q], b1 + scale * sum[2 * d + 1][q]);
+            }
+            *reinterpret_cast<u32x4_t*>(out + row_at[q] + now) = o;
+        }
+    }
+}
+
+// Workgroups of a fused launch's column parts, or 0 where two launches take less time: the
+// parts' repeated reads of x and w (16 rows and the ranks, of k) may come to kFusedBytes.
+constexpr int64_t kFusedBytes = 32 << 20;
+constexpr int64_t kFusedElements = 64 << 10;
+
+static int fused_parts(int64_t tokens, int64_t k, int64_t width, int rank, int adapters) {
+    // No registers for up's rows beside the loads of h past 32 ranks; and one CU streams
+    // a long w slower than two launches over all of them take.
+    if (rank > 32 || rank * k > kFusedElements) return 0;
+    const int64_t fragments = tokens / 16 + std::min<int64_t>(adapters + 1, tokens);
+    const int64_t columns = (width + kFusedCols - 1) / kFusedCols;
+    const int64_t parts = std::clamp<int64_t>(512 / fragments, 1, columns);
+    return fragments * parts * (rank + 16) * k * 2 <= kFusedBytes ? static_cast<int>(parts) : 0;
+}
+
+// contract and spread: h of x and down, then up; one launch for small batches. Without
+// out: h_out alone.
+static int launch_through(const uint16_t* x, const uint16_t* down, const uint16_t* up, const float* scales,
+                          const Groups& g, const uint16_t* base, uint16_t* out, float* h_out, float* partials,
+                          int64_t tokens, int64_t k, int64_t width, int rank, int adapters, hipStream_t stream) {
+    if (const int parts = out ? fused_parts(tokens, k, width, rank, adapters) : 0) {
+        const int columns = static_cast<int>((width + kFusedCols - 1) / kFusedCols);
+        const int turns = (columns + parts - 1) / parts;
+        const dim3 grid(4 * g.tile_bound, (columns + turns - 1) / turns);
+        const auto run = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, grid, dim3(64 * kFusedWaves), 0, stream, x, down, up, scales, g, base, out, h_out,
+                               static_cast<int>(k), width, rank, turns);
+            return check_launch("fused_kernel");
+        };
+        return rank <= 16 ? run(fused_kernel<1>) : run(fused_kernel<2>);
+    }
+    const int slices = contract_slices(g.tile_bound, k);
+    const int rc = launch_contract(x, down, g, partials, slices, tokens, k, rank, stream);
+    if (rc != MOE_OK) return rc;
+    return launch_spread(partials, slices, up, false, scales, g, base, out, h_out, tokens, width, rank, stream);
+}
+
+// ---------------------------------------------------------------------------
 // outer: out[c][j] = s sum_i h[i][c] x[i][j] over an adapter's rows.
 // The rows are the MFMA's k. A workgroup takes a split of one adapter's rows and 128
 // columns; its waves take 32 rows in turn. x's 8 x 8 blocks are transposed in registers
@@ -821,12 +1040,8 @@ int launch_low_rank_add(const uint16_t* x, const uint16_t* down, const uint16_t*
                         const void* table, const uint16_t* base, uint16_t* output, float* hidden_out, char* scratch,
                         int64_t tokens, int64_t hidden, int64_t width, int rank, int adapters, hipStream_t stream) {
     const Groups g = groups_of(table, tokens, adapters);
-    const int slices = contract_slices(g.tile_bound, hidden);
-    float* partials = reinterpret_cast<float*>(scratch);
-    int rc = launch_contract(x, down, g, partials, slices, tokens, hidden, rank, stream);
-    if (rc == MOE_OK)
-        rc = launch_spread(partials, slices, up, false, scales, g, base, output, hidden_out, tokens, width, rank, stream);
-    return rc;
+    return launch_through(x, down, up, scales, g, base, output, hidden_out, reinterpret_cast<float*>(scratch), tokens,
+                          hidden, width, rank, adapters, stream);
 }
 
 int launch_low_rank_backward(const uint16_t* grad_output, const uint16_t* x, const uint16_t* down, const uint16_t* up,
@@ -840,13 +1055,10 @@ int launch_low_rank_backward(const uint16_t* grad_output, const uint16_t* x, con
     float* dh = reinterpret_cast<float*>(scratch + up16(slices * row));
     float* partials = reinterpret_cast<float*>(scratch + up16(slices * row) + up16(row));
     int rc = MOE_OK;
-    if (tokens > 0 && (grad_x || grad_down)) {
-        rc = launch_contract(grad_output, up, g, dh_parts, slices, tokens, width, rank, stream);
-        // dx, and dh's sum for the outer product (the spread alone has no output without grad_x).
-        if (rc == MOE_OK)
-            rc = launch_spread(dh_parts, slices, down, false, scales, g, grad_x_base, grad_x, dh, tokens, hidden, rank,
-                               stream);
-    }
+    // dx, and dh for its outer product.
+    if (tokens > 0 && (grad_x || grad_down))
+        rc = launch_through(grad_output, up, down, scales, g, grad_x_base, grad_x, dh, dh_parts, tokens, width, hidden,
+                            rank, adapters, stream);
     if (rc == MOE_OK && (grad_down || grad_up)) {
         OuterJob jobs[2];
         if (grad_down) jobs[0] = {dh, x, partials, grad_down, hidden};

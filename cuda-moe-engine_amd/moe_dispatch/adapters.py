@@ -23,7 +23,7 @@ from typing import NamedTuple
 import torch
 
 from ._extension import DTYPE_CODES, current_stream_handle, get_extension
-from .training import _ptr, on_device, refuse_autograd, require_tensor, scratch_bytes, shape_of
+from .training import _ptr, on_device, refuse_autograd, require_tensor, shape_of
 
 MAX_ADAPTERS = 4096
 MAX_RANK = 128
@@ -55,6 +55,7 @@ class AdapterGroups:
         nbytes = self.extension.lib.moe_adapter_table_bytes(tokens, adapters)
         self.table = torch.empty(nbytes // 4, dtype=torch.int32, device=device)
         self.table_bytes = nbytes
+        self._sizes = {}  # shapes of x, down and up that fit -> _Sizes
 
     def assign(self, ids):
         require_tensor(ids, "ids", (self.tokens,), torch.int32, self.device)
@@ -85,26 +86,49 @@ def _check_width(n, name):
         raise ValueError(f"{name} must be a multiple of 8 up to 2^20")
 
 
+class _Sizes(NamedTuple):
+    hidden: int
+    width: int
+    rank: int
+    forward_bytes: int
+    backward_bytes: int
+
+
+def _check_sizes(x, down, up, groups):
+    """Sizes and scratch of operands whose shapes fit each other and the groups."""
+    tokens, adapters = groups.tokens, groups.adapters
+    hidden = shape_of(x, "x", 2)[1]
+    rank = shape_of(down, "down", 3)[1]
+    width = shape_of(up, "up", 3)[2]
+    for t, name, shape in ((x, "x", (tokens, hidden)), (down, "down", (adapters, rank, hidden)),
+                           (up, "up", (adapters, rank, width))):
+        if t.shape != shape:
+            raise ValueError(f"{name}: expected shape {list(shape)}, got {list(t.shape)}")
+    _check_width(hidden, "hidden")
+    _check_width(width, "width")
+    if not 1 <= rank <= MAX_RANK:
+        raise ValueError("rank must be in 1..128")
+    need = groups.extension.lib.moe_low_rank_scratch_bytes
+    sizes = _Sizes(hidden, width, rank, *(need(tokens, hidden, width, rank, adapters, b) for b in (0, 1)))
+    groups._sizes[(x.shape, down.shape, up.shape)] = sizes
+    return sizes
+
+
 def _check_operands(x, down, up, groups, scales):
     if not isinstance(groups, AdapterGroups):
         raise TypeError("groups must be AdapterGroups")
     if groups.assignment == 0:
         raise RuntimeError("AdapterGroups.assign has not grouped any rows yet")
     device = groups.device
-    tokens, adapters = groups.tokens, groups.adapters
-    hidden = shape_of(x, "x", 2)[1]
-    require_tensor(x, "x", (tokens, hidden), torch.bfloat16, device)
-    rank = shape_of(down, "down", 3)[1]
-    require_tensor(down, "down", (adapters, rank, hidden), torch.bfloat16, device)
-    width = shape_of(up, "up", 3)[2]
-    require_tensor(up, "up", (adapters, rank, width), torch.bfloat16, device)
-    _check_width(hidden, "hidden")
-    _check_width(width, "width")
-    if not 1 <= rank <= MAX_RANK:
-        raise ValueError("rank must be in 1..128")
+    for t, name in ((x, "x"), (down, "down"), (up, "up")):
+        if not isinstance(t, torch.Tensor) or t.dtype is not torch.bfloat16 or t.device != device or not t.is_contiguous():
+            require_tensor(t, name, getattr(t, "shape", ()), torch.bfloat16, device)
+    sizes = groups._sizes.get((x.shape, down.shape, up.shape))
+    if sizes is None:
+        sizes = _check_sizes(x, down, up, groups)
     if scales is not None:
-        require_tensor(scales, "scales", (adapters,), torch.float32, device)
-    return tokens, adapters, hidden, width, rank, device
+        require_tensor(scales, "scales", (groups.adapters,), torch.float32, device)
+    return sizes
 
 
 def _overlaps(a, b):
@@ -120,7 +144,8 @@ def low_rank_add(base, x, down, up, groups, *, scales=None, output=None, return_
     (in place); a new tensor when None. With ``return_hidden`` the result is
     ``(output, hidden)``, ``hidden`` for ``low_rank_backward``.
     """
-    tokens, adapters, hidden, width, rank, device = _check_operands(x, down, up, groups, scales)
+    hidden, width, rank, need, _ = _check_operands(x, down, up, groups, scales)
+    tokens, device = groups.tokens, groups.device
     if base is not None:
         require_tensor(base, "base", (tokens, width), torch.bfloat16, device)
     if output is not None:
@@ -132,14 +157,13 @@ def low_rank_add(base, x, down, up, groups, *, scales=None, output=None, return_
     lib = groups.extension.lib
     with on_device(device):
         if output is None:
-            output = x.new_empty((tokens, width))
+            output = torch.empty_like(base) if base is not None else x.new_empty((tokens, width))
         kept = x.new_empty((tokens, rank), dtype=torch.float32) if return_hidden else None
-        need = scratch_bytes("moe_low_rank_scratch_bytes", tokens, hidden, width, rank, adapters, 0)
         scratch = x.new_empty(need // 2)
         lib.check(lib.moe_low_rank_add(
             x.data_ptr(), down.data_ptr(), up.data_ptr(), _ptr(scales), groups.table.data_ptr(),
             groups.table_bytes, _ptr(base), output.data_ptr(), _ptr(kept), scratch.data_ptr(), need, tokens,
-            hidden, width, rank, adapters, current_stream_handle(device.index)), "low_rank_add")
+            hidden, width, rank, groups.adapters, current_stream_handle(device.index)), "low_rank_add")
     return (output, LowRankHidden(kept, groups, groups.assignment)) if return_hidden else output
 
 
@@ -153,7 +177,8 @@ def low_rank_backward(grad_output, x, down, up, groups, *, scales=None, hidden, 
     ``grad_dtype`` (fp32, or bf16 rounded once), zero for adapters without rows. scales get
     no gradient.
     """
-    tokens, adapters, h, width, rank, device = _check_operands(x, down, up, groups, scales)
+    h, width, rank, _, need = _check_operands(x, down, up, groups, scales)
+    tokens, device = groups.tokens, groups.device
     require_tensor(grad_output, "grad_output", (tokens, width), torch.bfloat16, device)
     if not isinstance(hidden, LowRankHidden):
         raise TypeError("hidden must be what low_rank_add returned with return_hidden")
@@ -170,12 +195,11 @@ def low_rank_backward(grad_output, x, down, up, groups, *, scales=None, hidden, 
         out_x = torch.empty_like(x)
         grad_down = torch.empty_like(down, dtype=grad_dtype)
         grad_up = torch.empty_like(up, dtype=grad_dtype)
-        need = scratch_bytes("moe_low_rank_scratch_bytes", tokens, h, width, rank, adapters, 1)
         scratch = x.new_empty(need // 2)
         lib.check(lib.moe_low_rank_backward(
             grad_output.data_ptr(), x.data_ptr(), down.data_ptr(), up.data_ptr(), _ptr(scales),
             groups.table.data_ptr(), groups.table_bytes, hidden.values.data_ptr(), _ptr(grad_x),
             out_x.data_ptr(), grad_down.data_ptr(), grad_up.data_ptr(), DTYPE_CODES[grad_dtype], scratch.data_ptr(),
-            need, tokens, h, width, rank, adapters, current_stream_handle(device.index)),
+            need, tokens, h, width, rank, groups.adapters, current_stream_handle(device.index)),
             "low_rank_backward")
     return out_x, grad_down, grad_up

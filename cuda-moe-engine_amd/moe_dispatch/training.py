@@ -29,11 +29,12 @@ from ._extension import DTYPE_CODES, current_stream_handle, get_extension
 from .workspace import MAX_EXPERTS, MAX_TOPK
 
 _CURRENT = nullcontext()
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def on_device(device):
     """Makes ``device`` current where it is not: streams and launches go by the current device."""
-    return _CURRENT if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _CURRENT if device.index == _current_device() else torch.cuda.device(device)
 
 
 def require_tensor(t, name, shape, dtype, device):
@@ -54,9 +55,9 @@ def require_tensor(t, name, shape, dtype, device):
 
 
 def shape_of(t, name, dims):
-    if not isinstance(t, torch.Tensor):
+    shape = t.shape if isinstance(t, torch.Tensor) else None
+    if shape is None:
         raise TypeError(f"{name} must be a tensor")
-    shape = t.shape
     if len(shape) != dims:
         raise ValueError(f"{name}: expected {dims} dimensions, got shape {list(shape)}")
     return shape
@@ -80,9 +81,13 @@ def _ptr(t):
 
 
 @lru_cache(maxsize=1024)
-def scratch_bytes(name, *sizes):
-    """What one of the library's ``*_scratch_bytes`` functions says (-1 for sizes it refuses)."""
-    return getattr(get_extension().lib, name)(*sizes)
+def _loss_scratch_bytes(tokens, experts):
+    return get_extension().lib.moe_router_loss_scratch_bytes(tokens, experts)
+
+
+@lru_cache(maxsize=1024)
+def _route_scratch_bytes(tokens, hidden, experts):
+    return get_extension().lib.moe_route_backward_scratch_bytes(tokens, hidden, experts)
 
 
 class RouterLoss(NamedTuple):
@@ -108,11 +113,14 @@ class RouterLoss(NamedTuple):
 def _check_routed(logits, expert_ids, bias, mask):
     tokens, experts = shape_of(logits, "logits", 2)
     device = logits.device
-    require_tensor(logits, "logits", (tokens, experts), torch.float32, device)
+    if logits.dtype is not torch.float32 or not logits.is_contiguous():
+        require_tensor(logits, "logits", logits.shape, torch.float32, device)
     if not 1 <= experts <= MAX_EXPERTS:
         raise ValueError("logits must have 1..64 experts")
-    topk = shape_of(expert_ids, "expert_ids", 2)[1]
-    require_tensor(expert_ids, "expert_ids", (tokens, topk), torch.int32, device)
+    rows, topk = shape_of(expert_ids, "expert_ids", 2)
+    if (rows != tokens or expert_ids.dtype is not torch.int32 or expert_ids.device != device
+            or not expert_ids.is_contiguous()):
+        require_tensor(expert_ids, "expert_ids", (tokens, topk), torch.int32, device)
     if not 1 <= topk <= MAX_TOPK:
         raise ValueError("topk must be in 1..8")
     if tokens * max(experts, topk) > 2**31 - 1:
@@ -145,7 +153,7 @@ def router_loss(logits, expert_ids, bias=None, *, mask=None):
     with on_device(device):
         losses = logits.new_empty(2)
         stats = expert_ids.new_empty(experts + 1)
-        need = scratch_bytes("moe_router_loss_scratch_bytes", tokens, experts)
+        need = _loss_scratch_bytes(tokens, experts)
         scratch = logits.new_empty(need // 4) if need else None
         lib.check(lib.moe_router_loss(
             logits.data_ptr(), _ptr(bias), expert_ids.data_ptr(), _ptr(mask), losses.data_ptr(), stats.data_ptr(),
@@ -214,7 +222,7 @@ def route_backward(x, router_weight, logits, expert_ids, bias=None, *, mask=None
         out_x = torch.empty_like(x)
         grad_router_weight = torch.empty_like(router_weight)
         grad_bias = logits.new_empty(experts)
-        need = scratch_bytes("moe_route_backward_scratch_bytes", tokens, hidden, experts)
+        need = _route_scratch_bytes(tokens, hidden, experts)
         if need < 0:
             raise ValueError("route_backward takes up to 2^21 tokens")
         scratch = logits.new_empty(need // 4)

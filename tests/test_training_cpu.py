@@ -1,5 +1,7 @@
 """Refusals of the training and adapter operators, checked where no kernel can launch."""
 
+from types import SimpleNamespace
+
 import pytest
 import torch
 
@@ -101,7 +103,8 @@ def test_transport_gradients_refuse_bad_tensors():
 def _groups(tokens=4, adapters=3, assigned=True):
     groups = object.__new__(AdapterGroups)
     groups.tokens, groups.adapters, groups.device = tokens, adapters, torch.device("cpu")
-    groups.assignment, groups.table_bytes = int(assigned), 0
+    groups.assignment, groups.table_bytes, groups._sizes = int(assigned), 0, {}
+    groups.extension = SimpleNamespace(lib=_lib.load_library())
     return groups
 
 
