@@ -75,12 +75,14 @@ inline Groups groups_of(const void* table, int64_t tokens, int64_t adapters) {
     return g;
 }
 
-// The splits of one group may follow the width too: about 512 workgroups.
-inline Groups one_group(int64_t tokens, int64_t width) {
+// The splits of one group may follow the width and rank too: about 512 workgroups, or 256
+// of the eight waves that more than 32 ranks take.
+inline Groups one_group(int64_t tokens, int64_t width, int64_t rank) {
     Groups g;
     const int64_t columns = (width + kOuterCols - 1) / kOuterCols;
+    const int64_t most = rank > 32 ? 256 : 512;
     g.split_rows = 128;
-    while (g.split_rows < 1024 && tokens * columns > static_cast<int64_t>(g.split_rows) * 512) g.split_rows <<= 1;
+    while (g.split_rows < 1024 && tokens * columns > g.split_rows * most) g.split_rows <<= 1;
     g.tile_bound = static_cast<int>((tokens + kTileRows - 1) / kTileRows);
     g.split_bound = static_cast<int>((tokens + g.split_rows - 1) / g.split_rows);
     return g;

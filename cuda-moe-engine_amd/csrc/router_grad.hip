@@ -411,7 +411,7 @@ int launch_router_logits_grad(const float* logits, const float* bias, const int3
 static int64_t aligned16(int64_t bytes) { return (bytes + 15) / 16 * 16; }
 
 int64_t route_backward_scratch_bytes(int64_t tokens, int64_t hidden, int64_t experts) {
-    const Groups g = one_group(tokens, hidden);
+    const Groups g = one_group(tokens, hidden, experts);
     return aligned16(tokens * experts * 4) + aligned16(static_cast<int64_t>(kLossBlocks) * experts * 4) +
            (g.split_bound > 1 ? g.split_bound * experts * hidden * 4 : 0);
 }
@@ -425,7 +425,7 @@ int launch_route_backward(const uint16_t* x, const float* router_w, const float*
     float* bias_part = reinterpret_cast<float*>(scratch + aligned16(tokens * experts * 4));
     float* partials = reinterpret_cast<float*>(scratch + aligned16(tokens * experts * 4) +
                                                aligned16(static_cast<int64_t>(kLossBlocks) * experts * 4));
-    const Groups g = one_group(tokens, hidden);
+    const Groups g = one_group(tokens, hidden, experts);
     ColumnSums sums;
     sums.part = bias_part;
     sums.out = grad_bias;
