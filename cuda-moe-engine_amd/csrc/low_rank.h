@@ -12,6 +12,7 @@ constexpr int64_t kMaxAdapterTokens = 1 << 21;  // tiles and adapters within a g
 constexpr int64_t kMaxLowRankWidth = 1 << 20;
 constexpr int kTileRows = 64;     // rows of one adapter per tile (contract, spread)
 constexpr int kOuterCols = 128;   // columns per workgroup of outer
+constexpr int kMaxSplitRows = 1024;
 
 // Where the parts of an adapter table lie, in int32 from its start:
 //   head         [4]     tiles, splits, 0, 0
@@ -30,7 +31,7 @@ struct TableLayout {
 // (splits * width / 128) to fill the card: about 8 splits of a batch.
 inline int outer_split_rows(int64_t tokens) {
     int rows = 128;
-    while (rows < 1024 && rows * 8 < tokens) rows <<= 1;
+    while (rows < kMaxSplitRows && rows * 8 < tokens) rows <<= 1;
     return rows;
 }
 
@@ -82,7 +83,7 @@ inline Groups one_group(int64_t tokens, int64_t width, int64_t rank) {
     const int64_t columns = (width + kOuterCols - 1) / kOuterCols;
     const int64_t most = rank > 32 ? 256 : 512;
     g.split_rows = 128;
-    while (g.split_rows < 1024 && tokens * columns > g.split_rows * most) g.split_rows <<= 1;
+    while (g.split_rows < kMaxSplitRows && tokens * columns > g.split_rows * most) g.split_rows <<= 1;
     g.tile_bound = static_cast<int>((tokens + kTileRows - 1) / kTileRows);
     g.split_bound = static_cast<int>((tokens + g.split_rows - 1) / g.split_rows);
     return g;
