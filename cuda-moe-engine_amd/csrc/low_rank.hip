@@ -674,7 +674,7 @@ __global__ __launch_bounds__(64 * kFusedWaves) void fused_kernel(
     if (adapter < 0) {  // no adapter: h is 0, the base as it is
         if (h_out && blockIdx.y == 0)
             for (int i = tid; i < rows * rank; i += 64 * kFusedWaves) h_out[static_cast<int64_t>(first) * rank + i] = 0.0f;
-        if (base == out) return;
+        if (base == out || !out) return;
         for (int turn = 0; turn < turns && col < width; ++turn, col += kFusedCols)
 #pragma unroll
             for (int q = 0; q < 4; ++q)
@@ -698,7 +698,7 @@ __global__ __launch_bounds__(64 * kFusedWaves) void fused_kernel(
 #pragma unroll
         for (int q = 0; q < 4; ++q) old[q] = base && inside ? load16(base + row_at[q] + col) : zero;
     };
-    fetch();
+    if (out) fetch();
     f32x4_t acc[NR];
 #pragma unroll
     for (int n = 0; n < NR; ++n) acc[n] = f32x4_t{0, 0, 0, 0};
@@ -777,6 +777,7 @@ __global__ __launch_bounds__(64 * kFusedWaves) void fused_kernel(
         else
             lo[row * KP + c] = rest;
     }
+    if (!out) return;
     __syncthreads();
     const float scale = scales ? scales[adapter] : 1.0f;
     for (int turn = 0; turn < turns; ++turn) {
@@ -834,12 +835,12 @@ static int fused_parts(int64_t tokens, int64_t k, int64_t width, int rank, int a
 }
 
 // contract and spread: h of x and down, then up; one launch for small batches. Without
-// out: h_out alone.
+// out: h_out alone, with the same sums.
 static int launch_through(const uint16_t* x, const uint16_t* down, const uint16_t* up, const float* scales,
                           const Groups& g, const uint16_t* base, uint16_t* out, float* h_out, float* partials,
                           int64_t tokens, int64_t k, int64_t width, int rank, int adapters, hipStream_t stream) {
-    if (const int parts = out ? fused_parts(tokens, k, width, rank, adapters) : 0) {
-        const int columns = static_cast<int>((width + kFusedCols - 1) / kFusedCols);
+    if (const int parts = fused_parts(tokens, k, width, rank, adapters)) {
+        const int columns = out ? static_cast<int>((width + kFusedCols - 1) / kFusedCols) : 1;
         const int turns = (columns + parts - 1) / parts;
         const dim3 grid(4 * g.tile_bound, (columns + turns - 1) / turns);
         const auto run = [&](auto kernel) {

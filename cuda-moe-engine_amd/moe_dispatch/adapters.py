@@ -168,14 +168,15 @@ def low_rank_add(base, x, down, up, groups, *, scales=None, output=None, return_
 
 
 def low_rank_backward(grad_output, x, down, up, groups, *, scales=None, hidden, grad_x=None,
-                      grad_dtype=torch.float32):
+                      grad_dtype=torch.float32, gradients=(True, True, True)):
     """Gradients of ``low_rank_add``: ``(grad_x, grad_down, grad_up)``; base's is ``grad_output``.
 
     ``hidden`` is what the forward returned with ``return_hidden``, on the groups' current
     assignment. ``grad_x`` bf16 [T, H] is x's gradient along its other paths (the shared
     projection): the result is the sum, rounded once. grad_down and grad_up are
     ``grad_dtype`` (fp32, or bf16 rounded once), zero for adapters without rows. scales get
-    no gradient.
+    no gradient. ``gradients``: which of the three are wanted; the others are None and
+    cost nothing.
     """
     h, width, rank, _, need = _check_operands(x, down, up, groups, scales)
     tokens, device = groups.tokens, groups.device
@@ -192,14 +193,15 @@ def low_rank_backward(grad_output, x, down, up, groups, *, scales=None, hidden, 
     refuse_autograd(grad_output, x, down, up, scales, grad_x)
     lib = groups.extension.lib
     with on_device(device):
-        out_x = torch.empty_like(x)
-        grad_down = torch.empty_like(down, dtype=grad_dtype)
-        grad_up = torch.empty_like(up, dtype=grad_dtype)
+        want_x, want_down, want_up = gradients
+        out_x = torch.empty_like(x) if want_x else None
+        grad_down = torch.empty_like(down, dtype=grad_dtype) if want_down else None
+        grad_up = torch.empty_like(up, dtype=grad_dtype) if want_up else None
         scratch = x.new_empty(need // 2)
         lib.check(lib.moe_low_rank_backward(
             grad_output.data_ptr(), x.data_ptr(), down.data_ptr(), up.data_ptr(), _ptr(scales),
             groups.table.data_ptr(), groups.table_bytes, hidden.values.data_ptr(), _ptr(grad_x),
-            out_x.data_ptr(), grad_down.data_ptr(), grad_up.data_ptr(), DTYPE_CODES[grad_dtype], scratch.data_ptr(),
+            _ptr(out_x), _ptr(grad_down), _ptr(grad_up), DTYPE_CODES[grad_dtype], scratch.data_ptr(),
             need, tokens, h, width, rank, groups.adapters, current_stream_handle(device.index)),
             "low_rank_backward")
     return out_x, grad_down, grad_up

@@ -131,6 +131,11 @@ def test_forward_and_gradients(tokens, hidden, width, rank, adapters, pattern):
     dx16, gd16, gu16 = low_rank_backward(case["grad"], *operands, scales=case["scales"], hidden=kept,
                                          grad_x=case["grad_x"], grad_dtype=torch.bfloat16)
     assert torch.equal(dx16, dx) and torch.equal(gd16, gd.bfloat16()) and torch.equal(gu16, gu.bfloat16())
+    for wanted in ((True, False, False), (False, True, False), (False, False, True), (False, False, False)):
+        some = low_rank_backward(case["grad"], *operands, scales=case["scales"], hidden=kept, grad_x=case["grad_x"],
+                                 gradients=wanted)
+        for got, full, want in zip(some, (dx, gd, gu), wanted):
+            assert (got is None) if not want else torch.equal(got, full)
     plain = (case["ids"] < 0) | (case["ids"] >= adapters)
     assert torch.equal(y[plain], case["base"][plain]) and torch.equal(dx[plain], case["grad_x"][plain])
 
