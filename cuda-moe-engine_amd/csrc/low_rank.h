@@ -118,7 +118,7 @@ __device__ __forceinline__ void sum_columns(const ColumnSums& c) {
 }
 
 // K slices of contract for this shape; partials holds that many [tokens, rank] sums.
-int contract_slices(int tile_bound, int64_t k);
+int contract_slices(int tile_bound, int64_t k, int64_t rank);
 
 // partials[s][i][c] = sum over slice s of x[order[i]][k] * w[adapter][c][k]; rows of no
 // adapter are not written.

@@ -340,10 +340,13 @@ __global__ __launch_bounds__(256) void contract_kernel(const uint16_t* __restric
     }
 }
 
-int contract_slices(int tile_bound, int64_t k) {
-    const int64_t most = (k + 255) / 256;
+// Up to about 600 workgroups; past 64 ranks, where spread reads each slice's sums again
+// for every 256 columns, 512 (contract and spread of 8192 x 4096 to 4096, rank 16: 46.9 us,
+// with 512 50.5; of 16384 rows, rank 128: 168 and 158).
+int contract_slices(int tile_bound, int64_t k, int64_t rank) {
+    const int64_t most = (k + 255) / 256, workgroups = rank <= 64 ? 600 : 512;
     int64_t s = 1;
-    while (s < 16 && s * 2 <= most && s * 2 * tile_bound <= 512) s <<= 1;
+    while (s < 16 && s * 2 <= most && s * 2 * tile_bound <= workgroups) s <<= 1;
     return static_cast<int>(s);
 }
 
@@ -850,7 +853,7 @@ static int launch_through(const uint16_t* x, const uint16_t* down, const uint16_
         };
         return rank <= 16 ? run(fused_kernel<1>) : run(fused_kernel<2>);
     }
-    const int slices = contract_slices(g.tile_bound, k);
+    const int slices = contract_slices(g.tile_bound, k, rank);
     const int rc = launch_contract(x, down, g, partials, slices, tokens, k, rank, stream);
     if (rc != MOE_OK) return rc;
     return launch_spread(partials, slices, up, false, scales, g, base, out, h_out, tokens, width, rank, stream);
@@ -1059,8 +1062,8 @@ int64_t low_rank_scratch_bytes(int64_t tokens, int64_t hidden, int64_t width, in
                                bool backward) {
     const TableLayout t = table_layout(tokens, adapters);
     const int64_t row = tokens * rank * 4;
-    if (!backward) return contract_slices(t.tile_bound, hidden) * row;
-    return up16(contract_slices(t.tile_bound, width) * row) + up16(row) +
+    if (!backward) return contract_slices(t.tile_bound, hidden, rank) * row;
+    return up16(contract_slices(t.tile_bound, width, rank) * row) + up16(row) +
            static_cast<int64_t>(t.split_bound) * rank * (hidden + width) * 4;
 }
 
@@ -1077,7 +1080,7 @@ int launch_low_rank_backward(const uint16_t* grad_output, const uint16_t* x, con
                              uint16_t* grad_x, void* grad_down, void* grad_up, bool grad_bf16, char* scratch,
                              int64_t tokens, int64_t hidden, int64_t width, int rank, int adapters, hipStream_t stream) {
     const Groups g = groups_of(table, tokens, adapters);
-    const int slices = contract_slices(g.tile_bound, width);
+    const int slices = contract_slices(g.tile_bound, width, rank);
     const int64_t row = tokens * rank * 4;
     float* dh_parts = reinterpret_cast<float*>(scratch);
     float* dh = reinterpret_cast<float*>(scratch + up16(slices * row));
