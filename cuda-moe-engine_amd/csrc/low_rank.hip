@@ -832,6 +832,7 @@ static int fused_parts(int64_t tokens, int64_t k, int64_t width, int rank, int a
     // a long w slower than two launches over all of them take.
     if (rank > 32 || rank * k > kFusedElements) return 0;
     const int64_t fragments = tokens / 16 + std::min<int64_t>(adapters + 1, tokens);
+    if (fragments == 0) return 0;
     const int64_t columns = (width + kFusedCols - 1) / kFusedCols;
     const int64_t parts = std::clamp<int64_t>(512 / fragments, 1, columns);
     return fragments * parts * (rank + 16) * k * 2 <= kFusedBytes ? static_cast<int>(parts) : 0;
@@ -1057,13 +1058,18 @@ int launch_outer(const OuterJob& first, const OuterJob& second, const float* sca
 // ---------------------------------------------------------------------------
 static int64_t up16(int64_t bytes) { return (bytes + 15) / 16 * 16; }
 
-// Forward: contract's partial sums. Backward: those of dh, dh itself, the two products' partial sums.
+// contract's partial sums, none where one launch does.
+static int64_t through_bytes(int64_t tokens, int64_t k, int64_t width, int64_t rank, int64_t adapters) {
+    if (fused_parts(tokens, k, width, static_cast<int>(rank), static_cast<int>(adapters))) return 0;
+    return contract_slices(table_layout(tokens, adapters).tile_bound, k, rank) * tokens * rank * 4;
+}
+
+// Forward: contract's sums. Backward: those of dh, dh itself, the two products' partial sums.
 int64_t low_rank_scratch_bytes(int64_t tokens, int64_t hidden, int64_t width, int64_t rank, int64_t adapters,
                                bool backward) {
     const TableLayout t = table_layout(tokens, adapters);
-    const int64_t row = tokens * rank * 4;
-    if (!backward) return contract_slices(t.tile_bound, hidden, rank) * row;
-    return up16(contract_slices(t.tile_bound, width, rank) * row) + up16(row) +
+    if (!backward) return through_bytes(tokens, hidden, width, rank, adapters);
+    return up16(through_bytes(tokens, width, hidden, rank, adapters)) + up16(tokens * rank * 4) +
            static_cast<int64_t>(t.split_bound) * rank * (hidden + width) * 4;
 }
 
@@ -1080,11 +1086,10 @@ int launch_low_rank_backward(const uint16_t* grad_output, const uint16_t* x, con
                              uint16_t* grad_x, void* grad_down, void* grad_up, bool grad_bf16, char* scratch,
                              int64_t tokens, int64_t hidden, int64_t width, int rank, int adapters, hipStream_t stream) {
     const Groups g = groups_of(table, tokens, adapters);
-    const int slices = contract_slices(g.tile_bound, width, rank);
-    const int64_t row = tokens * rank * 4;
     float* dh_parts = reinterpret_cast<float*>(scratch);
-    float* dh = reinterpret_cast<float*>(scratch + up16(slices * row));
-    float* partials = reinterpret_cast<float*>(scratch + up16(slices * row) + up16(row));
+    scratch += up16(through_bytes(tokens, width, hidden, rank, adapters));
+    float* dh = reinterpret_cast<float*>(scratch);
+    float* partials = reinterpret_cast<float*>(scratch + up16(tokens * rank * 4));
     int rc = MOE_OK;
     // dx, and dh for its outer product.
     if (tokens > 0 && (grad_x || grad_down))

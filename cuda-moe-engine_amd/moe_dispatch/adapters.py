@@ -159,10 +159,10 @@ def low_rank_add(base, x, down, up, groups, *, scales=None, output=None, return_
         if output is None:
             output = torch.empty_like(base) if base is not None else x.new_empty((tokens, width))
         kept = x.new_empty((tokens, rank), dtype=torch.float32) if return_hidden else None
-        scratch = x.new_empty(need // 2)
+        scratch = x.new_empty(need // 2) if need else None
         lib.check(lib.moe_low_rank_add(
             x.data_ptr(), down.data_ptr(), up.data_ptr(), _ptr(scales), groups.table.data_ptr(),
-            groups.table_bytes, _ptr(base), output.data_ptr(), _ptr(kept), scratch.data_ptr(), need, tokens,
+            groups.table_bytes, _ptr(base), output.data_ptr(), _ptr(kept), _ptr(scratch), need, tokens,
             hidden, width, rank, groups.adapters, current_stream_handle(device.index)), "low_rank_add")
     return (output, LowRankHidden(kept, groups, groups.assignment)) if return_hidden else output
 

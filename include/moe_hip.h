@@ -486,8 +486,8 @@ int64_t moe_adapter_table_bytes(int64_t tokens, int64_t adapters);
 int moe_adapter_group(const int32_t* ids, void* table, int64_t table_bytes, int64_t tokens, int64_t adapters,
                       void* stream);
 
-/* Bytes of scratch moe_low_rank_add (backward == 0) or moe_low_rank_backward needs; -1 for
- * invalid sizes. */
+/* Bytes of scratch moe_low_rank_add (backward == 0; 0: none) or moe_low_rank_backward needs;
+ * -1 for invalid sizes. */
 int64_t moe_low_rank_scratch_bytes(int64_t tokens, int64_t hidden, int64_t width, int64_t rank, int64_t adapters,
                                    int backward);
 

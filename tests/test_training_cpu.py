@@ -233,10 +233,11 @@ def test_c_entries_check_their_arguments_without_launching():
     assert lib.moe_adapter_group(A, A + 4, table, 4, 3, None) == 1
     assert lib.moe_adapter_group(A, A, table, 4, 0, None) == 2
     assert lib.moe_low_rank_scratch_bytes(4, 64, 32, 129, 3, 0) == -1
-    need = lib.moe_low_rank_scratch_bytes(4, 64, 32, 8, 3, 0)
-    assert need == 4 * 8 * 4  # one slice of 64: tokens * rank sums
+    assert lib.moe_low_rank_scratch_bytes(4, 64, 32, 8, 3, 0) == 0  # a small batch: one launch, nothing handed over
+    need = lib.moe_low_rank_scratch_bytes(4, 64, 32, 40, 3, 0)
+    assert need == 4 * 40 * 4  # one slice of 64: tokens * rank sums
 
-    def add(x=A, base=A, out=A, nbytes=need, table_bytes=table, hidden=64, width=32, rank=8, tokens=4):
+    def add(x=A, base=A, out=A, nbytes=need, table_bytes=table, hidden=64, width=32, rank=40, tokens=4):
         return lib.moe_low_rank_add(x, A, A, A, A, table_bytes, base, out, None, A, nbytes, tokens, hidden, width, rank,
                                     3, None)
 
