@@ -32,6 +32,17 @@ constexpr int kXor1 = 0xB1, kXor2 = 0x4E, kHalfMirror = 0x141, kRor8 = 0x128, kR
 
 __device__ __forceinline__ float max_nan(float a, float b) { return b > a || b != b ? b : a; }  // keeps a NaN
 
+// e^x for x <= 0 (a NaN stays one): 2^t with t = x log2 e rounded, times e^(what the
+// rounding left), to first order; the hardware's 2^t is good to about one rounding. Below
+// -100 it is 0, as no sum it enters beside e^0 = 1 can tell.
+__device__ __forceinline__ float exp_to_0(float x) {
+    const float log2e = 1.44269504f, rest = 1.92596303e-8f;  // log2 e, and beyond fp32
+    const float t = x * log2e;
+    const float left = __builtin_fmaf(x, log2e, -t) + x * rest;
+    const float y = __builtin_amdgcn_exp2f(t);
+    return x < -100.0f ? 0.0f : __builtin_fmaf(y * left, 0.693147181f, y);
+}
+
 // Over the G neighbouring lanes of a token.
 template <int G>
 __device__ __forceinline__ float token_max(float v) {
@@ -87,7 +98,7 @@ __device__ __forceinline__ void token_softmax(const float (&v)[kPer], float (&p)
     float total = 0.0f;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
-        p[j] = some ? expf(v[j] - top) : 0.0f;
+        p[j] = some ? exp_to_0(v[j] - top) : 0.0f;
         total += p[j];
     }
     total = token_sum<G>(total);
@@ -118,7 +129,8 @@ __device__ __forceinline__ void write_losses(const LossOut& out, float p, int co
 
 // A block's sums over its tokens: records[block] = p [E], z, counts [E], tokens (the
 // latter as integers), or the losses themselves where it is the only block.
-template <int G>
+// K: the most experts a token has here.
+template <int G, int K>
 __global__ __launch_bounds__(256) void router_loss_kernel(const float* __restrict__ logits,
                                                           const float* __restrict__ bias,
                                                           const int32_t* __restrict__ ids,
@@ -141,9 +153,9 @@ __global__ __launch_bounds__(256) void router_loss_kernel(const float* __restric
          t += static_cast<int64_t>(gridDim.x) * (256 / G)) {
         if (mask && !mask[t]) continue;  // the whole group
         float v[kPer], p[kPer], lse;
-        int id[kMaxTopk];
+        int id[K];
 #pragma unroll
-        for (int k = 0; k < kMaxTopk; ++k) id[k] = k < topk ? ids[t * topk + k] : -1;
+        for (int k = 0; k < K; ++k) id[k] = k < topk ? ids[t * topk + k] : -1;
         load_logits(logits + t * experts, b, e0, experts, v);
         token_softmax<G>(v, p, &lse);
         z_sum += lse * lse;
@@ -152,7 +164,7 @@ __global__ __launch_bounds__(256) void router_loss_kernel(const float* __restric
         for (int j = 0; j < kPer; ++j) {
             p_sum[j] += p[j];
 #pragma unroll
-            for (int k = 0; k < kMaxTopk; ++k) count[j] += id[k] == e0 + j;
+            for (int k = 0; k < K; ++k) count[j] += id[k] == e0 + j;
         }
     }
     // A wave's tokens, then the waves.
@@ -246,7 +258,7 @@ __global__ __launch_bounds__(1024) void router_loss_sum_kernel(const float* __re
 }
 
 // dv, and each block's sum over its tokens for the bias (bias_part may be null).
-template <int G>
+template <int G, int K>
 __global__ __launch_bounds__(256) void router_logits_grad_kernel(
     const float* __restrict__ logits, const float* __restrict__ bias, const int32_t* __restrict__ ids,
     const uint8_t* __restrict__ mask, const int32_t* __restrict__ stats, const float* __restrict__ grad_losses,
@@ -286,23 +298,23 @@ __global__ __launch_bounds__(256) void router_logits_grad_kernel(
             if (grad_weights) {
                 // The chosen experts' softmax, the same terms in every lane of the token; an
                 // id outside the experts was not routed and has no term.
-                float chosen[kMaxTopk], dw[kMaxTopk];
-                int id[kMaxTopk];
+                float chosen[K], dw[K];
+                int id[K];
 #pragma unroll
-                for (int k = 0; k < kMaxTopk; ++k) {
+                for (int k = 0; k < K; ++k) {
                     id[k] = k < topk ? ids[t * topk + k] : -1;
                     dw[k] = k < topk ? grad_weights[t * topk + k] : 0.0f;
                 }
                 float top = -__builtin_inff(), total = 0.0f, dot = 0.0f;
 #pragma unroll
-                for (int k = 0; k < kMaxTopk; ++k) {
+                for (int k = 0; k < K; ++k) {
                     const bool routed = static_cast<unsigned>(id[k]) < static_cast<unsigned>(experts);
                     chosen[k] = routed ? row[id[k]] + (bias ? bias[id[k]] : 0.0f) : -__builtin_inff();
                     top = max_nan(top, chosen[k]);
                 }
 #pragma unroll
-                for (int k = 0; k < kMaxTopk; ++k) {
-                    chosen[k] = chosen[k] == -__builtin_inff() ? 0.0f : chosen[k] == top ? 1.0f : expf(chosen[k] - top);
+                for (int k = 0; k < K; ++k) {
+                    chosen[k] = chosen[k] == -__builtin_inff() ? 0.0f : chosen[k] == top ? 1.0f : exp_to_0(chosen[k] - top);
                     total += chosen[k];
                     // A chosen expert of weight 0 passes nothing on, whatever its gradient.
                     dot += chosen[k] == 0.0f ? 0.0f : chosen[k] * dw[k];
@@ -311,7 +323,7 @@ __global__ __launch_bounds__(256) void router_logits_grad_kernel(
                     const float inverse = 1.0f / total;
                     dot *= inverse;
 #pragma unroll
-                    for (int k = 0; k < kMaxTopk; ++k) {
+                    for (int k = 0; k < K; ++k) {
                         const float term = chosen[k] == 0.0f ? 0.0f : chosen[k] * inverse * (dw[k] - dot);
 #pragma unroll
                         for (int j = 0; j < kPer; ++j) dv[j] += id[k] == e0 + j ? term : 0.0f;
@@ -358,13 +370,17 @@ static int token_blocks(int64_t tokens, int experts) {
     return lanes <= 1024 ? 1 : static_cast<int>(std::min<int64_t>((lanes + 255) / 256, kLossBlocks));
 }
 
+// f(lanes a token, most experts a token): top-1 and top-2, and the rest.
 template <typename F>
-static int by_lanes(int experts, F f) {
+static int by_shape(int experts, int topk, F f) {
+    const auto with = [&](auto g) {
+        return topk <= 2 ? f(g, std::integral_constant<int, 2>{}) : f(g, std::integral_constant<int, kMaxTopk>{});
+    };
     switch (group_lanes(experts)) {
-        case 1: return f(std::integral_constant<int, 1>{});
-        case 2: return f(std::integral_constant<int, 2>{});
-        case 4: return f(std::integral_constant<int, 4>{});
-        default: return f(std::integral_constant<int, 8>{});
+        case 1: return with(std::integral_constant<int, 1>{});
+        case 2: return with(std::integral_constant<int, 2>{});
+        case 4: return with(std::integral_constant<int, 4>{});
+        default: return with(std::integral_constant<int, 8>{});
     }
 }
 
@@ -377,8 +393,8 @@ int launch_router_loss(const float* logits, const float* bias, const int32_t* id
                        int32_t* stats, float* records, int64_t tokens, int experts, int topk, hipStream_t stream) {
     const int blocks = token_blocks(tokens, experts);
     const LossOut out{losses, stats};
-    int rc = by_lanes(experts, [&](auto g) {
-        hipLaunchKernelGGL(router_loss_kernel<decltype(g)::value>, dim3(blocks), dim3(256), 0, stream, logits, bias, ids,
+    int rc = by_shape(experts, topk, [&](auto g, auto k) {
+        hipLaunchKernelGGL((router_loss_kernel<decltype(g)::value, decltype(k)::value>), dim3(blocks), dim3(256), 0, stream, logits, bias, ids,
                            mask, tokens, experts, topk, records, out);
         return check_launch("router_loss_kernel");
     });
@@ -400,8 +416,8 @@ int launch_router_logits_grad(const float* logits, const float* bias, const int3
         sums->rows = blocks == 1 ? 0 : blocks;
         sums->columns = experts;
     }
-    return by_lanes(experts, [&](auto g) {
-        hipLaunchKernelGGL(router_logits_grad_kernel<decltype(g)::value>, dim3(blocks), dim3(256), 0, stream, logits,
+    return by_shape(experts, topk, [&](auto g, auto k) {
+        hipLaunchKernelGGL((router_logits_grad_kernel<decltype(g)::value, decltype(k)::value>), dim3(blocks), dim3(256), 0, stream, logits,
                            bias, ids, mask, stats, grad_losses, grad_weights, tokens, experts, topk, grad_logits, part);
         return check_launch("router_logits_grad_kernel");
     });
