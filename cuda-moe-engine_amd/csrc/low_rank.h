@@ -11,6 +11,10 @@ constexpr int kMaxRank = 128;
 constexpr int64_t kMaxAdapterTokens = 1 << 21;  // tiles and adapters within a grid's 65535
 constexpr int64_t kMaxLowRankWidth = 1 << 20;
 constexpr int kTileRows = 64;     // rows of one adapter per tile (contract, spread)
+// Rows per tile of one group of more than 32 ranks (the router's experts): their fp32
+// weights are taken apart into bf16 parts once a tile.
+constexpr int kWideTileRows = 128;
+inline int group_tile_rows(int64_t rank) { return rank > 32 ? kWideTileRows : kTileRows; }
 constexpr int kOuterCols = 128;   // columns per workgroup of outer
 constexpr int kMaxSplitRows = 1024;
 
@@ -84,7 +88,8 @@ inline Groups one_group(int64_t tokens, int64_t width, int64_t rank) {
     const int64_t most = rank > 32 ? 256 : 512;
     g.split_rows = 128;
     while (g.split_rows < kMaxSplitRows && tokens * columns > g.split_rows * most) g.split_rows <<= 1;
-    g.tile_bound = static_cast<int>((tokens + kTileRows - 1) / kTileRows);
+    const int rows = group_tile_rows(rank);
+    g.tile_bound = static_cast<int>((tokens + rows - 1) / rows);
     g.split_bound = static_cast<int>((tokens + g.split_rows - 1) / g.split_rows);
     return g;
 }

@@ -401,8 +401,8 @@ __device__ __forceinline__ void transpose8(const V (&v)[8], u32x4_t (&b)[N]) {
 // NK: 32-rank chunks. HALF (r <= 16): one chunk whose k 0-15 are h's first parts and
 // 16-31 the rests, w's rows twice. W32: w is fp32, taken as two bf16 parts as well
 // (the product of the two rests, below 2^-32 of the term, is left out). A workgroup takes
-// `fragments` 16-row fragments of a tile, blockIdx.z the first: 4, or 1 where whole tiles
-// would leave CUs idle. base's rows are on their way one fragment ahead.
+// `fragments` 16-row fragments of a tile, blockIdx.z the first: the whole tile, or 1 where
+// whole tiles would leave CUs idle. base's rows are on their way one fragment ahead.
 // COLS: columns a lane, 8, or 4 where w's operands for 8 would leave a SIMD one wave
 // (r > 32, fp32 w).
 template <int NK, bool HALF, bool W32, int COLS>
@@ -412,14 +412,15 @@ __global__ __launch_bounds__(256, NK == 1 && !W32 ? 3 : 1) void spread_kernel(co
                                                      int64_t width, int rank, int fragments, int columns) {
     constexpr int KP = 32 * NK + 8;  // 16-byte rows, off the banks' period
     constexpr int C = HALF ? 16 : 32 * NK;
-    __shared__ __attribute__((aligned(16))) uint16_t hi[kTileRows * KP];
-    __shared__ __attribute__((aligned(16))) uint16_t lo[HALF ? 8 : kTileRows * KP];
-    __shared__ int32_t row_of[kTileRows];
+    constexpr int R = W32 && NK == 2 ? kWideTileRows : kTileRows;
+    __shared__ __attribute__((aligned(16))) uint16_t hi[R * KP];
+    __shared__ __attribute__((aligned(16))) uint16_t lo[HALF ? 8 : R * KP];
+    __shared__ int32_t row_of[R];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int l = lane & 15, g = lane >> 4;
     int chunk, at_tile;
     if (!part_of(columns, gr.tile_bound, &chunk, &at_tile)) return;
-    int adapter = 0, first = at_tile * kTileRows, rows;
+    int adapter = 0, first = at_tile * R, rows;
     if (gr.order) {
         const int4 tile = gr.tiles[at_tile];
         if (at_tile >= gr.head[0]) return;
@@ -427,7 +428,7 @@ __global__ __launch_bounds__(256, NK == 1 && !W32 ? 3 : 1) void spread_kernel(co
         first = tile.y;
         rows = tile.z;
     } else {
-        rows = static_cast<int>(min(static_cast<int64_t>(kTileRows), tokens - first));
+        rows = static_cast<int>(min(static_cast<int64_t>(R), tokens - first));
     }
     first += 16 * fragments * blockIdx.z;
     rows = min(rows - static_cast<int>(16 * fragments * blockIdx.z), 16 * fragments);
@@ -623,8 +624,9 @@ int launch_spread(const float* partials, int slices, const void* w, bool w32, co
         // Without out: h_out alone.
         const int columns = out ? static_cast<int>((width + 64 * cols - 1) / (64 * cols)) : 1;
         const int64_t parts = static_cast<int64_t>(g.tile_bound) * columns;
-        const int fragments = parts > 256 ? 4 : 1;
-        hipLaunchKernelGGL(kernel, dim3(part_grid(columns, g.tile_bound), 1, 4 / fragments), dim3(256), 0, stream,
+        const int whole = g.order ? kTileRows / 16 : group_tile_rows(rank) / 16;
+        const int fragments = parts > 256 ? whole : 1;
+        hipLaunchKernelGGL(kernel, dim3(part_grid(columns, g.tile_bound), 1, whole / fragments), dim3(256), 0, stream,
                            partials, slices, w, scales, g, base, out, h_out, tokens, width, rank, fragments, columns);
         return check_launch("spread_kernel");
     };
