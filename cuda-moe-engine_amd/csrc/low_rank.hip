@@ -48,7 +48,8 @@ __device__ __forceinline__ int group_of(int id, int adapters) {
     return static_cast<unsigned>(id) < static_cast<unsigned>(adapters) ? id : adapters;
 }
 
-// The rows of group a, in order, to order[pos...]; `ids(i)` is row i's group.
+// The rows of group a, in order, to order[pos...end); `ids(i)` is row i's group. Never past
+// end, whatever the ids have become since they were counted.
 template <typename F>
 __device__ __forceinline__ void collect_rows(int a, int pos, int end, int tokens, int lane, int32_t* order, F ids) {
     constexpr int U = 4;
@@ -62,7 +63,8 @@ __device__ __forceinline__ void collect_rows(int a, int pos, int end, int tokens
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const uint64_t found = __ballot(group[u] == a);
-            if (group[u] == a) order[pos + __popcll(found & ((1ull << lane) - 1))] = base + 64 * u + lane;
+            const int at = pos + __popcll(found & ((1ull << lane) - 1));
+            if (group[u] == a && at < end) order[at] = base + 64 * u + lane;
             pos += __popcll(found);
         }
     }
@@ -185,12 +187,12 @@ int launch_adapter_group(const int32_t* ids, void* table, int64_t tokens, int ad
 // contract: h[i][c] = sum_k x[i][k] w[c][k].
 // A workgroup takes a tile of up to 64 rows of one adapter and a slice of k. A wave takes
 // 16 rows and the slice, or for r > 32, where w's lines are the more, 32 rows and half of
-// it; with fewer rows in the tile more waves share them and split the slice. Eight lanes load a 128-byte line of a row, D
-// steps of 64 k ahead, and the wave turns the step over in LDS of its own into the MFMA's
-// operands (lane l: row l % 16, 8 k from 8 (l / 16); k is permuted inside 64). Loaded as
-// operands, neighbouring lanes hold different rows and each 16 bytes is a line of its own
-// to the L1: T=4096, H=4096, r=16 and 64 took 17.2 and 38.6 us, 12.1 and 16.8 now.
-// Rows past the tile and ranks past r are read from the last one and not stored (an output
+// it; with fewer rows in the tile more waves share them and split the slice. Eight lanes
+// load a 128-byte line of a row, D steps of 64 k ahead, and the wave turns the step over
+// in LDS of its own into the MFMA's operands (lane l: row l % 16, 8 k from 8 (l / 16); k is
+// permuted inside 64). Loaded as operands, neighbouring lanes hold different rows and each
+// 16 bytes is a line of its own to the L1: T=4096, H=4096, r=16 and 64 took 17.2 and 38.6
+// us, 11.5 and 15.0 now (a plain reduction of rows that come from HBM takes 11.3). Rows past the tile and ranks past r are read from the last one and not stored (an output
 // depends on its own row and rank alone). Waves on one row meet in LDS, slices in the
 // consumer, both in order.
 // ---------------------------------------------------------------------------

@@ -260,6 +260,43 @@ def test_same_every_time_on_streams_and_under_replay(tokens, adapters):
             assert torch.equal(a, b), round_
 
 
+def test_two_streams_share_the_groups():
+    """Calls that only read the groups may run at once: their sums are their own."""
+    case = _case(2000, 512, 1024, 16, 5)
+    operands = (case["x"], case["down"], case["up"], case["groups"])
+    want, kept = low_rank_add(case["base"], *operands, return_hidden=True)
+    grads = low_rank_backward(case["grad"], *operands, hidden=kept)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    results = []
+    for stream in streams:
+        stream.wait_stream(torch.cuda.current_stream())
+    for _ in range(4):
+        for stream in streams:
+            with torch.cuda.stream(stream):
+                y, h = low_rank_add(case["base"], *operands, return_hidden=True)
+                results.append((y,) + low_rank_backward(case["grad"], *operands, hidden=h))
+    for stream in streams:
+        torch.cuda.current_stream().wait_stream(stream)
+    for result in results:
+        for a, b in zip(result, (want,) + grads):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("tokens,hidden,width,rank", [(40, 4096, 1000, 16), (40, 2056, 1000, 32), (300, 2048, 2048, 32),
+                                                      (16, 4104, 256, 16), (600, 64, 64, 33)])
+def test_where_one_launch_ends(tokens, hidden, width, rank):
+    """Sizes on either side of the rule that fuses the two products."""
+    case = _case(tokens, hidden, width, rank, 3, "runs")
+    ref = _reference(case)
+    operands = (case["x"], case["down"], case["up"], case["groups"])
+    y, kept = low_rank_add(case["base"], *operands, scales=case["scales"], return_hidden=True)
+    _check(y, ref["y"], "y")
+    dx, gd, gu = low_rank_backward(case["grad"], *operands, scales=case["scales"], hidden=kept, grad_x=case["grad_x"])
+    _check(dx, ref["dx"], "grad_x")
+    _check(gd, ref["gd"], "grad_down", U)
+    _check(gu, ref["gu"], "grad_up", U)
+
+
 def test_gradients_against_differences():
     """The 64-bit forward in random directions of x, down and up."""
     case = _case(60, 64, 72, 8, 3)

@@ -180,6 +180,55 @@ def test_disabled_experts_and_empty_rows():
     _within(got, ref["dv"], _logits_tolerance(ref), "dv")
 
 
+def test_the_lowest_value_masks_like_infinity():
+    """Logits masked with the type's lowest value give what -inf gives, bit for bit."""
+    results = []
+    for value in (torch.finfo(torch.float32).min, -float("inf")):
+        case = _router_case(200, 16, 2, 16)
+        case["logits"][:, 3] = value
+        case["logits"][5:50, 8:] = value
+        case["bias"] = None
+        case["ids"] = torch.topk(case["logits"], 2, dim=-1).indices.int().contiguous()
+        loss = router_loss(case["logits"], case["ids"])
+        results.append((loss.losses, loss.stats, route_logits_backward(
+            case["logits"], case["ids"], loss=loss, grad_losses=case["grad_losses"], grad_weights=case["grad_weights"])))
+    for a, b in zip(*results):
+        assert torch.equal(a, b) and torch.isfinite(a).all()
+
+
+def test_an_expert_chosen_twice():
+    """Ids of a program's own router may name an expert twice: both terms count."""
+    case = _router_case(300, 12, 4, 14)
+    case["ids"] = torch.randint(0, 12, (300, 4), device="cuda", dtype=torch.int32)
+    args = (case["logits"], case["ids"], case["bias"])
+    loss = router_loss(*args)
+    ref = _reference(case)
+    _check_losses(loss, ref, 300)
+    got = route_logits_backward(*args, loss=loss, grad_losses=case["grad_losses"], grad_weights=case["grad_weights"])
+    _within(got, ref["dv"], _logits_tolerance(ref), "dv")
+
+
+@pytest.mark.parametrize("tokens", [100, 3000])
+def test_each_gradient_alone(tokens):
+    """Through the C entry any gradient may be left out; the others stay the same."""
+    case = _router_case(tokens, 16, 2, 15, hidden=64)
+    args = (case["x"], case["w"], case["logits"], case["ids"], case["bias"])
+    full = route_backward(*args, grad_weights=case["grad_weights"], grad_x=case["grad_x"])
+    lib = get_extension().lib
+    need = lib.moe_route_backward_scratch_bytes(tokens, 64, 16)
+    scratch = torch.empty(need, device="cuda", dtype=torch.uint8)
+    # The entry takes the bias before the ids.
+    inputs = [case[name].data_ptr() for name in ("x", "w", "logits", "bias", "ids")]
+    for wanted in range(3):
+        out = torch.full_like(full[wanted], 7.0)
+        outs = [None, None, None]
+        outs[wanted] = out.data_ptr()
+        lib.check(lib.moe_route_backward(
+            *inputs, None, None, None, case["grad_weights"].data_ptr(), case["grad_x"].data_ptr(),
+            *outs, scratch.data_ptr(), need, tokens, 64, 16, 2, torch.cuda.current_stream().cuda_stream), "route")
+        assert torch.equal(out, full[wanted])
+
+
 def test_nan_and_infinite_logits_show():
     case = _router_case(64, 8, 2, 5)
     for value in (float("nan"), float("inf")):
@@ -245,7 +294,7 @@ def _check_route_backward(case, tokens, experts, topk, hidden):
 
 @pytest.mark.parametrize("tokens,hidden,experts,topk", [
     (1, 8, 1, 1), (1, 4096, 8, 2), (3, 72, 5, 2), (63, 512, 8, 2), (64, 1000, 12, 3), (65, 136, 16, 4), (129, 256, 17, 2),
-    (300, 2048, 32, 4), (777, 1000, 33, 3), (2049, 520, 64, 6), (5000, 128, 64, 8)])
+    (300, 2048, 32, 4), (777, 1000, 33, 3), (2049, 520, 64, 6), (5000, 128, 64, 8), (1100, 65536, 8, 2)])
 def test_route_backward(tokens, hidden, experts, topk):
     case = _router_case(tokens, experts, topk, tokens * 7 + experts, masked=tokens > 100, hidden=hidden)
     first = _check_route_backward(case, tokens, experts, topk, hidden)
