@@ -403,8 +403,8 @@ __device__ __forceinline__ void transpose8(const V (&v)[8], u32x4_t (&b)[N]) {
 // NK: 32-rank chunks. HALF (r <= 16): one chunk whose k 0-15 are h's first parts and
 // 16-31 the rests, w's rows twice. W32: w is fp32, taken as two bf16 parts as well
 // (the product of the two rests, below 2^-32 of the term, is left out). A workgroup takes
-// `fragments` 16-row fragments of a tile, blockIdx.z the first: the whole tile, or 1 where
-// whole tiles would leave CUs idle. base's rows are on their way one fragment ahead.
+// `fragments` 16-row fragments of a tile, blockIdx.z the first: the whole tile, or 2 or 1
+// where whole tiles would leave CUs idle. base's rows are on their way one fragment ahead.
 // COLS: columns a lane, 8, or 4 where w's operands for 8 would leave a SIMD one wave
 // (r > 32, fp32 w).
 template <int NK, bool HALF, bool W32, int COLS>
@@ -627,7 +627,10 @@ int launch_spread(const float* partials, int slices, const void* w, bool w32, co
         const int columns = out ? static_cast<int>((width + 64 * cols - 1) / (64 * cols)) : 1;
         const int64_t parts = static_cast<int64_t>(g.tile_bound) * columns;
         const int whole = g.order ? kTileRows / 16 : group_tile_rows(rank) / 16;
-        const int fragments = parts > 256 ? whole : 1;
+        // Whole tiles read w once a tile, parts of them fill the card: 512 rows of 4096
+        // columns at rank 64 (272 parts) 13.6 us with whole tiles, 10.9 with 2; 1024 rows at
+        // rank 16 (200) 10.8 with 1, 8.2 with 2; 256 rows at rank 64 (144) 8.5 and 7.7 with 1.
+        const int fragments = parts > 384 ? whole : parts > 192 ? 2 : 1;
         hipLaunchKernelGGL(kernel, dim3(part_grid(columns, g.tile_bound), 1, whole / fragments), dim3(256), 0, stream,
                            partials, slices, w, scales, g, base, out, h_out, tokens, width, rank, fragments, columns);
         return check_launch("spread_kernel");
