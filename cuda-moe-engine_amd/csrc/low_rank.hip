@@ -440,9 +440,15 @@ __global__ __launch_bounds__(256, NK == 1 && !W32 ? 3 : 1) void spread_kernel(co
     typedef uint32_t cols_t __attribute__((ext_vector_type(COLS / 2)));  // 16-bit columns
     typedef float wide_t __attribute__((ext_vector_type(COLS)));
     const cols_t zero = {};
-    if (tid < rows) row_of[tid] = gr.order ? gr.order[first + tid] : first + tid;
-    // This lane's rows of a fragment, 16 m + 4 g + q, and what base has there; the first
-    // fragment's rows come straight from the table.
+    // What a workgroup asks memory for, in this order and without a wait between but the one
+    // for its first rows' numbers: row numbers, w, base's first rows, h.
+    const auto listed = [&](int r) { return gr.order ? gr.order[first + r] : first + r; };
+    const auto kept = [&](int r) { return row_of[r]; };
+    const int own_row = tid < rows ? listed(tid) : 0;
+    int first_rows[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) first_rows[q] = listed(min(4 * g + q, rows - 1));
+    // This lane's rows of a fragment, 16 m + 4 g + q, and what base has there.
     int64_t at[4];
     cols_t old[4];
     const auto fetch = [&](int m, auto row) {
@@ -451,15 +457,12 @@ __global__ __launch_bounds__(256, NK == 1 && !W32 ? 3 : 1) void spread_kernel(co
 #pragma unroll
         for (int q = 0; q < 4; ++q) old[q] = base && inside ? *reinterpret_cast<const cols_t*>(base + at[q]) : zero;
     };
-    const auto listed = [&](int r) { return gr.order ? gr.order[first + r] : first + r; };
-    const auto kept = [&](int r) { return row_of[r]; };
-    if (out) fetch(0, listed);
     if (adapter < 0) {  // no adapter: h is 0, the base as it is
         if (h_out && chunk == 0)
             for (int i = tid; i < rows * rank; i += 256) h_out[static_cast<int64_t>(first) * rank + i] = 0.0f;
         if (base == out || !out || !inside) return;
         for (int m = 0; 16 * m < rows; ++m) {
-            if (m > 0) fetch(m, listed);
+            fetch(m, listed);
 #pragma unroll
             for (int q = 0; q < 4; ++q)
                 if (16 * m + 4 * g + q < rows) *reinterpret_cast<cols_t*>(out + at[q]) = old[q];
@@ -485,6 +488,12 @@ __global__ __launch_bounds__(256, NK == 1 && !W32 ? 3 : 1) void spread_kernel(co
             else
                 raw[n][j] = held ? *reinterpret_cast<const cols_t*>(wa + from) : zero;
         }
+    if (out) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) at[q] = first_rows[q] * width + col;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) old[q] = base && inside ? *reinterpret_cast<const cols_t*>(base + at[q]) : zero;
+    }
     // h: the slices' sums as bf16 parts; zero past the rank and past the rows, up to a
     // whole fragment. A thread takes four ranks of a row, U rows and S slices in flight.
     constexpr int Q = C / 4;
@@ -557,6 +566,7 @@ __global__ __launch_bounds__(256, NK == 1 && !W32 ? 3 : 1) void spread_kernel(co
         default: stage(std::integral_constant<int, 8>{}); break;
     }
     if (!out) return;
+    if (tid < rows) row_of[tid] = own_row;
     const float scale = scales ? scales[adapter] : 1.0f;
     __syncthreads();
     const int last = (rows - 1) / 16;
