@@ -342,11 +342,11 @@ __global__ __launch_bounds__(256) void contract_kernel(const uint16_t* __restric
     }
 }
 
-// Up to about 600 workgroups; past 64 ranks, where spread reads each slice's sums again
+// Up to about 600 workgroups; past 32 ranks, where spread reads each slice's sums again
 // for every 256 columns, 512 (contract and spread of 8192 x 4096 to 4096, rank 16: 46.9 us,
-// with 512 50.5; of 16384 rows, rank 128: 168 and 158).
+// with 512 50.5; of 4096 rows, rank 64: 43.8 and 40.0; of 16384, rank 128: 168 and 158).
 int contract_slices(int tile_bound, int64_t k, int64_t rank) {
-    const int64_t most = (k + 255) / 256, workgroups = rank <= 64 ? 600 : 512;
+    const int64_t most = (k + 255) / 256, workgroups = rank <= 32 ? 600 : 512;
     int64_t s = 1;
     while (s < 16 && s * 2 <= most && s * 2 * tile_bound <= workgroups) s <<= 1;
     return static_cast<int>(s);
