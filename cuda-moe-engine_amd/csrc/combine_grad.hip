@@ -4,9 +4,13 @@
 //
 // One pass: a wave takes a token, reads its dout row once, and each of its K expert rows
 // once, writing the row's gradient and keeping K running sums in fp32; the lanes' sums
-// meet by shuffles in one order. Bound by the bytes: K rows read and K written a token.
+// meet by shuffles in one order. Bound by the bytes: K rows read and K written a token
+// (4096 tokens, top-2, rows of 2048 bf16: 84 MB in 17.5 us beside the dispatch's gradient,
+// 14.6 alone, 5.7 TB/s). Four rows in flight a lane instead of two took 22.1 us.
 // Every packed row that holds no assignment gets a zero gradient, so that a program's
-// expert backward may run over whole spans.
+// expert backward may run over whole spans; with 64 experts and spans of 128 rows that is
+// half of the rows (8192 assignments of 4096 in 16384 rows: 155 us with two bytes a lane
+// and 64 blocks, 59 with 16 bytes, 55 with 256 blocks).
 #include <algorithm>
 
 #include "moe_common.h"
@@ -36,8 +40,13 @@ __global__ __launch_bounds__(256) void combine_grad_kernel(
         for (int e = 0; e <= experts; ++e) {
             const int64_t from = e < experts ? __shfl(lane_from, e) : end;
             const int64_t to = e < experts ? __shfl(lane_to, e) : rows;
-            for (int64_t r = (from > 0 ? from : 0) + self; r < to && r < rows; r += waves)
-                for (int64_t j = lane; j < hidden; j += 64) grad_y[r * hidden + j] = Elem<DT>::store(0.0f);
+            for (int64_t r = (from > 0 ? from : 0) + self; r < to && r < rows; r += waves) {
+                T* dst = grad_y + r * hidden;
+                const V zeros = {};
+                for (int64_t v = lane; v < hidden / VE; v += 64) *reinterpret_cast<V*>(dst + v * VE) = zeros;
+                const int64_t j = hidden / VE * VE + lane;
+                if (j < hidden) dst[j] = Elem<DT>::store(0.0f);
+            }
         }
         return;
     }
@@ -103,7 +112,7 @@ static int combine_grad_typed(const void* grad_output, const void* y, const int3
     const int64_t token_blocks = (tokens + 3) / 4;
     const int64_t spare = rows - tokens * topk;
     // One block also where every row should be taken: ids out of range leave some free.
-    const int64_t pad_blocks = std::clamp<int64_t>((spare + 3) / 4, 1, 64);
+    const int64_t pad_blocks = std::clamp<int64_t>((spare + 3) / 4, 1, 256);
     const auto run = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(token_blocks + pad_blocks)), dim3(256), 0, stream,
                            static_cast<const T*>(grad_output), static_cast<const T*>(y), inverse, weights, counts,
