@@ -63,6 +63,7 @@ struct Groups {
     const int4* tiles = nullptr;
     const int4* splits = nullptr;
     int tile_bound = 0, split_bound = 0, split_rows = 0;
+    const uint8_t* mask = nullptr;  // one group: outer reads no row of x whose byte is 0
 };
 
 inline Groups groups_of(const void* table, int64_t tokens, int64_t adapters) {

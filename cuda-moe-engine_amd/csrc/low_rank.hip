@@ -402,7 +402,7 @@ __device__ __forceinline__ void transpose8(const V (&v)[8], u32x4_t (&b)[N]) {
 
 // NK: 32-rank chunks. HALF (r <= 16): one chunk whose k 0-15 are h's first parts and
 // 16-31 the rests, w's rows twice. W32: w is fp32, taken as two bf16 parts as well
-// (the product of the two rests, below 2^-32 of the term, is left out). A workgroup takes
+// (the product of the two rests, below 2^-16 of the term, is left out). A workgroup takes
 // `fragments` 16-row fragments of a tile, blockIdx.z the first: the whole tile, or 2 or 1
 // where whole tiles would leave CUs idle. base's rows are on their way one fragment ahead.
 // COLS: columns a lane, 8, or 4 where w's operands for 8 would leave a SIMD one wave
@@ -928,7 +928,9 @@ __global__ __launch_bounds__(64 * W) void outer_kernel(OuterJobs jobs, const flo
     } else {
         rows = static_cast<int>(min(static_cast<int64_t>(gr.split_rows), tokens - first));
     }
-    for (int i = tid; i < rows; i += 64 * W) row_of[i] = gr.order ? gr.order[first + i] : first + i;
+    // -1: a masked row, which may hold anything (its h is 0, and 0 times NaN is not).
+    for (int i = tid; i < rows; i += 64 * W)
+        row_of[i] = gr.order ? gr.order[first + i] : gr.mask && !gr.mask[first + i] ? -1 : first + i;
     const int64_t col = static_cast<int64_t>(part_column) * kOuterCols + 8 * l;
     const bool inside = col < width;
     const int c0 = wave % RG * 16 * NR;
@@ -945,7 +947,8 @@ __global__ __launch_bounds__(64 * W) void outer_kernel(OuterJobs jobs, const flo
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const int i = t0 + 8 * g + j;
-            v[j] = i < rows && inside ? load16(job.x + row_of[i] * width + col) : zero;
+            const int row = i < rows ? row_of[i] : -1;
+            v[j] = row >= 0 && inside ? load16(job.x + row * width + col) : zero;
 #pragma unroll
             for (int n = 0; n < NR; ++n) {
                 const int c = c0 + 16 * n + l;

@@ -441,7 +441,8 @@ int launch_route_backward(const uint16_t* x, const float* router_w, const float*
     float* bias_part = reinterpret_cast<float*>(scratch + aligned16(tokens * experts * 4));
     float* partials = reinterpret_cast<float*>(scratch + aligned16(tokens * experts * 4) +
                                                aligned16(static_cast<int64_t>(kLossBlocks) * experts * 4));
-    const Groups g = one_group(tokens, hidden, experts);
+    Groups g = one_group(tokens, hidden, experts);
+    g.mask = mask;
     ColumnSums sums;
     sums.part = bias_part;
     sums.out = grad_bias;

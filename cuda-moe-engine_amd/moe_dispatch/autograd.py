@@ -27,6 +27,13 @@ def _eager_only():
                            "moe_dispatch.adapters instead")
 
 
+def _rows(grad):
+    """A gradient as the kernels take it: contiguous, and 16-byte aligned where it was cut
+    out of a larger one."""
+    grad = grad.contiguous()
+    return grad if grad.data_ptr() % 16 == 0 else grad.clone()
+
+
 class Routed(NamedTuple):
     """``weights`` fp32 [T, K] and ``losses`` fp32 [2] (balance, z) carry gradients;
     ``ids`` int32 [T, K], ``counts`` int32 [E] do not."""
@@ -48,11 +55,10 @@ class _Route(torch.autograd.Function):
         with _training.on_device(x.device):
             get_extension().router_fused_out(x, router_weight, bias, ids, None, weights, logits=logits)
         loss = _training.router_loss(logits, ids, bias, mask=mask)
-        ctx.save_for_backward(x, router_weight, bias, logits, ids, loss.losses, loss.stats)
-        ctx.mask = mask
+        ctx.save_for_backward(x, router_weight, bias, logits, ids, mask, loss.stats)
         ctx.mark_non_differentiable(ids, loss.stats)
         ctx.set_materialize_grads(False)
-        return weights, loss.losses.clone(), ids, loss.stats
+        return weights, loss.losses, ids, loss.stats
 
     @staticmethod
     @once_differentiable
@@ -60,12 +66,13 @@ class _Route(torch.autograd.Function):
         _eager_only()
         if grad_weights is None and grad_losses is None:
             return None, None, None, None, None
-        x, router_weight, bias, logits, ids, losses, stats = ctx.saved_tensors
+        x, router_weight, bias, logits, ids, mask, stats = ctx.saved_tensors
         grads = _training.route_backward(
-            x, router_weight, logits, ids, bias, mask=ctx.mask, loss=_training.RouterLoss(losses, stats),
+            x, router_weight, logits, ids, bias, mask=mask, loss=_training.RouterLoss(None, stats),
             grad_losses=None if grad_losses is None else grad_losses.contiguous(),
-            grad_weights=None if grad_weights is None else grad_weights.contiguous())
-        return (*(g if need else None for g, need in zip(grads, ctx.needs_input_grad)), None, None)
+            grad_weights=None if grad_weights is None else grad_weights.contiguous(),
+            gradients=ctx.needs_input_grad[:3])
+        return (*grads, None, None)
 
 
 def route(x, router_weight, bias, topk, *, mask=None):
@@ -163,7 +170,7 @@ class _LowRankAdd(torch.autograd.Function):
         grads = None, None, None
         if need_x or need_down or need_up:
             hidden = _adapters.LowRankHidden(values, ctx.groups, ctx.assignment)
-            grads = _adapters.low_rank_backward(grad_output.contiguous(), x, down, up, ctx.groups, scales=scales,
+            grads = _adapters.low_rank_backward(_rows(grad_output), x, down, up, ctx.groups, scales=scales,
                                                 hidden=hidden, grad_dtype=down.dtype,
                                                 gradients=(need_x, need_down, need_up))
         return (grad_output if ctx.needs_input_grad[0] else None, *grads, None, None)

@@ -196,13 +196,14 @@ def route_logits_backward(logits, expert_ids, bias=None, *, mask=None, loss=None
 
 
 def route_backward(x, router_weight, logits, expert_ids, bias=None, *, mask=None, loss=None, grad_losses=None,
-                   grad_weights=None, grad_x=None):
+                   grad_weights=None, grad_x=None, gradients=(True, True, True)):
     """Gradients of x, router weight and bias: ``(grad_x, grad_router_weight, grad_bias)``.
 
     x bf16 [T, H] and router_weight fp32 [E, H] are the router's inputs (H a multiple of 8),
     the rest is ``route_logits_backward``'s. ``grad_x`` bf16 [T, H] is x's gradient along its
     other paths: the result is the sum, rounded once. grad_router_weight [E, H] and grad_bias
-    [E] are fp32.
+    [E] are fp32. A masked token's row of x is not read. ``gradients``: which of the three
+    are wanted; the others are None and cost nothing.
     """
     tokens, experts, topk, device = _check_routed(logits, expert_ids, bias, mask)
     _check_gradients(logits, expert_ids, loss, grad_losses, grad_weights)
@@ -217,11 +218,15 @@ def route_backward(x, router_weight, logits, expert_ids, bias=None, *, mask=None
     refuse_autograd(x, router_weight, logits, bias, grad_losses, grad_weights, grad_x)
     lib = get_extension().lib
     with on_device(device):
+        want_x, want_weight, want_bias = gradients
+        out_x = torch.empty_like(x) if want_x else None
+        grad_router_weight = torch.empty_like(router_weight) if want_weight else None
+        grad_bias = logits.new_empty(experts) if want_bias else None
         if tokens == 0:
-            return torch.empty_like(x), torch.zeros_like(router_weight), torch.zeros(experts, device=device)
-        out_x = torch.empty_like(x)
-        grad_router_weight = torch.empty_like(router_weight)
-        grad_bias = logits.new_empty(experts)
+            for t in (grad_router_weight, grad_bias):
+                if t is not None:
+                    t.zero_()
+            return out_x, grad_router_weight, grad_bias
         need = _route_scratch_bytes(tokens, hidden, experts)
         if need < 0:
             raise ValueError("route_backward takes up to 2^21 tokens")
@@ -229,7 +234,7 @@ def route_backward(x, router_weight, logits, expert_ids, bias=None, *, mask=None
         lib.check(lib.moe_route_backward(
             x.data_ptr(), router_weight.data_ptr(), logits.data_ptr(), _ptr(bias), expert_ids.data_ptr(), _ptr(mask),
             loss.stats.data_ptr() if loss is not None else None, _ptr(grad_losses), _ptr(grad_weights), _ptr(grad_x),
-            out_x.data_ptr(), grad_router_weight.data_ptr(), grad_bias.data_ptr(), scratch.data_ptr(), need, tokens,
+            _ptr(out_x), _ptr(grad_router_weight), _ptr(grad_bias), scratch.data_ptr(), need, tokens,
             hidden, experts, topk, current_stream_handle(device.index)), "route_backward")
     return out_x, grad_router_weight, grad_bias
 

@@ -446,8 +446,9 @@ int64_t moe_route_backward_scratch_bytes(int64_t tokens, int64_t hidden, int64_t
  *            it may be grad_x itself)
  *   grad_router_w = dv^T . x  (fp32 [E, H]),  grad_bias = sum_t dv  (fp32 [E])
  * Any of the three may be NULL. Products of dv and x are exact and accumulate in fp32;
- * dv and router_w enter grad_x as two bf16 parts each (16 bits). Requires hidden % 8 == 0
- * and 16-byte aligned rows.
+ * dv and router_w enter grad_x as two bf16 parts each (16 bits). A masked token's row of x
+ * is not read and may hold anything; an infinite x of a valid one makes NaN, not infinity, of
+ * sums it enters. grad_x must not overlap x. Requires hidden % 8 == 0 and 16-byte aligned rows.
  */
 int moe_route_backward(const void* x, const float* router_w, const float* logits, const float* bias,
                        const int32_t* ids, const uint8_t* mask, const int32_t* stats, const float* grad_losses,
@@ -500,7 +501,9 @@ int64_t moe_low_rank_scratch_bytes(int64_t tokens, int64_t hidden, int64_t width
  * scales fp32 [N] (NULL: 1). base may be NULL (0) or output itself; output must not
  * overlap x. down . x is summed in fp32, written to hidden_out (fp32 [T, rank], in the
  * table's row order, unscaled, 0 for a row of no adapter) unless that is NULL, and enters
- * the second product as two bf16 parts (16 bits). An adapter of lower rank is padded with zero rows.
+ * the second product as two bf16 parts (16 bits); an infinite up makes NaN, not infinity. Rows
+ * of no adapter (padding among them) are read from base alone. An adapter of lower rank is
+ * padded with zero rows.
  * Limits: hidden and width multiples of 8 up to 2^20, 1 <= rank <= 128; rows 16-byte aligned.
  */
 int moe_low_rank_add(const void* x, const void* down, const void* up, const float* scales, const void* table,

@@ -52,6 +52,26 @@ def test_low_rank_add_gradients():
         y.backward(dy)
 
 
+def test_gradients_cut_out_of_a_larger_one():
+    """A result joined with others behind an odd number of elements: its gradient starts there."""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    groups = AdapterGroups(20, 2)
+    groups.assign(torch.zeros(20, device="cuda", dtype=torch.int32))
+    operands = [_normal(g, 20, 64), _normal(g, 2, 4, 64), _normal(g, 2, 4, 16)]
+    head, dy = _normal(g, 3), _normal(g, 320)
+    grads = []
+    for cut in (True, False):
+        leaves = [t.clone().requires_grad_() for t in operands]
+        y = autograd.low_rank_add(None, *leaves, groups)
+        if cut:
+            torch.cat((head, y.reshape(-1))).backward(torch.cat((head, dy)))
+        else:
+            y.backward(dy.reshape(20, 16))
+        grads.append([leaf.grad for leaf in leaves])
+    for a, b in zip(*grads):
+        assert torch.equal(a, b)
+
+
 def test_two_micro_batches_in_flight():
     """Forward twice, then backward twice: no call disturbs what another kept."""
     g = torch.Generator(device="cuda").manual_seed(1)

@@ -163,6 +163,35 @@ def test_masked_tokens_are_not_read():
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("tokens,experts", [(1, 4), (200, 16), (3000, 64)])
+def test_masked_rows_of_x_reach_nothing(tokens, experts):
+    """Padding tokens' activations may be anything: their gradients are 0, and 0 times NaN is not."""
+    case = _router_case(tokens, experts, 2, 21, masked=True, hidden=136)
+    if tokens == 1:
+        case["mask"][0] = False
+    args = (case["logits"], case["ids"], case["bias"])
+    loss = router_loss(*args, mask=case["mask"])
+    dirty = case["x"].clone()
+    dirty[~case["mask"]] = float("nan")
+    assert dirty.isnan().any()
+    clean, got = (route_backward(x, case["w"], *args, mask=case["mask"], loss=loss, grad_losses=case["grad_losses"],
+                                 grad_weights=case["grad_weights"], grad_x=case["grad_x"]) for x in (case["x"], dirty))
+    for a, b in zip(got, clean):
+        assert torch.equal(a, b)
+
+
+def test_gradients_not_wanted():
+    for tokens in (0, 100):
+        case = _router_case(tokens, 8, 2, 22, hidden=64)
+        args = (case["x"], case["w"], case["logits"], case["ids"], case["bias"])
+        full = route_backward(*args, grad_weights=case["grad_weights"])
+        for wanted in range(8):
+            flags = tuple(bool(wanted >> i & 1) for i in range(3))
+            got = route_backward(*args, grad_weights=case["grad_weights"], gradients=flags)
+            for flag, a, b in zip(flags, got, full):
+                assert torch.equal(a, b) if flag else a is None
+
+
 def test_disabled_experts_and_empty_rows():
     """-inf logits (disabled experts; a token with none left) and ids that were not routed."""
     case = _router_case(150, 8, 3, 4)
@@ -367,6 +396,23 @@ def test_transport_gradients(tokens, hidden, experts, topk, alignment, dtype):
     parts = back.double()[inverse.reshape(-1)].view(tokens, topk, hidden)
     want = parts.sum(1)
     _within(gx, want, want.abs() * _half(dtype) + parts.abs().sum(1) * (topk + 1) * U + tiny, "grad_x")
+
+
+@pytest.mark.parametrize("dtype,hidden", [(torch.bfloat16, 1000), (torch.float32, 1023), (torch.float16, 7)])
+def test_padding_rows_are_zero(dtype, hidden):
+    """64 experts of spans rounded up to 128 rows: most packed rows hold no assignment."""
+    g = torch.Generator(device="cuda").manual_seed(23)
+    tokens, experts = 500, 64
+    x = torch.randn(tokens, hidden, device="cuda", generator=g).to(dtype)
+    ids = torch.randint(0, experts, (tokens, 1), device="cuda", generator=g, dtype=torch.int32)
+    batch = dispatch(x, ids, experts, alignment=128)
+    y = torch.full(batch.packed.shape, float("nan"), device="cuda", dtype=dtype)
+    held = torch.zeros(batch.packed.shape[0], device="cuda", dtype=torch.bool)
+    held[batch.inverse.long().reshape(-1)] = True
+    y[held] = 1.0
+    dy, dw = combine_backward(x, y, batch, torch.ones(tokens, 1, device="cuda"))
+    assert int(held.sum()) == tokens and not dy[~held].any()
+    assert torch.equal(dy[batch.inverse.long().reshape(-1)], x) and dw.isfinite().all()
 
 
 def test_combine_gradient_against_differences():
