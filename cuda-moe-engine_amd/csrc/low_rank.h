@@ -10,6 +10,7 @@ constexpr int kMaxAdapters = 4096;
 constexpr int kMaxRank = 128;
 constexpr int64_t kMaxAdapterTokens = 1 << 21;  // tiles and adapters within a grid's 65535
 constexpr int64_t kMaxLowRankWidth = 1 << 20;
+constexpr int kChunkRows = 4096;  // rows that one workgroup sorts by adapter
 constexpr int kTileRows = 64;     // rows of one adapter per tile (contract, spread)
 // Rows per tile of one group of more than 32 ranks (the router's experts): their fp32
 // weights are taken apart into bf16 parts once a tile.
@@ -25,9 +26,11 @@ constexpr int kMaxSplitRows = 1024;
 //   split_start  [N + 1] first split of each adapter
 //   tiles        [tile_bound]  {adapter (-1: none), first sorted row, rows <= kTileRows, 0}
 //   splits       [split_bound] {adapter, first sorted row, rows <= split_rows, adapter's splits}
+//   chunks       [chunk_count][N + 1]  while it is made, of a batch of more rows than a chunk:
+//                        each chunk's rows of each adapter, then those of the chunks before
 struct TableLayout {
-    int64_t order, starts, split_start, tiles, splits, ints;
-    int tile_bound, split_bound, split_rows;
+    int64_t order, starts, split_start, tiles, splits, chunks, ints;
+    int tile_bound, split_bound, split_rows, chunk_count;
 };
 
 // Rows per split of the outer product: a split's partial result is written and read
@@ -51,7 +54,9 @@ inline TableLayout table_layout(int64_t tokens, int64_t adapters) {
     t.split_start = t.starts + up4(adapters + 2);
     t.tiles = t.split_start + up4(adapters + 1);
     t.splits = t.tiles + 4 * static_cast<int64_t>(t.tile_bound);
-    t.ints = t.splits + 4 * static_cast<int64_t>(t.split_bound);
+    t.chunks = t.splits + 4 * static_cast<int64_t>(t.split_bound);
+    t.chunk_count = tokens > kChunkRows ? static_cast<int>((tokens + kChunkRows - 1) / kChunkRows) : 0;
+    t.ints = t.chunks + up4(t.chunk_count * (adapters + 1));
     return t;
 }
 

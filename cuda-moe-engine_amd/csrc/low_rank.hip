@@ -34,75 +34,91 @@ __device__ __forceinline__ float bf16_rest(float f, uint32_t part) {
     return __builtin_isfinite(rest) ? rest : 0.0f;
 }
 
+// Orders a wave's LDS accesses: what its lanes wrote before is there for all of them after.
+// (A wave's LDS operations complete in order; this keeps the compiler from moving them.)
+__device__ __forceinline__ void wave_lds_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // ---------------------------------------------------------------------------
-// Rows sorted by adapter. One workgroup counts the ids in LDS, scans the counts into
-// starts, and writes the tile and split tables; then a wave per adapter collects its
-// rows in order (ballot ranks: stable, no atomics), in the same launch for up to
-// kGroupSmall rows and in a second one for more. A program groups once a step and uses
-// the table for all its projections.
+// Rows sorted by adapter: a stable counting sort. A wave ranks 64 rows at a time among
+// themselves (a ballot per bit of the group number) and behind its earlier rows (its own
+// counts in LDS), so that no order depends on timing; the waves' counts are then added up
+// in order, the groups scanned, and each row goes to its group's start plus its rank. Up
+// to kChunkRows rows are one launch of one workgroup: latency (4096 rows of 8, 256 and
+// 4096 adapters 7.5, 9.9 and 26 us, where a wave per adapter that looks through all rows
+// took 12, 140 and 910). More rows are counted by chunk, scanned by one workgroup and
+// placed by chunk (65536 rows 15, 18 and 46 us, where one workgroup counting took 190 to
+// 206). A program groups once a step and uses the table for all its projections.
 // ---------------------------------------------------------------------------
 constexpr int kGroupThreads = 1024;
-constexpr int kGroupSmall = 4096;
 
 __device__ __forceinline__ int group_of(int id, int adapters) {
     return static_cast<unsigned>(id) < static_cast<unsigned>(adapters) ? id : adapters;
 }
 
-// The rows of group a, in order, to order[pos...end); `ids(i)` is row i's group. Never past
-// end, whatever the ids have become since they were counted.
-template <typename F>
-__device__ __forceinline__ void collect_rows(int a, int pos, int end, int tokens, int lane, int32_t* order, F ids) {
-    constexpr int U = 4;
-    for (int base = 0; base < tokens && pos < end; base += 64 * U) {
-        int group[U];
+// This wave's rows of a chunk: each one's group and its rank among the wave's rows of that
+// group, group << 16 | rank, and in counts [groups] how many the wave has of each.
+template <int STEPS>
+__device__ __forceinline__ void rank_rows(const int32_t* __restrict__ ids, int first, int tokens, int adapters,
+                                          uint16_t* counts, uint32_t (&ranked)[STEPS]) {
+    const int lane = threadIdx.x & 63;
+    int group[STEPS];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int i = base + 64 * u + lane;
-            group[u] = i < tokens ? ids(i) : -1;
-        }
+    for (int s = 0; s < STEPS; ++s) {
+        const int i = first + 64 * s + lane;
+        group[s] = i < tokens ? group_of(ids[i], adapters) : 0;
+    }
+    for (int a = lane; a <= adapters; a += 64) counts[a] = 0;
+    wave_lds_order();
+    const int bits = 32 - __clz(adapters);  // adapters >= 1: the groups are 0...adapters
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const uint64_t found = __ballot(group[u] == a);
-            const int at = pos + __popcll(found & ((1ull << lane) - 1));
-            if (group[u] == a && at < end) order[at] = base + 64 * u + lane;
-            pos += __popcll(found);
+    for (int s = 0; s < STEPS; ++s) {
+        uint64_t same = __ballot(first + 64 * s + lane < tokens);
+        if (same == 0) break;
+        const bool held = same >> lane & 1;
+        for (int b = 0; b < bits; ++b) {
+            const bool bit = group[s] >> b & 1;
+            const uint64_t plane = __ballot(bit);
+            same &= bit ? plane : ~plane;
         }
+        const int rank = __popcll(same & ((1ull << lane) - 1));
+        const int before = held ? counts[group[s]] : 0;
+        wave_lds_order();
+        if (held && rank == 0) counts[group[s]] = static_cast<uint16_t>(before + __popcll(same));
+        wave_lds_order();
+        ranked[s] = static_cast<uint32_t>(group[s]) << 16 | static_cast<uint32_t>(before + rank);
     }
 }
 
-__global__ __launch_bounds__(kGroupThreads) void adapter_group_kernel(const int32_t* __restrict__ ids,
-                                                                      int32_t* __restrict__ table, TableLayout t,
-                                                                      int tokens, int adapters) {
-    extern __shared__ int32_t lds[];
-    int32_t* counts = lds;                    // [adapters + 1], then the groups' starts
-    int32_t* cached = lds + adapters + 1;     // [tokens] groups of a small batch
+// The waves' counts of a group become what the waves before them have; returns their sum.
+template <int WAVES>
+__device__ __forceinline__ int sum_waves(uint16_t* counts, int groups, int a) {
+    uint16_t n[WAVES];
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) n[w] = counts[w * groups + a];
+    int sum = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+        counts[w * groups + a] = static_cast<uint16_t>(sum);
+        sum += n[w];
+    }
+    return sum;
+}
+
+// start [groups + 1] in LDS: the groups' counts in, their starts out. Returns the first
+// tile and split of the thread's groups.
+__device__ __forceinline__ int2 scan_groups(int32_t* start, const TableLayout& t, int tokens, int groups) {
     __shared__ int32_t wave_sums[3][kGroupThreads / 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const bool small = tokens <= kGroupSmall;
-    for (int i = tid; i <= adapters; i += kGroupThreads) counts[i] = 0;
-    __syncthreads();
-    for (int i = tid; i < tokens; i += kGroupThreads) {
-        const int a = group_of(ids[i], adapters);
-        if (small) cached[i] = a;
-        // Rows of a request are neighbours: one add for a wave of one group.
-        const uint64_t active = __ballot(1);
-        const int first = __builtin_amdgcn_readfirstlane(a);
-        if (__ballot(a == first) == active) {
-            if (lane == __ffsll(static_cast<unsigned long long>(active)) - 1) atomicAdd(&counts[a], __popcll(active));
-        } else {
-            atomicAdd(&counts[a], 1);
-        }
-    }
-    __syncthreads();
-    // Exclusive scans of rows, tiles and splits over the groups; a thread owns `per` neighbours.
-    const int groups = adapters + 1;
     const int per = (groups + kGroupThreads - 1) / kGroupThreads;
     const int g0 = min(tid * per, groups), g1 = min(g0 + per, groups);
     int rows = 0, tiles = 0, splits = 0;
     for (int a = g0; a < g1; ++a) {
-        rows += counts[a];
-        tiles += (counts[a] + kTileRows - 1) / kTileRows;
-        if (a < adapters) splits += (counts[a] + t.split_rows - 1) / t.split_rows;
+        rows += start[a];
+        tiles += (start[a] + kTileRows - 1) / kTileRows;
+        if (a < groups - 1) splits += (start[a] + t.split_rows - 1) / t.split_rows;
     }
     int row_end = rows, tile_end = tiles, split_end = splits;
 #pragma unroll
@@ -125,62 +141,201 @@ __global__ __launch_bounds__(kGroupThreads) void adapter_group_kernel(const int3
         tile_end += wave_sums[1][w];
         split_end += wave_sums[2][w];
     }
-    int row = row_end - rows, tile = tile_end - tiles, split = split_end - splits;
-    int32_t* starts = table + t.starts;
-    int32_t* split_start = table + t.split_start;
-    int4* tile_table = reinterpret_cast<int4*>(table + t.tiles);
-    int4* split_table = reinterpret_cast<int4*>(table + t.splits);
+    int row = row_end - rows;
     for (int a = g0; a < g1; ++a) {
-        const int n = counts[a];
-        const int owner = a < adapters ? a : -1;
-        starts[a] = row;
-        for (int i = 0; i < n; i += kTileRows) tile_table[tile++] = make_int4(owner, row + i, min(kTileRows, n - i), 0);
-        if (a < adapters) {
-            const int parts = (n + t.split_rows - 1) / t.split_rows;
-            split_start[a] = split;
-            for (int i = 0; i < n; i += t.split_rows)
-                split_table[split++] = make_int4(a, row + i, min(t.split_rows, n - i), parts);
-        } else {
-            starts[adapters + 1] = tokens;
-            split_start[adapters] = split;
-            table[0] = tile;
-            table[1] = split;
-            table[2] = table[3] = 0;
-        }
-        counts[a] = row;  // this thread's own entry: its start from here on
+        const int n = start[a];
+        start[a] = row;
         row += n;
     }
-    if (!small) return;
-    __syncthreads();
-    for (int a = wave; a < groups; a += kGroupThreads / 64) {
-        const int end = a < adapters ? counts[a + 1] : tokens;
-        if (counts[a] < end)
-            collect_rows(a, counts[a], end, tokens, lane, table + t.order, [&](int i) { return cached[i]; });
-    }
+    if (tid == 0) start[groups] = tokens;
+    return make_int2(tile_end - tiles, split_end - splits);
 }
 
-__global__ __launch_bounds__(256) void adapter_order_kernel(const int32_t* __restrict__ ids, int32_t* __restrict__ table,
+// The table's parts but the rows, an entry a thread: a tile's or split's group is found in
+// LDS (first_of, twice groups + 1 entries).
+__device__ __forceinline__ void write_table(const int32_t* start, int32_t* first_of, int2 first, int32_t* __restrict__ table,
+                                            const TableLayout& t, int groups) {
+    const int tid = threadIdx.x;
+    const int per = (groups + kGroupThreads - 1) / kGroupThreads;
+    const int g0 = min(tid * per, groups), g1 = min(g0 + per, groups);
+    int32_t *tile_of = first_of, *split_of = first_of + groups + 1;
+    int tile = first.x, split = first.y;
+    for (int a = g0; a < g1; ++a) {
+        const int n = start[a + 1] - start[a];
+        tile_of[a] = tile;
+        split_of[a] = split;
+        tile += (n + kTileRows - 1) / kTileRows;
+        if (a < groups - 1) split += (n + t.split_rows - 1) / t.split_rows;
+        if (a == groups - 1) {
+            tile_of[groups] = tile;
+            split_of[groups] = split;
+        }
+    }
+    __syncthreads();
+    for (int a = tid; a <= groups; a += kGroupThreads) table[t.starts + a] = start[a];
+    for (int a = tid; a < groups; a += kGroupThreads) table[t.split_start + a] = split_of[a];
+    if (tid < 4) table[tid] = tid == 0 ? tile_of[groups] : tid == 1 ? split_of[groups] : 0;
+    const auto write = [&](const int32_t* entries, int rows, int4* to, auto last) {
+        const int count = entries[groups];
+        for (int i = tid; i < count; i += kGroupThreads) {
+            int low = 0, high = groups;  // entries[low] <= i < entries[high]
+            while (high - low > 1) {
+                const int mid = (low + high) / 2;
+                if (entries[mid] <= i)
+                    low = mid;
+                else
+                    high = mid;
+            }
+            const int at = start[low] + (i - entries[low]) * rows;
+            to[i] = make_int4(low < groups - 1 ? low : -1, at, min(rows, start[low + 1] - at),
+                              last(entries[low + 1] - entries[low]));
+        }
+    };
+    write(tile_of, kTileRows, reinterpret_cast<int4*>(table + t.tiles), [](int) { return 0; });
+    write(split_of, t.split_rows, reinterpret_cast<int4*>(table + t.splits), [](int parts) { return parts; });
+}
+
+// All rows of a small batch, ranked by the first WAVES waves.
+template <int WAVES>
+__global__ __launch_bounds__(kGroupThreads) void adapter_group_kernel(const int32_t* __restrict__ ids,
+                                                                      int32_t* __restrict__ table, TableLayout t,
+                                                                      int tokens, int adapters) {
+    constexpr int STEPS = kChunkRows / (64 * WAVES);
+    extern __shared__ int32_t lds[];
+    const int groups = adapters + 1;
+    int32_t* start = lds;                                              // [groups + 1]
+    uint16_t* counts = reinterpret_cast<uint16_t*>(lds + groups + 1);  // [WAVES][groups], then tile_of and split_of
+    const int tid = threadIdx.x, wave = tid >> 6;
+    const int steps = (tokens + 64 * WAVES - 1) / (64 * WAVES), first = wave * 64 * steps;
+    uint32_t ranked[STEPS];
+    if (wave < WAVES)
+        rank_rows<STEPS>(ids, first, min(first + 64 * steps, tokens), adapters, counts + wave * groups, ranked);
+    __syncthreads();
+    for (int a = tid; a < groups; a += kGroupThreads) start[a] = sum_waves<WAVES>(counts, groups, a);
+    __syncthreads();
+    const int2 tables = scan_groups(start, t, tokens, groups);
+    __syncthreads();
+    if (wave < WAVES) {
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            const int i = first + 64 * s + (tid & 63), group = ranked[s] >> 16;
+            if (s < steps && i < tokens)
+                table[t.order + start[group] + counts[wave * groups + group] + (ranked[s] & 0xffff)] = i;
+        }
+    }
+    __syncthreads();
+    write_table(start, reinterpret_cast<int32_t*>(counts), tables, table, t, groups);
+}
+
+// Larger batches: each chunk's counts,
+__global__ __launch_bounds__(256) void adapter_count_kernel(const int32_t* __restrict__ ids, int32_t* __restrict__ table,
                                                             TableLayout t, int tokens, int adapters) {
-    const int a = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (a > adapters) return;
-    const int pos = table[t.starts + a], end = table[t.starts + a + 1];
-    if (pos < end)
-        collect_rows(a, pos, end, tokens, threadIdx.x & 63, table + t.order,
-                     [&](int i) { return group_of(ids[i], adapters); });
+    extern __shared__ int32_t lds[];
+    const int tid = threadIdx.x, groups = adapters + 1;
+    for (int a = tid; a < groups; a += 256) lds[a] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int s = 0; s < kChunkRows / 256; ++s) {
+        const int i = blockIdx.x * kChunkRows + 256 * s + tid;
+        if (i >= tokens) break;
+        // Rows of a request are neighbours: one add for a wave of one group.
+        const int a = group_of(ids[i], adapters);
+        const uint64_t active = __ballot(1);
+        if (__ballot(a == __builtin_amdgcn_readfirstlane(a)) == active) {
+            if ((tid & 63) == 0) atomicAdd(&lds[a], __popcll(active));
+        } else {
+            atomicAdd(&lds[a], 1);
+        }
+    }
+    __syncthreads();
+    for (int a = tid; a < groups; a += 256) table[t.chunks + static_cast<int64_t>(blockIdx.x) * groups + a] = lds[a];
+}
+
+// their sums over the chunks before, the starts and the tables,
+__global__ __launch_bounds__(kGroupThreads) void adapter_scan_kernel(int32_t* __restrict__ table, TableLayout t, int tokens,
+                                                                    int adapters, int chunks) {
+    extern __shared__ int32_t lds[];
+    const int groups = adapters + 1;
+    int32_t *start = lds, *first_of = lds + groups + 1;
+    constexpr int U = 16;  // chunks in flight
+    for (int a = threadIdx.x; a < groups; a += kGroupThreads) {
+        int32_t* count = table + t.chunks + a;
+        int sum = 0;
+        for (int c0 = 0; c0 < chunks; c0 += U) {
+            int n[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) n[u] = c0 + u < chunks ? count[static_cast<int64_t>(c0 + u) * groups] : 0;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (c0 + u < chunks) count[static_cast<int64_t>(c0 + u) * groups] = sum;
+                sum += n[u];
+            }
+        }
+        start[a] = sum;
+    }
+    __syncthreads();
+    const int2 tables = scan_groups(start, t, tokens, groups);
+    __syncthreads();
+    write_table(start, first_of, tables, table, t, groups);
+}
+
+// and the rows to their places: never past the table, whatever the ids have become since
+// they were counted.
+template <int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void adapter_place_kernel(const int32_t* __restrict__ ids,
+                                                                   int32_t* __restrict__ table, TableLayout t, int tokens,
+                                                                   int adapters) {
+    constexpr int STEPS = kChunkRows / (64 * WAVES);
+    extern __shared__ int32_t lds[];
+    const int groups = adapters + 1;
+    int32_t* start = lds;
+    uint16_t* counts = reinterpret_cast<uint16_t*>(lds + groups + 1);
+    const int tid = threadIdx.x, wave = tid >> 6;
+    const int first = blockIdx.x * kChunkRows + wave * 64 * STEPS;
+    uint32_t ranked[STEPS];
+    rank_rows<STEPS>(ids, first, tokens, adapters, counts + wave * groups, ranked);
+    __syncthreads();
+    for (int a = tid; a < groups; a += 64 * WAVES) {
+        start[a] = table[t.starts + a] + table[t.chunks + static_cast<int64_t>(blockIdx.x) * groups + a];
+        sum_waves<WAVES>(counts, groups, a);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+        const int i = first + 64 * s + (tid & 63), group = ranked[s] >> 16;
+        if (i >= tokens) break;
+        const int at = start[group] + counts[wave * groups + group] + (ranked[s] & 0xffff);
+        if (at < tokens) table[t.order + at] = i;
+    }
 }
 
 int launch_adapter_group(const int32_t* ids, void* table, int64_t tokens, int adapters, hipStream_t stream) {
     const TableLayout t = table_layout(tokens, adapters);
     int32_t* base = static_cast<int32_t*>(table);
-    const bool small = tokens <= kGroupSmall;
-    const size_t lds = (static_cast<size_t>(adapters) + 1 + (small ? tokens : 0)) * 4;
-    hipLaunchKernelGGL(adapter_group_kernel, dim3(1), dim3(kGroupThreads), lds, stream, ids, base, t,
-                       static_cast<int>(tokens), adapters);
-    int rc = check_launch("adapter_group_kernel");
-    if (rc != MOE_OK || small) return rc;
-    hipLaunchKernelGGL(adapter_order_kernel, dim3((adapters + 4) / 4), dim3(256), 0, stream, ids, base, t,
-                       static_cast<int>(tokens), adapters);
-    return check_launch("adapter_order_kernel");
+    const int rows = static_cast<int>(tokens), groups = adapters + 1;
+    // Sixteen waves' counts, or four's, within 64 KiB of LDS beside the starts.
+    const bool many = groups > 1536;
+    const size_t lds = (groups + 1) * 4 + std::max((many ? 4 : 16) * groups * 2, 2 * (groups + 1) * 4);
+    if (t.chunk_count == 0) {
+        if (many)
+            hipLaunchKernelGGL(adapter_group_kernel<4>, dim3(1), dim3(kGroupThreads), lds, stream, ids, base, t, rows, adapters);
+        else
+            hipLaunchKernelGGL(adapter_group_kernel<16>, dim3(1), dim3(kGroupThreads), lds, stream, ids, base, t, rows, adapters);
+        return check_launch("adapter_group_kernel");
+    }
+    const dim3 chunks(t.chunk_count);
+    hipLaunchKernelGGL(adapter_count_kernel, chunks, dim3(256), groups * 4, stream, ids, base, t, rows, adapters);
+    int rc = check_launch("adapter_count_kernel");
+    if (rc != MOE_OK) return rc;
+    hipLaunchKernelGGL(adapter_scan_kernel, dim3(1), dim3(kGroupThreads), 3 * (groups + 1) * 4, stream, base, t, rows, adapters,
+                       t.chunk_count);
+    rc = check_launch("adapter_scan_kernel");
+    if (rc != MOE_OK) return rc;
+    if (many)
+        hipLaunchKernelGGL(adapter_place_kernel<4>, chunks, dim3(256), lds, stream, ids, base, t, rows, adapters);
+    else
+        hipLaunchKernelGGL(adapter_place_kernel<16>, chunks, dim3(1024), lds, stream, ids, base, t, rows, adapters);
+    return check_launch("adapter_place_kernel");
 }
 
 // ---------------------------------------------------------------------------
@@ -219,13 +374,6 @@ __device__ __forceinline__ void put_lines(uint16_t* lds, const Lines& s, int lan
 }
 __device__ __forceinline__ u32x4_t get_operand(const uint16_t* lds, int l, int g, int h) {
     return *reinterpret_cast<const u32x4_t*>(lds + l * 64 + (((2 * g + h) ^ (l & 7)) * 8));
-}
-
-// Orders a wave's LDS accesses: what its lanes wrote before is there for all of them after.
-// (A wave's LDS operations complete in order; this keeps the compiler from moving them.)
-__device__ __forceinline__ void wave_lds_order() {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
 }
 
 // NR: 16-rank fragments. F: 16-row fragments a wave.

@@ -140,6 +140,44 @@ def test_forward_and_gradients(tokens, hidden, width, rank, adapters, pattern):
     assert torch.equal(y[plain], case["base"][plain]) and torch.equal(dx[plain], case["grad_x"][plain])
 
 
+@pytest.mark.parametrize("tokens,adapters,pattern", [
+    (1000, 4096, "mixed"), (4096, 4096, "outside"), (4096, 1535, "mixed"), (4096, 1536, "runs"), (4095, 1, "mixed"),
+    (4097, 4096, "mixed"), (8192, 1536, "outside"), (8193, 2, "one"), (12289, 1535, "runs"), (70000, 4096, "mixed"),
+    (70000, 1, "none")])
+def test_many_adapters_and_rows(tokens, adapters, pattern):
+    """Both sides of where a batch is sorted in chunks, and by four waves instead of sixteen."""
+    case = _case(tokens, 8, 8, 2, adapters, pattern)
+    key = _check_groups(case)
+    groups = case["groups"]
+    y, kept = low_rank_add(case["base"], case["x"], case["down"], case["up"], groups, return_hidden=True)
+    got = low_rank_backward(case["grad"], case["x"], case["down"], case["up"], groups, hidden=kept)
+    # Every row of one adapter at a time would take a launch each; here each row's own factors.
+    safe = key.clamp(max=adapters - 1)
+    on = (key < adapters).double().unsqueeze(1)
+    x, dy = case["x"].double(), case["grad"].double()
+    down, up = case["down"].double()[safe], case["up"].double()[safe]
+    middle = 2 * (8 / 4 + 100) * U  # of the first product, as in _reference
+
+    def through(base, v, first, second):
+        h = (first * v.unsqueeze(1)).sum(2) * on
+        th = (first.abs() * v.abs().unsqueeze(1)).sum(2) * on * middle
+        want = base + (second * h.unsqueeze(2)).sum(1)
+        size = (second.abs() * h.abs().unsqueeze(2)).sum(1)
+        tol = (second.abs() * th.unsqueeze(2)).sum(1) + size * (2.0**-16 + 2 * (2 * 2 + 16) * U)
+        return h, th, (want, tol + (want.abs() + base.abs()) * 2 * U)
+
+    h, th, ref = through(case["base"].double(), x, down, up)
+    _check(y, ref, "output")
+    dh, tdh, ref = through(torch.zeros_like(x), dy, up, down)
+    _check(got[0], ref, "grad_x")
+    for g, a, ta, b in ((got[1], dh, tdh, x), (got[2], h, th, dy)):
+        want, size, tol = (torch.zeros(adapters + 1, 2, 8, device="cuda", dtype=torch.float64).index_add_(
+            0, key, m.unsqueeze(2) * v.unsqueeze(1)) for m, v in ((a, b), (a.abs(), b.abs()), (ta, b.abs())))
+        rows = torch.bincount(key, minlength=adapters + 1)[:-1].reshape(-1, 1, 1)
+        n = 3 * rows.clamp(max=1024) + rows / 128 + 20
+        _check(g, (want[:-1], tol[:-1] + size[:-1] * 2 * n * U), "adapter gradient", half=0.0)
+
+
 def test_without_base_and_scales_and_in_place():
     case = _case(150, 136, 264, 16, 3)
     ref = _reference(case, scaled=False)
