@@ -1042,8 +1042,24 @@ __device__ __forceinline__ void store4(void* out, int64_t at, f32x4_t v) {
         *reinterpret_cast<f32x4_t*>(static_cast<float*>(out) + at) = v;
 }
 
-// A wave holds NR 16-rank fragments; RG of the W waves share the ranks (r <= 16 NR RG)
-// and W / RG the rows. The split's row numbers are in LDS before the first row is asked
+// Eight fp32 values as three bf16 operands: their significands' 24 bits, eight at a time,
+// cut off and not rounded, so that each rest is exact (an infinite value leaves NaN).
+__device__ __forceinline__ void split3(const float (&f)[8], u32x4_t (&a)[3]) {
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+        float f0 = f[2 * p], f1 = f[2 * p + 1];
+#pragma unroll
+        for (int n = 0; n < 3; ++n) {
+            const uint32_t b0 = __float_as_uint(f0), b1 = __float_as_uint(f1);
+            a[n][p] = __builtin_amdgcn_perm(b1, b0, 0x07060302u);
+            f0 -= __uint_as_float(b0 & 0xffff0000u);
+            f1 -= __uint_as_float(b1 & 0xffff0000u);
+        }
+    }
+}
+
+// Up to 32 ranks: a wave holds NR 16-rank fragments of 128 columns, the waves share the
+// rows. The split's row numbers are in LDS before the first row is asked
 // for: read from the table beside each step's rows, every step waited for memory twice
 // (4096 rows of 4096 columns, rank 16, both products: 22.4 us, 14.8 now; loads one or two
 // steps ahead then gain nothing).
@@ -1053,35 +1069,64 @@ struct OuterJobs {
     int columns[2];  // column parts of each; the grid has both
 };
 
-template <int NR, int RG, int W, bool BF16>
-__global__ __launch_bounds__(64 * W) void outer_kernel(OuterJobs jobs, const float* __restrict__ scales, Groups gr,
-                                                              int64_t tokens, int rank) {
-    constexpr int TG = W / RG;
-    __shared__ __attribute__((aligned(16))) float lds[W * 16 * 128];
+// A workgroup's split, job and columns.
+struct OuterPart {
+    OuterJob job;
+    int column, adapter, first, rows, parts;
+};
+__device__ __forceinline__ bool outer_part(const OuterJobs& jobs, const Groups& gr, int64_t tokens, OuterPart* p) {
+    const bool second = static_cast<int>(blockIdx.y) >= jobs.columns[0];
+    p->job = jobs.job[second];
+    p->column = (blockIdx.y - (second ? jobs.columns[0] : 0)) * kOuterCols;
+    if (gr.order) {
+        const int4 split = gr.splits[blockIdx.x];
+        p->adapter = split.x;
+        p->first = split.y;
+        p->rows = split.z;
+        p->parts = split.w;
+        return static_cast<int>(blockIdx.x) < gr.head[1];
+    }
+    p->adapter = 0;
+    p->first = blockIdx.x * gr.split_rows;
+    p->rows = static_cast<int>(min(static_cast<int64_t>(gr.split_rows), tokens - p->first));
+    p->parts = gr.split_bound;
+    return true;
+}
+
+// The split's rows, up to whole 64s. -1: past its end, or a masked row, which may hold
+// anything (its h is 0, and 0 times NaN is not).
+__device__ __forceinline__ void list_rows(int32_t* row_of, const Groups& gr, const OuterPart& p) {
+    for (int i = threadIdx.x; i < (p.rows + 63) / 64 * 64; i += blockDim.x) {
+        const int at = p.first + i;
+        row_of[i] = i >= p.rows ? -1 : gr.order ? gr.order[at] : gr.mask && !gr.mask[at] ? -1 : at;
+    }
+}
+
+// Four columns of a rank: the result, or this split's share of it.
+template <bool BF16>
+__device__ __forceinline__ void store_outer(const OuterPart& p, int rank, int c, int64_t j, f32x4_t sum) {
+    if (c >= rank || j >= p.job.width) return;
+    if (p.parts == 1)
+        store4<BF16>(p.job.out, (static_cast<int64_t>(p.adapter) * rank + c) * p.job.width + j, sum);
+    else
+        store4<false>(p.job.partials, (static_cast<int64_t>(blockIdx.x) * rank + c) * p.job.width + j, sum);
+}
+
+template <int NR, bool BF16>
+__global__ __launch_bounds__(256, 3) void outer_kernel(OuterJobs jobs, const float* __restrict__ scales, Groups gr,
+                                                    int64_t tokens, int rank) {
+    constexpr int W = 4;
+    __shared__ __attribute__((aligned(16))) float lds[W * 16 * kOuterCols];
     __shared__ int32_t row_of[kMaxSplitRows];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int l = lane & 15, g = lane >> 4;
-    const bool second = static_cast<int>(blockIdx.y) >= jobs.columns[0];
-    const OuterJob job = jobs.job[second];
-    const int part_column = blockIdx.y - (second ? jobs.columns[0] : 0);
-    const int64_t width = job.width;
-    int adapter = 0, first = blockIdx.x * gr.split_rows, rows, parts = gr.split_bound;
-    if (gr.order) {
-        const int4 split = gr.splits[blockIdx.x];
-        if (static_cast<int>(blockIdx.x) >= gr.head[1]) return;
-        adapter = split.x;
-        first = split.y;
-        rows = split.z;
-        parts = split.w;
-    } else {
-        rows = static_cast<int>(min(static_cast<int64_t>(gr.split_rows), tokens - first));
-    }
-    // -1: a masked row, which may hold anything (its h is 0, and 0 times NaN is not).
-    for (int i = tid; i < rows; i += 64 * W)
-        row_of[i] = gr.order ? gr.order[first + i] : gr.mask && !gr.mask[first + i] ? -1 : first + i;
-    const int64_t col = static_cast<int64_t>(part_column) * kOuterCols + 8 * l;
+    OuterPart part;
+    if (!outer_part(jobs, gr, tokens, &part)) return;
+    list_rows(row_of, gr, part);
+    const int rows = part.rows;
+    const int64_t width = part.job.width;
+    const int64_t col = part.column + 8 * l;
     const bool inside = col < width;
-    const int c0 = wave % RG * 16 * NR;
     const u32x4_t zero = {0, 0, 0, 0};
     f32x4_t acc[NR][8];
 #pragma unroll
@@ -1089,73 +1134,161 @@ __global__ __launch_bounds__(64 * W) void outer_kernel(OuterJobs jobs, const flo
 #pragma unroll
         for (int i = 0; i < 8; ++i) acc[n][i] = f32x4_t{0, 0, 0, 0};
     __syncthreads();
-    for (int t0 = 32 * (wave / RG); t0 < rows; t0 += 32 * TG) {
+    for (int t0 = 32 * wave; t0 < rows; t0 += 32 * W) {
         u32x4_t v[8];
         float hv[NR][8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const int i = t0 + 8 * g + j;
             const int row = i < rows ? row_of[i] : -1;
-            v[j] = row >= 0 && inside ? load16(job.x + row * width + col) : zero;
+            v[j] = row >= 0 && inside ? load16(part.job.x + row * width + col) : zero;
 #pragma unroll
             for (int n = 0; n < NR; ++n) {
-                const int c = c0 + 16 * n + l;
-                hv[n][j] = i < rows && c < rank ? job.h[static_cast<int64_t>(first + i) * rank + c] : 0.0f;
+                const int c = 16 * n + l;
+                hv[n][j] = i < rows && c < rank ? part.job.h[static_cast<int64_t>(part.first + i) * rank + c] : 0.0f;
             }
         }
         u32x4_t b[8];
         transpose8(v, b);
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
-            u32x4_t a0, a1, a2;
-#pragma unroll
-            for (int p = 0; p < 4; ++p) {
-                float f0 = hv[n][2 * p], f1 = hv[n][2 * p + 1];
-                a0[p] = pack_bf16x2(f0, f1);
-                f0 = bf16_rest(f0, a0[p]);
-                f1 = bf16_rest(f1, a0[p] >> 16);
-                a1[p] = pack_bf16x2(f0, f1);
-                a2[p] = pack_bf16x2(bf16_rest(f0, a1[p]), bf16_rest(f1, a1[p] >> 16));
-            }
+            u32x4_t a[3];
+            split3(hv[n], a);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                acc[n][i] = mfma(a2, b[i], acc[n][i]);
-                acc[n][i] = mfma(a1, b[i], acc[n][i]);
-                acc[n][i] = mfma(a0, b[i], acc[n][i]);
+                acc[n][i] = mfma(a[2], b[i], acc[n][i]);
+                acc[n][i] = mfma(a[1], b[i], acc[n][i]);
+                acc[n][i] = mfma(a[0], b[i], acc[n][i]);
             }
         }
     }
-    const float scale = scales ? scales[adapter] : 1.0f;
-    // One fragment of every wave at a time: [wave][rank][column] in LDS, the row groups
-    // summed in order; a thread takes four columns.
+    const float scale = scales ? scales[part.adapter] : 1.0f;
+    // One fragment of every wave at a time: [wave][rank][column] in LDS, the waves summed
+    // in order; a thread takes four columns of two ranks.
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
         if (n > 0) __syncthreads();
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            float* dst = lds + (wave * 16 + 4 * g + q) * 128 + 8 * l;
+            float* dst = lds + (wave * 16 + 4 * g + q) * kOuterCols + 8 * l;
             *reinterpret_cast<f32x4_t*>(dst) = f32x4_t{acc[n][0][q], acc[n][1][q], acc[n][2][q], acc[n][3][q]};
             *reinterpret_cast<f32x4_t*>(dst + 4) = f32x4_t{acc[n][4][q], acc[n][5][q], acc[n][6][q], acc[n][7][q]};
         }
         __syncthreads();
-        const int64_t j = static_cast<int64_t>(part_column) * kOuterCols + 4 * (tid & 31);
-        // 2 W rows of 128 columns a turn.
 #pragma unroll
-        for (int r0 = 0; r0 < 16 * RG; r0 += 2 * W) {
-            const int r = r0 + tid / 32, rg = r / 16;
-            const int c = (rg * NR + n) * 16 + r % 16;
-            if (r >= 16 * RG || c >= rank || j >= width) continue;
-            const float* src = lds + r * 128 + 4 * (tid & 31);
+        for (int r0 = 0; r0 < 16; r0 += 8) {
+            const int r = r0 + tid / 32;
+            const float* src = lds + r * kOuterCols + 4 * (tid & 31);
             f32x4_t sum = *reinterpret_cast<const f32x4_t*>(src);
 #pragma unroll
-            for (int t = 1; t < TG; ++t) sum += *reinterpret_cast<const f32x4_t*>(src + t * RG * 2048);
-            sum *= scale;
-            if (parts == 1)
-                store4<BF16>(job.out, (static_cast<int64_t>(adapter) * rank + c) * width + j, sum);
-            else
-                store4<false>(job.partials, (static_cast<int64_t>(blockIdx.x) * rank + c) * width + j, sum);
+            for (int w = 1; w < W; ++w) sum += *reinterpret_cast<const f32x4_t*>(src + w * 16 * kOuterCols);
+            store_outer<BF16>(part, rank, 16 * n + r, part.column + 4 * (tid & 31), sum * scale);
         }
     }
+}
+
+// More than 32 ranks: every wave would load and transpose the same x, and each column part
+// split the same h, once per 32 ranks (4096 rows of 4096 columns, rank 64 and 128, both
+// products: 41.9 and 74.4 us). Here eight waves stage 64 rows a step in LDS as operands,
+// a wave eight of them (x transposed, h split), while the next rows' loads are on their
+// way; then a wave multiplies its quarter of the ranks and half of the columns: 23 and 46 us.
+// RF: 16-rank fragments, 4 or 8.
+template <int RF, bool BF16>
+__global__ __launch_bounds__(512, 4) void outer_wide_kernel(OuterJobs jobs, const float* __restrict__ scales, Groups gr,
+                                                            int64_t tokens, int rank) {
+    constexpr int R = 16 * RF, NR = RF / 4, HL = R / 64;
+    // [32 rows][8 of them][column, or rank], 16 bytes each: eight rows of a column or rank.
+    // Column c of a half lies at 16 (c % 4) + c / 4, so that a lane ends with four
+    // neighbours.
+    __shared__ u32x4_t xs[2][4][kOuterCols];
+    __shared__ u32x4_t hs[2][3][4][R];
+    __shared__ __attribute__((aligned(16))) int32_t row_of[kMaxSplitRows];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int l = lane & 15, g = lane >> 4;
+    OuterPart part;
+    if (!outer_part(jobs, gr, tokens, &part)) return;
+    list_rows(row_of, gr, part);
+    const int rows = part.rows;
+    const int64_t width = part.job.width;
+    const bool inside = part.column + 2 * lane < width;
+    const int rank0 = wave % 4 * 16 * NR, half = wave / 4;
+    f32x4_t acc[NR][4];
+#pragma unroll
+    for (int n = 0; n < NR; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[n][i] = f32x4_t{0, 0, 0, 0};
+    // This wave's eight rows of a step: two columns and a rank (two) a lane. Addresses are
+    // a scalar row and a lane's offset; rows of none are read from row 0 (and the last h) and
+    // taken as zeros of x.
+    const uint32_t x_at = inside ? 2 * lane : 0;
+    uint32_t xv[8], valid;
+    float hv[HL][8];
+    const int own = __builtin_amdgcn_readfirstlane(8 * wave);
+    const uint16_t* x0 = part.job.x + part.column;
+    const auto fetch = [&](int t0) {
+        valid = 0;
+        const int4 listed[2] = {*reinterpret_cast<const int4*>(row_of + t0 + own),
+                                *reinterpret_cast<const int4*>(row_of + t0 + own + 4)};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int i = min(t0 + own + j, rows - 1);
+            const int row = __builtin_amdgcn_readfirstlane(reinterpret_cast<const int*>(listed)[j]);
+            valid |= static_cast<uint32_t>(row >= 0) << j;
+            xv[j] = *reinterpret_cast<const uint32_t*>(x0 + max(row, 0) * width + x_at);
+            const float* h = part.job.h + static_cast<int64_t>(part.first + i) * rank;
+#pragma unroll
+            for (int n = 0; n < HL; ++n) hv[n][j] = h[min(64 * n + lane, rank - 1)];
+        }
+    };
+    __syncthreads();
+    fetch(0);
+    for (int t0 = 0; t0 < rows; t0 += 64) {
+        const int group = wave / 4, eight = wave % 4;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) xv[j] = valid >> j & 1 ? xv[j] : 0u;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            u32x4_t b;
+#pragma unroll
+            for (int p = 0; p < 4; ++p)
+                b[p] = __builtin_amdgcn_perm(xv[2 * p + 1], xv[2 * p], i ? 0x07060302u : 0x05040100u);
+            const int c = 2 * lane + i;
+            xs[group][eight][(c & 64) + 16 * (c & 3) + (c & 63) / 4] = b;
+        }
+#pragma unroll
+        for (int n = 0; n < HL; ++n) {
+            u32x4_t a[3];
+            split3(hv[n], a);
+#pragma unroll
+            for (int p = 0; p < 3; ++p) hs[group][p][eight][64 * n + lane] = a[p];
+        }
+        __syncthreads();
+        if (t0 + 64 < rows) fetch(t0 + 64);
+        if (rank0 < rank) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                u32x4_t b[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) b[i] = xs[k][g][64 * half + 16 * i + l];
+#pragma unroll
+                for (int n = 0; n < NR; ++n)
+#pragma unroll
+                    for (int p = 2; p >= 0; --p) {
+                        const u32x4_t a = hs[k][p][g][rank0 + 16 * n + l];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) acc[n][i] = mfma(a, b[i], acc[n][i]);
+                    }
+            }
+        }
+        __syncthreads();
+    }
+    const float scale = scales ? scales[part.adapter] : 1.0f;
+#pragma unroll
+    for (int n = 0; n < NR; ++n)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            store_outer<BF16>(part, rank, rank0 + 16 * n + 4 * g + q, part.column + 64 * half + 4 * l,
+                              f32x4_t{acc[n][0][q], acc[n][1][q], acc[n][2][q], acc[n][3][q]} * scale);
 }
 
 // An adapter's partial sums in split order, or zeros for one without rows.
@@ -1203,10 +1336,10 @@ int launch_outer(const OuterJob& first, const OuterJob& second, const float* sca
     };
     const auto by_rank = [&](auto bf16) {
         constexpr bool B = decltype(bf16)::value;
-        if (rank <= 16) return run(outer_kernel<1, 1, 4, B>, 4);
-        if (rank <= 32) return run(outer_kernel<2, 1, 4, B>, 4);
-        if (rank <= 64) return run(outer_kernel<2, 2, 8, B>, 8);
-        return run(outer_kernel<2, 4, 8, B>, 8);
+        if (rank <= 16) return run(outer_kernel<1, B>, 4);
+        if (rank <= 32) return run(outer_kernel<2, B>, 4);
+        if (rank <= 64) return run(outer_wide_kernel<4, B>, 8);
+        return run(outer_wide_kernel<8, B>, 8);
     };
     int rc = MOE_OK;
     if (g.split_bound > 0) rc = out_bf16 ? by_rank(std::true_type{}) : by_rank(std::false_type{});
