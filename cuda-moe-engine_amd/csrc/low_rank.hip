@@ -364,6 +364,13 @@ __device__ __forceinline__ void load_lines(Lines& s, const LineRows& r, int at, 
 #pragma unroll
     for (int h = 0; h < 2; ++h) s.v[h] = at < k ? load16(r.row[h] + at) : zero;
 }
+// Of `rows` rows: the others are zeros that cost no traffic (decoding 8.1 -> 7.9 us, 777 rows
+// 12.6 -> 12.4; contract, whose loads wait on HBM, gains nothing).
+__device__ __forceinline__ void load_lines(Lines& s, const LineRows& r, int at, int k, int rows, int lane) {
+    const u32x4_t zero = {0, 0, 0, 0};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) s.v[h] = at < k && lane / 8 + 8 * h < rows ? load16(r.row[h] + at) : zero;
+}
 
 // A wave's 2 KiB: piece p of row r lies at slot p ^ (r % 8) of its 128 bytes, so that the
 // operands' 16 rows fall on different banks.
@@ -810,7 +817,9 @@ int launch_spread(const float* partials, int slices, const void* w, bool w32, co
 // waves split all of k, add up in LDS, and each spread 128 columns. Every column part
 // computes h again, from w in the L2, so that nothing is handed over between workgroups.
 // The sums' order is k's over eight waves: results differ from the two launches' in fp32
-// rounding.
+// rounding. Latency, not bytes: one row of 4096 -> 4096 at rank 16 takes 7.9 us (two
+// launches 14.8), of 512 -> 512 4.6; 64 rows of 16 adapters 10.7. Loads five to seven steps
+// ahead took 8.4 to 8.7, sixteen waves of 64 columns 9.8 (their registers spill).
 // ---------------------------------------------------------------------------
 constexpr int kFusedWaves = 8;
 constexpr int kFusedCols = kFusedWaves * 128;
@@ -890,7 +899,7 @@ __global__ __launch_bounds__(64 * kFusedWaves) void fused_kernel(
         Step ring[D];
         const auto load = [&](Step& s, int k0) {
             const int at = k0 + 8 * (lane % 8);
-            load_lines(s.x, xr, at, k);
+            load_lines(s.x, xr, at, k, rows, lane);
 #pragma unroll
             for (int n = 0; n < NR; ++n) load_lines(s.w[n], wr[n], at, k);
         };
