@@ -347,9 +347,11 @@ int launch_adapter_group(const int32_t* ids, void* table, int64_t tokens, int ad
 // in LDS of its own into the MFMA's operands (lane l: row l % 16, 8 k from 8 (l / 16); k is
 // permuted inside 64). Loaded as operands, neighbouring lanes hold different rows and each
 // 16 bytes is a line of its own to the L1: T=4096, H=4096, r=16 and 64 took 17.2 and 38.6
-// us, 11.5 and 15.0 now (a plain reduction of rows that come from HBM takes 11.3). Rows past the tile and ranks past r are read from the last one and not stored (an output
+// us, 11.1 and 17.1 now (a plain reduction of rows that come from HBM takes 11.3). Rows
+// past the tile and ranks past r are read from the last one and not stored (an output
 // depends on its own row and rank alone). Waves on one row meet in LDS, slices in the
-// consumer, both in order.
+// consumer, both in order. Bound by x's bytes; past 64 ranks (21.7 us at r=128) by the LDS
+// that turns w's lines over for 32 rows.
 // ---------------------------------------------------------------------------
 // 16 rows of 64 k: lane i loads piece i % 8 (8 k) of rows i / 8 and i / 8 + 8.
 struct LineRows {
@@ -542,7 +544,10 @@ static unsigned part_grid(int64_t columns, int64_t rows) {
 // transposes the block in registers (v_perm_b32); MFMA i then covers columns n0 + 8 l + i,
 // and a lane ends with 8 neighbouring columns of a row: base and out move 16 bytes a lane.
 // h enters as two bf16 parts (rest below 2^-16 of it, under the result's own rounding to
-// bf16): for r <= 16 side by side in one MFMA's 32 k, else as two MFMAs on one w.
+// bf16): for r <= 16 side by side in one MFMA's 32 k, else as two MFMAs on one w. Bound by
+// base's and out's bytes: 67 MB (T=4096, 4096 columns) in 14.8 us at r=16, the rate of a
+// copy from HBM, 16.5 at r=32; at r=64 22.9 and at r=128 35, where every column part reads
+// the slices' sums of h again.
 // ---------------------------------------------------------------------------
 // The 8 x N block of 16-bit values v[j] (row j, two columns a dword) as B operands:
 // column i of all rows.
@@ -1041,6 +1046,8 @@ static int launch_through(const uint16_t* x, const uint16_t* down, const uint16_
 // as in spread; h (fp32, read along the ranks) enters as three bf16 parts, which hold
 // all its bits, so each product is exact and sums in fp32. The waves' sums meet in LDS;
 // an adapter of one split is done, of more its partial sums are added in split order.
+// Bound by x's bytes: both products of 4096 rows of 4096 columns, 67 MB, in 14.6 us at
+// r=16 and 18 at r=32, and 4 us for the splits' sums.
 // ---------------------------------------------------------------------------
 template <bool BF16>
 __device__ __forceinline__ void store4(void* out, int64_t at, f32x4_t v) {
