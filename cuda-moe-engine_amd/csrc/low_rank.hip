@@ -342,7 +342,9 @@ int launch_adapter_group(const int32_t* ids, void* table, int64_t tokens, int ad
 // contract: h[i][c] = sum_k x[i][k] w[c][k].
 // A workgroup takes a tile of up to 64 rows of one adapter and a slice of k. A wave takes
 // 16 rows and the slice, or for r > 32, where w's lines are the more, 32 rows and half of
-// it; with fewer rows in the tile more waves share them and split the slice. Eight lanes
+// it; with fewer rows in the tile more waves share them and split the slice. Up to 64 ranks
+// take eight waves and half the slices (rank 16 in eight waves spills: 29.4 -> 32.5 us with
+// spread). Eight lanes
 // load a 128-byte line of a row, D steps of 64 k ahead, and the wave turns the step over
 // in LDS of its own into the MFMA's operands (lane l: row l % 16, 8 k from 8 (l / 16); k is
 // permuted inside 64). Loaded as operands, neighbouring lanes hold different rows and each
@@ -385,22 +387,22 @@ __device__ __forceinline__ u32x4_t get_operand(const uint16_t* lds, int l, int g
     return *reinterpret_cast<const u32x4_t*>(lds + l * 64 + (((2 * g + h) ^ (l & 7)) * 8));
 }
 
-// NR: 16-rank fragments. F: 16-row fragments a wave.
-template <int NR, int F>
-__global__ __launch_bounds__(256) void contract_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict__ w,
+// NR: 16-rank fragments. F: 16-row fragments a wave. W: waves.
+template <int NR, int F, int W>
+__global__ __launch_bounds__(64 * W) void contract_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict__ w,
                                                        Groups gr, float* __restrict__ partials, int64_t tokens, int k,
                                                        int rank, int span) {
     constexpr int D = NR <= 2 ? 6 : NR == 4 ? 3 : 2;  // steps in flight
     constexpr int C = 16 * NR;
     constexpr int kWaveHalfs = 1024 * (F + NR);  // x's fragments and w's
-    __shared__ __attribute__((aligned(16))) uint16_t lines[4 * kWaveHalfs];
+    __shared__ __attribute__((aligned(16))) uint16_t lines[W * kWaveHalfs];
     const int4 tile = gr.tiles[blockIdx.x];
     if (static_cast<int>(blockIdx.x) >= gr.head[0] || tile.x < 0) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int l = lane & 15, g = lane >> 4;
     const int first = tile.y, rows = tile.z;
     // Waves on the same rows, this wave's rows and its part of the slice.
-    const int kw = rows > 32 ? F : rows > 16 ? 2 * F : 4;
+    const int kw = (rows > 32 ? F : rows > 16 ? 2 * F : 4) * (W / 4);
     const int m = wave / kw, kpart = wave % kw;
     const bool two = F == 2 && rows - 32 * m > 16;
     const int kb = blockIdx.y * span + kpart * (span / kw);
@@ -500,27 +502,34 @@ __global__ __launch_bounds__(256) void contract_kernel(const uint16_t* __restric
 }
 
 // Up to about 600 workgroups; past 32 ranks, where spread reads each slice's sums again
-// for every 256 columns, 512 (contract and spread of 8192 x 4096 to 4096, rank 16: 46.9 us,
-// with 512 50.5; of 4096 rows, rank 64: 43.8 and 40.0; of 16384, rank 128: 168 and 158).
+// for every 256 columns, 512, or one a CU of the eight waves of up to 64 ranks (contract
+// and spread of 8192 x 4096 to 4096, rank 16: 46.9 us, with 512 50.5; of 4096 rows, rank 64:
+// 45.5 with three slices, 46.3 with two, 46.8 with four of four waves; of 1024 rows 20.1 and
+// 22.6; of 16384, rank 128: 158, with 600 168).
 int contract_slices(int tile_bound, int64_t k, int64_t rank) {
-    const int64_t most = (k + 255) / 256, workgroups = rank <= 32 ? 600 : 512;
-    int64_t s = 1;
-    while (s < 16 && s * 2 <= most && s * 2 * tile_bound <= workgroups) s <<= 1;
-    return static_cast<int>(s);
+    const bool wide = rank > 32 && rank <= 64;
+    const int64_t most = wide ? (k + 511) / 512 : (k + 255) / 256;
+    const int64_t workgroups = rank <= 32 ? 600 : wide ? 256 : 512;
+    int best = 1;
+    for (int s : {2, 3, 4, 8, 16})
+        if (s <= most && static_cast<int64_t>(s) * tile_bound <= workgroups) best = s;
+    return best;
 }
 
 int launch_contract(const uint16_t* x, const uint16_t* w, const Groups& g, float* partials, int slices, int64_t tokens,
                     int64_t k, int rank, hipStream_t stream) {
-    const int span = static_cast<int>(((k + slices - 1) / slices + 255) / 256 * 256);
     const dim3 grid(g.tile_bound, slices);
-    const auto run = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, x, w, g, partials, tokens, static_cast<int>(k), rank, span);
+    const auto run = [&](auto kernel, int waves) {
+        const int unit = 64 * waves;  // whole steps for every wave
+        const int span = static_cast<int>(((k + slices - 1) / slices + unit - 1) / unit * unit);
+        hipLaunchKernelGGL(kernel, grid, dim3(64 * waves), 0, stream, x, w, g, partials, tokens, static_cast<int>(k),
+                           rank, span);
         return check_launch("contract_kernel");
     };
-    if (rank <= 16) return run(contract_kernel<1, 1>);
-    if (rank <= 32) return run(contract_kernel<2, 1>);
-    if (rank <= 64) return run(contract_kernel<4, 2>);
-    return run(contract_kernel<8, 2>);
+    if (rank <= 16) return run(contract_kernel<1, 1, 4>, 4);
+    if (rank <= 32) return run(contract_kernel<2, 1, 4>, 4);
+    if (rank <= 64) return run(contract_kernel<4, 2, 8>, 8);
+    return run(contract_kernel<8, 2, 4>, 4);
 }
 
 // Workgroup b as (column part, row part), the column parts of a row part next to each
@@ -660,7 +669,7 @@ __global__ __launch_bounds__(256, NK == 1 && !W32 ? 3 : 1) void spread_kernel(co
     const int filled = (rows + 15) / 16 * 16 * Q;
     const int64_t slice = tokens * rank;
     const auto stage = [&](auto count) {
-        constexpr int S = decltype(count)::value, U = C >= 64 && S <= 4 ? 2 : 1;
+        constexpr int S = decltype(count)::value, U = C >= 64 && S <= 4 && S != 3 ? 2 : 1;
         using V = Unaligned<float, 4>;
 #pragma unroll 1
         for (int i0 = tid; i0 < filled; i0 += 256 * U) {
@@ -722,6 +731,7 @@ __global__ __launch_bounds__(256, NK == 1 && !W32 ? 3 : 1) void spread_kernel(co
     else switch (slices) {
         case 1: stage(std::integral_constant<int, 1>{}); break;
         case 2: stage(std::integral_constant<int, 2>{}); break;
+        case 3: stage(std::integral_constant<int, 3>{}); break;
         case 4: stage(std::integral_constant<int, 4>{}); break;
         default: stage(std::integral_constant<int, 8>{}); break;
     }
