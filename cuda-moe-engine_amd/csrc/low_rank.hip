@@ -575,8 +575,8 @@ __device__ __forceinline__ void transpose8(const V (&v)[8], u32x4_t (&b)[N]) {
 // `fragments` 16-row fragments of a tile, blockIdx.z the first: the whole tile, or 2 or 1
 // where whole tiles would leave CUs idle. base's rows are on their way one fragment ahead.
 // COLS: columns a lane, 8, or 4 where w's operands for 8 would leave a SIMD one wave
-// (r > 32, fp32 w).
-template <int NK, bool HALF, bool W32, int COLS>
+// (r > 32, fp32 w). STREAM: base is read past the caches.
+template <int NK, bool HALF, bool W32, int COLS, bool STREAM>
 __global__ __launch_bounds__(256, NK == 1 && !W32 ? 3 : 1) void spread_kernel(const float* __restrict__ partials, int slices, const void* wv,
                                                      const float* __restrict__ scales, Groups gr, const uint16_t* base,
                                                      uint16_t* out, float* __restrict__ h_out, int64_t tokens,
@@ -617,6 +617,11 @@ __global__ __launch_bounds__(256, NK == 1 && !W32 ? 3 : 1) void spread_kernel(co
     int first_rows[4];
 #pragma unroll
     for (int q = 0; q < 4; ++q) first_rows[q] = listed(min(4 * g + q, rows - 1));
+    const auto from_base = [](const uint16_t* p) {
+        const cols_t* v = reinterpret_cast<const cols_t*>(p);
+        if constexpr (STREAM) return __builtin_nontemporal_load(v);
+        return *v;
+    };
     // This lane's rows of a fragment, 16 m + 4 g + q, and what base has there.
     int64_t at[4];
     cols_t old[4];
@@ -624,7 +629,7 @@ __global__ __launch_bounds__(256, NK == 1 && !W32 ? 3 : 1) void spread_kernel(co
 #pragma unroll
         for (int q = 0; q < 4; ++q) at[q] = row(min(16 * m + 4 * g + q, rows - 1)) * width + col;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) old[q] = base && inside ? *reinterpret_cast<const cols_t*>(base + at[q]) : zero;
+        for (int q = 0; q < 4; ++q) old[q] = base && inside ? from_base(base + at[q]) : zero;
     };
     if (adapter < 0) {  // no adapter: h is 0, the base as it is
         if (h_out && chunk == 0)
@@ -661,7 +666,7 @@ __global__ __launch_bounds__(256, NK == 1 && !W32 ? 3 : 1) void spread_kernel(co
 #pragma unroll
         for (int q = 0; q < 4; ++q) at[q] = first_rows[q] * width + col;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) old[q] = base && inside ? *reinterpret_cast<const cols_t*>(base + at[q]) : zero;
+        for (int q = 0; q < 4; ++q) old[q] = base && inside ? from_base(base + at[q]) : zero;
     }
     // h: the slices' sums as bf16 parts; zero past the rank and past the rows, up to a
     // whole fragment. A thread takes four ranks of a row, U rows and S slices in flight.
@@ -794,10 +799,18 @@ __global__ __launch_bounds__(256, NK == 1 && !W32 ? 3 : 1) void spread_kernel(co
                 const float b1 = bf16_to_f32(static_cast<uint16_t>(there[q][d] >> 16));
                 o[d] = pack_bf16x2(b0 + scale * acc[2 * d][q], b1 + scale * acc[2 * d + 1][q]);
             }
-            *reinterpret_cast<cols_t*>(out + now[q]) = o;
+            __builtin_nontemporal_store(o, reinterpret_cast<cols_t*>(out + now[q]));
         }
     }
 }
+
+// Results are stored past the caches, which then hold what the next workgroups read (1024
+// rows of 4096 columns with contract, rank 16: 15.2 -> 14.2 us; 4096 rows 29.5 -> 30.8 with
+// nothing in the caches, the same behind the kernels that wrote x and base), and from 48 MB
+// of base on it is read that way too (8192 rows behind those kernels, rank 16 and 64: 46.8
+// -> 39.7 and 68 -> 61, 71 -> 70 with nothing in the caches; at 32 MB and less it lost up to
+// 8%).
+constexpr int64_t kStreamElements = 24 << 20;
 
 int launch_spread(const float* partials, int slices, const void* w, bool w32, const float* scales, const Groups& g,
                   const uint16_t* base, uint16_t* out, float* h_out, int64_t tokens, int64_t width, int rank,
@@ -815,15 +828,19 @@ int launch_spread(const float* partials, int slices, const void* w, bool w32, co
                            partials, slices, w, scales, g, base, out, h_out, tokens, width, rank, fragments, columns);
         return check_launch("spread_kernel");
     };
-    if (w32) {  // the router: at most 64 experts
-        if (rank <= 16) return run(spread_kernel<1, true, true, 8>, 8);
-        if (rank <= 32) return run(spread_kernel<1, false, true, 8>, 8);
-        return run(spread_kernel<2, false, true, 4>, 4);
-    }
-    if (rank <= 16) return run(spread_kernel<1, true, false, 8>, 8);
-    if (rank <= 32) return run(spread_kernel<1, false, false, 8>, 8);
-    if (rank <= 64) return run(spread_kernel<2, false, false, 4>, 4);
-    return run(spread_kernel<4, false, false, 4>, 4);
+    const auto by_rank = [&](auto streamed) {
+        constexpr bool S = decltype(streamed)::value;
+        if (w32) {  // the router: at most 64 experts
+            if (rank <= 16) return run(spread_kernel<1, true, true, 8, S>, 8);
+            if (rank <= 32) return run(spread_kernel<1, false, true, 8, S>, 8);
+            return run(spread_kernel<2, false, true, 4, S>, 4);
+        }
+        if (rank <= 16) return run(spread_kernel<1, true, false, 8, S>, 8);
+        if (rank <= 32) return run(spread_kernel<1, false, false, 8, S>, 8);
+        if (rank <= 64) return run(spread_kernel<2, false, false, 4, S>, 4);
+        return run(spread_kernel<4, false, false, 4, S>, 4);
+    };
+    return tokens * width >= kStreamElements ? by_rank(std::true_type{}) : by_rank(std::false_type{});
 }
 
 // ---------------------------------------------------------------------------

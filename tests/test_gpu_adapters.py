@@ -140,6 +140,12 @@ def test_forward_and_gradients(tokens, hidden, width, rank, adapters, pattern):
     assert torch.equal(y[plain], case["base"][plain]) and torch.equal(dx[plain], case["grad_x"][plain])
 
 
+@pytest.mark.parametrize("rank", [7, 32, 33, 128])
+def test_batches_whose_base_is_streamed(rank):
+    """Past 24 M elements of base; every rank's variant of spread."""
+    test_forward_and_gradients(3100, 4104, 8192, rank, 3, "runs")
+
+
 @pytest.mark.parametrize("tokens,adapters,pattern", [
     (1000, 4096, "mixed"), (4096, 4096, "outside"), (4096, 1535, "mixed"), (4096, 1536, "runs"), (4095, 1, "mixed"),
     (4097, 4096, "mixed"), (8192, 1536, "outside"), (8193, 2, "one"), (12289, 1535, "runs"), (70000, 4096, "mixed"),

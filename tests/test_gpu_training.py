@@ -335,6 +335,13 @@ def test_route_backward(tokens, hidden, experts, topk):
     assert first[0].dtype == torch.bfloat16
 
 
+@pytest.mark.parametrize("experts", [8, 20, 64])
+def test_route_backward_of_a_streamed_base(experts):
+    """Past 24 M elements of x's gradient; every expert count's variant."""
+    case = _router_case(3100, experts, 2, 31, masked=True, hidden=8192)
+    _check_route_backward(case, 3100, experts, 2, 8192)
+
+
 def test_route_backward_follows_the_framework_router():
     """The routing weights' gradient belongs to the weights that the fused router returns."""
     ext = get_extension()
