@@ -344,12 +344,11 @@ int launch_adapter_group(const int32_t* ids, void* table, int64_t tokens, int ad
 // 16 rows and the slice, or for r > 32, where w's lines are the more, 32 rows and half of
 // it; with fewer rows in the tile more waves share them and split the slice. Up to 64 ranks
 // take eight waves and half the slices (rank 16 in eight waves spills: 29.4 -> 32.5 us with
-// spread). Eight lanes
-// load a 128-byte line of a row, D steps of 64 k ahead, and the wave turns the step over
+// spread). Eight lanes load a 128-byte line of a row, D steps of 64 k ahead, and the wave turns the step over
 // in LDS of its own into the MFMA's operands (lane l: row l % 16, 8 k from 8 (l / 16); k is
 // permuted inside 64). Loaded as operands, neighbouring lanes hold different rows and each
 // 16 bytes is a line of its own to the L1: T=4096, H=4096, r=16 and 64 took 17.2 and 38.6
-// us, 11.1 and 17.1 now (a plain reduction of rows that come from HBM takes 11.3). Rows
+// us, 11.4 and 15.7 now (a plain reduction of rows that come from HBM takes 11.3). Rows
 // past the tile and ranks past r are read from the last one and not stored (an output
 // depends on its own row and rank alone). Waves on one row meet in LDS, slices in the
 // consumer, both in order. Bound by x's bytes; past 64 ranks (21.7 us at r=128) by the LDS
