@@ -317,18 +317,16 @@ int launch_adapter_group(const int32_t* ids, void* table, int64_t tokens, int ad
     const bool many = groups > 1536;
     const size_t lds = (groups + 1) * 4 + std::max((many ? 4 : 16) * groups * 2, 2 * (groups + 1) * 4);
     if (t.chunk_count == 0) {
-        if (many)
-            hipLaunchKernelGGL(adapter_group_kernel<4>, dim3(1), dim3(kGroupThreads), lds, stream, ids, base, t, rows, adapters);
-        else
-            hipLaunchKernelGGL(adapter_group_kernel<16>, dim3(1), dim3(kGroupThreads), lds, stream, ids, base, t, rows, adapters);
+        const auto kernel = many ? adapter_group_kernel<4> : adapter_group_kernel<16>;
+        hipLaunchKernelGGL(kernel, dim3(1), dim3(kGroupThreads), lds, stream, ids, base, t, rows, adapters);
         return check_launch("adapter_group_kernel");
     }
     const dim3 chunks(t.chunk_count);
     hipLaunchKernelGGL(adapter_count_kernel, chunks, dim3(256), groups * 4, stream, ids, base, t, rows, adapters);
     int rc = check_launch("adapter_count_kernel");
     if (rc != MOE_OK) return rc;
-    hipLaunchKernelGGL(adapter_scan_kernel, dim3(1), dim3(kGroupThreads), 3 * (groups + 1) * 4, stream, base, t, rows, adapters,
-                       t.chunk_count);
+    hipLaunchKernelGGL(adapter_scan_kernel, dim3(1), dim3(kGroupThreads), 3 * (groups + 1) * 4, stream, base, t, rows,
+                       adapters, t.chunk_count);
     rc = check_launch("adapter_scan_kernel");
     if (rc != MOE_OK) return rc;
     if (many)
@@ -344,9 +342,9 @@ int launch_adapter_group(const int32_t* ids, void* table, int64_t tokens, int ad
 // 16 rows and the slice, or for r > 32, where w's lines are the more, 32 rows and half of
 // it; with fewer rows in the tile more waves share them and split the slice. Up to 64 ranks
 // take eight waves and half the slices (rank 16 in eight waves spills: 29.4 -> 32.5 us with
-// spread). Eight lanes load a 128-byte line of a row, D steps of 64 k ahead, and the wave turns the step over
-// in LDS of its own into the MFMA's operands (lane l: row l % 16, 8 k from 8 (l / 16); k is
-// permuted inside 64). Loaded as operands, neighbouring lanes hold different rows and each
+// spread). Eight lanes load a 128-byte line of a row, D steps of 64 k ahead, and the wave
+// turns the step over in LDS of its own into the MFMA's operands (lane l: row l % 16, 8 k
+// from 8 (l / 16); k is permuted inside 64). Loaded as operands, neighbouring lanes hold different rows and each
 // 16 bytes is a line of its own to the L1: T=4096, H=4096, r=16 and 64 took 17.2 and 38.6
 // us, 11.4 and 15.7 now (a plain reduction of rows that come from HBM takes 11.3). Rows
 // past the tile and ranks past r are read from the last one and not stored (an output
@@ -576,10 +574,10 @@ __device__ __forceinline__ void transpose8(const V (&v)[8], u32x4_t (&b)[N]) {
 // COLS: columns a lane, 8, or 4 where w's operands for 8 would leave a SIMD one wave
 // (r > 32, fp32 w). STREAM: base is read past the caches.
 template <int NK, bool HALF, bool W32, int COLS, bool STREAM>
-__global__ __launch_bounds__(256, NK == 1 && !W32 ? 3 : 1) void spread_kernel(const float* __restrict__ partials, int slices, const void* wv,
-                                                     const float* __restrict__ scales, Groups gr, const uint16_t* base,
-                                                     uint16_t* out, float* __restrict__ h_out, int64_t tokens,
-                                                     int64_t width, int rank, int fragments, int columns) {
+__global__ __launch_bounds__(256, NK == 1 && !W32 ? 3 : 1) void spread_kernel(
+    const float* __restrict__ partials, int slices, const void* wv, const float* __restrict__ scales, Groups gr,
+    const uint16_t* base, uint16_t* out, float* __restrict__ h_out, int64_t tokens, int64_t width, int rank,
+    int fragments, int columns) {
     constexpr int KP = 32 * NK + 8;  // 16-byte rows, off the banks' period
     constexpr int C = HALF ? 16 : 32 * NK;
     constexpr int R = W32 && NK == 2 ? kWideTileRows : kTileRows;

@@ -395,8 +395,8 @@ int launch_router_loss(const float* logits, const float* bias, const int32_t* id
     const int blocks = token_blocks(tokens, experts);
     const LossOut out{losses, stats};
     int rc = by_shape(experts, topk, [&](auto g, auto k) {
-        hipLaunchKernelGGL((router_loss_kernel<decltype(g)::value, decltype(k)::value>), dim3(blocks), dim3(256), 0, stream, logits, bias, ids,
-                           mask, tokens, experts, topk, records, out);
+        hipLaunchKernelGGL((router_loss_kernel<decltype(g)::value, decltype(k)::value>), dim3(blocks), dim3(256), 0,
+                           stream, logits, bias, ids, mask, tokens, experts, topk, records, out);
         return check_launch("router_loss_kernel");
     });
     if (rc != MOE_OK || blocks == 1) return rc;
@@ -418,8 +418,9 @@ int launch_router_logits_grad(const float* logits, const float* bias, const int3
         sums->columns = experts;
     }
     return by_shape(experts, topk, [&](auto g, auto k) {
-        hipLaunchKernelGGL((router_logits_grad_kernel<decltype(g)::value, decltype(k)::value>), dim3(blocks), dim3(256), 0, stream, logits,
-                           bias, ids, mask, stats, grad_losses, grad_weights, tokens, experts, topk, grad_logits, part);
+        hipLaunchKernelGGL((router_logits_grad_kernel<decltype(g)::value, decltype(k)::value>), dim3(blocks), dim3(256),
+                           0, stream, logits, bias, ids, mask, stats, grad_losses, grad_weights, tokens, experts, topk,
+                           grad_logits, part);
         return check_launch("router_logits_grad_kernel");
     });
 }
