@@ -145,8 +145,10 @@ class _Combine(torch.autograd.Function):
 
 def combine(expert_output, batch, weights):
     """The weighted combine of ``batch``'s packed rows, [T, H], with gradients to the rows
-    and to the fp32 weights [T, K]."""
+    and to the fp32 weights [T, K]. The batch's workspace must not be dispatched again before
+    the backward pass has run (``RuntimeError``)."""
     _eager_only()
+    batch.require_current()
     _training.require_tensor(expert_output, "expert_output", batch.packed.shape, batch.workspace.dtype,
                              batch.workspace.device)
     _training.require_tensor(weights, "weights", batch.inverse.shape, torch.float32, batch.workspace.device)

@@ -433,6 +433,7 @@ class _FusedLaunches:
         self.device_index = x.device.index if x.device.index is not None else torch.cuda.current_device()
         self.fingerprint = self._fingerprint(block)
         self.keep = (ids32, ids64, weights, t, state)  # the buffers below stay allocated
+        self.transport = t
         self.output = t.output
         tokens, hidden = x.shape
         scratch = block._router_scratch
@@ -498,6 +499,7 @@ class _FusedLaunches:
 
     def __call__(self, block, x):
         router_weight, split_of = block._router_split_plan()
+        self.transport.dispatches += 1
         status = self.lib.moe_block_forward(self.args_address, x.data_ptr(), router_weight,
                                             current_stream_handle(self.device_index))
         if status:

@@ -12,7 +12,7 @@ maximum back to the host in one transfer (it synchronises the stream): hot
 loops should validate once and then call ``CudaWorkspace.dispatch`` directly.
 """
 
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 
 import torch
 
@@ -26,13 +26,24 @@ _ID_DTYPES = (torch.int32, torch.int64)
 class PackedTokens:
     """The packed rows, inverse map, counts and offsets of one dispatch, as views of
     its workspace's buffers: the next call on that workspace overwrites them, so
-    clone what must outlive it."""
+    clone what must outlive it. ``dispatches`` is the workspace's count when the batch was
+    formed; the transport's gradients raise ``RuntimeError`` once it has moved on. A
+    dispatch replayed from a graph moves no count: that its buffers are still the batch's is
+    the program's to know."""
 
     packed: torch.Tensor
     inverse: torch.Tensor
     counts: torch.Tensor
     offsets: torch.Tensor
     workspace: CudaWorkspace
+    dispatches: int = field(init=False, repr=False, compare=False)
+
+    def __post_init__(self):
+        object.__setattr__(self, "dispatches", getattr(self.workspace, "dispatches", 0))
+
+    def require_current(self):
+        if self.dispatches != getattr(self.workspace, "dispatches", 0):
+            raise RuntimeError("the batch's workspace has been dispatched again: its index buffers are another batch's")
 
 
 # (predicate over (x, ids, experts), exception type, message), checked in order.

@@ -243,9 +243,10 @@ def combine_backward(grad_output, expert_output, batch, weights):
     """Gradients of ``combine(expert_output, batch, weights)``: ``(grad_expert_output, grad_weights)``.
 
     ``batch`` is the ``PackedTokens`` of the dispatch, its workspace not dispatched again
-    since. grad_expert_output has the packed rows' shape and dtype; rows that hold no
+    since (``RuntimeError``). grad_expert_output has the packed rows' shape and dtype; rows that hold no
     assignment (padding) are zero. grad_weights is fp32 [T, K].
     """
+    batch.require_current()
     workspace = batch.workspace
     tokens, hidden, experts, topk = workspace.shape
     dtype, device = workspace.dtype, workspace.device
@@ -268,7 +269,8 @@ def combine_backward(grad_output, expert_output, batch, weights):
 
 def dispatch_backward(grad_packed, batch):
     """Gradient of ``dispatch(x, ...)``: [T, H], each token's K packed rows' gradients summed
-    in fp32 in k order and rounded once."""
+    in fp32 in k order and rounded once. ``batch`` as in ``combine_backward``."""
+    batch.require_current()
     workspace = batch.workspace
     tokens, hidden, _, topk = workspace.shape
     dtype, device = workspace.dtype, workspace.device

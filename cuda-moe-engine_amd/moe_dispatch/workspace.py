@@ -24,7 +24,8 @@ of ``packed``, ``row_src`` receives each packed row's token (-1 for padding),
 which the gathered gate/up GEMM reads x through.
 
 One workspace serves one invocation at a time: its outputs are views that the
-next call overwrites.
+next call overwrites. ``dispatches`` counts the calls that wrote its index buffers, so that
+a ``PackedTokens`` can tell whether they are still its own.
 """
 
 import torch
@@ -185,12 +186,14 @@ class CudaWorkspace:
             "row_src": ((rows,), torch.int32),
         }
         self._names = tuple(layout)
+        self.dispatches = 0
         for name, (shape, kind) in layout.items():
             setattr(self, name, torch.empty(shape, device=device, dtype=kind))
         self._bound = _Bound(self)
 
     def dispatch(self, x, ids32, ids64=None):
         """Hot path: contiguous x[T,H] and int32 ids[T,K] with in-range ids (ids64 is unused)."""
+        self.dispatches += 1
         self._bound.dispatch(x, ids32)
 
     def dispatch_ranked(self, x, ids32):
@@ -198,17 +201,20 @@ class CudaWorkspace:
         and ``tile_counts`` for these ids (``rank_tile`` > 0): the pack pass only."""
         if self.rank_tile <= 0:
             raise RuntimeError("this workspace's shape has no ranked route (rank_tile == 0)")
+        self.dispatches += 1
         self._bound.dispatch_ranked(x, ids32)
 
     def dispatch_rows(self, ids32):
         """The dispatch layout (counts, offsets, slots, inverse) without copying
         rows: ``row_src`` receives each packed row's token, -1 for padding rows."""
+        self.dispatches += 1
         self._bound.dispatch_rows(ids32, ranked=False)
 
     def dispatch_ranked_rows(self, ids32):
         """dispatch_rows() after a ranked route (as ``dispatch_ranked``)."""
         if self.rank_tile <= 0:
             raise RuntimeError("this workspace's shape has no ranked route (rank_tile == 0)")
+        self.dispatches += 1
         self._bound.dispatch_rows(ids32, ranked=True)
 
     def combine(self, expert_output, weights):

@@ -1,0 +1,68 @@
+"""Buffers that are used again between a forward and its backward pass."""
+
+import pytest
+import torch
+
+from moe_dispatch import MoEBlock, MoEConfig, autograd, combine_backward, dispatch, dispatch_backward
+from moe_dispatch.ops import PackedTokens
+from tests._helpers import gpu
+
+pytestmark = gpu
+
+BF16 = torch.bfloat16
+
+
+def _normal(g, *shape, dtype=BF16):
+    return torch.randn(*shape, device="cuda", generator=g).to(dtype)
+
+
+def _ids(g, tokens, experts, topk):
+    return torch.randint(0, experts, (tokens, topk), device="cuda", generator=g, dtype=torch.int32)
+
+
+@pytest.mark.parametrize("again", ["ops", "workspace"])
+def test_a_batch_of_an_earlier_dispatch_gets_no_gradients(again):
+    """The second dispatch has put its own rows where the first batch's views look."""
+    g = torch.Generator(device="cuda").manual_seed(0)
+    tokens, hidden, experts, topk = 50, 64, 4, 2
+    x = _normal(g, tokens, hidden).requires_grad_()
+    ids, others = _ids(g, tokens, experts, topk), _ids(g, tokens, experts, topk)
+    weights = torch.rand(tokens, topk, device="cuda", generator=g).requires_grad_()
+    packed, batch = autograd.dispatch(x, ids, experts)
+    out = autograd.combine(packed * 2, batch, weights)
+    y, dout = _normal(g, *batch.packed.shape), _normal(g, tokens, hidden)
+    want = combine_backward(dout, y, batch, weights.detach())
+    if again == "ops":
+        second = dispatch(x.detach(), others, experts, workspace=batch.workspace)
+    else:
+        workspace = batch.workspace
+        workspace.dispatch(x.detach(), others)
+        second = PackedTokens(workspace.packed, workspace.inverse, workspace.counts, workspace.offsets, workspace)
+    for call in (lambda: out.sum().backward(), lambda: packed.float().sum().backward(),
+                 lambda: combine_backward(dout, y, batch, weights.detach()), lambda: dispatch_backward(y, batch),
+                 lambda: autograd.combine(packed, batch, weights)):
+        with pytest.raises(RuntimeError, match="dispatched again"):
+            call()
+    # The second batch is current; dispatched as the first was, so is a third.
+    assert not torch.equal(combine_backward(dout, y, second, weights.detach())[1], want[1])
+    third = dispatch(x.detach(), ids, experts, workspace=batch.workspace)
+    for a, b in zip(combine_backward(dout, y, third, weights.detach()), want):
+        assert torch.equal(a, b)
+
+
+def test_a_batch_of_a_blocks_transport_ends_with_the_next_forward():
+    """Both forms of a block's forward write its transport's index buffers."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    block = MoEBlock(MoEConfig(hidden=64, intermediate=128, experts=4, topk=2), device="cuda:0",
+                     implementation="cuda_fused", seed=0)
+    x = _normal(g, 40, 64)
+    grad = None
+    for _ in range(3):  # validated, then by one native call
+        block(x)
+        t = block.workspace(x).transport
+        batch = PackedTokens(t.packed, t.inverse, t.counts, t.offsets, t)
+        grad = _normal(g, *t.packed.shape)
+        dispatch_backward(grad, batch)
+        block(x)
+        with pytest.raises(RuntimeError, match="dispatched again"):
+            dispatch_backward(grad, batch)
