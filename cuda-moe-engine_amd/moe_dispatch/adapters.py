@@ -37,6 +37,11 @@ class AdapterGroups:
     ``assign(ids)`` groups the rows by their int32 adapter ids [T]; an id outside
     [0, adapters) means no adapter. The groups hold until the next ``assign``. One object
     serves one sequential stream of calls; a graph that captured its calls needs it kept.
+
+    The first ``assign`` must run, not be captured (``RuntimeError``): a captured one writes
+    nothing before its graph is replayed, and calls before that would read row numbers that
+    nobody wrote. A replayed ``assign`` changes the groups without a host call:
+    ``low_rank_backward`` cannot tell that a ``hidden`` is older than it.
     """
 
     def __init__(self, tokens, adapters, *, device="cuda", extension=None):
@@ -59,6 +64,9 @@ class AdapterGroups:
 
     def assign(self, ids):
         require_tensor(ids, "ids", (self.tokens,), torch.int32, self.device)
+        if self.assignment == 0 and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("assign the groups once before capturing: until the graph's first replay they would "
+                               "hold no rows' numbers")
         lib = self.extension.lib
         with on_device(self.device):
             lib.check(lib.moe_adapter_group(ids.data_ptr(), self.table.data_ptr(), self.table_bytes, self.tokens,

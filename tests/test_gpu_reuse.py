@@ -3,7 +3,8 @@
 import pytest
 import torch
 
-from moe_dispatch import MoEBlock, MoEConfig, autograd, combine_backward, dispatch, dispatch_backward
+from moe_dispatch import (AdapterGroups, MoEBlock, MoEConfig, autograd, combine_backward, dispatch, dispatch_backward,
+                          low_rank_add)
 from moe_dispatch.ops import PackedTokens
 from tests._helpers import gpu
 
@@ -66,3 +67,34 @@ def test_a_batch_of_a_blocks_transport_ends_with_the_next_forward():
         block(x)
         with pytest.raises(RuntimeError, match="dispatched again"):
             dispatch_backward(grad, batch)
+
+
+def test_a_captured_assignment_takes_effect_when_it_is_replayed():
+    """Between capture and replay the groups are those of the last assignment that ran."""
+    g = torch.Generator(device="cuda").manual_seed(2)
+    x, base = _normal(g, 70, 64), _normal(g, 70, 72)
+    down, up = _normal(g, 3, 8, 64), _normal(g, 3, 8, 72)
+    first, second = (torch.randint(-1, 3, (70,), device="cuda", generator=g, dtype=torch.int32) for _ in range(2))
+
+    def alone(ids):
+        groups = AdapterGroups(70, 3)
+        groups.assign(ids)
+        return low_rank_add(base, x, down, up, groups)
+
+    want = alone(first), alone(second)
+    assert not torch.equal(*want)
+    groups = AdapterGroups(70, 3)
+    groups.assign(first)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        groups.assign(second)
+        captured = low_rank_add(base, x, down, up, groups)
+    assert torch.equal(low_rank_add(base, x, down, up, groups), want[0])
+    for _ in range(3):
+        captured.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(captured, want[1])
+        assert torch.equal(low_rank_add(base, x, down, up, groups), want[1])
+        groups.assign(first)
+        assert torch.equal(low_rank_add(base, x, down, up, groups), want[0])

@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from moe_dispatch import autograd, combine_backward, dispatch_backward
+from moe_dispatch import AdapterGroups, autograd, combine_backward, dispatch_backward
 from moe_dispatch.ops import PackedTokens
 
 
@@ -27,3 +27,12 @@ def test_gradients_refuse_a_batch_whose_workspace_was_dispatched_again():
             call()
     # A batch formed after that dispatch is current.
     PackedTokens(torch.zeros(8, 16), *indices, workspace).require_current()
+
+
+def test_the_first_assignment_is_not_captured(monkeypatch):
+    groups = object.__new__(AdapterGroups)
+    groups.tokens, groups.device, groups.assignment = 4, torch.device("cpu"), 0
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="before capturing"):
+        groups.assign(torch.zeros(4, dtype=torch.int32))
+    assert groups.assignment == 0
