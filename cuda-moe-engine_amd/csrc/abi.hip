@@ -240,9 +240,10 @@ static int check_dispatch(const void* x, int dtype, const int32_t* ids, int32_t*
     MOE_REQUIRE(experts >= 1 && experts <= kMaxExperts, MOE_ERR_UNSUPPORTED, "supports 1..64 experts");
     MOE_REQUIRE(topk >= 1 && topk <= kMaxTopk, MOE_ERR_UNSUPPORTED, "topk must be in 1..8");
     MOE_REQUIRE(alignment >= 1 && alignment <= 128, MOE_ERR_INVALID_ARGUMENT, "alignment must be 1..128");
+    MOE_REQUIRE(tokens <= INT_MAX / topk, MOE_ERR_CAPACITY, "shape exceeds int32 indexing capacity");
     const int64_t n = tokens * topk;
     const int64_t required = aligned_capacity(n, experts, alignment);
-    MOE_REQUIRE(n <= INT_MAX && hidden <= INT_MAX && required <= INT_MAX, MOE_ERR_CAPACITY,
+    MOE_REQUIRE(hidden <= INT_MAX && required <= INT_MAX, MOE_ERR_CAPACITY,
                 "shape exceeds int32 indexing capacity");
     MOE_REQUIRE(packed_rows >= required, MOE_ERR_WORKSPACE,
                 "packed workspace has %lld rows, needs %lld", (long long)packed_rows,
@@ -323,9 +324,10 @@ static int check_dispatch_rows(const int32_t* ids, int32_t* counts, int32_t* off
     MOE_REQUIRE(experts >= 1 && experts <= kMaxExperts, MOE_ERR_UNSUPPORTED, "supports 1..64 experts");
     MOE_REQUIRE(topk >= 1 && topk <= kMaxTopk, MOE_ERR_UNSUPPORTED, "topk must be in 1..8");
     MOE_REQUIRE(alignment >= 1 && alignment <= 128, MOE_ERR_INVALID_ARGUMENT, "alignment must be 1..128");
+    MOE_REQUIRE(tokens <= INT_MAX / topk, MOE_ERR_CAPACITY, "shape exceeds int32 indexing capacity");
     const int64_t n = tokens * topk;
     const int64_t required = aligned_capacity(n, experts, alignment);
-    MOE_REQUIRE(n <= INT_MAX && required <= INT_MAX, MOE_ERR_CAPACITY, "shape exceeds int32 indexing capacity");
+    MOE_REQUIRE(required <= INT_MAX, MOE_ERR_CAPACITY, "shape exceeds int32 indexing capacity");
     MOE_REQUIRE(packed_rows >= required, MOE_ERR_WORKSPACE, "row table has %lld rows, needs %lld",
                 (long long)packed_rows, (long long)required);
     MOE_REQUIRE(counts && offsets, MOE_ERR_INVALID_ARGUMENT, "null pointer");
@@ -414,7 +416,7 @@ int moe_combine(const void* expert_output, int dtype, const int32_t* inverse,
     MOE_REQUIRE(valid_dtype(dtype), MOE_ERR_INVALID_ARGUMENT, "unsupported output dtype");
     MOE_REQUIRE(topk >= 1 && topk <= kMaxTopk, MOE_ERR_UNSUPPORTED, "topk must be in 1..8");
     MOE_REQUIRE(tokens >= 0 && hidden > 0, MOE_ERR_INVALID_ARGUMENT, "invalid output shape");
-    MOE_REQUIRE(tokens * topk <= INT_MAX && hidden <= INT_MAX && packed_rows <= INT_MAX,
+    MOE_REQUIRE(tokens <= INT_MAX / topk && hidden <= INT_MAX && packed_rows <= INT_MAX,
                 MOE_ERR_CAPACITY, "invalid output shape");
     MOE_REQUIRE(packed_rows >= tokens * topk, MOE_ERR_INVALID_ARGUMENT, "shape/dtype mismatch");
     if (tokens == 0) return MOE_OK;
@@ -693,7 +695,7 @@ int moe_combine_backward(const void* grad_output, const void* expert_output, int
     MOE_REQUIRE(topk >= 1 && topk <= kMaxTopk, MOE_ERR_UNSUPPORTED, "topk must be in 1..8");
     MOE_REQUIRE(experts >= 1 && experts <= kMaxExperts, MOE_ERR_UNSUPPORTED, "supports 1..64 experts");
     MOE_REQUIRE(tokens >= 0 && hidden > 0, MOE_ERR_INVALID_ARGUMENT, "invalid shape");
-    MOE_REQUIRE(tokens * topk <= INT_MAX && hidden <= INT_MAX && packed_rows <= INT_MAX, MOE_ERR_CAPACITY,
+    MOE_REQUIRE(tokens <= INT_MAX / topk && hidden <= INT_MAX && packed_rows <= INT_MAX, MOE_ERR_CAPACITY,
                 "shape exceeds int32 indexing capacity");
     MOE_REQUIRE(packed_rows >= tokens * topk, MOE_ERR_INVALID_ARGUMENT, "packed rows hold fewer than the assignments");
     if (packed_rows == 0) return MOE_OK;
@@ -716,7 +718,7 @@ int moe_dispatch_backward(const void* grad_packed, int dtype, const int32_t* inv
     MOE_REQUIRE(valid_dtype(dtype), MOE_ERR_INVALID_ARGUMENT, "only FP32, FP16 and BF16 are supported");
     MOE_REQUIRE(topk >= 1 && topk <= kMaxTopk, MOE_ERR_UNSUPPORTED, "topk must be in 1..8");
     MOE_REQUIRE(tokens >= 0 && hidden > 0, MOE_ERR_INVALID_ARGUMENT, "invalid shape");
-    MOE_REQUIRE(tokens * topk <= INT_MAX && hidden <= INT_MAX && packed_rows <= INT_MAX, MOE_ERR_CAPACITY,
+    MOE_REQUIRE(tokens <= INT_MAX / topk && hidden <= INT_MAX && packed_rows <= INT_MAX, MOE_ERR_CAPACITY,
                 "shape exceeds int32 indexing capacity");
     MOE_REQUIRE(packed_rows >= tokens * topk, MOE_ERR_INVALID_ARGUMENT, "packed rows hold fewer than the assignments");
     if (tokens == 0) return MOE_OK;
