@@ -52,7 +52,8 @@ int launch_route_backward(const uint16_t*, const float*, const float*, const flo
 int launch_combine_grad(const void*, const void*, int, const int32_t*, const float*, const int32_t*, const int32_t*,
                         void*, float*, int64_t, int64_t, int, int, int64_t, hipStream_t);
 int launch_adapter_group(const int32_t*, void*, int64_t, int, hipStream_t);
-int64_t low_rank_scratch_bytes(int64_t, int64_t, int64_t, int64_t, int64_t, bool);
+int64_t low_rank_add_scratch_bytes(int64_t, int64_t, int64_t, int64_t, int64_t);
+int64_t low_rank_backward_scratch_bytes(int64_t, int64_t, int64_t, int64_t, int64_t, bool, bool, bool);
 int launch_low_rank_add(const uint16_t*, const uint16_t*, const uint16_t*, const float*, const void*, const uint16_t*,
                         uint16_t*, float*, char*, int64_t, int64_t, int64_t, int, int, hipStream_t);
 int launch_low_rank_backward(const uint16_t*, const uint16_t*, const uint16_t*, const uint16_t*, const float*,
@@ -764,17 +765,19 @@ int64_t moe_low_rank_scratch_bytes(int64_t tokens, int64_t hidden, int64_t width
     if (tokens < 0 || tokens > kMaxAdapterTokens || adapters < 1 || adapters > kMaxAdapters ||
         !valid_low_rank_width(hidden) || !valid_low_rank_width(width) || rank < 1 || rank > kMaxRank)
         return -1;
-    return low_rank_scratch_bytes(tokens, hidden, width, rank, adapters, backward != 0);
+    if (backward == 0) return low_rank_add_scratch_bytes(tokens, hidden, width, rank, adapters);
+    return low_rank_backward_scratch_bytes(tokens, hidden, width, rank, adapters, !(backward & MOE_WITHOUT_GRAD_X),
+                                           !(backward & MOE_WITHOUT_GRAD_DOWN), !(backward & MOE_WITHOUT_GRAD_UP));
 }
 
 static int check_low_rank(const void* table, int64_t table_bytes, const void* scratch, int64_t scratch_bytes,
-                          int64_t tokens, int64_t hidden, int64_t width, int64_t rank, int64_t adapters, bool backward) {
+                          int64_t tokens, int64_t hidden, int64_t width, int64_t rank, int64_t adapters, int backward) {
     const int rc = check_adapter_table(table, table_bytes, tokens, adapters);
     if (rc != MOE_OK) return rc;
     MOE_REQUIRE(valid_low_rank_width(hidden) && valid_low_rank_width(width), MOE_ERR_UNSUPPORTED,
                 "low-rank widths must be multiples of 8 up to %lld", (long long)kMaxLowRankWidth);
     MOE_REQUIRE(rank >= 1 && rank <= kMaxRank, MOE_ERR_UNSUPPORTED, "rank must be in 1..%d", kMaxRank);
-    const int64_t need = low_rank_scratch_bytes(tokens, hidden, width, rank, adapters, backward);
+    const int64_t need = moe_low_rank_scratch_bytes(tokens, hidden, width, rank, adapters, backward);
     MOE_REQUIRE((scratch || need == 0) && scratch_bytes >= need, MOE_ERR_WORKSPACE,
                 "low-rank scratch needs %lld bytes, got %lld", (long long)need, (long long)scratch_bytes);
     MOE_REQUIRE(aligned_to(scratch, 16), MOE_ERR_INVALID_ARGUMENT, "scratch must be 16-byte aligned");
@@ -785,8 +788,7 @@ int moe_low_rank_add(const void* x, const void* down, const void* up, const floa
                      int64_t table_bytes, const void* base, void* output, float* hidden_out, void* scratch,
                      int64_t scratch_bytes, int64_t tokens, int64_t hidden, int64_t width, int64_t rank,
                      int64_t adapters, void* stream) {
-    const int rc = check_low_rank(table, table_bytes, scratch, scratch_bytes, tokens, hidden, width, rank, adapters,
-                                  false);
+    const int rc = check_low_rank(table, table_bytes, scratch, scratch_bytes, tokens, hidden, width, rank, adapters, 0);
     if (rc != MOE_OK || tokens == 0) return rc;
     MOE_REQUIRE(x && down && up && output, MOE_ERR_INVALID_ARGUMENT, "null pointer");
     MOE_REQUIRE(aligned_to(x, 16) && aligned_to(down, 16) && aligned_to(up, 16) && aligned_to(base, 16) &&
@@ -803,7 +805,10 @@ int moe_low_rank_backward(const void* grad_output, const void* x, const void* do
                           void* grad_x, void* grad_down, void* grad_up, int grad_dtype, void* scratch,
                           int64_t scratch_bytes, int64_t tokens, int64_t hidden, int64_t width, int64_t rank,
                           int64_t adapters, void* stream) {
-    const int rc = check_low_rank(table, table_bytes, scratch, scratch_bytes, tokens, hidden, width, rank, adapters, true);
+    const int wanted = 1 | (grad_x ? 0 : MOE_WITHOUT_GRAD_X) | (grad_down ? 0 : MOE_WITHOUT_GRAD_DOWN) |
+                       (grad_up ? 0 : MOE_WITHOUT_GRAD_UP);
+    const int rc =
+        check_low_rank(table, table_bytes, scratch, scratch_bytes, tokens, hidden, width, rank, adapters, wanted);
     if (rc != MOE_OK) return rc;
     MOE_REQUIRE(grad_dtype == MOE_DTYPE_F32 || grad_dtype == MOE_DTYPE_BF16, MOE_ERR_INVALID_ARGUMENT,
                 "adapter gradients are FP32 or BF16");

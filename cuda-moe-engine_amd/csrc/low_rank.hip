@@ -1405,13 +1405,30 @@ static int64_t through_bytes(int64_t tokens, int64_t k, int64_t width, int64_t r
     return contract_slices(table_layout(tokens, adapters).tile_bound, k, rank) * tokens * rank * 4;
 }
 
-// Forward: contract's sums. Backward: those of dh, dh itself, the two products' partial sums.
-int64_t low_rank_scratch_bytes(int64_t tokens, int64_t hidden, int64_t width, int64_t rank, int64_t adapters,
-                               bool backward) {
-    const TableLayout t = table_layout(tokens, adapters);
-    if (!backward) return through_bytes(tokens, hidden, width, rank, adapters);
-    return up16(through_bytes(tokens, width, hidden, rank, adapters)) + up16(tokens * rank * 4) +
-           static_cast<int64_t>(t.split_bound) * rank * (hidden + width) * 4;
+int64_t low_rank_add_scratch_bytes(int64_t tokens, int64_t hidden, int64_t width, int64_t rank, int64_t adapters) {
+    return through_bytes(tokens, hidden, width, rank, adapters);
+}
+
+// Where the backward pass' scratch lies: contract's sums of dh and dh itself (for grad_x and
+// grad_down), and the partial sums of the products that are wanted.
+struct BackwardScratch {
+    int64_t dh, down, up, bytes;
+};
+static BackwardScratch backward_scratch(int64_t tokens, int64_t hidden, int64_t width, int64_t rank, int64_t adapters,
+                                        bool want_x, bool want_down, bool want_up) {
+    const int64_t rows = static_cast<int64_t>(table_layout(tokens, adapters).split_bound) * rank;
+    BackwardScratch s{};
+    if (want_x || want_down) {
+        s.dh = up16(through_bytes(tokens, width, hidden, rank, adapters));
+        s.down = s.dh + up16(tokens * rank * 4);
+    }
+    s.up = s.down + (want_down ? rows * hidden * 4 : 0);
+    s.bytes = s.up + (want_up ? rows * width * 4 : 0);
+    return s;
+}
+int64_t low_rank_backward_scratch_bytes(int64_t tokens, int64_t hidden, int64_t width, int64_t rank, int64_t adapters,
+                                        bool want_x, bool want_down, bool want_up) {
+    return backward_scratch(tokens, hidden, width, rank, adapters, want_x, want_down, want_up).bytes;
 }
 
 int launch_low_rank_add(const uint16_t* x, const uint16_t* down, const uint16_t* up, const float* scales,
@@ -1427,10 +1444,9 @@ int launch_low_rank_backward(const uint16_t* grad_output, const uint16_t* x, con
                              uint16_t* grad_x, void* grad_down, void* grad_up, bool grad_bf16, char* scratch,
                              int64_t tokens, int64_t hidden, int64_t width, int rank, int adapters, hipStream_t stream) {
     const Groups g = groups_of(table, tokens, adapters);
+    const BackwardScratch at = backward_scratch(tokens, hidden, width, rank, adapters, grad_x, grad_down, grad_up);
     float* dh_parts = reinterpret_cast<float*>(scratch);
-    scratch += up16(through_bytes(tokens, width, hidden, rank, adapters));
-    float* dh = reinterpret_cast<float*>(scratch);
-    float* partials = reinterpret_cast<float*>(scratch + up16(tokens * rank * 4));
+    float* dh = reinterpret_cast<float*>(scratch + at.dh);
     int rc = MOE_OK;
     // dx, and dh for its outer product.
     if (tokens > 0 && (grad_x || grad_down))
@@ -1438,9 +1454,8 @@ int launch_low_rank_backward(const uint16_t* grad_output, const uint16_t* x, con
                             rank, adapters, stream);
     if (rc == MOE_OK && (grad_down || grad_up)) {
         OuterJob jobs[2];
-        if (grad_down) jobs[0] = {dh, x, partials, grad_down, hidden};
-        if (grad_up)
-            jobs[1] = {hidden_in, grad_output, partials + g.split_bound * rank * hidden, grad_up, width};
+        if (grad_down) jobs[0] = {dh, x, reinterpret_cast<float*>(scratch + at.down), grad_down, hidden};
+        if (grad_up) jobs[1] = {hidden_in, grad_output, reinterpret_cast<float*>(scratch + at.up), grad_up, width};
         rc = launch_outer(jobs[0], jobs[1], scales, g, grad_bf16, tokens, rank, adapters, stream);
     }
     return rc;

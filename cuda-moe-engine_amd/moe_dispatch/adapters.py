@@ -99,7 +99,7 @@ class _Sizes(NamedTuple):
     width: int
     rank: int
     forward_bytes: int
-    backward_bytes: int
+    backward_bytes: dict  # by which gradients are wanted
 
 
 def _check_sizes(x, down, up, groups):
@@ -117,7 +117,7 @@ def _check_sizes(x, down, up, groups):
     if not 1 <= rank <= MAX_RANK:
         raise ValueError("rank must be in 1..128")
     need = groups.extension.lib.moe_low_rank_scratch_bytes
-    sizes = _Sizes(hidden, width, rank, *(need(tokens, hidden, width, rank, adapters, b) for b in (0, 1)))
+    sizes = _Sizes(hidden, width, rank, need(tokens, hidden, width, rank, adapters, 0), {})
     groups._sizes[(x.shape, down.shape, up.shape)] = sizes
     return sizes
 
@@ -186,7 +186,7 @@ def low_rank_backward(grad_output, x, down, up, groups, *, scales=None, hidden, 
     no gradient. ``gradients``: which of the three are wanted; the others are None and
     cost nothing.
     """
-    h, width, rank, _, need = _check_operands(x, down, up, groups, scales)
+    h, width, rank, _, scratch_bytes = _check_operands(x, down, up, groups, scales)
     tokens, device = groups.tokens, groups.device
     require_tensor(grad_output, "grad_output", (tokens, width), torch.bfloat16, device)
     if not isinstance(hidden, LowRankHidden):
@@ -202,14 +202,19 @@ def low_rank_backward(grad_output, x, down, up, groups, *, scales=None, hidden, 
     lib = groups.extension.lib
     with on_device(device):
         want_x, want_down, want_up = gradients
+        without = (0 if want_x else 2) + (0 if want_down else 4) + (0 if want_up else 8)  # MOE_WITHOUT_GRAD_*
+        need = scratch_bytes.get(without)
+        if need is None:
+            need = scratch_bytes[without] = lib.moe_low_rank_scratch_bytes(tokens, h, width, rank, groups.adapters,
+                                                                           1 + without)
         out_x = torch.empty_like(x) if want_x else None
         grad_down = torch.empty_like(down, dtype=grad_dtype) if want_down else None
         grad_up = torch.empty_like(up, dtype=grad_dtype) if want_up else None
-        scratch = x.new_empty(need // 2)
+        scratch = x.new_empty(need // 2) if need else None
         lib.check(lib.moe_low_rank_backward(
             grad_output.data_ptr(), x.data_ptr(), down.data_ptr(), up.data_ptr(), _ptr(scales),
             groups.table.data_ptr(), groups.table_bytes, hidden.values.data_ptr(), _ptr(grad_x),
-            _ptr(out_x), _ptr(grad_down), _ptr(grad_up), DTYPE_CODES[grad_dtype], scratch.data_ptr(),
+            _ptr(out_x), _ptr(grad_down), _ptr(grad_up), DTYPE_CODES[grad_dtype], _ptr(scratch),
             need, tokens, h, width, rank, groups.adapters, current_stream_handle(device.index)),
             "low_rank_backward")
     return out_x, grad_down, grad_up

@@ -487,8 +487,14 @@ int64_t moe_adapter_table_bytes(int64_t tokens, int64_t adapters);
 int moe_adapter_group(const int32_t* ids, void* table, int64_t table_bytes, int64_t tokens, int64_t adapters,
                       void* stream);
 
-/* Bytes of scratch moe_low_rank_add (backward == 0; 0: none) or moe_low_rank_backward needs;
- * -1 for invalid sizes. */
+/* What moe_low_rank_scratch_bytes' backward leaves out. */
+#define MOE_WITHOUT_GRAD_X 2
+#define MOE_WITHOUT_GRAD_DOWN 4
+#define MOE_WITHOUT_GRAD_UP 8
+
+/* Bytes of scratch moe_low_rank_add (backward == 0) or moe_low_rank_backward needs (0: none);
+ * -1 for invalid sizes. backward is 1 for all three gradients, and any of MOE_WITHOUT_GRAD_* besides
+ * for a call that passes NULL for them: scratch for one that is not wanted is not asked for. */
 int64_t moe_low_rank_scratch_bytes(int64_t tokens, int64_t hidden, int64_t width, int64_t rank, int64_t adapters,
                                    int backward);
 

@@ -19,3 +19,31 @@ def test_tokens_times_topk_is_bounded_before_it_is_formed(tokens, topk):
     assert lib.moe_dispatch_backward(A, 2, A, A, tokens, 64, topk, 8, None) == capacity
     assert lib.moe_dispatch(A, 2, A, A, A, A, A, A, A, 1 << 40, tokens, 64, 8, topk, 1, 8, 1, None) == capacity
     assert lib.moe_dispatch_rows(A, A, A, A, A, A, A, 1 << 40, tokens, 8, topk, 1, 8, None) == capacity
+
+
+def test_gradients_that_are_not_wanted_ask_for_no_scratch():
+    lib = _lib.load_library()
+    tokens, hidden, width, rank, adapters = 4096, 4096, 1408, 16, 8
+
+    def need(backward):
+        return lib.moe_low_rank_scratch_bytes(tokens, hidden, width, rank, adapters, backward)
+
+    x, down, up = 2, 4, 8  # MOE_WITHOUT_GRAD_*
+    assert need(1 + x + down + up) == 0
+    # Without both products: dh's sums and dh, no partial sums of a whole gradient's size.
+    assert tokens * rank * 4 <= need(1 + down + up) <= (16 + 1) * tokens * rank * 4
+    partial_down, partial_up = need(1 + up) - need(1 + down + up), need(1 + down) - need(1 + down + up)
+    assert partial_down > 0 and partial_up > 0 and partial_down * width == partial_up * hidden
+    assert need(1) == need(1 + x) == need(1 + down + up) + partial_down + partial_up
+    assert need(1 + x + down) == partial_up and need(1 + x + up) == need(1 + up)
+
+
+@stand_in_addresses
+def test_a_backward_call_is_held_to_the_scratch_of_its_gradients():
+    lib = _lib.load_library()
+    sizes = 4096, 4096, 1408, 40, 8
+    table = lib.moe_adapter_table_bytes(4096, 8)
+    for grads, without in (((A, None, None), 12), ((None, A, None), 10), ((None, None, A), 6), ((A, A, None), 8)):
+        need = lib.moe_low_rank_scratch_bytes(*sizes, 1 + without)
+        back = (lambda nbytes: lib.moe_low_rank_backward(A, A, A, A, A, A, table, A, A, *grads, 0, A, nbytes, *sizes, None))
+        assert back(need - 1) == 4 and back(need) == 5  # workspace too small; no GPU to launch on

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from moe_dispatch import (AdapterGroups, MoEBlock, MoEConfig, autograd, combine_backward, dispatch, dispatch_backward,
-                          low_rank_add)
+                          low_rank_add, low_rank_backward)
 from moe_dispatch.ops import PackedTokens
 from tests._helpers import gpu
 
@@ -98,3 +98,23 @@ def test_a_captured_assignment_takes_effect_when_it_is_replayed():
         assert torch.equal(low_rank_add(base, x, down, up, groups), want[1])
         groups.assign(first)
         assert torch.equal(low_rank_add(base, x, down, up, groups), want[0])
+
+
+def test_the_gradient_of_x_alone_takes_no_memory_of_the_others():
+    """Frozen adapters: no scratch of the size of their gradients."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    tokens, hidden, rank, adapters = 4096, 1024, 16, 64
+    x, grad = _normal(g, tokens, hidden), _normal(g, tokens, hidden)
+    down, up = _normal(g, adapters, rank, hidden), _normal(g, adapters, rank, hidden)
+    groups = AdapterGroups(tokens, adapters)
+    groups.assign(torch.randint(0, adapters, (tokens,), device="cuda", generator=g, dtype=torch.int32))
+    _, kept = low_rank_add(None, x, down, up, groups, return_hidden=True)
+    want = low_rank_backward(grad, x, down, up, groups, hidden=kept)[0]
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    got, _, _ = low_rank_backward(grad, x, down, up, groups, hidden=kept, gradients=(True, False, False))
+    peak = torch.cuda.max_memory_allocated() - before
+    assert torch.equal(got, want)
+    # The result, dh and up to sixteen slices' sums of it, and the allocator's 512-byte steps.
+    assert peak <= tokens * hidden * 2 + 17 * tokens * rank * 4 + 4096
