@@ -23,14 +23,15 @@ constexpr int kMaxSplitRows = 1024;
 //   head         [4]     tiles, splits, 0, 0
 //   order        [T]     rows sorted by adapter (stable); rows of no adapter last
 //   starts       [N + 2] first sorted row of each adapter, of the rows of none, T
-//   split_start  [N + 1] first split of each adapter
+//   partial_start [N + 1] first partial sum of each adapter: a split's of those that have several
 //   tiles        [tile_bound]  {adapter (-1: none), first sorted row, rows <= kTileRows, 0}
-//   splits       [split_bound] {adapter, first sorted row, rows <= split_rows, adapter's splits}
+//   splits       [split_bound] {adapter, first sorted row, rows <= split_rows, partial sum (-1: the
+//                        adapter's only split)}
 //   chunks       [chunk_count][N + 1]  while it is made, of a batch of more rows than a chunk:
 //                        each chunk's rows of each adapter, then those of the chunks before
 struct TableLayout {
-    int64_t order, starts, split_start, tiles, splits, chunks, ints;
-    int tile_bound, split_bound, split_rows, chunk_count;
+    int64_t order, starts, partial_start, tiles, splits, chunks, ints;
+    int tile_bound, split_bound, partial_bound, split_rows, chunk_count;
 };
 
 // Rows per split of the outer product: a split's partial result is written and read
@@ -49,10 +50,14 @@ inline TableLayout table_layout(int64_t tokens, int64_t adapters) {
     // Each group has at most one partial tile (split).
     t.tile_bound = static_cast<int>(tokens / kTileRows + (adapters + 1 < tokens ? adapters + 1 : tokens));
     t.split_bound = static_cast<int>(tokens / t.split_rows + (adapters < tokens ? adapters : tokens));
+    // An adapter of n > split_rows rows has fewer than 2 n / split_rows splits; the others' one
+    // split writes the result itself, so that a large bank asks for no more partial sums.
+    const int64_t partials = tokens > t.split_rows ? 2 * tokens / t.split_rows : 0;
+    t.partial_bound = partials < t.split_bound ? static_cast<int>(partials) : t.split_bound;
     t.order = 4;
     t.starts = t.order + up4(tokens);
-    t.split_start = t.starts + up4(adapters + 2);
-    t.tiles = t.split_start + up4(adapters + 1);
+    t.partial_start = t.starts + up4(adapters + 2);
+    t.tiles = t.partial_start + up4(adapters + 1);
     t.splits = t.tiles + 4 * static_cast<int64_t>(t.tile_bound);
     t.chunks = t.splits + 4 * static_cast<int64_t>(t.split_bound);
     t.chunk_count = tokens > kChunkRows ? static_cast<int>((tokens + kChunkRows - 1) / kChunkRows) : 0;
@@ -64,7 +69,8 @@ inline TableLayout table_layout(int64_t tokens, int64_t adapters) {
 struct Groups {
     const int32_t* head = nullptr;
     const int32_t* order = nullptr;
-    const int32_t* split_start = nullptr;
+    const int32_t* starts = nullptr;
+    const int32_t* partial_start = nullptr;
     const int4* tiles = nullptr;
     const int4* splits = nullptr;
     int tile_bound = 0, split_bound = 0, split_rows = 0;
@@ -77,7 +83,8 @@ inline Groups groups_of(const void* table, int64_t tokens, int64_t adapters) {
     Groups g;
     g.head = base;
     g.order = base + t.order;
-    g.split_start = base + t.split_start;
+    g.starts = base + t.starts;
+    g.partial_start = base + t.partial_start;
     g.tiles = reinterpret_cast<const int4*>(base + t.tiles);
     g.splits = reinterpret_cast<const int4*>(base + t.splits);
     g.tile_bound = t.tile_bound;
@@ -144,7 +151,8 @@ int launch_spread(const float* partials, int slices, const void* w, bool w32, co
                   hipStream_t stream);
 
 // out[a][c][j] = scale_a * sum over a's rows of h[i][c] * x[order[i]][j], fp32 or bf16;
-// 0 for an adapter without rows. partials: split_bound * rank * width fp32.
+// 0 for an adapter without rows. partials: partial_bound * rank * width fp32 (one group:
+// split_bound, none where that is 1).
 struct OuterJob {
     const float* h = nullptr;
     const uint16_t* x = nullptr;

@@ -107,39 +107,54 @@ __device__ __forceinline__ int sum_waves(uint16_t* counts, int groups, int a) {
     return sum;
 }
 
+__device__ __forceinline__ int split_count(int rows, const TableLayout& t) {
+    return (rows + t.split_rows - 1) / t.split_rows;
+}
+// Splits whose sums are added up: none of an adapter that has only one.
+__device__ __forceinline__ int partial_count(int rows, const TableLayout& t) {
+    return rows > t.split_rows ? split_count(rows, t) : 0;
+}
+
 // start [groups + 1] in LDS: the groups' counts in, their starts out. Returns the first
-// tile and split of the thread's groups.
-__device__ __forceinline__ int2 scan_groups(int32_t* start, const TableLayout& t, int tokens, int groups) {
-    __shared__ int32_t wave_sums[3][kGroupThreads / 64];
+// tile, split and partial sum of the thread's groups.
+__device__ __forceinline__ int3 scan_groups(int32_t* start, const TableLayout& t, int tokens, int groups) {
+    __shared__ int32_t wave_sums[4][kGroupThreads / 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int per = (groups + kGroupThreads - 1) / kGroupThreads;
     const int g0 = min(tid * per, groups), g1 = min(g0 + per, groups);
-    int rows = 0, tiles = 0, splits = 0;
+    int rows = 0, tiles = 0, splits = 0, partials = 0;
     for (int a = g0; a < g1; ++a) {
         rows += start[a];
         tiles += (start[a] + kTileRows - 1) / kTileRows;
-        if (a < groups - 1) splits += (start[a] + t.split_rows - 1) / t.split_rows;
+        if (a < groups - 1) {
+            splits += split_count(start[a], t);
+            partials += partial_count(start[a], t);
+        }
     }
-    int row_end = rows, tile_end = tiles, split_end = splits;
+    int row_end = rows, tile_end = tiles, split_end = splits, partial_end = partials;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
         const int r = __shfl_up(row_end, d), i = __shfl_up(tile_end, d), s = __shfl_up(split_end, d);
+        const int p = __shfl_up(partial_end, d);
         if (lane >= d) {
             row_end += r;
             tile_end += i;
             split_end += s;
+            partial_end += p;
         }
     }
     if (lane == 63) {
         wave_sums[0][wave] = row_end;
         wave_sums[1][wave] = tile_end;
         wave_sums[2][wave] = split_end;
+        wave_sums[3][wave] = partial_end;
     }
     __syncthreads();
     for (int w = 0; w < wave; ++w) {
         row_end += wave_sums[0][w];
         tile_end += wave_sums[1][w];
         split_end += wave_sums[2][w];
+        partial_end += wave_sums[3][w];
     }
     int row = row_end - rows;
     for (int a = g0; a < g1; ++a) {
@@ -148,32 +163,38 @@ __device__ __forceinline__ int2 scan_groups(int32_t* start, const TableLayout& t
         row += n;
     }
     if (tid == 0) start[groups] = tokens;
-    return make_int2(tile_end - tiles, split_end - splits);
+    return make_int3(tile_end - tiles, split_end - splits, partial_end - partials);
 }
 
 // The table's parts but the rows, an entry a thread: a tile's or split's group is found in
-// LDS (first_of, twice groups + 1 entries).
-__device__ __forceinline__ void write_table(const int32_t* start, int32_t* first_of, int2 first, int32_t* __restrict__ table,
-                                            const TableLayout& t, int groups) {
+// LDS (first_of, table_lds bytes: twice groups + 1 entries, and as many of 16 bits for the
+// partial sums, of which there are at most 2 kMaxAdapterTokens / kMaxSplitRows).
+constexpr int table_lds(int groups) { return 10 * (groups + 1); }
+__device__ __forceinline__ void write_table(const int32_t* start, int32_t* first_of, int3 first,
+                                            int32_t* __restrict__ table, const TableLayout& t, int groups) {
     const int tid = threadIdx.x;
     const int per = (groups + kGroupThreads - 1) / kGroupThreads;
     const int g0 = min(tid * per, groups), g1 = min(g0 + per, groups);
     int32_t *tile_of = first_of, *split_of = first_of + groups + 1;
-    int tile = first.x, split = first.y;
+    uint16_t* partial_of = reinterpret_cast<uint16_t*>(split_of + groups + 1);
+    int tile = first.x, split = first.y, partial = first.z;
     for (int a = g0; a < g1; ++a) {
         const int n = start[a + 1] - start[a];
         tile_of[a] = tile;
         split_of[a] = split;
+        partial_of[a] = static_cast<uint16_t>(partial);
         tile += (n + kTileRows - 1) / kTileRows;
-        if (a < groups - 1) split += (n + t.split_rows - 1) / t.split_rows;
-        if (a == groups - 1) {
+        if (a < groups - 1) {
+            split += split_count(n, t);
+            partial += partial_count(n, t);
+        } else {
             tile_of[groups] = tile;
             split_of[groups] = split;
         }
     }
     __syncthreads();
     for (int a = tid; a <= groups; a += kGroupThreads) table[t.starts + a] = start[a];
-    for (int a = tid; a < groups; a += kGroupThreads) table[t.split_start + a] = split_of[a];
+    for (int a = tid; a < groups; a += kGroupThreads) table[t.partial_start + a] = partial_of[a];
     if (tid < 4) table[tid] = tid == 0 ? tile_of[groups] : tid == 1 ? split_of[groups] : 0;
     const auto write = [&](const int32_t* entries, int rows, int4* to, auto last) {
         const int count = entries[groups];
@@ -188,11 +209,12 @@ __device__ __forceinline__ void write_table(const int32_t* start, int32_t* first
             }
             const int at = start[low] + (i - entries[low]) * rows;
             to[i] = make_int4(low < groups - 1 ? low : -1, at, min(rows, start[low + 1] - at),
-                              last(entries[low + 1] - entries[low]));
+                              last(low, i - entries[low]));
         }
     };
-    write(tile_of, kTileRows, reinterpret_cast<int4*>(table + t.tiles), [](int) { return 0; });
-    write(split_of, t.split_rows, reinterpret_cast<int4*>(table + t.splits), [](int parts) { return parts; });
+    write(tile_of, kTileRows, reinterpret_cast<int4*>(table + t.tiles), [](int, int) { return 0; });
+    write(split_of, t.split_rows, reinterpret_cast<int4*>(table + t.splits),
+          [&](int a, int i) { return split_of[a + 1] - split_of[a] > 1 ? partial_of[a] + i : -1; });
 }
 
 // All rows of a small batch, ranked by the first WAVES waves.
@@ -213,7 +235,7 @@ __global__ __launch_bounds__(kGroupThreads) void adapter_group_kernel(const int3
     __syncthreads();
     for (int a = tid; a < groups; a += kGroupThreads) start[a] = sum_waves<WAVES>(counts, groups, a);
     __syncthreads();
-    const int2 tables = scan_groups(start, t, tokens, groups);
+    const int3 tables = scan_groups(start, t, tokens, groups);
     __syncthreads();
     if (wave < WAVES) {
 #pragma unroll
@@ -274,7 +296,7 @@ __global__ __launch_bounds__(kGroupThreads) void adapter_scan_kernel(int32_t* __
         start[a] = sum;
     }
     __syncthreads();
-    const int2 tables = scan_groups(start, t, tokens, groups);
+    const int3 tables = scan_groups(start, t, tokens, groups);
     __syncthreads();
     write_table(start, first_of, tables, table, t, groups);
 }
@@ -315,7 +337,7 @@ int launch_adapter_group(const int32_t* ids, void* table, int64_t tokens, int ad
     const int rows = static_cast<int>(tokens), groups = adapters + 1;
     // Sixteen waves' counts, or four's, within 64 KiB of LDS beside the starts.
     const bool many = groups > 1536;
-    const size_t lds = (groups + 1) * 4 + std::max((many ? 4 : 16) * groups * 2, 2 * (groups + 1) * 4);
+    const size_t lds = (groups + 1) * 4 + std::max((many ? 4 : 16) * groups * 2, table_lds(groups));
     if (t.chunk_count == 0) {
         const auto kernel = many ? adapter_group_kernel<4> : adapter_group_kernel<16>;
         hipLaunchKernelGGL(kernel, dim3(1), dim3(kGroupThreads), lds, stream, ids, base, t, rows, adapters);
@@ -325,8 +347,8 @@ int launch_adapter_group(const int32_t* ids, void* table, int64_t tokens, int ad
     hipLaunchKernelGGL(adapter_count_kernel, chunks, dim3(256), groups * 4, stream, ids, base, t, rows, adapters);
     int rc = check_launch("adapter_count_kernel");
     if (rc != MOE_OK) return rc;
-    hipLaunchKernelGGL(adapter_scan_kernel, dim3(1), dim3(kGroupThreads), 3 * (groups + 1) * 4, stream, base, t, rows,
-                       adapters, t.chunk_count);
+    hipLaunchKernelGGL(adapter_scan_kernel, dim3(1), dim3(kGroupThreads), (groups + 1) * 4 + table_lds(groups), stream,
+                       base, t, rows, adapters, t.chunk_count);
     rc = check_launch("adapter_scan_kernel");
     if (rc != MOE_OK) return rc;
     if (many)
@@ -1112,7 +1134,7 @@ struct OuterJobs {
 // A workgroup's split, job and columns.
 struct OuterPart {
     OuterJob job;
-    int column, adapter, first, rows, parts;
+    int column, adapter, first, rows, partial;
 };
 __device__ __forceinline__ bool outer_part(const OuterJobs& jobs, const Groups& gr, int64_t tokens, OuterPart* p) {
     const bool second = static_cast<int>(blockIdx.y) >= jobs.columns[0];
@@ -1123,13 +1145,13 @@ __device__ __forceinline__ bool outer_part(const OuterJobs& jobs, const Groups& 
         p->adapter = split.x;
         p->first = split.y;
         p->rows = split.z;
-        p->parts = split.w;
+        p->partial = split.w;
         return static_cast<int>(blockIdx.x) < gr.head[1];
     }
     p->adapter = 0;
     p->first = blockIdx.x * gr.split_rows;
     p->rows = static_cast<int>(min(static_cast<int64_t>(gr.split_rows), tokens - p->first));
-    p->parts = gr.split_bound;
+    p->partial = gr.split_bound > 1 ? static_cast<int>(blockIdx.x) : -1;
     return true;
 }
 
@@ -1146,10 +1168,10 @@ __device__ __forceinline__ void list_rows(int32_t* row_of, const Groups& gr, con
 template <bool BF16>
 __device__ __forceinline__ void store_outer(const OuterPart& p, int rank, int c, int64_t j, f32x4_t sum) {
     if (c >= rank || j >= p.job.width) return;
-    if (p.parts == 1)
+    if (p.partial < 0)
         store4<BF16>(p.job.out, (static_cast<int64_t>(p.adapter) * rank + c) * p.job.width + j, sum);
     else
-        store4<false>(p.job.partials, (static_cast<int64_t>(blockIdx.x) * rank + c) * p.job.width + j, sum);
+        store4<false>(p.job.partials, (static_cast<int64_t>(p.partial) * rank + c) * p.job.width + j, sum);
 }
 
 template <int NR, bool BF16>
@@ -1344,9 +1366,9 @@ __global__ __launch_bounds__(256) void outer_sum_kernel(OuterJobs jobs, Groups g
     const bool second = static_cast<int64_t>(blockIdx.x) >= blocks0;
     const OuterJob job = jobs.job[second];
     const int64_t elements = job.width * rank;
-    const int s0 = gr.order ? gr.split_start[a] : 0;
-    const int s1 = gr.order ? gr.split_start[a + 1] : gr.split_bound;
-    if (s1 - s0 == 1) return;
+    const int s0 = gr.order ? gr.partial_start[a] : 0;
+    const int s1 = gr.order ? gr.partial_start[a + 1] : gr.split_bound;
+    if (s0 == s1 && gr.starts[a] < gr.starts[a + 1]) return;  // its one split wrote the result
     const int64_t at = ((static_cast<int64_t>(blockIdx.x) - (second ? blocks0 : 0)) * 256 + threadIdx.x) * 4;
     if (at >= elements) return;
     f32x4_t sum = {0, 0, 0, 0};
@@ -1416,7 +1438,7 @@ struct BackwardScratch {
 };
 static BackwardScratch backward_scratch(int64_t tokens, int64_t hidden, int64_t width, int64_t rank, int64_t adapters,
                                         bool want_x, bool want_down, bool want_up) {
-    const int64_t rows = static_cast<int64_t>(table_layout(tokens, adapters).split_bound) * rank;
+    const int64_t rows = static_cast<int64_t>(table_layout(tokens, adapters).partial_bound) * rank;
     BackwardScratch s{};
     if (want_x || want_down) {
         s.dh = up16(through_bytes(tokens, width, hidden, rank, adapters));

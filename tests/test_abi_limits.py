@@ -47,3 +47,26 @@ def test_a_backward_call_is_held_to_the_scratch_of_its_gradients():
         need = lib.moe_low_rank_scratch_bytes(*sizes, 1 + without)
         back = (lambda nbytes: lib.moe_low_rank_backward(A, A, A, A, A, A, table, A, A, *grads, 0, A, nbytes, *sizes, None))
         assert back(need - 1) == 4 and back(need) == 5  # workspace too small; no GPU to launch on
+
+
+@pytest.mark.parametrize("tokens", [1, 128, 129, 257, 1024, 1025, 4096, 8192, 8193, 100_000, 1 << 21])
+@pytest.mark.parametrize("adapters", [1, 7, 256, 4096])
+def test_partial_sums_are_those_of_adapters_of_several_splits(tokens, adapters):
+    """Their number does not grow with the bank, and holds the worst batch: as many adapters
+    as there are rows for, each one row past a split."""
+    lib = _lib.load_library()
+    rank, width = 16, 64
+    split = 128
+    while split < 1024 and split * 8 < tokens:
+        split *= 2
+    size = lib.moe_low_rank_scratch_bytes(tokens, width, width, rank, adapters, 1 + 2 + 4)
+    assert size % (rank * width * 4) == 0
+    bound = size // (rank * width * 4)
+    assert bound <= 2 * tokens / split
+    for rows in (split + 1, split + 2, 2 * split, 2 * split + 1, tokens):
+        whole = min(tokens // rows, adapters) if rows <= tokens else 0
+        rest = tokens - whole * rows if whole < adapters else 0
+        partials = whole * -(-rows // split) if rows > split else 0
+        if rest > split:
+            partials += -(-rest // split)
+        assert partials <= bound, rows
