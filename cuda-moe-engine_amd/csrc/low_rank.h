@@ -23,7 +23,8 @@ constexpr int kMaxSplitRows = 1024;
 //   head         [4]     tiles, splits, 0, 0
 //   order        [T]     rows sorted by adapter (stable); rows of no adapter last
 //   starts       [N + 2] first sorted row of each adapter, of the rows of none, T
-//   partial_start [N + 1] first partial sum of each adapter: a split's of those that have several
+//   partial_start [N + 1] twice the first partial sum of each adapter (a split's, of the adapters
+//                        that have several), plus 1 where the adapter has rows
 //   tiles        [tile_bound]  {adapter (-1: none), first sorted row, rows <= kTileRows, 0}
 //   splits       [split_bound] {adapter, first sorted row, rows <= split_rows, partial sum (-1: the
 //                        adapter's only split)}
@@ -69,7 +70,6 @@ inline TableLayout table_layout(int64_t tokens, int64_t adapters) {
 struct Groups {
     const int32_t* head = nullptr;
     const int32_t* order = nullptr;
-    const int32_t* starts = nullptr;
     const int32_t* partial_start = nullptr;
     const int4* tiles = nullptr;
     const int4* splits = nullptr;
@@ -83,7 +83,6 @@ inline Groups groups_of(const void* table, int64_t tokens, int64_t adapters) {
     Groups g;
     g.head = base;
     g.order = base + t.order;
-    g.starts = base + t.starts;
     g.partial_start = base + t.partial_start;
     g.tiles = reinterpret_cast<const int4*>(base + t.tiles);
     g.splits = reinterpret_cast<const int4*>(base + t.splits);

@@ -107,54 +107,47 @@ __device__ __forceinline__ int sum_waves(uint16_t* counts, int groups, int a) {
     return sum;
 }
 
-__device__ __forceinline__ int split_count(int rows, const TableLayout& t) {
-    return (rows + t.split_rows - 1) / t.split_rows;
-}
-// Splits whose sums are added up: none of an adapter that has only one.
-__device__ __forceinline__ int partial_count(int rows, const TableLayout& t) {
-    return rows > t.split_rows ? split_count(rows, t) : 0;
+// An adapter's splits, and those of them whose sums are added up (none of an only one) in the
+// upper 16 bits: a batch has at most kMaxAdapters + 2 kMaxAdapterTokens / kMaxSplitRows of
+// them, and the halves are scanned as one.
+__device__ __forceinline__ int split_counts(int rows, const TableLayout& t) {
+    const int splits = (rows + t.split_rows - 1) >> __builtin_ctz(t.split_rows);
+    return splits > 1 ? splits * 0x10001 : splits;
 }
 
 // start [groups + 1] in LDS: the groups' counts in, their starts out. Returns the first
-// tile, split and partial sum of the thread's groups.
-__device__ __forceinline__ int3 scan_groups(int32_t* start, const TableLayout& t, int tokens, int groups) {
-    __shared__ int32_t wave_sums[4][kGroupThreads / 64];
+// tile and split (with the first partial sum) of the thread's groups.
+__device__ __forceinline__ int2 scan_groups(int32_t* start, const TableLayout& t, int tokens, int groups) {
+    __shared__ int32_t wave_sums[3][kGroupThreads / 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int per = (groups + kGroupThreads - 1) / kGroupThreads;
     const int g0 = min(tid * per, groups), g1 = min(g0 + per, groups);
-    int rows = 0, tiles = 0, splits = 0, partials = 0;
+    int rows = 0, tiles = 0, splits = 0;
     for (int a = g0; a < g1; ++a) {
         rows += start[a];
         tiles += (start[a] + kTileRows - 1) / kTileRows;
-        if (a < groups - 1) {
-            splits += split_count(start[a], t);
-            partials += partial_count(start[a], t);
-        }
+        if (a < groups - 1) splits += split_counts(start[a], t);
     }
-    int row_end = rows, tile_end = tiles, split_end = splits, partial_end = partials;
+    int row_end = rows, tile_end = tiles, split_end = splits;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
         const int r = __shfl_up(row_end, d), i = __shfl_up(tile_end, d), s = __shfl_up(split_end, d);
-        const int p = __shfl_up(partial_end, d);
         if (lane >= d) {
             row_end += r;
             tile_end += i;
             split_end += s;
-            partial_end += p;
         }
     }
     if (lane == 63) {
         wave_sums[0][wave] = row_end;
         wave_sums[1][wave] = tile_end;
         wave_sums[2][wave] = split_end;
-        wave_sums[3][wave] = partial_end;
     }
     __syncthreads();
     for (int w = 0; w < wave; ++w) {
         row_end += wave_sums[0][w];
         tile_end += wave_sums[1][w];
         split_end += wave_sums[2][w];
-        partial_end += wave_sums[3][w];
     }
     int row = row_end - rows;
     for (int a = g0; a < g1; ++a) {
@@ -163,30 +156,25 @@ __device__ __forceinline__ int3 scan_groups(int32_t* start, const TableLayout& t
         row += n;
     }
     if (tid == 0) start[groups] = tokens;
-    return make_int3(tile_end - tiles, split_end - splits, partial_end - partials);
+    return make_int2(tile_end - tiles, split_end - splits);
 }
 
 // The table's parts but the rows, an entry a thread: a tile's or split's group is found in
-// LDS (first_of, table_lds bytes: twice groups + 1 entries, and as many of 16 bits for the
-// partial sums, of which there are at most 2 kMaxAdapterTokens / kMaxSplitRows).
-constexpr int table_lds(int groups) { return 10 * (groups + 1); }
-__device__ __forceinline__ void write_table(const int32_t* start, int32_t* first_of, int3 first,
+// LDS (first_of, twice groups + 1 entries).
+__device__ __forceinline__ void write_table(const int32_t* start, int32_t* first_of, int2 first,
                                             int32_t* __restrict__ table, const TableLayout& t, int groups) {
     const int tid = threadIdx.x;
     const int per = (groups + kGroupThreads - 1) / kGroupThreads;
     const int g0 = min(tid * per, groups), g1 = min(g0 + per, groups);
     int32_t *tile_of = first_of, *split_of = first_of + groups + 1;
-    uint16_t* partial_of = reinterpret_cast<uint16_t*>(split_of + groups + 1);
-    int tile = first.x, split = first.y, partial = first.z;
+    int tile = first.x, split = first.y;
     for (int a = g0; a < g1; ++a) {
         const int n = start[a + 1] - start[a];
         tile_of[a] = tile;
         split_of[a] = split;
-        partial_of[a] = static_cast<uint16_t>(partial);
         tile += (n + kTileRows - 1) / kTileRows;
         if (a < groups - 1) {
-            split += split_count(n, t);
-            partial += partial_count(n, t);
+            split += split_counts(n, t);
         } else {
             tile_of[groups] = tile;
             split_of[groups] = split;
@@ -194,27 +182,30 @@ __device__ __forceinline__ void write_table(const int32_t* start, int32_t* first
     }
     __syncthreads();
     for (int a = tid; a <= groups; a += kGroupThreads) table[t.starts + a] = start[a];
-    for (int a = tid; a < groups; a += kGroupThreads) table[t.partial_start + a] = partial_of[a];
-    if (tid < 4) table[tid] = tid == 0 ? tile_of[groups] : tid == 1 ? split_of[groups] : 0;
-    const auto write = [&](const int32_t* entries, int rows, int4* to, auto last) {
-        const int count = entries[groups];
+    for (int a = tid; a < groups; a += kGroupThreads)
+        table[t.partial_start + a] = split_of[a] >> 16 << 1 | (start[a] < start[a + 1]);
+    if (tid < 4) table[tid] = tid == 0 ? tile_of[groups] : tid == 1 ? split_of[groups] & 0xffff : 0;
+    const auto write = [&](const int32_t* firsts, int mask, int rows, int4* to, auto last) {
+        const auto entry = [&](int a) { return firsts[a] & mask; };
+        const int count = entry(groups);
         for (int i = tid; i < count; i += kGroupThreads) {
-            int low = 0, high = groups;  // entries[low] <= i < entries[high]
+            int low = 0, high = groups;  // entry(low) <= i < entry(high)
             while (high - low > 1) {
                 const int mid = (low + high) / 2;
-                if (entries[mid] <= i)
+                if (entry(mid) <= i)
                     low = mid;
                 else
                     high = mid;
             }
-            const int at = start[low] + (i - entries[low]) * rows;
+            const int at = start[low] + (i - entry(low)) * rows;
             to[i] = make_int4(low < groups - 1 ? low : -1, at, min(rows, start[low + 1] - at),
-                              last(low, i - entries[low]));
+                              last(low, i - entry(low)));
         }
     };
-    write(tile_of, kTileRows, reinterpret_cast<int4*>(table + t.tiles), [](int, int) { return 0; });
-    write(split_of, t.split_rows, reinterpret_cast<int4*>(table + t.splits),
-          [&](int a, int i) { return split_of[a + 1] - split_of[a] > 1 ? partial_of[a] + i : -1; });
+    write(tile_of, -1, kTileRows, reinterpret_cast<int4*>(table + t.tiles), [](int, int) { return 0; });
+    write(split_of, 0xffff, t.split_rows, reinterpret_cast<int4*>(table + t.splits), [&](int a, int i) {
+        return split_of[a + 1] - split_of[a] == 1 ? -1 : (split_of[a] >> 16) + i;  // one split, none added up
+    });
 }
 
 // All rows of a small batch, ranked by the first WAVES waves.
@@ -235,7 +226,7 @@ __global__ __launch_bounds__(kGroupThreads) void adapter_group_kernel(const int3
     __syncthreads();
     for (int a = tid; a < groups; a += kGroupThreads) start[a] = sum_waves<WAVES>(counts, groups, a);
     __syncthreads();
-    const int3 tables = scan_groups(start, t, tokens, groups);
+    const int2 tables = scan_groups(start, t, tokens, groups);
     __syncthreads();
     if (wave < WAVES) {
 #pragma unroll
@@ -296,7 +287,7 @@ __global__ __launch_bounds__(kGroupThreads) void adapter_scan_kernel(int32_t* __
         start[a] = sum;
     }
     __syncthreads();
-    const int3 tables = scan_groups(start, t, tokens, groups);
+    const int2 tables = scan_groups(start, t, tokens, groups);
     __syncthreads();
     write_table(start, first_of, tables, table, t, groups);
 }
@@ -337,7 +328,7 @@ int launch_adapter_group(const int32_t* ids, void* table, int64_t tokens, int ad
     const int rows = static_cast<int>(tokens), groups = adapters + 1;
     // Sixteen waves' counts, or four's, within 64 KiB of LDS beside the starts.
     const bool many = groups > 1536;
-    const size_t lds = (groups + 1) * 4 + std::max((many ? 4 : 16) * groups * 2, table_lds(groups));
+    const size_t lds = (groups + 1) * 4 + std::max((many ? 4 : 16) * groups * 2, 2 * (groups + 1) * 4);
     if (t.chunk_count == 0) {
         const auto kernel = many ? adapter_group_kernel<4> : adapter_group_kernel<16>;
         hipLaunchKernelGGL(kernel, dim3(1), dim3(kGroupThreads), lds, stream, ids, base, t, rows, adapters);
@@ -347,8 +338,8 @@ int launch_adapter_group(const int32_t* ids, void* table, int64_t tokens, int ad
     hipLaunchKernelGGL(adapter_count_kernel, chunks, dim3(256), groups * 4, stream, ids, base, t, rows, adapters);
     int rc = check_launch("adapter_count_kernel");
     if (rc != MOE_OK) return rc;
-    hipLaunchKernelGGL(adapter_scan_kernel, dim3(1), dim3(kGroupThreads), (groups + 1) * 4 + table_lds(groups), stream,
-                       base, t, rows, adapters, t.chunk_count);
+    hipLaunchKernelGGL(adapter_scan_kernel, dim3(1), dim3(kGroupThreads), 3 * (groups + 1) * 4, stream, base, t, rows,
+                       adapters, t.chunk_count);
     rc = check_launch("adapter_scan_kernel");
     if (rc != MOE_OK) return rc;
     if (many)
@@ -1366,9 +1357,9 @@ __global__ __launch_bounds__(256) void outer_sum_kernel(OuterJobs jobs, Groups g
     const bool second = static_cast<int64_t>(blockIdx.x) >= blocks0;
     const OuterJob job = jobs.job[second];
     const int64_t elements = job.width * rank;
-    const int s0 = gr.order ? gr.partial_start[a] : 0;
-    const int s1 = gr.order ? gr.partial_start[a + 1] : gr.split_bound;
-    if (s0 == s1 && gr.starts[a] < gr.starts[a + 1]) return;  // its one split wrote the result
+    const int first = gr.order ? gr.partial_start[a] : 0;
+    const int s0 = first >> 1, s1 = gr.order ? gr.partial_start[a + 1] >> 1 : gr.split_bound;
+    if (s0 == s1 && (first & 1)) return;  // its one split wrote the result
     const int64_t at = ((static_cast<int64_t>(blockIdx.x) - (second ? blocks0 : 0)) * 256 + threadIdx.x) * 4;
     if (at >= elements) return;
     f32x4_t sum = {0, 0, 0, 0};
