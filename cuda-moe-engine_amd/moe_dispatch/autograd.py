@@ -76,15 +76,18 @@ class _Route(torch.autograd.Function):
 
 
 def route(x, router_weight, bias, topk, *, mask=None):
-    """Routes x bf16 [T, H] (T at least 1) by router_weight fp32 [E, H] and bias fp32 [E]
-    through the fused router, with the losses of ``training.router_loss``: ``Routed``.
-    ``mask`` bool [T] is false for padding tokens: they count in no loss and pass no
+    """Routes x bf16 [T, H] by router_weight fp32 [E, H] and bias fp32 [E] through the fused
+    router, with the losses of ``training.router_loss``: ``Routed``. T is at least 1, and up to
+    2^21 where a gradient is recorded. ``mask`` bool [T] is false for padding tokens: they count in no loss and pass no
     gradient on, though they get ids and weights as any token."""
     _eager_only()
     _training.shape_of(x, "x", 2)
     experts = _training.shape_of(router_weight, "router_weight", 2)[0]
     if x.shape[0] == 0:
         raise ValueError("route needs at least one token")
+    if x.shape[0] > _training.MAX_ROUTED and torch.is_grad_enabled() and any(
+            isinstance(t, torch.Tensor) and t.requires_grad for t in (x, router_weight, bias)):
+        raise ValueError("route records gradients of up to 2^21 tokens")
     if not isinstance(topk, int) or not 1 <= topk <= min(experts, _training.MAX_TOPK):
         raise ValueError("topk must be in 1..min(experts, 8)")
     weights, losses, ids, stats = _Route.apply(x, router_weight, bias, topk, mask)

@@ -28,6 +28,8 @@ import torch
 from ._extension import DTYPE_CODES, current_stream_handle, get_extension
 from .workspace import MAX_EXPERTS, MAX_TOPK
 
+MAX_ROUTED = 2**21  # tokens of route_backward
+
 _CURRENT = nullcontext()
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
@@ -200,7 +202,7 @@ def route_backward(x, router_weight, logits, expert_ids, bias=None, *, mask=None
     """Gradients of x, router weight and bias: ``(grad_x, grad_router_weight, grad_bias)``.
 
     x bf16 [T, H] and router_weight fp32 [E, H] are the router's inputs (H a multiple of 8),
-    the rest is ``route_logits_backward``'s. ``grad_x`` bf16 [T, H] is x's gradient along its
+    T is up to 2^21, the rest is ``route_logits_backward``'s. ``grad_x`` bf16 [T, H] is x's gradient along its
     other paths: the result is the sum, rounded once. grad_router_weight [E, H] and grad_bias
     [E] are fp32. A masked token's row of x is not read. ``gradients``: which of the three
     are wanted; the others are None and cost nothing.
@@ -211,6 +213,8 @@ def route_backward(x, router_weight, logits, expert_ids, bias=None, *, mask=None
     require_tensor(x, "x", (tokens, hidden), torch.bfloat16, device)
     if hidden < 8 or hidden % 8 or hidden > 2**20:
         raise ValueError("hidden must be a multiple of 8 up to 2^20")
+    if tokens > MAX_ROUTED:
+        raise ValueError("route_backward takes up to 2^21 tokens")
     require_tensor(router_weight, "router_weight", (experts, hidden), torch.float32, device)
     if grad_x is not None:
         require_tensor(grad_x, "grad_x", (tokens, hidden), torch.bfloat16, device)
@@ -228,8 +232,6 @@ def route_backward(x, router_weight, logits, expert_ids, bias=None, *, mask=None
                     t.zero_()
             return out_x, grad_router_weight, grad_bias
         need = _route_scratch_bytes(tokens, hidden, experts)
-        if need < 0:
-            raise ValueError("route_backward takes up to 2^21 tokens")
         scratch = logits.new_empty(need // 4)
         lib.check(lib.moe_route_backward(
             x.data_ptr(), router_weight.data_ptr(), logits.data_ptr(), _ptr(bias), expert_ids.data_ptr(), _ptr(mask),

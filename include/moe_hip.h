@@ -448,7 +448,8 @@ int64_t moe_route_backward_scratch_bytes(int64_t tokens, int64_t hidden, int64_t
  * Any of the three may be NULL. Products of dv and x are exact and accumulate in fp32;
  * dv and router_w enter grad_x as two bf16 parts each (16 bits). A masked token's row of x
  * is not read and may hold anything; an infinite x of a valid one makes NaN, not infinity, of
- * sums it enters. grad_x must not overlap x. Requires hidden % 8 == 0 and 16-byte aligned rows.
+ * sums it enters. grad_x must not overlap x. Requires 1 <= T <= 2^21, hidden % 8 == 0 and 16-byte
+ * aligned rows.
  */
 int moe_route_backward(const void* x, const float* router_w, const float* logits, const float* bias,
                        const int32_t* ids, const uint8_t* mask, const int32_t* stats, const float* grad_losses,

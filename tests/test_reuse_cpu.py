@@ -36,3 +36,10 @@ def test_the_first_assignment_is_not_captured(monkeypatch):
     with pytest.raises(RuntimeError, match="before capturing"):
         groups.assign(torch.zeros(4, dtype=torch.int32))
     assert groups.assignment == 0
+
+
+def test_route_refuses_before_its_forward_what_its_gradient_would():
+    x = torch.zeros(2**21 + 1, 8, dtype=torch.bfloat16)
+    w, bias = torch.zeros(4, 8, requires_grad=True), torch.zeros(4)
+    with pytest.raises(ValueError, match="2.21 tokens"):
+        autograd.route(x, w, bias, 2)
