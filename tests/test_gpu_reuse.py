@@ -118,32 +118,3 @@ def test_the_gradient_of_x_alone_takes_no_memory_of_the_others():
     assert torch.equal(got, want)
     # The result, dh and up to sixteen slices' sums of it, and the allocator's 512-byte steps.
     assert peak <= tokens * hidden * 2 + 17 * tokens * rank * 4 + 4096
-
-
-@pytest.mark.parametrize("sizes", [
-    (0, 1, 127, 128, 129, 0, 255, 256, 257, 130, 17), (129,) * 7 + (121,), (1024,), (128,) * 8, (0, 0, 300, 0, 300, 1),
-    (256, 257, 255, 512, 0, 513, 1, 254, 700)])
-@pytest.mark.parametrize("rank", [5, 40])
-def test_adapter_gradients_on_either_side_of_a_split(sizes, rank):
-    """Whole-number factors: sums are exact, so that a split or an adapter in another's place
-    shows. Splits are of 128 rows up to 1024 rows, of 256 up to 2048, and of 512 behind."""
-    g = torch.Generator(device="cuda").manual_seed(sum(sizes) + rank)
-    tokens, hidden, width = sum(sizes), 136, 72
-    ids = torch.repeat_interleave(torch.arange(len(sizes), device="cuda"), torch.tensor(sizes, device="cuda")).int()
-    ids = ids[torch.randperm(tokens, device="cuda", generator=g)].contiguous()
-
-    def whole(*shape):
-        return torch.randint(-2, 3, shape, device="cuda", generator=g).bfloat16()
-
-    x, grad, down, up = whole(tokens, hidden), whole(tokens, width), whole(len(sizes), rank, hidden), whole(len(sizes),
-                                                                                                           rank, width)
-    groups = AdapterGroups(tokens, len(sizes))
-    groups.assign(ids)
-    _, kept = low_rank_add(None, x, down, up, groups, return_hidden=True)
-    _, grad_down, grad_up = low_rank_backward(grad, x, down, up, groups, hidden=kept)
-    for a in range(len(sizes)):
-        rows = ids == a
-        h = x[rows].double() @ down[a].double().t()
-        dh = grad[rows].double() @ up[a].double().t()
-        assert torch.equal(grad_down[a].double(), dh.t() @ x[rows].double()), a
-        assert torch.equal(grad_up[a].double(), h.t() @ grad[rows].double()), a
