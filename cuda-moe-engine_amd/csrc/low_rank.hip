@@ -359,11 +359,12 @@ int launch_adapter_group(const int32_t* ids, void* table, int64_t tokens, int ad
 // turns the step over in LDS of its own into the MFMA's operands (lane l: row l % 16, 8 k
 // from 8 (l / 16); k is permuted inside 64). Loaded as operands, neighbouring lanes hold different rows and each
 // 16 bytes is a line of its own to the L1: T=4096, H=4096, r=16 and 64 took 17.2 and 38.6
-// us, 11.4 and 15.7 now (a plain reduction of rows that come from HBM takes 11.3). Rows
+// us, 11.1 and 15.9 now. Its 33.5 MB of x are 6.5 us at a copy's rate, and outer reads as
+// many in 8.8: no bound is known for the rest. Rows
 // past the tile and ranks past r are read from the last one and not stored (an output
 // depends on its own row and rank alone). Waves on one row meet in LDS, slices in the
-// consumer, both in order. Bound by x's bytes; past 64 ranks (21.7 us at r=128) by the LDS
-// that turns w's lines over for 32 rows.
+// consumer, both in order. Past 64 ranks (21.7 us at r=128) the LDS that turns w's lines
+// over for 32 rows takes longer than x's bytes.
 // ---------------------------------------------------------------------------
 // 16 rows of 64 k: lane i loads piece i % 8 (8 k) of rows i / 8 and i / 8 + 8.
 struct LineRows {
@@ -511,11 +512,15 @@ __global__ __launch_bounds__(64 * W) void contract_kernel(const uint16_t* __rest
     }
 }
 
-// Up to about 600 workgroups; past 32 ranks, where spread reads each slice's sums again
-// for every 256 columns, 512, or one a CU of the eight waves of up to 64 ranks (contract
-// and spread of 8192 x 4096 to 4096, rank 16: 46.9 us, with 512 50.5; of 4096 rows, rank 64:
-// 45.5 with three slices, 46.3 with two, 46.8 with four of four waves; of 1024 rows 20.1 and
-// 22.6; of 16384, rank 128: 158, with 600 168).
+// Up to about 600 workgroups of the tiles that the table could hold; past 32 ranks, where
+// spread reads each slice's sums again for every 256 columns, 512, or one a CU of the eight
+// waves of up to 64 ranks (contract and spread of 8192 x 4096 to 4096, rank 16: 46.9 us, with
+// 512 50.5; of 4096 rows, rank 64: 45.5 with three slices, 46.3 with two, 46.8 with four of
+// four waves; of 1024 rows 20.1 and 22.6; of 16384, rank 128: 158, with 600 168). The host
+// knows the bank and not how many of its adapters a batch uses, so few adapters of a large one
+// get few slices (contract and spread of 4096 rows of six adapters beside 8, 64 and 256, rank
+// 16: 25.5, 30.3 and 55.4 us, rank 64: 38.7, 49.7 and 74.1). Ranks 17 to 32 and past 64 keep
+// fewer workgroups on a CU than their rule supposes (186 registers; one workgroup).
 int contract_slices(int tile_bound, int64_t k, int64_t rank) {
     const bool wide = rank > 32 && rank <= 64;
     const int64_t most = wide ? (k + 511) / 512 : (k + 255) / 256;
@@ -564,9 +569,9 @@ static unsigned part_grid(int64_t columns, int64_t rows) {
 // and a lane ends with 8 neighbouring columns of a row: base and out move 16 bytes a lane.
 // h enters as two bf16 parts (rest below 2^-16 of it, under the result's own rounding to
 // bf16): for r <= 16 side by side in one MFMA's 32 k, else as two MFMAs on one w. Bound by
-// base's and out's bytes: 67 MB (T=4096, 4096 columns) in 14.8 us at r=16, the rate of a
-// copy from HBM, 16.5 at r=32; at r=64 22.9 and at r=128 35, where every column part reads
-// the slices' sums of h again.
+// base's and out's bytes: 67 MB (T=4096, 4096 columns) at r=16 in 17.9 us on average and 14.1
+// at best inside a training pass, 3.8 and 4.8 TB/s; at r=64 22.8 and at r=128 35, where
+// every column part reads the slices' sums of h again.
 // ---------------------------------------------------------------------------
 // The 8 x N block of 16-bit values v[j] (row j, two columns a dword) as B operands:
 // column i of all rows.
@@ -859,9 +864,10 @@ int launch_spread(const float* partials, int slices, const void* w, bool w32, co
 // waves split all of k, add up in LDS, and each spread 128 columns. Every column part
 // computes h again, from w in the L2, so that nothing is handed over between workgroups.
 // The sums' order is k's over eight waves: results differ from the two launches' in fp32
-// rounding. Latency, not bytes: one row of 4096 -> 4096 at rank 16 takes 7.9 us (two
-// launches 14.8), of 512 -> 512 4.6; 64 rows of 16 adapters 10.7. Loads five to seven steps
-// ahead took 8.4 to 8.7, sixteen waves of 64 columns 9.8 (their registers spill).
+// rounding. Latency, not bytes: one row of 4096 -> 4096 at rank 16 takes 7.5 us under replay
+// and 8.3 a call (two launches 7.2, and 11.5 with the host's second launch and scratch), of
+// 512 -> 512 4.6; 64 rows of 16 adapters 10.6. Loads five to seven steps ahead took 8.4 to
+// 8.7 where four took 8.1, sixteen waves of 64 columns 9.8 (their registers spill).
 // ---------------------------------------------------------------------------
 constexpr int kFusedWaves = 8;
 constexpr int kFusedCols = kFusedWaves * 128;
@@ -1038,8 +1044,15 @@ __global__ __launch_bounds__(64 * kFusedWaves) void fused_kernel(
     }
 }
 
-// Workgroups of a fused launch's column parts, or 0 where two launches take less time: the
-// parts' repeated reads of x and w (16 rows and the ranks, of k) may come to kFusedBytes.
+// Workgroups of a fused launch's column parts, or 0 where two launches take less time. A call
+// from Python pays 3 us for the second launch and its scratch, a replay nothing, and the rule
+// is for calls. The parts' repeated reads of x and w (16 rows and the ranks, of k) may come
+// to kFusedBytes: 64 rows of 16 adapters, 4096 to 4096 at rank 16, take 10.8 us a call and
+// 11.7 in two launches (replayed 10.6 and 7.8), 256 rows of 8 adapters 12.1 and 12.5 (12.2 and
+// 8.6); with 64 MB, 48 rows of 64 adapters took 23.6 where two launches take 12.0 (23.1 and
+// 8.6). A workgroup walks all of k, so rank * k is limited too: one row of 4096 columns at
+// rank 16, at the limit, 8.3 us a call and 11.5 in two launches (7.5 and 7.2); of 8192, past
+// it, 10.9 and 11.6 (10.6 and 7.3); of 4096 at rank 32, 9.5 and 11.6 (9.1 and 7.7).
 constexpr int64_t kFusedBytes = 32 << 20;
 constexpr int64_t kFusedElements = 64 << 10;
 
@@ -1083,7 +1096,7 @@ static int launch_through(const uint16_t* x, const uint16_t* down, const uint16_
 // as in spread; h (fp32, read along the ranks) enters as three bf16 parts, which hold
 // all its bits, so each product is exact and sums in fp32. The waves' sums meet in LDS;
 // an adapter of one split is done, of more its partial sums are added in split order.
-// Bound by x's bytes: both products of 4096 rows of 4096 columns, 67 MB, in 14.6 us at
+// Bound by x's bytes: both products of 4096 rows of 4096 columns, 67 MB, in 14.4 us at
 // r=16 and 18 at r=32, and 4 us for the splits' sums.
 // ---------------------------------------------------------------------------
 template <bool BF16>

@@ -364,8 +364,10 @@ __global__ __launch_bounds__(256) void router_bias_grad_kernel(ColumnSums bias) 
 // ---------------------------------------------------------------------------
 static int group_lanes(int experts) { return experts <= 8 ? 1 : experts <= 16 ? 2 : experts <= 32 ? 4 : 8; }
 
-// Blocks of the token kernels: one for up to four rounds of its lanes (a second launch
-// takes longer), else as many as there are tokens for, at most kLossBlocks.
+// Blocks of the token kernels: one for up to four rounds of its lanes, else as many as there
+// are tokens for, at most kLossBlocks. The losses of 1024 lanes (1024 tokens of 8 experts) take
+// 5.9 us in one block and as long in four with the second launch, 8.6 and 12.1 a call from
+// Python; 2048 lanes 8.8 and 5.9, 9.1 and 12.2 a call.
 static int token_blocks(int64_t tokens, int experts) {
     const int64_t lanes = tokens * group_lanes(experts);
     return lanes <= 1024 ? 1 : static_cast<int>(std::min<int64_t>((lanes + 255) / 256, kLossBlocks));

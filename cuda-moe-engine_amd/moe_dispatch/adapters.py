@@ -183,8 +183,8 @@ def low_rank_backward(grad_output, x, down, up, groups, *, scales=None, hidden, 
     assignment. ``grad_x`` bf16 [T, H] is x's gradient along its other paths (the shared
     projection): the result is the sum, rounded once. grad_down and grad_up are
     ``grad_dtype`` (fp32, or bf16 rounded once), zero for adapters without rows. scales get
-    no gradient. ``gradients``: which of the three are wanted; the others are None and
-    cost nothing.
+    no gradient. ``gradients``: which of the three are wanted; the others are None, are not
+    computed and take no memory.
     """
     h, width, rank, _, scratch_bytes = _check_operands(x, down, up, groups, scales)
     tokens, device = groups.tokens, groups.device

@@ -78,8 +78,8 @@ class _Route(torch.autograd.Function):
 def route(x, router_weight, bias, topk, *, mask=None):
     """Routes x bf16 [T, H] by router_weight fp32 [E, H] and bias fp32 [E] through the fused
     router, with the losses of ``training.router_loss``: ``Routed``. T is at least 1, and up to
-    2^21 where a gradient is recorded. ``mask`` bool [T] is false for padding tokens: they count in no loss and pass no
-    gradient on, though they get ids and weights as any token."""
+    2^21 where a gradient is recorded. ``mask`` bool [T] is false for padding tokens: they count
+    in no loss and pass no gradient on, though they get ids and weights as any token."""
     _eager_only()
     _training.shape_of(x, "x", 2)
     experts = _training.shape_of(router_weight, "router_weight", 2)[0]

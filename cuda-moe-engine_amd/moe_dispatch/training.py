@@ -204,8 +204,8 @@ def route_backward(x, router_weight, logits, expert_ids, bias=None, *, mask=None
     x bf16 [T, H] and router_weight fp32 [E, H] are the router's inputs (H a multiple of 8),
     T is up to 2^21, the rest is ``route_logits_backward``'s. ``grad_x`` bf16 [T, H] is x's gradient along its
     other paths: the result is the sum, rounded once. grad_router_weight [E, H] and grad_bias
-    [E] are fp32. A masked token's row of x is not read. ``gradients``: which of the three
-    are wanted; the others are None and cost nothing.
+    [E] are fp32. A masked token's row of x may hold anything. ``gradients``: which of the
+    three are wanted; the others are None and are not computed.
     """
     tokens, experts, topk, device = _check_routed(logits, expert_ids, bias, mask)
     _check_gradients(logits, expert_ids, loss, grad_losses, grad_weights)

@@ -447,7 +447,7 @@ int64_t moe_route_backward_scratch_bytes(int64_t tokens, int64_t hidden, int64_t
  *   grad_router_w = dv^T . x  (fp32 [E, H]),  grad_bias = sum_t dv  (fp32 [E])
  * Any of the three may be NULL. Products of dv and x are exact and accumulate in fp32;
  * dv and router_w enter grad_x as two bf16 parts each (16 bits). A masked token's row of x
- * is not read and may hold anything; an infinite x of a valid one makes NaN, not infinity, of
+ * may hold anything (none of it reaches a result); an infinite x of a valid one makes NaN, not infinity, of
  * sums it enters. grad_x must not overlap x. Requires 1 <= T <= 2^21, hidden % 8 == 0 and 16-byte
  * aligned rows.
  */
@@ -482,7 +482,8 @@ int64_t moe_adapter_table_bytes(int64_t tokens, int64_t adapters);
  * Sorts the rows of a batch by adapter: ids [T] int32, an id outside [0, N) being a row
  * of no adapter. The table (16-byte aligned, moe_adapter_table_bytes(T, N) bytes) serves
  * every low-rank call of the same T and N until it is written again; calls that read
- * it must not overlap with one that writes it. The order is stable, so results do not
+ * it must not overlap with one that writes it, nor come before the first (a captured one
+ * writes when its graph is replayed). The order is stable, so results do not
  * vary from call to call. Limits: 1 <= N <= 4096, T <= 2^21.
  */
 int moe_adapter_group(const int32_t* ids, void* table, int64_t table_bytes, int64_t tokens, int64_t adapters,
@@ -526,7 +527,8 @@ int moe_low_rank_add(const void* x, const void* down, const void* up, const floa
  * hidden_in is the forward's hidden_out on the same table (needed for grad_up). Any of the
  * three gradients may be NULL. grad_down and grad_up are [N, rank, hidden] and
  * [N, rank, width] of grad_dtype (FP32, or BF16 rounded once from the fp32 sums), zero for
- * an adapter without rows; their products are exact and accumulate in fp32 in row order.
+ * an adapter without rows; their products are exact and accumulate in fp32 in one fixed order (32
+ * rows at a time over the waves of a split of the rows, then the splits).
  * grad_x must not overlap x or grad_output.
  */
 int moe_low_rank_backward(const void* grad_output, const void* x, const void* down, const void* up,

@@ -45,8 +45,9 @@ def test_a_backward_call_is_held_to_the_scratch_of_its_gradients():
     table = lib.moe_adapter_table_bytes(4096, 8)
     for grads, without in (((A, None, None), 12), ((None, A, None), 10), ((None, None, A), 6), ((A, A, None), 8)):
         need = lib.moe_low_rank_scratch_bytes(*sizes, 1 + without)
-        back = (lambda nbytes: lib.moe_low_rank_backward(A, A, A, A, A, A, table, A, A, *grads, 0, A, nbytes, *sizes, None))
-        assert back(need - 1) == 4 and back(need) == 5  # workspace too small; no GPU to launch on
+        status = [lib.moe_low_rank_backward(A, A, A, A, A, A, table, A, A, *grads, 0, A, nbytes, *sizes, None)
+                  for nbytes in (need - 1, need)]
+        assert status == [4, 5]  # workspace too small; no GPU to launch on
 
 
 @pytest.mark.parametrize("tokens", [1, 128, 129, 257, 1024, 1025, 4096, 8192, 8193, 100_000, 1 << 21])
