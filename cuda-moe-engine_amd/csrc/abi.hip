@@ -83,16 +83,6 @@ int check_launch(const char* what) {
     return MOE_OK;
 }
 
-static bool valid_dtype(int dtype) {
-    return dtype == MOE_DTYPE_F32 || dtype == MOE_DTYPE_F16 || dtype == MOE_DTYPE_BF16;
-}
-
-// True when p is a multiple of `bytes` (a null pointer counts as aligned: the
-// null checks report it).
-static bool aligned_to(const void* p, uintptr_t bytes) {
-    return reinterpret_cast<uintptr_t>(p) % bytes == 0;
-}
-
 static int64_t aligned_capacity(int64_t n, int64_t experts, int64_t alignment) {
     if (alignment == 1) return n;
     return (n + experts * (alignment - 1) + 1 + alignment - 1) / alignment * alignment;

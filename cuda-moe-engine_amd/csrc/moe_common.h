@@ -133,6 +133,14 @@ inline int dtype_size(int dtype) {
     }
 }
 
+inline bool valid_dtype(int64_t dtype) {
+    return dtype == MOE_DTYPE_F32 || dtype == MOE_DTYPE_F16 || dtype == MOE_DTYPE_BF16;
+}
+
+// True when p is a multiple of `bytes` (a null pointer counts as aligned: the
+// null checks report it).
+inline bool aligned_to(const void* p, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
 // ---------------------------------------------------------------------------
 // Host-side error reporting: a status code plus a thread-local message.
 // ---------------------------------------------------------------------------

@@ -9,7 +9,8 @@ from __future__ import annotations
 
 import ctypes
 import os
-from functools import lru_cache
+import struct
+from functools import lru_cache, partial
 from pathlib import Path
 
 LIBRARY_NAME = "libmoe_hip.so"
@@ -77,6 +78,17 @@ _SIGNATURES = {
     "moe_low_rank_add": (_int, [_c_void_p] * 5 + [_i64] + [_c_void_p] * 4 + [_i64] * 6 + [_c_void_p]),
     "moe_low_rank_backward": (_int, [_c_void_p] * 6 + [_i64] + [_c_void_p] * 5 + [_int, _c_void_p] + [_i64] * 6
                               + [_c_void_p]),
+    "moe_rms_norm": (_int, [_c_void_p] * 2),
+    "moe_quantize_rows": (_int, [_c_void_p, _int, _c_void_p, _c_void_p, _i64, _i64, _c_void_p]),
+    "moe_rms_norm_backward_scratch_bytes": (_i64, [_i64, _i64]),
+    "moe_rms_norm_backward": (_int, [_c_void_p, _c_void_p, _int, _c_void_p, _int] + [_c_void_p] * 5 + [_i64] * 3
+                              + [_c_void_p]),
+    "moe_route_scored": (_int, [_c_void_p] * 2),
+    "moe_route_scored_backward": (_int, [_c_void_p] * 2),
+    "moe_linear_scratch_bytes": (_i64, [_i64] * 4 + [_int]),
+    "moe_linear": (_int, [_c_void_p] * 2),
+    "moe_clip_scratch_bytes": (_i64, []),
+    "moe_clip_gradients": (_int, [_c_void_p] * 2),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
@@ -100,6 +112,22 @@ BlockArgs._fields_ = [(name, _c_void_p if name in BlockArgs._POINTERS else _i64)
 
 
 BLOCK_ARGS_BYTES = ctypes.sizeof(BlockArgs)
+
+
+def _argument_struct(fields):
+    """A struct of eight-byte fields as a packer of its values, the
+    size in front: ``P`` a pointer, ``q`` an int64, ``d`` a double. The packed bytes are passed
+    as the call's first argument, which copies nothing and keeps no ctypes object."""
+    layout = struct.Struct("@q" + fields)
+    return partial(layout.pack, layout.size)
+
+
+# The header's *_args structs.
+RMS_NORM_ARGS = _argument_struct("PPPPPPPqqqqd")
+ROUTE_SCORED_ARGS = _argument_struct("PPPPqqqqqqqqd")
+ROUTE_SCORED_BACKWARD_ARGS = _argument_struct("PPPPqqqqqd")
+LINEAR_ARGS = _argument_struct("PPPPPPPPqqqqqqq")
+CLIP_ARGS = _argument_struct("PPPPqPPqd")
 
 
 def library_path() -> Path:

@@ -1,13 +1,13 @@
 """The training operators as differentiable functions, for ``loss.backward()``.
 
-``route``, ``dispatch``, ``combine`` and ``low_rank_add`` run the forward kernels and
-record the gradients of ``training`` and ``adapters``. Each returns new tensors, so that
+``route``, ``dispatch``, ``combine``, ``low_rank_add``, ``rms_norm`` and ``route_scored`` run
+the forward kernels and record the gradients of ``training``, ``adapters``, ``norms`` and ``scored``. Each returns new tensors, so that
 several layers and micro-batches may be in flight; none keeps a buffer for the next call.
 Gradients are first order (a second differentiation raises).
 
 They are eager: under graph capture they raise, since a backward pass recorded beside a
 live eager graph of the same leaves is more than torch survives. Capture the plain calls
-of ``training`` and ``adapters`` instead; they take buffers in and give gradients out.
+of those modules instead; they take buffers in and give gradients out.
 """
 
 from typing import NamedTuple
@@ -16,7 +16,9 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import adapters as _adapters
+from . import norms as _norms
 from . import ops as _ops
+from . import scored as _scored
 from . import training as _training
 from ._extension import get_extension
 
@@ -24,7 +26,7 @@ from ._extension import get_extension
 def _eager_only():
     if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
         raise RuntimeError("moe_dispatch.autograd is eager: capture the calls of moe_dispatch.training and "
-                           "moe_dispatch.adapters instead")
+                           "moe_dispatch.adapters (or norms, scored) instead")
 
 
 def _rows(grad):
@@ -188,3 +190,62 @@ def low_rank_add(base, x, down, up, groups, *, scales=None):
     if scales is not None and scales.requires_grad:
         raise ValueError("scales get no gradient; detach them")
     return _LowRankAdd.apply(base, x, down, up, groups, scales)
+
+
+class _RmsNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        normed = _norms.rms_norm(x, weight, residual=residual, eps=eps, return_rstd=True)
+        ctx.save_for_backward(x if residual is None else normed.total, weight, normed.rstd)
+        ctx.set_materialize_grads(False)
+        return normed.output, normed.total
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_output, grad_total):
+        _eager_only()
+        total, weight, rstd = ctx.saved_tensors
+        need_x, need_weight, need_residual, _ = ctx.needs_input_grad
+        if grad_output is None:
+            return (grad_total if need_x else None, None, grad_total if need_residual else None, None)
+        grad_x, grad_weight = _norms.rms_norm_backward(
+            grad_output.contiguous(), total, weight, rstd, grad_x=None if grad_total is None else grad_total.contiguous(),
+            gradients=(need_x or need_residual, need_weight))
+        if grad_weight is not None:
+            grad_weight = grad_weight.to(weight.dtype)
+        return grad_x if need_x else None, grad_weight, grad_x if need_residual else None, None
+
+
+def rms_norm(x, weight=None, *, residual=None, eps=1e-6):
+    """``norms.rms_norm`` with gradients to x, weight and residual: ``(output, total)``, total =
+    x + residual (None without a residual), to be the next residual. The gradient takes the normed
+    rows as total holds them, rounded to their type."""
+    _eager_only()
+    return _RmsNorm.apply(x, weight, residual, eps)
+
+
+class _RouteScored(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, topk, options, choice):
+        ids, weights = _scored.route_scored(logits, topk, **options, **choice)
+        ctx.save_for_backward(logits, ids)
+        ctx.options = options
+        ctx.mark_non_differentiable(ids)
+        return ids, weights
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, _ids, grad_weights):
+        _eager_only()
+        logits, ids = ctx.saved_tensors
+        return _scored.route_scored_backward(grad_weights.contiguous(), logits, ids, **ctx.options), None, None, None
+
+
+def route_scored(logits, topk, *, scoring="softmax", bias=None, groups=1, top_groups=1, group_best=2,
+                 renormalize=True, scale=1.0):
+    """``scored.route_scored`` with the weights' gradient to the logits: ``(ids, weights)``."""
+    _eager_only()
+    if bias is not None and bias.requires_grad:
+        raise ValueError("the selection bias gets no gradient; detach it")
+    return _RouteScored.apply(logits, topk, {"scoring": scoring, "renormalize": renormalize, "scale": scale},
+                              {"bias": bias, "groups": groups, "top_groups": top_groups, "group_best": group_best})

@@ -537,6 +537,188 @@ int moe_low_rank_backward(const void* grad_output, const void* x, const void* do
                           void* scratch, int64_t scratch_bytes, int64_t tokens, int64_t hidden, int64_t width,
                           int64_t rank, int64_t adapters, void* stream);
 
+/*
+ * ---------------------------------------------------------------------------
+ * The layer around the experts: norm, scored routing, dense products, gradient
+ * clipping. None of it has a counterpart in the reference. The calls with many
+ * arguments take a struct of eight-byte fields; struct_bytes is its size.
+ * ---------------------------------------------------------------------------
+ */
+
+/*
+ * Root-mean-square norm of the rows of x [T, H] (dtype a MOE_DTYPE_*):
+ *   h = x + residual (residual NULL: x),  rstd = 1 / sqrt(mean_j h_j^2 + eps),  y = h * rstd * weight
+ * in fp32 from the unrounded sum h; total = round(h) (with a residual only; it may be
+ * x or residual itself), rstd [T] fp32 (may be NULL). weight [H] has weight_dtype, dtype or
+ * MOE_DTYPE_F32 (NULL: 1). scales NULL: output = round(y) in dtype (it may be x or residual
+ * itself). scales fp32 [T]: output is e4m3 (OCP, one byte),
+ *   scales[t] = max(max_j |y_j|, 2^-100) / 448,  output = round_e4m3(y / scales[t]).
+ * A NaN stays NaN; an infinite y makes its row's scale infinite, so that nothing finite stands
+ * for it. fp32 rows have finite squares. Limits: 1 <= H <= 16384, T <= 2^21, eps >= 0.
+ */
+typedef struct moe_rms_norm_args {
+    int64_t struct_bytes;
+    const void* x;
+    const void* residual;
+    const void* weight;
+    void* total;
+    void* output;
+    float* scales;
+    float* rstd;
+    int64_t tokens;
+    int64_t hidden;
+    int64_t dtype;
+    int64_t weight_dtype;
+    double eps;
+} moe_rms_norm_args;
+
+int moe_rms_norm(const moe_rms_norm_args* args, void* stream);
+
+/* Rows in e4m3 with a scale each, as moe_rms_norm writes its y = x: activations between two 8-bit
+ * products, and weights (rows: output columns) when they are loaded. */
+int moe_quantize_rows(const void* x, int dtype, void* values, float* scales, int64_t tokens, int64_t hidden,
+                      void* stream);
+
+/* Bytes of scratch moe_rms_norm_backward needs for grad_weight; -1 for invalid sizes. */
+int64_t moe_rms_norm_backward_scratch_bytes(int64_t tokens, int64_t hidden);
+
+/*
+ * Gradients of y = x * rstd * weight, x the normed rows (total, with a residual), rstd as
+ * moe_rms_norm wrote it: with u = x * rstd and g = grad_output,
+ *   grad_x = round(grad_x_base + rstd * (g * weight - u * mean_j(g_j weight_j u_j)))  (base NULL: 0, or grad_x)
+ *   grad_weight = sum_t g * u  (fp32 [H], in a fixed order; 0 for no rows)
+ * Either may be NULL; scratch is needed for grad_weight. grad_x may be grad_output or x itself.
+ */
+int moe_rms_norm_backward(const void* grad_output, const void* x, int dtype, const void* weight, int weight_dtype,
+                          const float* rstd, const void* grad_x_base, void* grad_x, float* grad_weight, void* scratch,
+                          int64_t scratch_bytes, int64_t tokens, int64_t hidden, void* stream);
+
+/*
+ * Experts and weights of each token from its logits (fp32 [T, E]):
+ *   s = softmax(logits), or sigmoid(logits) when `sigmoid` is non-zero
+ *   key = s + bias (fp32 [E], finite; the bias takes part in the choice only), or the logit
+ *         without a bias, which orders the experts alike
+ *   groups > 1: experts lie in `groups` equal consecutive groups; a group's score is the sum of
+ *         its group_best (1 or 2) highest s + bias; the top_groups highest groups take part
+ *   ids [T, K]: the K highest keys in them, highest first
+ *   weights [T, K]: scale * s, or with renormalize scale * s / (sum of the chosen s)
+ * Ties go to the lower index. The choice is that of the exact values: it does not depend on
+ * how fp32 rounds a score (values that are nearer than 64 bits tell apart count as ties).
+ * A logit of -inf takes an expert out: it counts in no group's score and is chosen, with
+ * weight 0, only when its groups have nothing else left, lowest index first. A NaN logit is
+ * out as well and makes the token's weights NaN; so does +inf under softmax. ids are always K
+ * different experts. Limits: 1 <= E <= 512, 1 <= K <= 8, K <= top_groups * E / groups,
+ * groups <= 64, T <= 2^21.
+ */
+typedef struct moe_route_scored_args {
+    int64_t struct_bytes;
+    const float* logits;
+    const float* bias;
+    int32_t* ids;
+    float* weights;
+    int64_t tokens;
+    int64_t experts;
+    int64_t topk;
+    int64_t groups;
+    int64_t top_groups;
+    int64_t group_best;
+    int64_t sigmoid;
+    int64_t renormalize;
+    double scale;
+} moe_route_scored_args;
+
+int moe_route_scored(const moe_route_scored_args* args, void* stream);
+
+/*
+ * The gradient of the logits, fp32 [T, E], from the weights' (grad_weights [T, K]) for ids as
+ * moe_route_scored chose them (ids out of range count nowhere; the choice has no gradient).
+ */
+typedef struct moe_route_scored_backward_args {
+    int64_t struct_bytes;
+    const float* grad_weights;
+    const float* logits;
+    const int32_t* ids;
+    float* grad_logits;
+    int64_t tokens;
+    int64_t experts;
+    int64_t topk;
+    int64_t sigmoid;
+    int64_t renormalize;
+    double scale;
+} moe_route_scored_backward_args;
+
+int moe_route_scored_backward(const moe_route_scored_backward_args* args, void* stream);
+
+/* What moe_linear applies behind the product. */
+#define MOE_ACT_NONE 0
+#define MOE_ACT_RELU 1
+#define MOE_ACT_SILU 2
+#define MOE_ACT_GELU 3      /* z/2 (1 + erf(z / sqrt 2)) */
+#define MOE_ACT_GELU_TANH 4 /* its tanh form */
+#define MOE_ACT_SWIGLU 5    /* weight rows 0..N-1 gate, N..2N-1 up: silu(gate) * up */
+
+/*
+ * Dense product with its epilogue: output = round_bf16(act(x . weight^T + bias) + residual)
+ * x [T, K] and weight [R, K] (R = N, or 2N for MOE_ACT_SWIGLU), rows of weight row_stride elements
+ * apart, both bf16, or with x_scales [T] and weight_scales [R] both e4m3 (a product is then
+ * scaled by the two). bias [R] is bias_dtype, MOE_DTYPE_F32 or MOE_DTYPE_BF16 (NULL: 0), residual [T, N]
+ * bf16 (NULL: 0; it may be output itself), output [T, N] bf16. Sums, bias and activation are
+ * fp32; of e4m3 the matrix instruction first adds eight neighbouring products to 2^-13 of the
+ * largest, which is far below what 8 bits keep of each operand. Rows are multiples of 16 bytes and 16-byte aligned, N is a multiple of 8. Limits: T <=
+ * 2^21, K and N <= 2^20, weight below 4 GiB. scratch: moe_linear_scratch_bytes bytes, for this
+ * call alone (NULL when that is 0), 16-byte aligned.
+ */
+typedef struct moe_linear_args {
+    int64_t struct_bytes;
+    const void* x;
+    const void* weight;
+    const float* x_scales;
+    const float* weight_scales;
+    const void* bias;
+    const void* residual;
+    void* output;
+    void* scratch;
+    int64_t scratch_bytes;
+    int64_t tokens;
+    int64_t hidden;
+    int64_t width;
+    int64_t row_stride;
+    int64_t bias_dtype;
+    int64_t activation;
+} moe_linear_args;
+
+/* Bytes of scratch moe_linear needs (0: none); -1 for invalid sizes. `e4m3`: 8-bit operands. */
+int64_t moe_linear_scratch_bytes(int64_t tokens, int64_t hidden, int64_t width, int64_t activation, int e4m3);
+
+int moe_linear(const moe_linear_args* args, void* stream);
+
+/* Bytes of scratch moe_clip_gradients needs. */
+int64_t moe_clip_scratch_bytes(void);
+
+/*
+ * The global norm of many tensors and the tensors scaled to it:
+ *   norm = sqrt(sum over all of g^2),  outputs[i] = round(g_i * min(1, max_norm / (norm + 1e-6)))
+ * grads, outputs, elements and dtypes (MOE_DTYPE_*) are host arrays of `tensors` entries, read
+ * before the call returns; tensors are contiguous, aligned to their element, and outputs[i]
+ * is grads[i] (in place) or of its type and overlaps nothing else. Sums are 64 bits, in an
+ * order that the sizes fix. A norm that is infinite or NaN leaves the values as they are. norm: one fp32 on the
+ * device. Limits: 2^16 tensors, 2^40 elements.
+ */
+typedef struct moe_clip_args {
+    int64_t struct_bytes;
+    const void* const* grads;
+    void* const* outputs;
+    const int64_t* elements;
+    const int64_t* dtypes;
+    int64_t tensors;
+    float* norm;
+    void* scratch;
+    int64_t scratch_bytes;
+    double max_norm;
+} moe_clip_args;
+
+int moe_clip_gradients(const moe_clip_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
