@@ -1,0 +1,592 @@
+// Tiles of the dense products (linear.h): operands through an LDS ring, four waves a workgroup.
+//
+// Work is counted in bytes: a stage is 128 bytes of k of TM rows of x and BN rows of the weight, 64 bf16 or 128
+// e4m3, so both types move the same lines and differ in the matrix instruction alone (two
+// 16x16x32 bf16 steps or one 16x16x128 e4m3 step a stage, of the same duration).
+//
+//  * buffer_load ... lds moves 8 rows of one 128-byte line a wave instruction. Rows past the
+//    operand's end read as zero through the resource's range; chunks past K in the last stage
+//    by an offset past every range, so padding between rows never enters a sum.
+//  * Chunk c (16 bytes) of LDS row r lies at chunk c ^ ((r >> 1) & 7): 16 rows read at one chunk
+//    touch all banks once.
+//  * One barrier a stage. A stage's fragments are read between the matrix instructions of the step
+//    before, its slot is refilled from the barrier on that follows its last read.
+//  * Persistent workgroups chain tiles: the last windows of one load the next one's first stages.
+#pragma once
+
+#include "linear.h"
+
+namespace moe {
+
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef int intx4 __attribute__((ext_vector_type(4)));
+typedef int intx8 __attribute__((ext_vector_type(8)));
+
+constexpr int kStageBytes = 128;
+constexpr int kRingWaves = 4;
+
+// A launch's tiles: row tiles fastest, then column tiles, then splits of k.
+struct LinearPlan {
+    int row_tiles;
+    int col_tiles;
+    int splits;       // parts of k; more than one: partial sums in `partial`
+    int steps;        // stages of a whole row
+    int split_steps;  // stages of a part (the last may have fewer)
+    float* partial;   // [splits, T, rows] fp32
+};
+
+struct LinearTile {
+    bool valid;
+    int row0, col0, step0, steps, split;  // col0 in weight rows (of the gate half)
+};
+
+__device__ __forceinline__ int ring_swizzle(int row) { return (row >> 1) & 7; }
+
+constexpr int dense_stages(uint32_t stage_a, uint32_t stage_b, uint32_t bytes, int cap) {
+    const int fit = static_cast<int>(bytes / (stage_a + stage_b));
+    return fit < cap ? fit : cap;
+}
+
+// What the epilogue applies: nothing, one of the elementwise activations, or the gated one.
+enum LinearAct { kActNone, kActElement, kActSwiglu };
+
+template <int TM_, int BN_, LinearAct ACT_, bool FP8_, uint32_t LDS_, int WC_ = 2, int CAP = 6>
+struct DenseShape {
+    static constexpr int TM = TM_, BN = BN_, WC = WC_;
+    static constexpr LinearAct ACT = ACT_;
+    static constexpr bool SWIGLU = ACT == kActSwiglu, FP8 = FP8_;
+    static constexpr uint32_t LDS = LDS_;
+    static constexpr int COLS = SWIGLU ? BN / 2 : BN;  // output columns of a tile
+    static constexpr int WTM = TM / (kRingWaves / WC), WTN = BN / WC;
+    static constexpr int FA = WTM / 16, FB = WTN / 16;
+    static constexpr int A_LOADS = TM / 8 / kRingWaves, B_LOADS = BN / 8 / kRingWaves, LOADS = A_LOADS + B_LOADS;
+    static constexpr uint32_t A_STAGE = TM * kStageBytes, B_STAGE = BN * kStageBytes;
+    // Three or more whole stages where they fit, else two of x and what fits of the weight.
+    static constexpr int EQUAL = dense_stages(A_STAGE, B_STAGE, LDS, CAP);
+    static constexpr int SB = EQUAL >= 3 ? EQUAL : static_cast<int>((LDS - 2 * A_STAGE) / B_STAGE);
+    static constexpr int SA = EQUAL >= 3 ? EQUAL : 2;
+    static constexpr uint32_t B_BASE = SA * A_STAGE;
+    static constexpr uint32_t FRAG = 16 * kStageBytes;
+    // Loads younger than a stage's own when its first read waits for it: A of stage u + SA, then B of
+    // stage u + SB are issued in each window.
+    static constexpr int VM_STEADY = (SB > SA ? B_LOADS : 0) + (SA - 2) * LOADS;
+    static constexpr int VM_FIRST = (SB > SA ? B_LOADS : 0) + (SA - 1) * LOADS;
+    static_assert(A_LOADS >= 1 && B_LOADS >= 1 && FA >= 1 && FB >= 2 && FB % 2 == 0, "tile shape");
+    static_assert(SA >= 2 && SB >= SA && SA * A_STAGE + SB * B_STAGE <= LDS, "ring does not fit");
+    static_assert(VM_FIRST < 64, "loads in flight fit the counter");
+};
+
+template <typename S>
+struct DenseLoads {
+    __amdgpu_buffer_rsrc_t ra, rb;
+    uint32_t a_off[S::A_LOADS], b_off[S::B_LOADS];
+    char* lds;
+    int wave;
+    bool in_tail[2];  // the lane's chunk of even and odd row groups lies below K in a row's last stage
+
+    struct Rsrc {
+        __amdgpu_buffer_rsrc_t a, b;
+    };
+    static __device__ __forceinline__ Rsrc resources(const LinearArgs& p, const LinearTile& t) {
+        const int64_t skip = static_cast<int64_t>(t.step0) * kStageBytes;
+        const int64_t rows = min<int64_t>(p.tokens - t.row0, S::TM);
+        Rsrc r;
+        r.a = make_rsrc(p.x + t.row0 * p.k_bytes + skip, static_cast<uint32_t>(rows * p.k_bytes - skip));
+        r.b = make_rsrc(p.weight + t.col0 * p.w_stride + skip,
+                        static_cast<uint32_t>((p.rows - t.col0) * p.w_stride - skip));
+        return r;
+    }
+    __device__ __forceinline__ DenseLoads(const LinearArgs& p, char* lds_, const Rsrc& r) : lds(lds_) {
+        const int lane = threadIdx.x & 63;
+        wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        ra = r.a;
+        rb = r.b;
+        const int lrow = lane >> 3, chunk = lane & 7;
+        const int tail = static_cast<int>((p.k_bytes - 1) % kStageBytes) + 1;
+#pragma unroll
+        for (int g = 0; g < 2; ++g) in_tail[g] = (chunk ^ ring_swizzle(8 * g + lrow)) * 16 < tail;
+#pragma unroll
+        for (int i = 0; i < S::A_LOADS; ++i) {
+            const int row = (wave * S::A_LOADS + i) * 8 + lrow;
+            a_off[i] = static_cast<uint32_t>(row * p.k_bytes + (chunk ^ ring_swizzle(row)) * 16);
+        }
+#pragma unroll
+        for (int i = 0; i < S::B_LOADS; ++i) {
+            const int row = (wave * S::B_LOADS + i) * 8 + lrow;
+            int64_t from = row;
+            if constexpr (S::SWIGLU) {
+                // A wave's columns: WTN / 2 gate rows, then their up rows.
+                const int half = S::WTN / 2, col = row / S::WTN * half + row % half;
+                from = row % S::WTN < half ? col : p.n + col;
+            }
+            b_off[i] = static_cast<uint32_t>(from * p.w_stride + (chunk ^ ring_swizzle(row)) * 16);
+        }
+    }
+    // Load l of stage kt into slot st. `last`: stage kt ends the rows.
+    __device__ __forceinline__ void issue_a(__amdgpu_buffer_rsrc_t r, int kt, int st, int l, bool last) const {
+        const int g = wave * S::A_LOADS + l;
+        dma16(r, lds + st * S::A_STAGE + g * 1024, offset(a_off[l], kt, g, last), static_cast<uint32_t>(kt) * kStageBytes);
+    }
+    __device__ __forceinline__ void issue_b(__amdgpu_buffer_rsrc_t r, int kt, int st, int l, bool last) const {
+        const int g = wave * S::B_LOADS + l;
+        dma16(r, lds + S::B_BASE + st * S::B_STAGE + g * 1024, offset(b_off[l], kt, g, last),
+              static_cast<uint32_t>(kt) * kStageBytes);
+    }
+    __device__ __forceinline__ uint32_t offset(uint32_t off, int kt, int g, bool last) const {
+        return last && !in_tail[g & 1] ? 0xfffffff0u - static_cast<uint32_t>(kt) * kStageBytes : off;
+    }
+    // The loads of the windows before stage 0, in the loop's order (only the last window's when
+    // `chained`: the others went out in the tile before). Stages past the end load the last one again,
+    // so that every window counts the same loads.
+    __device__ __forceinline__ void prologue(int steps, bool ends, int a0, int b0, bool chained) const {
+#pragma unroll
+        for (int v = -S::SB; v < 0; ++v) {
+            if (chained && v != -1) continue;
+            if (v + S::SA >= 0) {
+                const int st = a0 + v + S::SA >= S::SA ? a0 + v : a0 + v + S::SA, kt = min(v + S::SA, steps - 1);
+#pragma unroll
+                for (int l = 0; l < S::A_LOADS; ++l) issue_a(ra, kt, st, l, ends && kt == steps - 1);
+            }
+            const int st = b0 + v + S::SB >= S::SB ? b0 + v : b0 + v + S::SB, kt = min(v + S::SB, steps - 1);
+#pragma unroll
+            for (int l = 0; l < S::B_LOADS; ++l) issue_b(rb, kt, st, l, ends && kt == steps - 1);
+        }
+    }
+};
+
+// One 16-row fragment of the current step: 16 bytes a lane (bf16) or 32 (e4m3).
+template <bool FP8>
+struct DenseFrag {
+    intx4 h[FP8 ? 2 : 1];
+};
+
+template <bool FP8>
+__device__ __forceinline__ floatx4 dense_mma(const DenseFrag<FP8>& w, const DenseFrag<FP8>& x, floatx4 acc) {
+    if constexpr (FP8) {
+        const intx8 a = __builtin_shufflevector(w.h[0], w.h[1], 0, 1, 2, 3, 4, 5, 6, 7);
+        const intx8 b = __builtin_shufflevector(x.h[0], x.h[1], 0, 1, 2, 3, 4, 5, 6, 7);
+        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 0, 0, 0, 0, 0, 0);
+    } else {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, w.h[0]),
+                                                       __builtin_bit_cast(bf16x8_t, x.h[0]), acc, 0, 0, 0);
+    }
+}
+
+// -- epilogue ----------------------------------------------------------------
+
+// z / (1 + e^-z) and its like: hardware exp2 and reciprocal, about 1 ulp each and the rounding of the
+// exponent, below 2e-6 of the value up to |z| of 30 (where e^-|z| is gone), before bf16's 4e-3.
+__device__ __forceinline__ float sigmoid_times(float z, float u) {
+    return z * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(u * -1.4426950408889634f));
+}
+
+// z Phi(z): with a = |z| / sqrt 2 and t = 1 / (1 + a / 2), erfc(a) = t P(t) e^(-a^2), P of degree 8 by weighted
+// least squares over a in [0, 12] (within 3e-7 of erfc in fp32), so that the negative side, where
+// 1 + erf cancels, keeps its relative precision.
+__device__ __forceinline__ float gelu_erf(float z) {
+    const float a = fabsf(z) * 0.70710678118654752f;
+    const float t = __builtin_amdgcn_rcpf(1.0f + 0.5f * a);
+    float p = -0.05936202353897773f;
+    p = p * t + 0.28600591597164415f;
+    p = p * t - 0.4901644081133491f;
+    p = p * t + 0.28145938040851415f;
+    p = p * t - 0.028961970795025077f;
+    p = p * t + 0.20367457674410538f;
+    p = p * t + 0.24285453204440827f;
+    p = p * t + 0.2824094757421122f;
+    p = p * t + 0.2820844776905523f;
+    const float q = 0.5f * t * p * __builtin_amdgcn_exp2f(a * a * -1.4426950408889634f);
+    return z < 0.0f ? z * q : z - z * q;
+}
+
+__device__ __forceinline__ void linear_activate(float (&y)[4], int act) {
+    if (act == MOE_ACT_RELU) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) y[r] = y[r] < 0.0f ? 0.0f : y[r];  // NaN stays
+    } else if (act == MOE_ACT_GELU) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) y[r] = gelu_erf(y[r]);
+    } else {
+        // silu, or z / 2 (1 + tanh u) = z / (1 + e^-2u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float z = y[r];
+            const float u = act == MOE_ACT_SILU ? z : 1.5957691216057308f * (z + 0.044715f * z * z * z);
+            y[r] = sigmoid_times(z, u);
+        }
+    }
+}
+
+// Columns col .. col + 3 of the weight row set at `base`: scales (1 for bf16) and bias (0 without).
+template <bool FP8>
+__device__ __forceinline__ void column_terms(const LinearArgs& p, int64_t row, float (&scale)[4], float (&bias)[4]) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        scale[r] = 1.0f;
+        bias[r] = 0.0f;
+    }
+    if constexpr (FP8) {
+        const auto v = *reinterpret_cast<const Unaligned<float, 4>*>(p.w_scales + row);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) scale[r] = v.v[r];
+    }
+    if (p.bias != nullptr) {
+        if (p.bias_bf16) {
+            const auto v = *reinterpret_cast<const Unaligned<uint16_t, 4>*>(static_cast<const uint16_t*>(p.bias) + row);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) bias[r] = bf16_to_f32(v.v[r]);
+        } else {
+            const auto v = *reinterpret_cast<const Unaligned<float, 4>*>(static_cast<const float*>(p.bias) + row);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) bias[r] = v.v[r];
+        }
+    }
+}
+
+// Four columns of one row of x: sums to bf16, with the residual's four values (0 without).
+template <bool FP8, LinearAct ACT>
+__device__ __forceinline__ uint2 finish4(const float (&z)[4], const float (&up)[4], float sx, const float (&scale)[4],
+                                         const float (&bias)[4], const float (&up_scale)[4], const float (&up_bias)[4],
+                                         int act, uint2 residual) {
+    float y[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const float v = (FP8 ? z[r] * (sx * scale[r]) : z[r]) + bias[r];
+        if constexpr (ACT == kActSwiglu) {
+            const float u = (FP8 ? up[r] * (sx * up_scale[r]) : up[r]) + up_bias[r];
+            y[r] = sigmoid_times(v, v) * u;
+        } else {
+            y[r] = v;
+        }
+    }
+    if constexpr (ACT == kActElement) linear_activate(y, act);
+    y[0] += __uint_as_float(residual.x << 16);
+    y[1] += __uint_as_float(residual.x & 0xffff0000u);
+    y[2] += __uint_as_float(residual.y << 16);
+    y[3] += __uint_as_float(residual.y & 0xffff0000u);
+    return make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
+}
+
+__device__ __forceinline__ void to_vgpr(floatx4& v) { asm volatile("" : "+v"(v)); }
+
+// One tile. Its prologue has been issued; `wait_all`: stores of the tile before may be in flight (they share the
+// loads' counter). With `chain` the last windows load the first stages of the next tile (resources
+// `next`), otherwise its whole prologue goes out in `hook`, once every wave is done with the ring.
+template <typename S, typename Hook>
+__device__ __forceinline__ void dense_tile(const LinearArgs& p, const LinearPlan& plan, char* lds, const LinearTile& t,
+                                           bool wait_all, int sa0, int sb0, bool chain,
+                                           typename DenseLoads<S>::Rsrc next, bool next_ends, int next_steps,
+                                           const Hook& hook) {
+    constexpr bool FP8 = S::FP8, SWIGLU = S::SWIGLU;
+    constexpr int FA = S::FA, FB = S::FB, SA = S::SA, SB = S::SB, HB = FB / 2, HM = FA * HB;
+    constexpr int A_LOADS = S::A_LOADS, B_LOADS = S::B_LOADS, LOADS = S::LOADS;
+    constexpr int SUBS = FP8 ? 1 : 2;         // steps of a stage
+    constexpr int SLOTS = 2 * SUBS * HM;      // matrix instructions of a window
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave / S::WC, wn = wave % S::WC;
+    const DenseLoads<S> ops(p, lds, DenseLoads<S>::resources(p, t));
+    const bool ends = t.step0 + t.steps == plan.steps;
+
+    // Lane l reads row l % 16 of a fragment at chunks l / 16 and 4 + l / 16: the two bf16 steps, or an e4m3
+    // step's two halves. Fragments 16 rows apart share the swizzle.
+    const int ar = wm * S::WTM + (lane & 15), br = wn * S::WTN + (lane & 15), chunk = lane >> 4;
+    uint32_t va[2], vb[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        va[h] = static_cast<uint32_t>(ar * kStageBytes + (((4 * h + chunk) ^ ring_swizzle(ar)) << 4));
+        vb[h] = S::B_BASE + static_cast<uint32_t>(br * kStageBytes + (((4 * h + chunk) ^ ring_swizzle(br)) << 4));
+    }
+    floatx4 acc[FA][FB];
+#pragma unroll
+    for (int i = 0; i < FA; ++i)
+#pragma unroll
+        for (int j = 0; j < FB; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[i][j][r] = 0.0f;
+
+    using Frag = DenseFrag<FP8>;
+    // Fragment idx of the step whose (first) address is va[sub] or vb[sub] plus the slot's offset.
+    auto read_at = [&](const uint32_t (&v)[2], uint32_t slot, auto sub_c, int idx) {
+        Frag f;
+        constexpr int sub = decltype(sub_c)::value;
+        f.h[0] = *reinterpret_cast<const intx4*>(lds + v[sub] + slot + idx * S::FRAG);
+        if constexpr (FP8) f.h[1] = *reinterpret_cast<const intx4*>(lds + v[1] + slot + idx * S::FRAG);
+        return f;
+    };
+    auto fence = [] { __builtin_amdgcn_sched_barrier(0); };
+    Frag fa[FA], fb[FB];
+    struct Refill {
+        int kt_a, slot_a, kt_b, slot_b;
+        __amdgpu_buffer_rsrc_t ra, rb;
+        bool a_last, b_last;
+    };
+    // Loads of a window: x in its first quarter, the weight in the two after it, where the quarters hold them.
+    constexpr bool kQuarters = A_LOADS <= SLOTS / 4 && B_LOADS <= SLOTS / 2;
+    auto refill_at = [&](auto g_c, const Refill& r) {
+        constexpr int g = decltype(g_c)::value;
+        static_for<A_LOADS>([&](auto l_c) {
+            constexpr int l = decltype(l_c)::value;
+            constexpr int slot = kQuarters ? l * (SLOTS / 4) / A_LOADS : l * SLOTS / LOADS;
+            if constexpr (slot == g) ops.issue_a(r.ra, r.kt_a, r.slot_a, l, r.a_last);
+        });
+        static_for<B_LOADS>([&](auto l_c) {
+            constexpr int l = decltype(l_c)::value;
+            constexpr int slot = kQuarters ? SLOTS / 4 + l * (SLOTS / 2) / B_LOADS : (A_LOADS + l) * SLOTS / LOADS;
+            if constexpr (slot == g) ops.issue_b(r.rb, r.kt_b, r.slot_b, l, r.b_last);
+        });
+    };
+    constexpr auto first_slot = [](int b) constexpr { return 2 * b < HM - 1 ? 2 * b : HM - 1; };
+    constexpr auto second_slot = [](int b) constexpr { return 2 * b + 1 < HM - 1 ? 2 * b + 1 : HM - 1; };
+    // Weight fragments [0, HB) by every x fragment (in snake order: one operand changes at a time), reading this
+    // step's fragments [HB, FB).
+    auto first_half = [&](uint32_t slot_b, auto sub_c, auto q_c, const Refill& rf) {
+        constexpr int q = decltype(q_c)::value;
+        static_for<HM>([&](auto m_c) {
+            constexpr int m = decltype(m_c)::value;
+            constexpr int i = m / HB, j = (i % 2) ? HB - 1 - m % HB : m % HB;
+            if constexpr (q >= 0) refill_at(std::integral_constant<int, q * HM + m>{}, rf);
+            acc[i][j] = dense_mma<FP8>(fb[j], fa[i], acc[i][j]);
+            static_for<HB>([&](auto b_c) {
+                constexpr int b = decltype(b_c)::value;
+                if constexpr (first_slot(b) == m) fb[HB + b] = read_at(vb, slot_b, sub_c, HB + b);
+            });
+            fence();
+        });
+    };
+    // The other weight fragments, reading the next step's x fragments and weight fragments [0, HB).
+    auto second_half = [&](uint32_t slot_a, uint32_t slot_b, auto sub_c, auto last_c, auto q_c, const Refill& rf) {
+        constexpr bool last = decltype(last_c)::value;
+        constexpr int q = decltype(q_c)::value;
+        static_for<HM>([&](auto m_c) {
+            constexpr int m = decltype(m_c)::value;
+            constexpr int i = m / HB, j = HB + ((i % 2) ? HB - 1 - m % HB : m % HB);
+            if constexpr (q >= 0) refill_at(std::integral_constant<int, q * HM + m>{}, rf);
+            acc[i][j] = dense_mma<FP8>(fb[j], fa[i], acc[i][j]);
+            if constexpr (!last) {
+                static_for<HB>([&](auto b_c) {
+                    constexpr int b = decltype(b_c)::value;
+                    if constexpr (second_slot(b) == m) fb[b] = read_at(vb, slot_b, sub_c, b);
+                });
+                if constexpr (m % HB == HB - 1) fa[i] = read_at(va, slot_a, sub_c, i);
+            }
+            fence();
+        });
+    };
+    using C0 = std::integral_constant<int, 0>;
+    using C1 = std::integral_constant<int, 1>;
+    using NoLoads = std::integral_constant<int, -1>;
+    using More = std::false_type;
+    const Refill none{0, 0, 0, 0, ops.ra, ops.rb, false, false};
+    const int steps = t.steps;
+    if (wait_all)
+        wait_vm_lgkm<0>();
+    else
+        wait_vm_lgkm<S::VM_FIRST>();
+    ring_barrier();
+    fence();
+    {
+        const uint32_t a0 = sa0 * S::A_STAGE, b0 = sb0 * S::B_STAGE;
+#pragma unroll
+        for (int b = 0; b < HB; ++b) fb[b] = read_at(vb, b0, C0{}, b);
+#pragma unroll
+        for (int i = 0; i < FA; ++i) fa[i] = read_at(va, a0, C0{}, i);
+        first_half(b0, C0{}, NoLoads{}, none);
+        if constexpr (SUBS == 2) {
+            second_half(a0, b0, C1{}, More{}, NoLoads{}, none);
+            first_half(b0, C1{}, NoLoads{}, none);
+        }
+    }
+    int sa = sa0, sb = sb0;  // slots of the stage whose last half is pending
+    auto window = [&](const Refill& rf, int na, int nb) {
+        const uint32_t a0 = na * S::A_STAGE, b0 = nb * S::B_STAGE;
+        fence();
+        wait_vm_lgkm<S::VM_STEADY>();
+        ring_barrier();
+        fence();
+        second_half(a0, b0, C0{}, More{}, C0{}, rf);
+        first_half(b0, C0{}, C1{}, rf);
+        if constexpr (SUBS == 2) {
+            second_half(a0, b0, C1{}, More{}, std::integral_constant<int, 2>{}, rf);
+            first_half(b0, C1{}, std::integral_constant<int, 3>{}, rf);
+        }
+    };
+    int u = 0;
+    // Refills of this tile's whole stages, without selects; then the last windows in full.
+    for (; u < steps - SB - 1; ++u) {
+        const int na = sa + 1 == SA ? 0 : sa + 1, nb = sb + 1 == SB ? 0 : sb + 1;
+        window(Refill{u + SA, sa, u + SB, sb, ops.ra, ops.rb, false, false}, na, nb);
+        sa = na;
+        sb = nb;
+    }
+    for (; u + 1 < steps; ++u) {
+        const int na = sa + 1 == SA ? 0 : sa + 1, nb = sb + 1 == SB ? 0 : sb + 1;
+        const bool a_next = chain && u + SA >= steps, b_next = chain && u + SB >= steps;
+        const int kt_a = a_next ? u + SA - steps : min(u + SA, steps - 1);
+        const int kt_b = b_next ? u + SB - steps : min(u + SB, steps - 1);
+        window(Refill{kt_a, sa, kt_b, sb, a_next ? next.a : ops.ra, b_next ? next.b : ops.rb,
+                      a_next ? next_ends && kt_a == next_steps - 1 : ends && kt_a == steps - 1,
+                      b_next ? next_ends && kt_b == next_steps - 1 : ends && kt_b == steps - 1},
+               na, nb);
+        sa = na;
+        sb = nb;
+    }
+    second_half(0u, 0u, C0{}, std::true_type{}, NoLoads{}, none);
+    wait_vm_lgkm<0>();
+    ring_barrier();
+    hook();
+
+    // Lane l holds, of each 16 x 16 block, row l % 16 and columns 4 (l / 16) + 0..3. The empty asm moves a row of
+    // accumulators to plain registers before the epilogue's pairs could shape their assignment in the loop.
+    const int lane_row = lane >> 4;
+    const int col4 = 4 * lane_row;
+    const int col8 = 8 * (((lane_row & 1) << 1) | (lane_row >> 1));
+    constexpr int OUT = SWIGLU ? FB / 2 : FB;
+    const int64_t first_col = t.col0 + wn * (SWIGLU ? S::WTN / 2 : S::WTN);
+    if (plan.splits > 1) {
+        // Partial sums of weight rows, as they are.
+        static_for<FA>([&](auto i_c) {
+            constexpr int i = decltype(i_c)::value;
+            const int64_t row = t.row0 + wm * S::WTM + i * 16 + (lane & 15);
+            float* to = plan.partial + (t.split * p.tokens + row) * p.rows;
+            static_for<FB>([&](auto j_c) {
+                constexpr int j = decltype(j_c)::value;
+                to_vgpr(acc[i][j]);
+                constexpr bool up = SWIGLU && j >= OUT;
+                const int64_t col = first_col + (up ? j - OUT : j) * 16 + col4;
+                if (row < p.tokens && col < p.n) *reinterpret_cast<floatx4*>(to + (up ? p.n : 0) + col) = acc[i][j];
+            });
+        });
+        return;
+    }
+    float scale[OUT][4], bias[OUT][4], up_scale[OUT][4], up_bias[OUT][4];
+    static_for<OUT>([&](auto j_c) {
+        constexpr int j = decltype(j_c)::value;
+        const int64_t col = min(first_col + j * 16 + col4, p.n - 4);
+        column_terms<FP8>(p, col, scale[j], bias[j]);
+        if constexpr (SWIGLU) column_terms<FP8>(p, p.n + col, up_scale[j], up_bias[j]);
+    });
+    static_for<FA>([&](auto i_c) {
+        constexpr int i = decltype(i_c)::value;
+        static_for<FB>([&](auto j_c) { to_vgpr(acc[i][decltype(j_c)::value]); });
+        const int64_t row = t.row0 + wm * S::WTM + i * 16 + (lane & 15);
+        const bool row_ok = row < p.tokens;
+        const int64_t at = (row_ok ? row : t.row0) * p.n;
+        const float sx = FP8 && row_ok ? p.x_scales[row] : 1.0f;
+        uint2 out[OUT];
+        static_for<OUT>([&](auto j_c) {
+            constexpr int j = decltype(j_c)::value;
+            const int64_t col = first_col + j * 16 + col4;
+            uint2 residual = make_uint2(0, 0);
+            if (p.residual != nullptr && row_ok && col < p.n)
+                residual = *reinterpret_cast<const uint2*>(p.residual + at + col);
+            float z[4], v[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                z[r] = acc[i][j][r];
+                v[r] = SWIGLU ? acc[i][SWIGLU ? j + OUT : j][r] : 0.0f;
+            }
+            out[j] = finish4<FP8, S::ACT>(z, v, sx, scale[j], bias[j], up_scale[j], up_bias[j], p.activation, residual);
+        });
+        // Lanes 16 apart trade halves of two neighbouring blocks: 16-byte stores of 8 columns.
+        static_for<OUT / 2>([&](auto h_c) {
+            constexpr int j = 2 * decltype(h_c)::value;
+            const auto s0 = __builtin_amdgcn_permlane16_swap(out[j].x, out[j + 1].x, false, false);
+            const auto s1 = __builtin_amdgcn_permlane16_swap(out[j].y, out[j + 1].y, false, false);
+            const int64_t col = first_col + j * 16 + col8;
+            if (row_ok && col < p.n)
+                *reinterpret_cast<uint4*>(p.output + at + col) = make_uint4(s0[0], s1[0], s0[1], s1[1]);
+        });
+        if constexpr (OUT % 2 == 1) {
+            const int64_t col = first_col + (OUT - 1) * 16 + col4;
+            if (row_ok && col < p.n) *reinterpret_cast<uint2*>(p.output + at + col) = out[OUT - 1];
+        }
+    });
+}
+
+// Persistent: workgroups on XCD i % 8 take a contiguous share of the tiles, in order, so that the CUs of one L2
+// work on neighbouring rows of x and the same weight rows.
+template <typename S>
+__global__ __launch_bounds__(256) void dense_ring_kernel(LinearArgs p, LinearPlan plan) {
+    __shared__ __attribute__((aligned(1024))) char lds[S::LDS];
+    using Loads = DenseLoads<S>;
+    const int tiles = plan.row_tiles * plan.col_tiles * plan.splits;
+    const int grid = static_cast<int>(gridDim.x);
+    const int xcds = grid < kNumXcd ? 1 : kNumXcd;
+    // XCD x has tiles [x tiles / xcds, (x + 1) tiles / xcds), its workgroups every (grid / xcds)-th of them.
+    const int xcd = blockIdx.x % xcds, per = grid / xcds;
+    const int first = static_cast<int>(static_cast<int64_t>(xcd) * tiles / xcds);
+    const int end = static_cast<int>(static_cast<int64_t>(xcd + 1) * tiles / xcds);
+    auto locate = [&](int index) {
+        LinearTile t{false, 0, 0, 0, 0, 0};
+        if (index >= end) return t;
+        const int column = index / plan.row_tiles;
+        t.split = column / plan.col_tiles;
+        t.row0 = (index - column * plan.row_tiles) * S::TM;
+        t.col0 = (column - t.split * plan.col_tiles) * S::COLS;
+        t.step0 = t.split * plan.split_steps;
+        t.steps = min(plan.split_steps, plan.steps - t.step0);
+        t.valid = true;
+        return t;
+    };
+    int at = first + static_cast<int>(blockIdx.x) / xcds;
+    LinearTile cur = locate(at);
+    if (!cur.valid) return;
+    Loads(p, lds, Loads::resources(p, cur)).prologue(cur.steps, cur.step0 + cur.steps == plan.steps, 0, 0, false);
+    bool after = false;
+    int sa = 0, sb = 0;
+    for (;;) {
+        at += per;
+        LinearTile nxt = locate(at);
+        {
+            // Opaque copies: nothing of the next tile is formed early and kept through the loop.
+            int v = nxt.valid, r = nxt.row0, c = nxt.col0, k = nxt.step0, n = nxt.steps, s = nxt.split;
+            asm volatile("" : "+s"(v), "+s"(r), "+s"(c), "+s"(k), "+s"(n), "+s"(s));
+            nxt = LinearTile{v != 0, r, c, k, n, s};
+        }
+        const bool chain = nxt.valid && cur.steps >= S::SB && nxt.steps >= S::SB;
+        const bool next_ends = nxt.step0 + nxt.steps == plan.steps;
+        typename Loads::Rsrc next{};
+        if (chain) next = Loads::resources(p, nxt);
+        const int na = (sa + cur.steps) % S::SA, nb = (sb + cur.steps) % S::SB;
+        auto hook = [&] {
+            if (!nxt.valid) return;
+            const Loads ops(p, lds, Loads::resources(p, nxt));
+            ops.prologue(nxt.steps, next_ends, chain ? na : 0, chain ? nb : 0, chain);
+        };
+        dense_tile<S>(p, plan, lds, cur, after, sa, sb, chain, next, next_ends, nxt.steps, hook);
+        if (!nxt.valid) break;
+        sa = chain ? na : 0;
+        sb = chain ? nb : 0;
+        cur = nxt;
+        after = true;
+    }
+}
+
+// f(constant<LinearAct>, constant<FP8>) for these operands.
+template <typename F>
+void linear_instance(const LinearArgs& a, F&& f) {
+    auto by_type = [&](auto act) { a.fp8 ? f(act, std::true_type{}) : f(act, std::false_type{}); };
+    if (a.activation == MOE_ACT_SWIGLU)
+        by_type(std::integral_constant<LinearAct, kActSwiglu>{});
+    else if (a.activation == MOE_ACT_NONE)
+        by_type(std::integral_constant<LinearAct, kActNone>{});
+    else
+        by_type(std::integral_constant<LinearAct, kActElement>{});
+}
+
+// The shape's kernel for these operands.
+template <int TM, int BN, uint32_t LDS, int WC>
+void run_dense(const LinearArgs& a, const LinearPlan& plan, int grid, hipStream_t stream) {
+    linear_instance(a, [&](auto act, auto fp8) {
+        using S = DenseShape<TM, BN, decltype(act)::value, decltype(fp8)::value, LDS, WC>;
+        dense_ring_kernel<S><<<grid, 256, 0, stream>>>(a, plan);
+    });
+}
+
+extern template void run_dense<256, 256, 160 * 1024, 2>(const LinearArgs&, const LinearPlan&, int, hipStream_t);
+extern template void run_dense<128, 128, 80 * 1024, 2>(const LinearArgs&, const LinearPlan&, int, hipStream_t);
+extern template void run_dense<64, 64, 53 * 1024, 2>(const LinearArgs&, const LinearPlan&, int, hipStream_t);
+
+}  // namespace moe

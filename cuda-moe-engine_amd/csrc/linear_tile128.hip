@@ -1,0 +1,6 @@
+// The 128 x 128 tiles of the dense products, in a file of their own for the time they take to compile.
+#include "linear_ring.h"
+
+namespace moe {
+template void run_dense<128, 128, 80 * 1024, 2>(const LinearArgs&, const LinearPlan&, int, hipStream_t);
+}  // namespace moe

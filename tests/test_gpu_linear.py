@@ -223,5 +223,6 @@ def test_weights_past_two_gib():
     for tokens in (1, 80):
         x = _normal(g, tokens, hidden).bfloat16()
         got = linear(x, w)
-        assert torch.equal(got[:, -64:], linear(x, w[-64:].contiguous()))
+        # A product of another width may split its sums elsewhere: the formula, not the bits.
+        _check(got[:, -64:], x, w[-64:], None, None, None, tokens)
         assert not bool(got[:, :-64].any())
