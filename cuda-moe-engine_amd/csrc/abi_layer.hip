@@ -1,6 +1,8 @@
 // extern "C" entry points of the operators around the experts: norm, scored routing, dense
 // products and gradient clipping. Argument checks, then the launches on the caller's stream;
 // nothing here allocates, synchronises or throws.
+#include <algorithm>
+
 #include "linear.h"
 #include "row_ops.h"
 
@@ -87,9 +89,9 @@ int moe_quantize_rows(const void* x, int dtype, void* values, float* scales, int
     return launch_quantize_rows(a, static_cast<hipStream_t>(stream));
 }
 
-int64_t moe_rms_norm_backward_scratch_bytes(int64_t tokens, int64_t hidden) {
-    if (tokens < 0 || tokens > kMaxLayerTokens || hidden < 1 || hidden > kMaxNormWidth) return -1;
-    return rms_norm_backward_scratch_bytes(tokens, hidden);
+int64_t moe_rms_norm_backward_scratch_bytes(int64_t tokens, int64_t hidden, int dtype) {
+    if (tokens < 0 || tokens > kMaxLayerTokens || hidden < 1 || hidden > kMaxNormWidth || !valid_dtype(dtype)) return -1;
+    return rms_norm_backward_scratch_bytes(tokens, hidden, dtype);
 }
 
 int moe_rms_norm_backward(const void* grad_output, const void* x, int dtype, const void* weight, int weight_dtype,
@@ -102,7 +104,7 @@ int moe_rms_norm_backward(const void* grad_output, const void* x, int dtype, con
     MOE_REQUIRE(tokens >= 1, MOE_ERR_INVALID_ARGUMENT, "norm gradients need at least one token");
     if (!grad_x && !grad_weight) return MOE_OK;
     MOE_REQUIRE(grad_output && x && rstd, MOE_ERR_INVALID_ARGUMENT, "null pointer");
-    const int64_t need = grad_weight ? rms_norm_backward_scratch_bytes(tokens, hidden) : 0;
+    const int64_t need = grad_weight ? rms_norm_backward_scratch_bytes(tokens, hidden, dtype) : 0;
     MOE_REQUIRE(need == 0 || (scratch && scratch_bytes >= need), MOE_ERR_WORKSPACE,
                 "norm gradient scratch needs %lld bytes, got %lld", (long long)need, (long long)scratch_bytes);
     const uintptr_t elem = dtype_size(dtype);
@@ -217,6 +219,26 @@ int moe_clip_gradients(const moe_clip_args* p, void* stream) {
     }
     return launch_clip_gradients(p->grads, p->outputs, p->elements, p->dtypes, p->tensors, p->max_norm, p->norm,
                                  static_cast<double*>(p->scratch), static_cast<hipStream_t>(stream));
+}
+
+int moe_clip_overlap(const void* const* grads, const void* const* outputs, const int64_t* elements,
+                     const int64_t* dtypes, uint64_t* room, int64_t tensors) {
+    struct Range {
+        uint64_t from, to;
+    };
+    Range* ranges = reinterpret_cast<Range*>(room);
+    int64_t count = 0;
+    for (int64_t i = 0; i < tensors; ++i) {
+        const uint64_t bytes = static_cast<uint64_t>(elements[i]) * dtype_size(static_cast<int>(dtypes[i]));
+        if (bytes == 0) continue;
+        const uint64_t g = reinterpret_cast<uint64_t>(grads[i]), o = reinterpret_cast<uint64_t>(outputs[i]);
+        ranges[count++] = Range{g, g + bytes};
+        if (o != g) ranges[count++] = Range{o, o + bytes};
+    }
+    std::sort(ranges, ranges + count, [](const Range& a, const Range& b) { return a.from < b.from; });
+    for (int64_t i = 1; i < count; ++i)
+        if (ranges[i - 1].to > ranges[i].from) return 1;
+    return 0;
 }
 
 }  // extern "C"

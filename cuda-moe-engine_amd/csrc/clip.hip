@@ -15,8 +15,9 @@ namespace moe {
 namespace {
 
 constexpr int kClipTensors = 112;   // of one launch: their table fits the kernel's arguments
-constexpr int kChunk = 1 << 15;     // elements a workgroup takes at a time
 constexpr int kThreads = 256;
+constexpr int kLeastChunk = 1 << 11, kMostChunk = 1 << 16;
+constexpr int kUnroll = 4;          // vectors of 16 bytes a lane has in flight
 
 struct ClipTable {
     const void* in[kClipTensors];
@@ -25,6 +26,7 @@ struct ClipTable {
     int32_t first[kClipTensors + 1];  // chunks before each tensor
     int8_t dtype[kClipTensors];
     int tensors;
+    int chunk;  // elements a workgroup takes at a time
 };
 static_assert(sizeof(ClipTable) + 64 <= 4096, "kernel arguments");
 
@@ -57,18 +59,36 @@ __device__ __forceinline__ double block_sum(double x, double* lds) {
     return sum;
 }
 
+// f(first element, v[N]) of a chunk of n elements from g, kUnroll vectors a lane in flight: whole
+// rounds of the workgroup, then vector by vector, the last one short.
+template <int DT, typename F>
+__device__ __forceinline__ void each_vector(const typename Elem<DT>::T* g, int n, const F& f) {
+    constexpr int N = DT == MOE_DTYPE_F32 ? 4 : 8, STEP = kThreads * N;
+    int at = threadIdx.x * N;
+    for (; at + (kUnroll - 1) * STEP + N <= n; at += kUnroll * STEP) {
+        typename Bytes<16>::V v[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) v[u] = load_bytes<16>(g + at + u * STEP);
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            float x[N];
+            unpack<DT>(v[u], x);
+            f(at + u * STEP, x);
+        }
+    }
+    for (; at < n; at += STEP) {
+        float x[N];
+        load_row<DT, N>(g, at, n, x);
+        f(at, x);
+    }
+}
+
 template <int DT>
 __device__ __forceinline__ double squares(const void* in, int64_t from, int n) {
-    using T = typename Elem<DT>::T;
-    constexpr int N = DT == MOE_DTYPE_F32 ? 4 : 8;
-    const T* g = static_cast<const T*>(in) + from;
     double sum = 0.0;
-    for (int at = threadIdx.x * N; at < n; at += kThreads * N) {
-        float v[N];
-        load_row<DT, N>(g, at, n, v);
-#pragma unroll
-        for (int i = 0; i < N; ++i) sum += static_cast<double>(v[i]) * static_cast<double>(v[i]);
-    }
+    each_vector<DT>(static_cast<const typename Elem<DT>::T*>(in) + from, n, [&](int, const auto& x) {
+        for (float v : x) sum += static_cast<double>(v) * static_cast<double>(v);
+    });
     return sum;
 }
 
@@ -78,8 +98,8 @@ __global__ __launch_bounds__(kThreads) void clip_norm_kernel(ClipTable t, double
     const int chunks = t.first[t.tensors];
     for (int chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
         const int i = tensor_of(t, chunk);
-        const int64_t from = static_cast<int64_t>(chunk - t.first[i]) * kChunk;
-        const int n = static_cast<int>(min<int64_t>(kChunk, t.elements[i] - from));
+        const int64_t from = static_cast<int64_t>(chunk - t.first[i]) * t.chunk;
+        const int n = static_cast<int>(min<int64_t>(t.chunk, t.elements[i] - from));
         const int dt = t.dtype[i];
         if (dt == MOE_DTYPE_F32)
             sum += squares<MOE_DTYPE_F32>(t.in[i], from, n);
@@ -94,17 +114,11 @@ __global__ __launch_bounds__(kThreads) void clip_norm_kernel(ClipTable t, double
 
 template <int DT>
 __device__ __forceinline__ void scale(const void* in, void* out, int64_t from, int n, float factor) {
-    using T = typename Elem<DT>::T;
-    constexpr int N = DT == MOE_DTYPE_F32 ? 4 : 8;
-    const T* g = static_cast<const T*>(in) + from;
-    T* o = static_cast<T*>(out) + from;
-    for (int at = threadIdx.x * N; at < n; at += kThreads * N) {
-        float v[N];
-        load_row<DT, N>(g, at, n, v);
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] *= factor;
-        store_row<DT, N>(o, at, n, v);
-    }
+    typename Elem<DT>::T* o = static_cast<typename Elem<DT>::T*>(out) + from;
+    each_vector<DT>(static_cast<const typename Elem<DT>::T*>(in) + from, n, [&](int at, auto& x) {
+        for (float& v : x) v *= factor;
+        store_row<DT>(o, at, n, x);
+    });
 }
 
 // `count` partial sums of all the norm launches; the first launch's first workgroup writes the norm.
@@ -119,11 +133,12 @@ __global__ __launch_bounds__(kThreads) void clip_scale_kernel(ClipTable t, const
     const double ratio = max_norm / (norm + 1e-6);
     const float factor = norm < __builtin_inf() && ratio < 1.0 ? static_cast<float>(ratio) : 1.0f;
     const int chunks = t.first[t.tensors];
-    for (int chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
+    // Backwards: what the pass before read last may still be in the caches.
+    for (int chunk = chunks - 1 - static_cast<int>(blockIdx.x); chunk >= 0; chunk -= gridDim.x) {
         const int i = tensor_of(t, chunk);
         if (factor == 1.0f && t.in[i] == t.out[i]) continue;
-        const int64_t from = static_cast<int64_t>(chunk - t.first[i]) * kChunk;
-        const int n = static_cast<int>(min<int64_t>(kChunk, t.elements[i] - from));
+        const int64_t from = static_cast<int64_t>(chunk - t.first[i]) * t.chunk;
+        const int n = static_cast<int>(min<int64_t>(t.chunk, t.elements[i] - from));
         const int dt = t.dtype[i];
         if (dt == MOE_DTYPE_F32)
             scale<MOE_DTYPE_F32>(t.in[i], t.out[i], from, n, factor);
@@ -139,6 +154,8 @@ int blocks_of(int chunks, int launches) {
     return chunks < most ? (chunks < 1 ? 1 : chunks) : most;
 }
 
+int chunks_of(int64_t elements, int chunk) { return static_cast<int>((elements + chunk - 1) / chunk); }
+
 }  // namespace
 
 // The entry point has bounded tensors and elements, so that chunks fit 32 bits and every
@@ -146,18 +163,18 @@ int blocks_of(int chunks, int launches) {
 int launch_clip_gradients(const void* const* grads, void* const* outputs, const int64_t* elements, const int64_t* dtypes,
                           int64_t tensors, double max_norm, float* norm, double* partials, hipStream_t stream) {
     const int launches = tensors <= kClipTensors ? 1 : static_cast<int>((tensors + kClipTensors - 1) / kClipTensors);
+    // A chunk for each of kClipPartials workgroups, within bounds: small batches spread over the chip, large
+    // ones do not search for their tensor all the time.
+    int64_t total = 0;
+    for (int64_t i = 0; i < tensors; ++i) total += elements[i];
+    int chunk = kLeastChunk;
+    while (chunk < kMostChunk && chunk * kClipPartials < total) chunk *= 2;
+    int used = 0;
     for (int pass = 0; pass < 2; ++pass) {
-        int used = 0, total = 0;
-        if (pass == 1)
-            for (int l = 0; l < launches; ++l) {
-                int64_t chunks = 0;
-                for (int64_t i = l * kClipTensors; i < tensors && i < (l + 1) * kClipTensors; ++i)
-                    chunks += (elements[i] + kChunk - 1) / kChunk;
-                total += blocks_of(static_cast<int>(chunks), launches);
-            }
         for (int l = 0; l < launches; ++l) {
             ClipTable t;
             t.tensors = 0;
+            t.chunk = chunk;
             int chunks = 0;
             for (int64_t i = l * kClipTensors; i < tensors && i < (l + 1) * kClipTensors; ++i) {
                 const int k = t.tensors++;
@@ -166,7 +183,7 @@ int launch_clip_gradients(const void* const* grads, void* const* outputs, const 
                 t.elements[k] = elements[i];
                 t.dtype[k] = static_cast<int8_t>(dtypes[i]);
                 t.first[k] = chunks;
-                chunks += static_cast<int>((elements[i] + kChunk - 1) / kChunk);
+                chunks += chunks_of(elements[i], chunk);
             }
             t.first[t.tensors] = chunks;
             const int blocks = blocks_of(chunks, launches);
@@ -174,7 +191,7 @@ int launch_clip_gradients(const void* const* grads, void* const* outputs, const 
                 clip_norm_kernel<<<blocks, kThreads, 0, stream>>>(t, partials + used);
                 used += blocks;
             } else {
-                clip_scale_kernel<<<blocks, kThreads, 0, stream>>>(t, partials, total, max_norm, l == 0 ? norm : nullptr);
+                clip_scale_kernel<<<blocks, kThreads, 0, stream>>>(t, partials, used, max_norm, l == 0 ? norm : nullptr);
             }
         }
     }

@@ -7,6 +7,8 @@
 // A row is read once: it waits in registers between its sum of squares, its largest value
 // and its output (the norm is taken of the fp32 sum of x and residual, not of its rounded
 // copy, so y is rounded once). Bound by the bytes.
+#include <algorithm>
+
 #include "row_ops.h"
 
 namespace moe {
@@ -53,9 +55,9 @@ __device__ __forceinline__ void store_e4m3(uint8_t* row, int at, int n, const fl
         words[i] = __builtin_amdgcn_cvt_pk_fp8_f32(in[4 * i + 2], in[4 * i + 3], word, true);
     }
     if (at + N <= n) {
-        Unaligned<uint8_t, N> v;
+        typename Bytes<N>::V v;
         __builtin_memcpy(&v, words, N);
-        *reinterpret_cast<Unaligned<uint8_t, N>*>(row + at) = v;
+        store_bytes<N>(row + at, v);
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i)
@@ -63,7 +65,8 @@ __device__ __forceinline__ void store_e4m3(uint8_t* row, int at, int n, const fl
     }
 }
 
-// WAVES waves a row (a workgroup of max(WAVES, 4) waves takes 4 / WAVES rows), NV vectors a lane.
+// WAVES waves a row, NV vectors a lane; a workgroup of four waves takes four rows at a time where a wave is enough.
+// Workgroups walk the rows, the next row's loads in flight while one is summed and written.
 // NORM false: the rows are only written in 8 bits (quantize_rows).
 template <int DT, int NV, int WAVES, bool QUANT, bool NORM>
 __global__ __launch_bounds__(WAVES < 4 ? 256 : WAVES * 64) void rms_norm_kernel(NormArgs a) {
@@ -71,85 +74,112 @@ __global__ __launch_bounds__(WAVES < 4 ? 256 : WAVES * 64) void rms_norm_kernel(
     constexpr int N = kVec<DT>;
     constexpr int ROWS = WAVES < 4 ? 4 / WAVES : 1;
     static_assert(WAVES == 1 || WAVES >= 4, "rows share no barrier");
-    __shared__ float lds[2][WAVES];
+    __shared__ float lds[2][2][WAVES];
     const int thread = WAVES == 1 ? threadIdx.x & 63 : threadIdx.x;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + (WAVES == 1 ? threadIdx.x >> 6 : 0);
-    if (row >= a.tokens) return;
     const int n = a.hidden;
-    const bool same = a.weight_dtype == DT;
-    const T* x = static_cast<const T*>(a.x) + row * n;
-    float h[NV][N];
-    float sum = 0.0f;
+    const int64_t stride = static_cast<int64_t>(gridDim.x) * ROWS;
+    int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + (WAVES == 1 ? threadIdx.x >> 6 : 0);
+    if (row >= a.tokens) return;
+    using V = typename Bytes<N * sizeof(T)>::V;
+    V xv[NV], rv[NV];
+    const bool add = NORM && a.residual != nullptr;
+    auto fetch = [&](int64_t at_row) {
+        const T* x = static_cast<const T*>(a.x) + at_row * n;
+        const T* r = static_cast<const T*>(a.residual) + at_row * n;
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-        const int at = (v * WAVES * 64 + thread) * N;
-        if (at < n) {
-            load_row<DT, N>(x, at, n, h[v]);
-        } else {
+        for (int v = 0; v < NV; ++v) {
+            const int at = (v * WAVES * 64 + thread) * N;
+            if (at < n) {
+                xv[v] = load_vector<T, N>(x, at, n);
+                if (add) rv[v] = load_vector<T, N>(r, at, n);
+            }
+        }
+    };
+    fetch(row);
+    float w[NORM ? NV : 1][N];
+    if constexpr (NORM) {
+        const bool same = a.weight_dtype == DT;
 #pragma unroll
-            for (int i = 0; i < N; ++i) h[v][i] = 0.0f;
+        for (int v = 0; v < NV; ++v) {
+            const int at = (v * WAVES * 64 + thread) * N;
+            if (at < n) load_weights<DT, N>(a.weight, same, at, n, w[v]);
         }
     }
-    if constexpr (NORM) {
-        if (a.residual != nullptr) {
-            const T* r = static_cast<const T*>(a.residual) + row * n;
-            T* total = static_cast<T*>(a.total) + row * n;
+    for (int turn = 0; row < a.tokens; turn ^= 1) {
+        float h[NV][N];
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const int at = (v * WAVES * 64 + thread) * N;
+            if (at >= n) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) h[v][i] = 0.0f;
+                continue;
+            }
+            unpack<DT>(xv[v], h[v]);
+            if (add) {
+                float r[N];
+                unpack<DT>(rv[v], r);
+#pragma unroll
+                for (int i = 0; i < N; ++i) h[v][i] += r[i];
+            }
+        }
+        const int64_t this_row = row;
+        row += stride;
+        if (row < a.tokens) fetch(row);
+        if (add) {
+            T* total = static_cast<T*>(a.total) + this_row * n;
 #pragma unroll
             for (int v = 0; v < NV; ++v) {
                 const int at = (v * WAVES * 64 + thread) * N;
-                if (at >= n) continue;
-                float add[N];
-                load_row<DT, N>(r, at, n, add);
-#pragma unroll
-                for (int i = 0; i < N; ++i) h[v][i] += add[i];
-                store_row<DT, N>(total, at, n, h[v]);
+                if (at < n) store_row<DT, N>(total, at, n, h[v]);
             }
         }
+        if constexpr (NORM) {
+            float sum = 0.0f;
 #pragma unroll
-        for (int v = 0; v < NV; ++v)
+            for (int v = 0; v < NV; ++v)
 #pragma unroll
-            for (int i = 0; i < N; ++i) sum += h[v][i] * h[v][i];
-        sum = row_reduce<SumOp, WAVES>(sum, lds[0]);
-        const float rstd = 1.0f / sqrtf(sum / static_cast<float>(n) + a.eps);
-        if (a.rstd != nullptr && thread == 0) a.rstd[row] = rstd;
+                for (int i = 0; i < N; ++i) sum += h[v][i] * h[v][i];
+            sum = row_reduce<SumOp, WAVES>(sum, lds[turn][0]);
+            const float rstd = 1.0f / sqrtf(sum / static_cast<float>(n) + a.eps);
+            if (a.rstd != nullptr && thread == 0) a.rstd[this_row] = rstd;
+#pragma unroll
+            for (int v = 0; v < NV; ++v)
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const int at = (v * WAVES * 64 + thread) * N;
+                    if (at < n) h[v][i] = h[v][i] * rstd * w[v][i];
+                }
+        }
+        float inverse = 1.0f;
+        if constexpr (QUANT) {
+            float most = 0.0f;
+#pragma unroll
+            for (int v = 0; v < NV; ++v)
+#pragma unroll
+                for (int i = 0; i < N; ++i) most = fmaxf(most, fabsf(h[v][i]));
+            most = fmaxf(row_reduce<MaxOp, WAVES>(most, lds[turn][1]), kLeastAmax);
+            const float scale = most / kE4m3Most;
+            if (thread == 0) a.scales[this_row] = scale;
+            inverse = 1.0f / scale;
+        }
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
             const int at = (v * WAVES * 64 + thread) * N;
             if (at >= n) continue;
-            float w[N];
-            load_weights<DT, N>(a.weight, same, at, n, w);
+            if constexpr (QUANT) {
+                // The largest value may come out a rounding past 448: it is held there. A minimum
+                // would hide a NaN, which the conversion keeps.
+                float q[N];
 #pragma unroll
-            for (int i = 0; i < N; ++i) h[v][i] = h[v][i] * rstd * w[i];
-        }
-    }
-    float inverse = 1.0f;
-    if constexpr (QUANT) {
-        float most = 0.0f;
-#pragma unroll
-        for (int v = 0; v < NV; ++v)
-#pragma unroll
-            for (int i = 0; i < N; ++i) most = fmaxf(most, fabsf(h[v][i]));
-        most = fmaxf(row_reduce<MaxOp, WAVES>(most, lds[1]), kLeastAmax);
-        const float scale = most / kE4m3Most;
-        if (thread == 0) a.scales[row] = scale;
-        inverse = 1.0f / scale;
-    }
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-        const int at = (v * WAVES * 64 + thread) * N;
-        if (at >= n) continue;
-        if constexpr (QUANT) {
-            // The largest value may come out a rounding past 448: it is held there.
-            // fmed3 would hide a NaN, which the conversion keeps.
-            float q[N];
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const float y = h[v][i] * inverse;
-                q[i] = fabsf(y) > kE4m3Most ? copysignf(kE4m3Most, y) : y;
+                for (int i = 0; i < N; ++i) {
+                    const float y = h[v][i] * inverse;
+                    q[i] = fabsf(y) > kE4m3Most ? copysignf(kE4m3Most, y) : y;
+                }
+                store_e4m3<N>(static_cast<uint8_t*>(a.output) + this_row * n, at, n, q);
+            } else {
+                store_row<DT, N>(static_cast<T*>(a.output) + this_row * n, at, n, h[v]);
             }
-            store_e4m3<N>(static_cast<uint8_t*>(a.output) + row * n, at, n, q);
-        } else {
-            store_row<DT, N>(static_cast<T*>(a.output) + row * n, at, n, h[v]);
         }
     }
 }
@@ -157,7 +187,10 @@ __global__ __launch_bounds__(WAVES < 4 ? 256 : WAVES * 64) void rms_norm_kernel(
 template <int DT, int NV, int WAVES>
 void run_norm(const NormArgs& a, bool norm, hipStream_t stream) {
     constexpr int ROWS = WAVES < 4 ? 4 / WAVES : 1;
-    const dim3 grid(static_cast<unsigned>((a.tokens + ROWS - 1) / ROWS)), block(WAVES < 4 ? 256 : WAVES * 64);
+    // As many workgroups as the chip holds at 32 waves a CU, an equal number of rows each.
+    const int64_t blocks = (a.tokens + ROWS - 1) / ROWS, most = 256 * (WAVES < 4 ? 8 : 32 / WAVES);
+    const int64_t turns = (blocks + most - 1) / most;
+    const dim3 grid(static_cast<unsigned>((blocks + turns - 1) / turns)), block(WAVES < 4 ? 256 : WAVES * 64);
     if (!norm)
         rms_norm_kernel<DT, NV, WAVES, true, false><<<grid, block, 0, stream>>>(a);
     else if (a.scales != nullptr)
@@ -170,11 +203,13 @@ template <int DT>
 void norm_by_width(const NormArgs& a, bool norm, hipStream_t stream) {
     constexpr int lane = kVec<DT>;
     const int vectors = (a.hidden + lane - 1) / lane;  // of the row
+    // A vector a lane where 16 waves allow it: 8 waves of one against 4 of two at 8192 x 4096 bf16 in 8
+    // bits 41 against 42 us, one row 3.1 against 3.5; a wave for the whole row 94 and 9.2.
     if (vectors <= 64) return run_norm<DT, 1, 1>(a, norm, stream);
     if (vectors <= 128) return run_norm<DT, 2, 1>(a, norm, stream);
     if (vectors <= 256) return run_norm<DT, 1, 4>(a, norm, stream);
-    if (vectors <= 512) return run_norm<DT, 2, 4>(a, norm, stream);
-    if (vectors <= 1024) return run_norm<DT, 4, 4>(a, norm, stream);
+    if (vectors <= 512) return run_norm<DT, 1, 8>(a, norm, stream);
+    if (vectors <= 1024) return run_norm<DT, 1, 16>(a, norm, stream);
     if (DT != MOE_DTYPE_F32 || vectors <= 2048) return run_norm<DT, 2, 16>(a, norm, stream);
     run_norm<DT, DT == MOE_DTYPE_F32 ? 4 : 2, 16>(a, norm, stream);
 }
@@ -204,35 +239,69 @@ int launch_quantize_rows(const NormArgs& a, hipStream_t stream) {
 
 namespace {
 
-constexpr int kGradBlocks = 512;  // partial weight gradients
 
+// WAVES waves a row, NV vectors a lane. A workgroup walks rows and keeps its share of the weight's gradient in
+// registers; where a lane has one vector, the weight stays there too and the next row's loads are in flight
+// (with two, the registers of 16 waves do not hold that).
 template <int DT, int NV, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void rms_norm_grad_kernel(NormGradArgs a) {
     using T = typename Elem<DT>::T;
     constexpr int N = kVec<DT>;
+    using V = typename Bytes<N * sizeof(T)>::V;
     __shared__ float lds[2][WAVES];
     const int thread = threadIdx.x, n = a.hidden;
-    const bool same = a.weight_dtype == DT;
-    float dw[NV][N];
+    const bool has_base = a.grad_x_base != nullptr && a.grad_x != nullptr;
+    constexpr bool AHEAD = NV == 1;
+    float dw[NV][N], kept[AHEAD ? NV : 1][N];
+    V xv[NV], gv[NV], bv[AHEAD ? NV : 1];
+    float rstd = 0.0f;
+    auto fetch = [&](int64_t row) {
+        rstd = a.rstd[row];
 #pragma unroll
-    for (int v = 0; v < NV; ++v)
+        for (int v = 0; v < NV; ++v) {
+            const int at = (v * WAVES * 64 + thread) * N;
+            if (at < n) {
+                xv[v] = load_vector<T, N>(static_cast<const T*>(a.x) + row * n, at, n);
+                gv[v] = load_vector<T, N>(static_cast<const T*>(a.grad_output) + row * n, at, n);
+                if constexpr (AHEAD) {
+                    if (has_base) bv[v] = load_vector<T, N>(static_cast<const T*>(a.grad_x_base) + row * n, at, n);
+                }
+            }
+        }
+    };
+    int64_t row = blockIdx.x;
+    if constexpr (AHEAD) fetch(row);
+    const bool same = a.weight_dtype == DT;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+        const int at = (v * WAVES * 64 + thread) * N;
+        if constexpr (AHEAD) {
+            if (at < n) load_weights<DT, N>(a.weight, same, at, n, kept[v]);
+        }
 #pragma unroll
         for (int i = 0; i < N; ++i) dw[v][i] = 0.0f;
-    int half = 0;
-    for (int64_t row = blockIdx.x; row < a.tokens; row += gridDim.x, half ^= 1) {
-        const T* x = static_cast<const T*>(a.x) + row * n;
-        const T* g = static_cast<const T*>(a.grad_output) + row * n;
-        const float rstd = a.rstd[row];
-        float u[NV][N], gw[NV][N];
+    }
+    for (int turn = 0; row < a.tokens; turn ^= 1) {
+        if constexpr (!AHEAD) fetch(row);
+        float u[NV][N], gw[NV][N], d[AHEAD ? NV : 1][N];
         float dot = 0.0f;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
             const int at = (v * WAVES * 64 + thread) * N;
             if (at < n) {
-                load_row<DT, N>(x, at, n, u[v]);
-                load_row<DT, N>(g, at, n, gw[v]);
                 float w[N];
-                load_weights<DT, N>(a.weight, same, at, n, w);
+                if constexpr (AHEAD) {
+#pragma unroll
+                    for (int i = 0; i < N; ++i) {
+                        w[i] = kept[v][i];
+                        d[v][i] = 0.0f;
+                    }
+                    if (has_base) unpack<DT>(bv[v], d[v]);
+                } else {
+                    load_weights<DT, N>(a.weight, same, at, n, w);
+                }
+                unpack<DT>(xv[v], u[v]);
+                unpack<DT>(gv[v], gw[v]);
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     u[v][i] *= rstd;
@@ -242,23 +311,29 @@ __global__ __launch_bounds__(WAVES * 64) void rms_norm_grad_kernel(NormGradArgs 
                 }
             }
         }
+        const int64_t this_row = row;
+        const float this_rstd = rstd;
+        row += gridDim.x;
+        if (AHEAD && row < a.tokens) fetch(row);
         if (a.grad_x != nullptr) {
-            const float c = row_reduce<SumOp, WAVES>(dot, lds[half]) / static_cast<float>(n);
-            const T* base = static_cast<const T*>(a.grad_x_base);
+            const float c = row_reduce<SumOp, WAVES>(dot, lds[turn]) / static_cast<float>(n);
 #pragma unroll
             for (int v = 0; v < NV; ++v) {
                 const int at = (v * WAVES * 64 + thread) * N;
                 if (at >= n) continue;
-                float d[N];
-                if (base != nullptr) {
-                    load_row<DT, N>(base + row * n, at, n, d);
+                float out[N];
+                if constexpr (AHEAD) {
+#pragma unroll
+                    for (int i = 0; i < N; ++i) out[i] = d[v][i];
                 } else {
 #pragma unroll
-                    for (int i = 0; i < N; ++i) d[i] = 0.0f;
+                    for (int i = 0; i < N; ++i) out[i] = 0.0f;
+                    if (has_base)
+                        load_row<DT, N>(static_cast<const T*>(a.grad_x_base) + this_row * n, at, n, out);
                 }
 #pragma unroll
-                for (int i = 0; i < N; ++i) d[i] += rstd * (gw[v][i] - u[v][i] * c);
-                store_row<DT, N>(static_cast<T*>(a.grad_x) + row * n, at, n, d);
+                for (int i = 0; i < N; ++i) out[i] += this_rstd * (gw[v][i] - u[v][i] * c);
+                store_row<DT, N>(static_cast<T*>(a.grad_x) + this_row * n, at, n, out);
             }
         }
     }
@@ -272,47 +347,79 @@ __global__ __launch_bounds__(WAVES * 64) void rms_norm_grad_kernel(NormGradArgs 
     }
 }
 
-// grad_weight[j] = sum of the partial rows, in order: 32 columns by 8 slices a workgroup.
-__global__ __launch_bounds__(256) void column_sum_kernel(const float* __restrict__ part, float* __restrict__ out, int rows,
-                                                         int n) {
-    __shared__ float lds[8][33];
+// grad_weight[j] = sum of the partial rows, in a fixed order: 32 columns by 32 slices a workgroup, a
+// slice's rows in flight together.
+__global__ __launch_bounds__(1024) void column_sum_kernel(const float* __restrict__ part, float* __restrict__ out, int rows,
+                                                          int n) {
+    constexpr int SLICES = 32, UNROLL = 8;
+    __shared__ float lds[SLICES][33];
     const int col = threadIdx.x & 31, slice = threadIdx.x >> 5;
     const int j = blockIdx.x * 32 + col;
     float sum = 0.0f;
-    if (j < n)
-        for (int r = slice; r < rows; r += 8) sum += part[static_cast<int64_t>(r) * n + j];
+    if (j < n) {
+        for (int r0 = slice; r0 < rows; r0 += SLICES * UNROLL) {
+            float v[UNROLL];
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u) {
+                const int r = r0 + u * SLICES;
+                v[u] = r < rows ? part[static_cast<int64_t>(r) * n + j] : 0.0f;
+            }
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u) sum += v[u];
+        }
+    }
     lds[slice][col] = sum;
     __syncthreads();
     if (slice == 0 && j < n) {
-#pragma unroll
-        for (int s = 1; s < 8; ++s) sum += lds[s][col];
+        for (int s = 1; s < SLICES; ++s) sum += lds[s][col];
         out[j] = sum;
     }
 }
 
-int grad_blocks(int64_t tokens) { return static_cast<int>(tokens < kGradBlocks ? tokens : kGradBlocks); }
+// Waves a row of the gradient kernel.
+int grad_waves(int vectors) {
+    if (vectors <= 64) return 1;
+    if (vectors <= 128) return 2;
+    if (vectors <= 256) return 4;
+    return vectors <= 512 ? 8 : 16;
+}
+
+// Workgroups, each of which leaves a partial weight gradient: eight rows each, fewer where that leaves CUs
+// idle (512 x 4096: 256 workgroups 10.0 us, 64 12.1), and not so many that the partial rows cost what they
+// save (4096 x 2048: 512 17.3 us, 1024 19.4; 2048 x 8192: 256 27, 512 30).
+int grad_blocks(int64_t tokens, int64_t hidden, int dtype) {
+    const int lane = dtype == MOE_DTYPE_F32 ? 4 : 8;
+    const int waves = grad_waves(static_cast<int>((hidden + lane - 1) / lane));
+    const int64_t most = waves <= 2 ? 2048 / waves : waves <= 8 ? 512 : 256;
+    const int64_t blocks = std::max<int64_t>(tokens / 8, std::min<int64_t>(tokens, 256));
+    return static_cast<int>(std::min(blocks, most));
+}
 
 template <int DT, int NV, int WAVES>
 void run_grad(const NormGradArgs& a, hipStream_t stream) {
-    rms_norm_grad_kernel<DT, NV, WAVES><<<grad_blocks(a.tokens), WAVES * 64, 0, stream>>>(a);
+    rms_norm_grad_kernel<DT, NV, WAVES><<<grad_blocks(a.tokens, a.hidden, a.dtype), WAVES * 64, 0, stream>>>(a);
 }
 
 template <int DT>
 void grad_by_width(const NormGradArgs& a, hipStream_t stream) {
     constexpr int lane = kVec<DT>;
     const int vectors = (a.hidden + lane - 1) / lane;
-    if (vectors <= 64) return run_grad<DT, 1, 1>(a, stream);
-    if (vectors <= 256) return run_grad<DT, 1, 4>(a, stream);
-    if (vectors <= 512) return run_grad<DT, 2, 4>(a, stream);
-    if (vectors <= 1024) return run_grad<DT, 2, 8>(a, stream);
+    switch (grad_waves(vectors)) {
+        case 1: return run_grad<DT, 1, 1>(a, stream);
+        case 2: return run_grad<DT, 1, 2>(a, stream);
+        case 4: return run_grad<DT, 1, 4>(a, stream);
+        case 8: return run_grad<DT, 1, 8>(a, stream);
+        default: break;
+    }
+    if (vectors <= 1024) return run_grad<DT, 1, 16>(a, stream);
     if (DT != MOE_DTYPE_F32 || vectors <= 2048) return run_grad<DT, 2, 16>(a, stream);
     run_grad<DT, DT == MOE_DTYPE_F32 ? 4 : 2, 16>(a, stream);
 }
 
 }  // namespace
 
-int64_t rms_norm_backward_scratch_bytes(int64_t tokens, int64_t hidden) {
-    return static_cast<int64_t>(grad_blocks(tokens)) * hidden * 4;
+int64_t rms_norm_backward_scratch_bytes(int64_t tokens, int64_t hidden, int dtype) {
+    return static_cast<int64_t>(grad_blocks(tokens, hidden, dtype)) * hidden * 4;
 }
 
 int launch_rms_norm_backward(const NormGradArgs& a, hipStream_t stream) {
@@ -323,8 +430,8 @@ int launch_rms_norm_backward(const NormGradArgs& a, hipStream_t stream) {
     else
         grad_by_width<MOE_DTYPE_BF16>(a, stream);
     if (a.grad_weight != nullptr)
-        column_sum_kernel<<<(a.hidden + 31) / 32, 256, 0, stream>>>(a.scratch, a.grad_weight, grad_blocks(a.tokens),
-                                                                    a.hidden);
+        column_sum_kernel<<<(a.hidden + 31) / 32, 1024, 0, stream>>>(
+            a.scratch, a.grad_weight, grad_blocks(a.tokens, a.hidden, a.dtype), a.hidden);
     return check_launch("rms_norm_backward");
 }
 

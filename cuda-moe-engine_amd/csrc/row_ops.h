@@ -2,6 +2,8 @@
 // (norm.hip, scored_route.hip, clip.hip) and their entry points (abi_layer.hip).
 #pragma once
 
+#include <type_traits>
+
 #include "moe_common.h"
 
 namespace moe {
@@ -32,6 +34,29 @@ struct MaxOp {
     static __device__ __forceinline__ float of(float a, float b) { return fmaxf(a, b); }
 };
 
+// The largest of aligned groups of WIDTH lanes, for unsigned integers (which, unlike floats, need no
+// quieting of each operand: one instruction a step).
+template <int WIDTH>
+__device__ __forceinline__ uint32_t lanes_max(uint32_t x) {
+    auto step = [&](auto ctrl) {
+        const uint32_t other = __builtin_amdgcn_update_dpp(0, static_cast<int>(x), decltype(ctrl)::value, 0xf, 0xf, true);
+        x = other > x ? other : x;
+    };
+    if constexpr (WIDTH >= 2) step(std::integral_constant<int, kDppXor1>{});
+    if constexpr (WIDTH >= 4) step(std::integral_constant<int, kDppXor2>{});
+    if constexpr (WIDTH >= 8) step(std::integral_constant<int, kDppHalfMirror>{});
+    if constexpr (WIDTH >= 16) step(std::integral_constant<int, kDppMirror>{});
+    if constexpr (WIDTH >= 32) {
+        const auto s = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+        x = s[0] > s[1] ? s[0] : s[1];
+    }
+    if constexpr (WIDTH >= 64) {
+        const auto s = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+        x = s[0] > s[1] ? s[0] : s[1];
+    }
+    return x;
+}
+
 // OP over aligned groups of WIDTH lanes (a power of two up to 64), the result in each lane.
 template <typename OP, int WIDTH = kWave>
 __device__ __forceinline__ float lanes_reduce(float x) {
@@ -50,34 +75,98 @@ __device__ __forceinline__ float lanes_reduce(float x) {
     return x;
 }
 
-// Elements [at, at + N) of a row of n, as fp32, 0 past its end. One vector access unless the
-// row ends inside it.
-template <int DT, int N>
-__device__ __forceinline__ void load_row(const typename Elem<DT>::T* row, int at, int n, float (&out)[N]) {
+// 16, 8 or 4 bytes at any address, as one instruction: a copy through a struct of elements is
+// split into narrow loads where its elements are converted one by one (the norm of 8192 x 4096 in 8 bits took
+// 68 us with such copies, 41 without).
+template <int BYTES> struct Bytes;
+template <> struct Bytes<16> {
+    typedef uint32_t V __attribute__((ext_vector_type(4)));
+    typedef uint32_t At __attribute__((ext_vector_type(4), aligned(1)));
+};
+template <> struct Bytes<8> {
+    typedef uint32_t V __attribute__((ext_vector_type(2)));
+    typedef uint32_t At __attribute__((ext_vector_type(2), aligned(1)));
+};
+template <> struct Bytes<4> {
+    typedef uint32_t V;
+    typedef uint32_t At __attribute__((aligned(1)));
+};
+
+template <int BYTES>
+__device__ __forceinline__ typename Bytes<BYTES>::V load_bytes(const void* p) {
+    return *static_cast<const typename Bytes<BYTES>::At*>(p);
+}
+
+template <int BYTES>
+__device__ __forceinline__ void store_bytes(void* p, typename Bytes<BYTES>::V v) {
+    *static_cast<typename Bytes<BYTES>::At*>(p) = v;
+}
+
+// Elements [at, at + N) of a row of n as they lie, 0 past its end. One access unless the row ends
+// inside it.
+template <typename T, int N>
+__device__ __forceinline__ typename Bytes<N * sizeof(T)>::V load_vector(const T* row, int at, int n) {
+    if (at + N <= n) return load_bytes<N * sizeof(T)>(row + at);
+    T v[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = at + i < n ? row[at + i] : T(0);
+    return __builtin_bit_cast(typename Bytes<N * sizeof(T)>::V, v);
+}
+
+// The N elements of such a vector as fp32, and back.
+template <int DT, int N, typename V>
+__device__ __forceinline__ void unpack(V v, float (&out)[N]) {
     using T = typename Elem<DT>::T;
-    Unaligned<T, N> v;
-    if (at + N <= n) {
-        v = *reinterpret_cast<const Unaligned<T, N>*>(row + at);
-    } else {
+    static_assert(sizeof(V) == N * sizeof(T), "vector");
+    T e[N];
+    __builtin_memcpy(e, &v, sizeof(V));
 #pragma unroll
-        for (int i = 0; i < N; ++i) v.v[i] = at + i < n ? row[at + i] : T(0);
-    }
-#pragma unroll
-    for (int i = 0; i < N; ++i) out[i] = Elem<DT>::load(v.v[i]);
+    for (int i = 0; i < N; ++i) out[i] = Elem<DT>::load(e[i]);
 }
 
 template <int DT, int N>
-__device__ __forceinline__ void store_row(typename Elem<DT>::T* row, int at, int n, const float (&in)[N]) {
+__device__ __forceinline__ auto pack(const float (&in)[N]) {
     using T = typename Elem<DT>::T;
-    Unaligned<T, N> v;
+    T e[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) v.v[i] = Elem<DT>::store(in[i]);
-    if (at + N <= n) {
-        *reinterpret_cast<Unaligned<T, N>*>(row + at) = v;
-    } else {
+    for (int i = 0; i < N; ++i) e[i] = Elem<DT>::store(in[i]);
+    return __builtin_bit_cast(typename Bytes<N * sizeof(T)>::V, e);
+}
+
+// As fp32, in accesses of up to 16 bytes.
+template <int DT, int N>
+__device__ __forceinline__ void load_row(const typename Elem<DT>::T* row, int at, int n, float (&out)[N]) {
+    using T = typename Elem<DT>::T;
+    constexpr int STEP = N * sizeof(T) > 16 ? 16 / sizeof(T) : N;
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (at + i < n) row[at + i] = v.v[i];
+    for (int i = 0; i < N; i += STEP) {
+        float part[STEP];
+        unpack<DT>(load_vector<T, STEP>(row, at + i, n), part);
+#pragma unroll
+        for (int j = 0; j < STEP; ++j) out[i + j] = part[j];
+    }
+}
+
+template <int DT, int N>
+__device__ __forceinline__ void store_row(typename Elem<DT>::T* row, int at, int n, const float (&in)[N],
+                                          bool stream = false) {
+    using T = typename Elem<DT>::T;
+    constexpr int STEP = N * sizeof(T) > 16 ? 16 / sizeof(T) : N;
+#pragma unroll
+    for (int i = 0; i < N; i += STEP) {
+        float part[STEP];
+#pragma unroll
+        for (int j = 0; j < STEP; ++j) part[j] = in[i + j];
+        const auto v = pack<DT>(part);
+        if (at + i + STEP <= n) {
+            store_bytes<STEP * sizeof(T)>(row + at + i, v);
+        } else {
+            T e[STEP];
+            __builtin_memcpy(e, &v, sizeof(v));
+#pragma unroll
+            for (int j = 0; j < STEP; ++j)
+                if (at + i + j < n) row[at + i + j] = e[j];
+        }
     }
 }
 
@@ -143,7 +232,7 @@ struct ScoreGradArgs {
 
 int launch_rms_norm(const NormArgs& a, hipStream_t stream);
 int launch_quantize_rows(const NormArgs& a, hipStream_t stream);
-int64_t rms_norm_backward_scratch_bytes(int64_t tokens, int64_t hidden);
+int64_t rms_norm_backward_scratch_bytes(int64_t tokens, int64_t hidden, int dtype);
 int launch_rms_norm_backward(const NormGradArgs& a, hipStream_t stream);
 int launch_route_scored(const ScoreArgs& a, hipStream_t stream);
 int launch_route_scored_backward(const ScoreGradArgs& a, hipStream_t stream);

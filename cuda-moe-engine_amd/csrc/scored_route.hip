@@ -7,47 +7,28 @@
 //   w = scale s_j / sum_chosen s  or  scale s_j.
 //
 // A token is a segment of LANES lanes of a wave, V experts a lane, every group in lanes of
-// its own. The choice is by exact value: scores are fp32 first, and a token whose order
-// hangs on a difference within their rounding is decided again with fp64 scores by its
-// wave, so that the ids are the definition's and do not depend on how exp rounds.
+// its own. A lane sorts its keys once; each choice is then a maximum over the segment of the lanes' first
+// keys, which the owner removes. The choice is by exact value: keys are fp32 first, and a token whose
+// order hangs on a difference within their rounding (or on a tie, or that has no K experts left) is decided
+// again by its wave in 64 bits, so that the ids are the definition's and do not depend on how exp rounds.
+// About one token in a thousand at 256 experts. Bound by instructions, not bytes: see the figures at the
+// launcher.
 #include "row_ops.h"
 
 namespace moe {
 
 namespace {
 
-template <int CTRL>
-__device__ __forceinline__ double dpp_move(double x) {
-    const uint64_t u = __double_as_longlong(x);
-    const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(u), CTRL, 0xf, 0xf, true);
-    const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(u >> 32), CTRL, 0xf, 0xf, true);
-    return __longlong_as_double(static_cast<uint64_t>(hi) << 32 | lo);
-}
-
-__device__ __forceinline__ float lane_xor(float x, int mask) { return __shfl_xor(x, mask); }
 __device__ __forceinline__ double lane_xor(double x, int mask) { return __shfl_xor(x, mask); }
-
-__device__ __forceinline__ float most(float a, float b) { return fmaxf(a, b); }
 __device__ __forceinline__ double most(double a, double b) { return fmax(a, b); }
 
 // The largest over aligned segments of `lanes` lanes, in each lane.
-template <int LANES>
-__device__ __forceinline__ float segment_max(float x) {
-    return lanes_reduce<MaxOp, LANES>(x);
-}
 template <int LANES>
 __device__ __forceinline__ double segment_max(double x) {
 #pragma unroll
     for (int d = 1; d < LANES; d <<= 1) x = most(x, lane_xor(x, d));
     return x;
 }
-
-__device__ __forceinline__ float exp_of(float x) { return expf(x); }
-__device__ __forceinline__ double exp_of(double x) { return exp(x); }
-
-template <typename F> __device__ __forceinline__ F minus_inf();
-template <> __device__ __forceinline__ float minus_inf<float>() { return -__builtin_inff(); }
-template <> __device__ __forceinline__ double minus_inf<double>() { return -__builtin_inf(); }
 
 // Where a lane's V experts lie.
 struct Place {
@@ -57,28 +38,26 @@ struct Place {
     int group_lanes;
 };
 
-// Chooses the token's experts by keys of type F: rank[i] = the slot of the lane's expert i
-// or -1. Returns whether the order hangs on a difference of at most `doubt` times the
-// largest key (fp32's rounding; 0 in fp64).
-template <typename F, int LANES, int V>
-__device__ __forceinline__ bool choose(const ScoreArgs& a, const Place& p, const float (&l)[V], const float (&b)[V],
-                                       F doubt, int (&rank)[V]) {
+// Chooses the token's experts in 64 bits, ties to the lower index: rank[i] = the slot
+// of the lane's expert i or -1.
+template <int LANES, int V>
+__device__ __forceinline__ void choose(const ScoreArgs& a, const Place& p, const float (&l)[V], const float (&b)[V],
+                                       int (&rank)[V]) {
     const bool has_bias = a.bias != nullptr;
-    F key[V], score[V];
-    F largest = 0;
+    double key[V], score[V];
     if (has_bias || a.groups > 1) {
         if (a.sigmoid) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) score[i] = F(1) / (F(1) + exp_of(-static_cast<F>(l[i])));
+            for (int i = 0; i < V; ++i) score[i] = 1.0 / (1.0 + exp(-static_cast<double>(l[i])));
         } else {
-            F top = minus_inf<F>();
+            double top = -__builtin_inf();
 #pragma unroll
-            for (int i = 0; i < V; ++i) top = most(top, static_cast<F>(l[i]));
+            for (int i = 0; i < V; ++i) top = most(top, static_cast<double>(l[i]));
             top = segment_max<LANES>(top);
-            F total = 0;
+            double total = 0;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                score[i] = l[i] == -__builtin_inff() ? F(0) : exp_of(static_cast<F>(l[i]) - top);
+                score[i] = l[i] == -__builtin_inff() ? 0.0 : exp(static_cast<double>(l[i]) - top);
                 total += score[i];
             }
 #pragma unroll
@@ -88,23 +67,18 @@ __device__ __forceinline__ bool choose(const ScoreArgs& a, const Place& p, const
         }
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            score[i] += static_cast<F>(b[i]);
+            score[i] += static_cast<double>(b[i]);
             // An expert that is out (a logit of -inf, or no number) has no key.
-            if (!(l[i] > -__builtin_inff()) || !(score[i] == score[i])) score[i] = minus_inf<F>();
-            if (score[i] > minus_inf<F>()) largest = most(largest, most(most(score[i], -score[i]), most(static_cast<F>(b[i]), static_cast<F>(-b[i]))));
+            if (!(l[i] > -__builtin_inff()) || !(score[i] == score[i])) score[i] = -__builtin_inf();
         }
-        largest = segment_max<LANES>(largest);
     }
 #pragma unroll
     for (int i = 0; i < V; ++i)
-        key[i] = has_bias ? score[i] : (l[i] > -__builtin_inff() ? static_cast<F>(l[i]) : minus_inf<F>());
-    // Keys of a bias are rounded; logits are what they are.
-    const F near = doubt * largest;
-    bool unsure = false;
+        key[i] = has_bias ? score[i] : (l[i] > -__builtin_inff() ? static_cast<double>(l[i]) : -__builtin_inf());
     bool open = true;
     if (a.groups > 1) {
         // The lane's best two, then the group's.
-        F first = minus_inf<F>(), second = minus_inf<F>();
+        double first = -__builtin_inf(), second = -__builtin_inf();
 #pragma unroll
         for (int i = 0; i < V; ++i)
             if (i < p.count) {
@@ -112,69 +86,252 @@ __device__ __forceinline__ bool choose(const ScoreArgs& a, const Place& p, const
                 first = most(first, score[i]);
             }
         for (int d = 1; d < p.group_lanes; d <<= 1) {
-            const F f = lane_xor(first, d), s = lane_xor(second, d);
+            const double f = lane_xor(first, d), s = lane_xor(second, d);
             second = most(most(second, s), f < first ? f : first);
             first = most(first, f);
         }
-        F group = first;
-        if (a.group_best == 2 && second > minus_inf<F>()) group += second;
+        double group = first;
+        if (a.group_best == 2 && second > -__builtin_inf()) group += second;
         // Its place among the groups, ties to the lower one; lanes without a group are last.
         const int mine = p.lane / p.group_lanes;
         const bool real = mine < a.groups;
         int before = 0;
         for (int o = 1; o < LANES / p.group_lanes; ++o) {
-            const F other = lane_xor(group, o * p.group_lanes);
+            const double other = lane_xor(group, o * p.group_lanes);
             const int index = mine ^ o;
             if (index < a.groups && (other > group || (other == group && index < mine))) ++before;
-            const F gap = other > group ? other - group : group - other;
-            unsure |= real && index < a.groups && gap <= 4 * near;
         }
         open = real && before < a.top_groups;
     }
-    // Chosen experts hold no key any more; those that have none in an open group are
-    // chosen last, in order, with the key below every other.
+    // Keys as unsigned integers of the same order. Chosen experts and those of other groups hold 0, as do those
+    // that are out, which are chosen last, in order.
+    uint64_t order[V];
     uint32_t left = 0;  // experts of the lane that can be chosen
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         rank[i] = -1;
-        if (open && i < p.count) left |= 1u << i;
-        if (!open || i >= p.count) key[i] = minus_inf<F>();
+        const bool can = open && i < p.count;
+        if (can) left |= 1u << i;
+        const uint64_t u = __double_as_longlong(key[i] + 0.0);  // -0 is 0
+        order[i] = can && key[i] > -__builtin_inf() ? u ^ (static_cast<uint64_t>(static_cast<int64_t>(u) >> 63) | (1ull << 63)) : 0;
     }
     const uint32_t lane = threadIdx.x & 63;
     const uint64_t segment = (LANES == 64 ? ~0ull : ((1ull << (LANES & 63)) - 1)) << (lane / LANES * LANES);
-    F previous = 0;
-    for (int k = 0; k <= a.topk; ++k) {
-        F best = minus_inf<F>();
+    for (int k = 0; k < a.topk; ++k) {
+        uint64_t best = 0;
 #pragma unroll
-        for (int i = 0; i < V; ++i) best = most(best, key[i]);
-        const F top = segment_max<LANES>(best);
-        // The order of neighbours, the first one left out among them.
-        if (has_bias && k > 0) unsure |= previous > minus_inf<F>() && top > minus_inf<F>() && previous - top <= 2 * near;
-        previous = top;
-        if (k == a.topk) break;
+        for (int i = 0; i < V; ++i) best = order[i] > best ? order[i] : best;
+        const uint32_t high = static_cast<uint32_t>(best >> 32);
+        const uint32_t top_high = lanes_max<LANES>(high);
+        const uint32_t top_low = lanes_max<LANES>(high == top_high ? static_cast<uint32_t>(best) : 0u);
+        const uint64_t top = static_cast<uint64_t>(top_high) << 32 | top_low;
         const uint64_t with = __ballot(left != 0 && best == top) & segment;
-        const bool owner = __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(with >> 32),
-                                                     __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(with), 0)) == 0 &&
-                           (with >> lane & 1);
-        if (owner) {
+        if (with >> lane & 1 && (with & ((1ull << lane) - 1)) == 0) {
             bool done = false;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const bool take = !done && (left >> i & 1) && key[i] == top;
+                const bool take = !done && (left >> i & 1) && order[i] == top;
                 rank[i] = take ? k : rank[i];
-                key[i] = take ? minus_inf<F>() : key[i];
+                order[i] = take ? 0 : order[i];
                 left &= take ? ~(1u << i) : ~0u;
                 done |= take;
             }
         }
     }
-    return unsure;
+}
+
+// `count` values from row[first] on, the rest `without`: 16 bytes a load, at any alignment, where there are four.
+template <int V>
+__device__ __forceinline__ void load_some(const float* row, int first, int count, float without, float (&out)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; i += 4) {
+        if (i + 4 <= count) {
+            float four[4];
+            unpack<MOE_DTYPE_F32>(load_bytes<16>(row + first + i), four);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) out[i + j] = four[j];
+        } else {
+#pragma unroll
+            for (int j = i; j < i + 4; ++j) out[j] = j < count ? row[first + j] : without;
+        }
+    }
+}
+
+// e^x and 1 / (1 + e^-x) by hardware exp2 and reciprocal. For scores that only order: within 2^-24 |x| for the
+// argument and 2^-23 for each of the two.
+__device__ __forceinline__ float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
+
+// A token's lanes are one wave, whose LDS accesses are in order: only the compiler has to keep it.
+__device__ __forceinline__ void wave_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
+
+// The lane's best two of a group, then the group's, over group_lanes lanes (a power of two).
+template <int LANES>
+__device__ __forceinline__ void best_two(float& first, float& second, int group_lanes) {
+    auto merge = [&](float f, float s) {
+        second = fmaxf(fmaxf(second, s), fminf(first, f));
+        first = fmaxf(first, f);
+    };
+    if (LANES >= 2 && group_lanes >= 2) merge(dpp_move<kDppXor1>(first), dpp_move<kDppXor1>(second));
+    if (LANES >= 4 && group_lanes >= 4) merge(dpp_move<kDppXor2>(first), dpp_move<kDppXor2>(second));
+    if (LANES >= 8 && group_lanes >= 8) merge(dpp_move<kDppHalfMirror>(first), dpp_move<kDppHalfMirror>(second));
+    if (LANES >= 16 && group_lanes >= 16) merge(dpp_move<kDppMirror>(first), dpp_move<kDppMirror>(second));
+    if (LANES >= 32 && group_lanes >= 32) merge(__shfl_xor(first, 16), __shfl_xor(second, 16));
+}
+
+// A float's bits as an unsigned integer of the same order; 0 stands for no key.
+__device__ __forceinline__ uint32_t ordered(float x) {
+    const uint32_t u = __float_as_uint(x);
+    return u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float unordered(uint32_t k) {
+    return __uint_as_float(k ^ (k >> 31 ? 0x80000000u : 0xffffffffu));
+}
+
+// Orders the lane's keys, largest first, with their places (an odd-even merge network).
+template <int V>
+__device__ __forceinline__ void sort_keys(uint32_t (&key)[V], int (&place)[V]) {
+#pragma unroll
+    for (int p = 1; p < V; p *= 2)
+#pragma unroll
+        for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+            for (int j = k % p; j + k < V; j += 2 * k)
+#pragma unroll
+                for (int i = 0; i < k; ++i)
+                    if (i + j + k < V && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+                        const int x = i + j, y = i + j + k;
+                        const uint32_t kx = key[x], ky = key[y];
+                        const int px = place[x], py = place[y];
+                        const bool swap = ky > kx;
+                        key[x] = swap ? ky : kx;
+                        key[y] = swap ? kx : ky;
+                        place[x] = swap ? py : px;
+                        place[y] = swap ? px : py;
+                    }
+}
+
+// Chooses by fp32 keys into picked[0..topk); true where fp32 does not decide it. `scores`: the token's
+// room for a score a group.
+template <int LANES, int V>
+__device__ __forceinline__ bool choose_fast(const ScoreArgs& a, const Place& p, const float (&l)[V], const float (&b)[V],
+                                            int* picked, float* scores) {
+    const bool has_bias = a.bias != nullptr;
+    const float minus = -__builtin_inff();
+    bool unsure = false;
+    uint32_t key[V];
+    float near = 0.0f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) key[i] = l[i] > minus ? ordered(l[i]) : 0u;
+    if (has_bias || a.groups > 1) {
+        float s[V];
+        // A score's roundings: sigmoid 6 of 2^-24 (argument, exp, sum, reciprocal), softmax up to V + 16 (its sum
+        // besides), one more for the bias, of the largest key or bias.
+        float error = 0x1p-21f;
+        if (a.sigmoid) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) s[i] = __builtin_amdgcn_rcpf(1.0f + fast_exp(-l[i]));
+        } else {
+            error = (V + 20) * 0x1p-24f;
+            float top = l[0];
+#pragma unroll
+            for (int i = 1; i < V; ++i) top = fmaxf(top, l[i]);
+            top = lanes_reduce<MaxOp, LANES>(top);
+            float total = 0.0f;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                s[i] = fast_exp(l[i] - top);
+                total += s[i];
+            }
+            const float inverse = __builtin_amdgcn_rcpf(lanes_reduce<SumOp, LANES>(total));
+#pragma unroll
+            for (int i = 0; i < V; ++i) s[i] *= inverse;
+        }
+        // Magnitudes as integers: of numbers they order alike, and a NaN's or infinity's are the largest.
+        uint32_t largest = 0;
+        float first = minus, second = minus;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const bool in = l[i] > minus;
+            const float k = in ? s[i] + b[i] : minus;
+            const uint32_t size = max(__float_as_uint(k) & 0x7fffffffu, __float_as_uint(b[i]) & 0x7fffffffu);
+            largest = max(largest, in ? size : 0u);
+            second = fmaxf(second, fminf(first, k));
+            first = fmaxf(first, k);
+            if (has_bias) key[i] = in ? ordered(k) : 0u;
+        }
+        largest = lanes_max<LANES>(largest);
+        near = 2.0f * error * __uint_as_float(largest);
+        // A key that is no number or infinite: the other path sorts that out.
+        unsure = largest >= 0x7f800000u;
+        if (a.groups > 1) {
+            best_two<LANES>(first, second, p.group_lanes);
+            const float group = a.group_best == 2 && second > minus ? first + second : first;
+            const int mine = p.lane / p.group_lanes;
+            // Lanes past the last group bring -inf, which is before and close to none.
+            if (p.lane % p.group_lanes == 0) scores[mine] = group;
+            wave_fence();
+            int before = 0, close = 0;
+            const int places = LANES / p.group_lanes;  // a power of two
+            for (int g = 0; g < places; g += 4) {
+                float other[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) other[j] = j < 2 || places > 2 ? scores[g + j] : minus;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    before += other[j] > group;
+                    close += fabsf(other[j] - group) <= 2.0f * near;  // itself among them
+                }
+            }
+            const bool real = mine < a.groups;
+            unsure |= real && close > 1;
+            if (!real || before >= a.top_groups) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) key[i] = 0u;
+            }
+        }
+    }
+    int place[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) place[i] = p.first + i;
+    sort_keys<V>(key, place);
+    const uint32_t lane = threadIdx.x & 63;
+    const uint64_t segment = (LANES == 64 ? ~0ull : ((1ull << (LANES & 63)) - 1)) << (lane / LANES * LANES);
+    const uint64_t lower = segment & ((1ull << lane) - 1);
+    float previous = __builtin_inff();
+    for (int k = 0; k < a.topk; ++k) {
+        const uint32_t top = lanes_max<LANES>(key[0]);
+        const uint64_t with = __ballot(key[0] == top);
+        // The lowest lane that has it.
+        const bool owner = LANES == 64 ? static_cast<int>(lane) == __builtin_ctzll(with)
+                                       : key[0] == top && (with & lower) == 0;
+        if (owner) {
+            picked[k] = place[0];
+#pragma unroll
+            for (int i = 0; i + 1 < V; ++i) {
+                key[i] = key[i + 1];
+                place[i] = place[i + 1];
+            }
+            key[V - 1] = 0u;
+        }
+        // Neighbours in the order that are too near (equal ones included), no expert left, or no numbers.
+        const float value = unordered(top);
+        unsure |= !(previous - value > near) || top == 0u;
+        previous = value;
+    }
+    // The first one left out.
+    const uint32_t next = lanes_max<LANES>(key[0]);
+    return unsure || (next != 0u && !(previous - unordered(next) > near));
 }
 
 template <int LANES, int V>
 __global__ __launch_bounds__(256) void route_scored_kernel(ScoreArgs a) {
+    constexpr int TOKENS = 256 / LANES;
+    constexpr int GROUPS = LANES < 64 ? LANES : 64;  // a lane each at least
+    __shared__ int picked[TOKENS][kMaxTopk];
+    __shared__ float scores[TOKENS][GROUPS];
     const int lane = threadIdx.x & 63;
-    const int64_t token = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / LANES;
+    const int slot = threadIdx.x / LANES;  // the token's place in the workgroup: one wave's
+    const int64_t token = static_cast<int64_t>(blockIdx.x) * TOKENS + slot;
     Place p;
     p.lane = lane % LANES;
     const int size = a.experts / a.groups;
@@ -183,61 +340,83 @@ __global__ __launch_bounds__(256) void route_scored_kernel(ScoreArgs a) {
     const int group = p.lane / p.group_lanes, part = p.lane % p.group_lanes;
     p.first = group * size + part * V;
     p.count = group < a.groups ? max(0, min(V, size - part * V)) : 0;
-    if (token >= a.tokens) p.count = 0;  // these lanes take part in the reductions only
+    const bool live = token < a.tokens;
+    if (!live) p.count = 0;  // these lanes take part in the reductions only
     float l[V], b[V];
-    const float* row = a.logits + token * a.experts + p.first;
+    const float* row = a.logits + token * a.experts;
+    load_some<V>(row, p.first, p.count, -__builtin_inff(), l);
+    if (a.bias != nullptr) {
+        load_some<V>(a.bias, p.first, p.count, 0.0f, b);
+    } else {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        l[i] = i < p.count ? row[i] : -__builtin_inff();
-        b[i] = i < p.count && a.bias != nullptr ? a.bias[p.first + i] : 0.0f;
+        for (int i = 0; i < V; ++i) b[i] = 0.0f;
     }
-    int rank[V];
-    // A score is within 14 roundings of 2^-24 (exp's argument and value, a sum of at most 16
-    // and 6 levels, a division), its key 15 of the largest key or bias: 2^-20 of that.
-    const bool unsure = choose<float, LANES, V>(a, p, l, b, 0x1p-20f, rank);
-    if (__ballot(unsure && token < a.tokens) != 0) choose<double, LANES, V>(a, p, l, b, 0.0, rank);
-    if (token >= a.tokens) return;
-
-    // Weights. Renormalised ones from scores relative to the largest chosen logit, so that
-    // scores too small for fp32 keep their ratio: softmax e^(l - m); sigmoid
-    // e^(min(l, 0) - min(m, 0)) / (1 + e^-|l|).
     bool number = true;
-    float top = -__builtin_inff(), top_all = -__builtin_inff();
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        number &= l[i] == l[i];
-        top_all = fmaxf(top_all, l[i]);
-        if (rank[i] >= 0) top = fmaxf(top, l[i]);
-    }
+    for (int i = 0; i < V; ++i) number &= l[i] == l[i];
     const uint64_t segment = (LANES == 64 ? ~0ull : ((1ull << (LANES & 63)) - 1)) << (lane / LANES * LANES);
     number = (__ballot(!number) & segment) == 0;
-    const bool all = !a.sigmoid && !a.renormalize;
-    top = lanes_reduce<MaxOp, LANES>(all ? top_all : top);
-    float w[V];
-    float sum = 0.0f;
+    const bool unsure = choose_fast<LANES, V>(a, p, l, b, picked[slot], scores[slot]) || !number;
+    if (__ballot(unsure && live) != 0) {
+        int rank[V];
+        choose<LANES, V>(a, p, l, b, rank);
+        wave_fence();
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        float s = 0.0f;
-        if (l[i] > -__builtin_inff()) {
-            if (!a.sigmoid)
-                s = expf(l[i] - top);
-            else if (a.renormalize)
-                s = expf(fminf(l[i], 0.0f) - fminf(top, 0.0f)) / (1.0f + expf(-fabsf(l[i])));
-            else
-                s = 1.0f / (1.0f + expf(-l[i]));
-        }
-        w[i] = s;
-        if (all || rank[i] >= 0) sum += s;
+        for (int i = 0; i < V; ++i)
+            if (rank[i] >= 0) picked[slot][rank[i]] = p.first + i;
     }
-    sum = lanes_reduce<SumOp, LANES>(sum);
+    wave_fence();
+
+    // Weights: slot k on lane k, several a lane where the segment has fewer than eight. Renormalised ones from
+    // scores relative to the largest chosen logit, so that scores too small for fp32 keep their ratio:
+    // softmax e^(l - m); sigmoid e^(min(l, 0) - min(m, 0)) / (1 + e^-|l|).
+    constexpr int WIDTH = LANES < kMaxTopk ? LANES : kMaxTopk, SLOTS = kMaxTopk / WIDTH;
+    const float minus = -__builtin_inff();
+    const bool all = !a.sigmoid && !a.renormalize;
+    float top = minus, sum = 0.0f;
+    if (all) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) top = fmaxf(top, l[i]);
+        top = lanes_reduce<MaxOp, LANES>(top);
+#pragma unroll
+        for (int i = 0; i < V; ++i) sum += l[i] > minus ? fast_exp(l[i] - top) : 0.0f;
+        sum = lanes_reduce<SumOp, LANES>(sum);
+    }
+    int id[SLOTS];
+    float chosen[SLOTS], w[SLOTS];
+#pragma unroll
+    for (int j = 0; j < SLOTS; ++j) {
+        const int k = j * WIDTH + p.lane;
+        const bool mine = live && p.lane < WIDTH && k < a.topk;
+        id[j] = mine ? picked[slot][k] : -1;
+        chosen[j] = mine ? row[id[j]] : minus;
+        if (!all) top = fmaxf(top, chosen[j]);
+    }
+    if (!all) top = lanes_reduce<MaxOp, WIDTH>(top);
+#pragma unroll
+    for (int j = 0; j < SLOTS; ++j) {
+        const float x = chosen[j];
+        w[j] = 0.0f;
+        if (x > minus) {
+            if (!a.sigmoid)
+                w[j] = fast_exp(x - top);
+            else if (a.renormalize)
+                w[j] = fast_exp(fminf(x, 0.0f) - fminf(top, 0.0f)) * __builtin_amdgcn_rcpf(1.0f + fast_exp(-fabsf(x)));
+            else
+                w[j] = __builtin_amdgcn_rcpf(1.0f + fast_exp(-x));
+        }
+        if (!all) sum += w[j];
+    }
+    if (!all) sum = lanes_reduce<SumOp, WIDTH>(sum);
     // Nothing but experts that are out: weights 0.
     float divisor = a.renormalize || !a.sigmoid ? (sum == 0.0f ? 1.0f : sum) : 1.0f;
     if (!number) divisor = __builtin_nanf("");
 #pragma unroll
-    for (int i = 0; i < V; ++i)
-        if (rank[i] >= 0) {
-            a.ids[token * a.topk + rank[i]] = p.first + i;
-            a.weights[token * a.topk + rank[i]] = w[i] / divisor * a.scale;
+    for (int j = 0; j < SLOTS; ++j)
+        if (id[j] >= 0) {
+            const int64_t at = token * a.topk + j * WIDTH + p.lane;
+            a.ids[at] = id[j];
+            a.weights[at] = w[j] / divisor * a.scale;
         }
 }
 
@@ -275,8 +454,12 @@ int lanes_of(const ScoreArgs& a, int v) {
 }  // namespace
 
 int launch_route_scored(const ScoreArgs& a, hipStream_t stream) {
-    // Four experts a lane where that fits a wave, else eight or sixteen.
-    if (lanes_of(a, 4) <= kWave)
+    // Four experts a lane where that fits a wave, else eight or sixteen. Eight as well for large batches of more than
+    // 64 experts, where instructions count and not the length of a lane's chain: two tokens share a wave's
+    // choices. Four against eight, 16384 tokens, top-8: 256 experts in 8 groups (sigmoid, bias) 21.2 and 19.8 us,
+    // 128 experts 7.7 and 6.2; 8192 of 64 in 8 groups 7.7 and 9.7; one token of 256 4.4 and 4.9.
+    const bool large = a.tokens >= 4096 && a.experts > 64 && lanes_of(a, 8) <= kWave;
+    if (!large && lanes_of(a, 4) <= kWave)
         by_lanes<4>(a, lanes_of(a, 4), stream);
     else if (lanes_of(a, 8) <= kWave)
         by_lanes<8>(a, lanes_of(a, 8), stream);
@@ -295,85 +478,111 @@ int launch_route_scored(const ScoreArgs& a, hipStream_t stream) {
 
 namespace {
 
-// LANES lanes a token, V experts of its row each.
+// LANES lanes a token, V experts of its row each. Slot k of the chosen ones is worked out by lane k alone
+// (several by a lane where the segment has fewer than eight) and reaches the others through LDS.
 template <int LANES, int V>
 __global__ __launch_bounds__(256) void route_scored_grad_kernel(ScoreGradArgs a) {
-    const int64_t token = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / LANES;
-    const int first = (threadIdx.x % LANES) * V;
+    constexpr int TOKENS = 256 / LANES, WIDTH = LANES < kMaxTopk ? LANES : kMaxTopk, SLOTS = kMaxTopk / WIDTH;
+    __shared__ int ids[TOKENS][kMaxTopk];
+    __shared__ float grads[TOKENS][kMaxTopk];
+    const int slot = threadIdx.x / LANES, lane = threadIdx.x % LANES;
+    const int64_t token = static_cast<int64_t>(blockIdx.x) * TOKENS + slot;
+    const int first = lane * V;
     const bool live = token < a.tokens;
     const int count = live ? max(0, min(V, a.experts - first)) : 0;
     const float* row = a.logits + token * a.experts;
     const float minus = -__builtin_inff();
     const bool dense = !a.sigmoid && !a.renormalize;
-    float l[V];
-    float top = minus, total = 0.0f;
-    if (dense) {
+    int id[SLOTS];
+    float chosen[SLOTS], g[SLOTS];
+    float top = minus;
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            l[i] = i < count ? row[first + i] : minus;
-            top = fmaxf(top, l[i]);
-        }
+    for (int j = 0; j < SLOTS; ++j) {
+        const int k = j * WIDTH + lane;
+        const bool mine = live && lane < WIDTH && k < a.topk;
+        id[j] = mine ? a.ids[token * a.topk + k] : -1;
+        const bool in = id[j] >= 0 && id[j] < a.experts;
+        chosen[j] = in ? row[id[j]] : minus;
+        g[j] = in ? a.grad_weights[token * a.topk + k] : 0.0f;
+        if (!dense) top = fmaxf(top, chosen[j]);
+    }
+    float l[V];
+    float total = 0.0f;
+    if (dense) {
+        load_some<V>(row, first, count, minus, l);
+#pragma unroll
+        for (int i = 0; i < V; ++i) top = fmaxf(top, l[i]);
         top = lanes_reduce<MaxOp, LANES>(top);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            l[i] = l[i] == minus ? 0.0f : expf(l[i] - top);
+            l[i] = l[i] == minus ? 0.0f : fast_exp(l[i] - top);
             total += l[i];
         }
         total = lanes_reduce<SumOp, LANES>(total);
         total = total == 0.0f ? 0.0f : 1.0f / total;
-    }
-    if (!live) return;
-    int id[kMaxTopk];
-    float chosen[kMaxTopk], g[kMaxTopk];
-#pragma unroll
-    for (int k = 0; k < kMaxTopk; ++k) {
-        id[k] = k < a.topk ? a.ids[token * a.topk + k] : -1;
-        const bool in = id[k] >= 0 && id[k] < a.experts;
-        chosen[k] = in ? row[id[k]] : minus;
-        g[k] = in ? a.grad_weights[token * a.topk + k] : 0.0f;
-    }
-    if (!dense) {
-#pragma unroll
-        for (int k = 0; k < kMaxTopk; ++k) top = fmaxf(top, chosen[k]);
+    } else {
+        top = lanes_reduce<MaxOp, WIDTH>(top);
     }
     // Scores (relative to `top` where they are renormalised), and 1 - s of a sigmoid.
-    float s[kMaxTopk], rest[kMaxTopk];
+    float s[SLOTS], rest[SLOTS];
     float sum = 0.0f, dot = 0.0f;
 #pragma unroll
-    for (int k = 0; k < kMaxTopk; ++k) {
-        rest[k] = 1.0f;
-        s[k] = 0.0f;
-        if (!(chosen[k] == minus)) {
+    for (int j = 0; j < SLOTS; ++j) {
+        const float x = chosen[j];
+        rest[j] = 1.0f;
+        s[j] = 0.0f;
+        if (!(x == minus)) {
             if (a.sigmoid) {
-                rest[k] = 1.0f / (1.0f + expf(chosen[k]));
-                s[k] = a.renormalize ? expf(fminf(chosen[k], 0.0f) - fminf(top, 0.0f)) / (1.0f + expf(-fabsf(chosen[k])))
-                                     : 1.0f / (1.0f + expf(-chosen[k]));
+                rest[j] = __builtin_amdgcn_rcpf(1.0f + fast_exp(x));
+                s[j] = a.renormalize ? fast_exp(fminf(x, 0.0f) - fminf(top, 0.0f)) * __builtin_amdgcn_rcpf(1.0f + fast_exp(-fabsf(x)))
+                                     : __builtin_amdgcn_rcpf(1.0f + fast_exp(-x));
             } else {
-                s[k] = expf(chosen[k] - top) * (dense ? total : 1.0f);
+                s[j] = fast_exp(x - top) * (dense ? total : 1.0f);
             }
         }
-        sum += s[k];
+        sum += s[j];
     }
+    sum = lanes_reduce<SumOp, WIDTH>(sum);
     const float divisor = a.renormalize && sum != 0.0f ? sum : 1.0f;
 #pragma unroll
-    for (int k = 0; k < kMaxTopk; ++k) {
-        s[k] /= divisor;  // one of a single chosen expert is exactly 1
-        dot += s[k] * g[k];
+    for (int j = 0; j < SLOTS; ++j) {
+        s[j] /= divisor;  // one of a single chosen expert is exactly 1
+        dot += s[j] * g[j];
     }
+    dot = lanes_reduce<SumOp, WIDTH>(dot);
     const float mean = a.sigmoid && !a.renormalize ? 0.0f : dot;
+#pragma unroll
+    for (int j = 0; j < SLOTS; ++j) {
+        const int k = j * WIDTH + lane;
+        if (lane < WIDTH) {
+            ids[slot][k] = id[j];
+            grads[slot][k] = a.scale * s[j] * rest[j] * (dense ? g[j] : g[j] - mean);
+        }
+    }
+    wave_fence();
+    if constexpr (LANES > WIDTH) dot = __shfl(dot, 0, LANES);  // the lanes without slots
     float out[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) out[i] = dense ? -(l[i] * total) * mean * a.scale : 0.0f;
+    for (int i = 0; i < V; ++i) out[i] = dense ? -(l[i] * total) * dot * a.scale : 0.0f;
 #pragma unroll
     for (int k = 0; k < kMaxTopk; ++k) {
-        const float d = a.scale * s[k] * rest[k] * (dense ? g[k] : g[k] - mean);
+        const int at = ids[slot][k] - first;
+        const float d = grads[slot][k];
 #pragma unroll
-        for (int i = 0; i < V; ++i) out[i] += id[k] == first + i ? d : 0.0f;
+        for (int i = 0; i < V; ++i) out[i] += at == i ? d : 0.0f;
     }
     float* to = a.grad_logits + token * a.experts + first;
 #pragma unroll
-    for (int i = 0; i < V; ++i)
-        if (i < count) to[i] = out[i];
+    for (int i = 0; i < V; i += 4) {
+        if (i + 4 <= count) {
+            const float four[4] = {out[i], out[i + 1], out[i + 2], out[i + 3]};
+            store_bytes<16>(to + i, pack<MOE_DTYPE_F32>(four));
+        } else {
+#pragma unroll
+            for (int j = i; j < i + 4; ++j)
+                if (j < count) to[j] = out[j];
+        }
+    }
 }
 
 template <int LANES, int V>

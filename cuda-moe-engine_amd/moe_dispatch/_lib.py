@@ -80,7 +80,7 @@ _SIGNATURES = {
                               + [_c_void_p]),
     "moe_rms_norm": (_int, [_c_void_p] * 2),
     "moe_quantize_rows": (_int, [_c_void_p, _int, _c_void_p, _c_void_p, _i64, _i64, _c_void_p]),
-    "moe_rms_norm_backward_scratch_bytes": (_i64, [_i64, _i64]),
+    "moe_rms_norm_backward_scratch_bytes": (_i64, [_i64, _i64, _int]),
     "moe_rms_norm_backward": (_int, [_c_void_p, _c_void_p, _int, _c_void_p, _int] + [_c_void_p] * 5 + [_i64] * 3
                               + [_c_void_p]),
     "moe_route_scored": (_int, [_c_void_p] * 2),
@@ -88,6 +88,7 @@ _SIGNATURES = {
     "moe_linear_scratch_bytes": (_i64, [_i64] * 4 + [_int]),
     "moe_linear": (_int, [_c_void_p] * 2),
     "moe_clip_scratch_bytes": (_i64, []),
+    "moe_clip_overlap": (_int, [_c_void_p] * 5 + [_i64]),
     "moe_clip_gradients": (_int, [_c_void_p] * 2),
 }
 

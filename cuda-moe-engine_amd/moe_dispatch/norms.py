@@ -122,8 +122,8 @@ def quantize_rows(x):
 
 
 @lru_cache(maxsize=1024)
-def _scratch_bytes(tokens, hidden):
-    return get_extension().lib.moe_rms_norm_backward_scratch_bytes(tokens, hidden)
+def _scratch_bytes(tokens, hidden, dtype_code):
+    return get_extension().lib.moe_rms_norm_backward_scratch_bytes(tokens, hidden, dtype_code)
 
 
 def rms_norm_backward(grad_output, x, weight, rstd, *, grad_x=None, gradients=(True, True)):
@@ -153,7 +153,7 @@ def rms_norm_backward(grad_output, x, weight, rstd, *, grad_x=None, gradients=(T
             if grad_weight is not None:
                 grad_weight.zero_()
             return out_x, grad_weight
-        need = _scratch_bytes(tokens, hidden) if grad_weight is not None else 0
+        need = _scratch_bytes(tokens, hidden, DTYPE_CODES[x.dtype]) if grad_weight is not None else 0
         scratch = x.new_empty(need // 4, dtype=torch.float32) if need else None
         lib.check(lib.moe_rms_norm_backward(
             grad_output.data_ptr(), x.data_ptr(), DTYPE_CODES[x.dtype], _ptr(weight), weight_code, rstd.data_ptr(),

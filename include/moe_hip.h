@@ -580,7 +580,7 @@ int moe_quantize_rows(const void* x, int dtype, void* values, float* scales, int
                       void* stream);
 
 /* Bytes of scratch moe_rms_norm_backward needs for grad_weight; -1 for invalid sizes. */
-int64_t moe_rms_norm_backward_scratch_bytes(int64_t tokens, int64_t hidden);
+int64_t moe_rms_norm_backward_scratch_bytes(int64_t tokens, int64_t hidden, int dtype);
 
 /*
  * Gradients of y = x * rstd * weight, x the normed rows (total, with a residual), rstd as
@@ -718,6 +718,12 @@ typedef struct moe_clip_args {
 } moe_clip_args;
 
 int moe_clip_gradients(const moe_clip_args* args, void* stream);
+
+/* Whether any two of the tensors share memory (1) or none do (0), an output that is its own
+ * gradient aside: the check that moe_clip_gradients leaves to its caller. Host work alone; room: 4 * tensors
+ * uint64_t of host memory. */
+int moe_clip_overlap(const void* const* grads, const void* const* outputs, const int64_t* elements,
+                     const int64_t* dtypes, uint64_t* room, int64_t tensors);
 
 #ifdef __cplusplus
 }

@@ -165,9 +165,9 @@ def test_clip_gradients_refuses_bad_lists():
         clip_gradients([g[:4], g[4:]], 1.0, outputs=[torch.zeros(4), g[:4]])
     with pytest.raises(ValueError, match="for each"):
         clip_gradients([g], 1.0, outputs=[])
-    with pytest.raises(ValueError, match="shape and type"):
+    with pytest.raises(ValueError, match="sizes and types"):
         clip_gradients([g], 1.0, outputs=[torch.zeros(9)])
-    with pytest.raises(ValueError, match="shape and type"):
+    with pytest.raises(ValueError, match="sizes and types"):
         clip_gradients([g], 1.0, outputs=[torch.zeros(8, dtype=BF16)])
 
 
@@ -199,8 +199,9 @@ def test_entry_points_check_their_arguments_without_launching():
     assert lib.moe_quantize_rows(A, 2, A, None, 4, 64, None) == invalid
     assert lib.moe_quantize_rows(A, 2, A, A, 0, 64, None) == ok
 
-    need = lib.moe_rms_norm_backward_scratch_bytes(100, 64)
-    assert need >= 64 * 4 and lib.moe_rms_norm_backward_scratch_bytes(100, 0) == -1
+    need = lib.moe_rms_norm_backward_scratch_bytes(100, 64, 2)
+    assert need >= 64 * 4 and lib.moe_rms_norm_backward_scratch_bytes(100, 0, 2) == -1
+    assert lib.moe_rms_norm_backward_scratch_bytes(100, 64, 3) == -1
 
     def grad(g=A, rstd=A, out=A, grad_weight=A, scratch=A, nbytes=need, tokens=100):
         return lib.moe_rms_norm_backward(g, A, 2, A, 2, rstd, None, out, grad_weight, scratch, nbytes, tokens, 64, None)
