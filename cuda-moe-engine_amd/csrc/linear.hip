@@ -29,7 +29,7 @@ __global__ __launch_bounds__(WAVES * 64) void linear_few_kernel(LinearArgs p, in
     const int64_t col0 = static_cast<int64_t>(blockIdx.x) * COLS;
     const auto rw = make_rsrc(p.weight + col0 * p.w_stride, static_cast<uint32_t>((p.rows - col0) * p.w_stride));
     const auto rx = make_rsrc(p.x, static_cast<uint32_t>(p.tokens * p.k_bytes));
-    const uint32_t chunk = (lane >> 4) * 32;
+    const uint32_t chunk = (lane >> 4) * 16;  // of each half of a line
     constexpr uint32_t kPast = 0xfffffff0u;
     uint32_t w_off[WF], x_off[XF];
 #pragma unroll
@@ -43,23 +43,26 @@ __global__ __launch_bounds__(WAVES * 64) void linear_few_kernel(LinearArgs p, in
         x_off[f] = row < p.tokens ? static_cast<uint32_t>(row * p.k_bytes + chunk) : kPast;
     }
     floatx4 acc[XF][WF] = {};
-    auto load = [](auto rsrc, uint32_t off, uint32_t at, bool in) {
-        return __builtin_bit_cast(intx4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, in ? off : kPast, in ? at : 0u, 0));
+    auto load = [](auto rsrc, uint32_t off, bool in) {
+        return __builtin_bit_cast(intx4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, in ? off : kPast, 0u, 0));
     };
+    // Workgroups start at different k: rows a multiple of 4 KiB apart lie on the same memory channels, and in step
+    // all CUs would read the same ones (2 x 14336 rows of 4096 e4m3, one row of x: 24.5 -> 23.9 us).
+    const int turn = static_cast<int>(blockIdx.x) % steps;
     for (int s0 = wave; s0 < steps; s0 += WAVES * UNROLL) {
         intx4 w[UNROLL][WF][2], x[UNROLL][XF][2];
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u) {
             const int s = s0 + u * WAVES;
             if (s < steps) {
-                const uint32_t at = static_cast<uint32_t>(s) * kStageBytes;
+                const uint32_t at = static_cast<uint32_t>(s + turn < steps ? s + turn : s + turn - steps) * kStageBytes;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const bool in = at + chunk + h * 16 < p.k_bytes;
+                    const bool in = at + chunk + h * 64 < p.k_bytes;
 #pragma unroll
-                    for (int f = 0; f < WF; ++f) w[u][f][h] = load(rw, w_off[f] + h * 16 + at, 0u, in);
+                    for (int f = 0; f < WF; ++f) w[u][f][h] = load(rw, w_off[f] + h * 64 + at, in);
 #pragma unroll
-                    for (int f = 0; f < XF; ++f) x[u][f][h] = load(rx, x_off[f] == kPast ? kPast : x_off[f] + h * 16 + at, 0u, in);
+                    for (int f = 0; f < XF; ++f) x[u][f][h] = load(rx, x_off[f] + h * 64 + at, in && x_off[f] != kPast);
                 }
             }
         }
@@ -155,48 +158,69 @@ void run_few(const LinearArgs& a, hipStream_t stream) {
     });
 }
 
-enum Kernel { kFew, kTile64, kTile128, kTile256 };
+// The tile shapes, and what a stage of each costs a CU: 128 bytes of k of TM + BN rows go into LDS and are read from
+// there by two waves each, 3 (TM + BN) cycles at 128 bytes a cycle, about 1.25 of that as measured (128 x 128 950
+// cycles, 64 x 64 470); the 256 x 256 tile alone is bound by its matrix instructions (2048 cycles).
+struct TileShape {
+    int tm, bn;
+    int cycles;    // a stage
+    int overhead;  // first loads and epilogue
+};
+enum Kernel { kTile64, kTile64x128, kTile128, kTile256, kFew };
+constexpr TileShape kShapes[] = {{64, 64, 470, 2500}, {64, 128, 700, 3200}, {128, 128, 950, 4500}, {256, 256, 2150, 8000}};
 
 struct Choice {
     Kernel kernel;
     LinearPlan plan;
     int grid;
+    bool deep;  // 128 x 128: a CU's whole LDS, where no second tile shares it and k is long (16 stages lose 0.5 us
+                // of 16 by it, 64 gain 3 of 38)
 };
 
 constexpr int kCus = 256;
+constexpr int kJoinCycles = 6000;   // the second launch of a split product
+constexpr int kJoinBytes = 1800;    // of partial sums a cycle, written and read
 
+// The cheapest shape and split of k: tiles share a CU's LDS, so a CU takes its tiles one after the other whatever
+// the ring depths are. Chosen against the best of all shapes and splits, timed: 48 x 14336 x 4096 bf16 four parts
+// of 64 x 64 27 us (37 as one part a tile of 128 columns), 333 x 4096 x 4096 64 x 128 21 (27 with 64 x 64), 1024 x 4096 x
+// 4096 128 x 128 35, 200 x 1000 x 2744 64 x 64 7.5 (11 with two parts).
 Choice choose(const LinearArgs& a) {
-    Choice c{};
-    LinearPlan& plan = c.plan;
-    plan.steps = static_cast<int>((a.k_bytes + kStageBytes - 1) / kStageBytes);
-    plan.splits = 1;
+    Choice best{};
+    best.plan.steps = static_cast<int>((a.k_bytes + kStageBytes - 1) / kStageBytes);
+    best.plan.splits = 1;
     if (a.tokens <= 16) {
-        c.kernel = kFew;
-        return c;
+        best.kernel = kFew;
+        return best;
     }
-    const int64_t big = ((a.tokens + 255) / 256) * ((a.rows + 255) / 256);
-    const int64_t mid = ((a.tokens + 127) / 128) * ((a.rows + 127) / 128);
-    int tile = 64, slots = 3 * kCus;
-    c.kernel = kTile64;
-    if (big >= kCus) {
-        tile = 256, slots = kCus;
-        c.kernel = kTile256;
-    } else if (mid >= kCus) {
-        tile = 128, slots = 2 * kCus;
-        c.kernel = kTile128;
+    const int steps = best.plan.steps;
+    const bool element = a.activation != MOE_ACT_NONE && a.activation != MOE_ACT_SWIGLU;
+    int64_t least = INT64_MAX;
+    for (int k = kTile64; k <= kTile256; ++k) {
+        const TileShape& s = kShapes[k];
+        const int cols = a.activation == MOE_ACT_SWIGLU ? s.bn / 2 : s.bn;
+        const int64_t row_tiles = (a.tokens + s.tm - 1) / s.tm, col_tiles = (a.n + cols - 1) / cols;
+        const int64_t tiles = row_tiles * col_tiles;
+        // An elementwise activation takes about as long again as the rest of the epilogue.
+        const int overhead = element ? 7 * s.overhead / 4 : s.overhead;
+        for (int splits = 1; splits <= 16 && 8 * splits <= std::max(steps, 8); ++splits) {
+            if (splits > 1 && tiles * splits > 2 * kCus) break;
+            const int part = (steps + splits - 1) / splits;
+            const int64_t rounds = (tiles * splits + kCus - 1) / kCus;
+            int64_t cost = rounds * (static_cast<int64_t>(part) * s.cycles + overhead);
+            if (splits > 1) cost += kJoinCycles + splits * a.tokens * a.rows * 8 / kJoinBytes;
+            if (cost >= least) continue;
+            least = cost;
+            best.kernel = static_cast<Kernel>(k);
+            best.plan.row_tiles = static_cast<int>(row_tiles);
+            best.plan.col_tiles = static_cast<int>(col_tiles);
+            best.plan.split_steps = part;
+            best.plan.splits = (steps + part - 1) / part;
+            best.deep = tiles * best.plan.splits <= kCus && part >= 32;
+            best.grid = static_cast<int>(std::min<int64_t>((tiles + kNumXcd - 1) / kNumXcd * kNumXcd, kCus));
+        }
     }
-    plan.row_tiles = static_cast<int>((a.tokens + tile - 1) / tile);
-    plan.col_tiles = static_cast<int>((a.rows + tile - 1) / tile);
-    if (a.activation == MOE_ACT_SWIGLU) plan.col_tiles = static_cast<int>((a.n + tile / 2 - 1) / (tile / 2));
-    const int64_t tiles = static_cast<int64_t>(plan.row_tiles) * plan.col_tiles;
-    // At least eight stages a part.
-    if (2 * tiles <= slots)
-        plan.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(slots / tiles, plan.steps / 8)));
-    plan.split_steps = (plan.steps + plan.splits - 1) / plan.splits;
-    plan.splits = (plan.steps + plan.split_steps - 1) / plan.split_steps;
-    c.grid = static_cast<int>(std::min<int64_t>(tiles * plan.splits, slots));
-    c.grid = std::min((c.grid + kNumXcd - 1) / kNumXcd * kNumXcd, slots);
-    return c;
+    return best;
 }
 
 }  // namespace
@@ -212,9 +236,15 @@ int launch_linear(const LinearArgs& a, void* scratch, hipStream_t stream) {
     c.plan.partial = static_cast<float*>(scratch);
     switch (c.kernel) {
         case kFew: run_few(a, stream); break;
-        case kTile64: run_dense<64, 64, 53 * 1024, 2>(a, c.plan, c.grid, stream); break;
-        case kTile128: run_dense<128, 128, 80 * 1024, 2>(a, c.plan, c.grid, stream); break;
-        case kTile256: run_dense<256, 256, 160 * 1024, 2>(a, c.plan, c.grid, stream); break;
+        case kTile64: run_dense<64, 64, 80 * 1024, false>(a, c.plan, c.grid, stream); break;
+        case kTile64x128: run_dense<64, 128, 80 * 1024, false>(a, c.plan, c.grid, stream); break;
+        case kTile128:
+            if (c.deep)
+                run_dense<128, 128, 160 * 1024, false>(a, c.plan, c.grid, stream);
+            else
+                run_dense<128, 128, 80 * 1024, false>(a, c.plan, c.grid, stream);
+            break;
+        case kTile256: run_dense<256, 256, 160 * 1024, true>(a, c.plan, c.grid, stream); break;
     }
     if (c.plan.splits > 1) {
         const unsigned grid = static_cast<unsigned>((a.tokens * (a.n / 4) + 255) / 256);

@@ -51,10 +51,12 @@ constexpr int dense_stages(uint32_t stage_a, uint32_t stage_b, uint32_t bytes, i
 // What the epilogue applies: nothing, one of the elementwise activations, or the gated one.
 enum LinearAct { kActNone, kActElement, kActSwiglu };
 
-template <int TM_, int BN_, LinearAct ACT_, bool FP8_, uint32_t LDS_, int WC_ = 2, int CAP = 6>
+template <int TM_, int BN_, LinearAct ACT_, bool FP8_, uint32_t LDS_, bool CHAIN_, int WC_ = 2, int CAP = 6>
 struct DenseShape {
     static constexpr int TM = TM_, BN = BN_, WC = WC_;
     static constexpr LinearAct ACT = ACT_;
+    // Persistent workgroups that chain tiles, or a workgroup a tile.
+    static constexpr bool CHAIN = CHAIN_;
     static constexpr bool SWIGLU = ACT == kActSwiglu, FP8 = FP8_;
     static constexpr uint32_t LDS = LDS_;
     static constexpr int COLS = SWIGLU ? BN / 2 : BN;  // output columns of a tile
@@ -268,9 +270,41 @@ __device__ __forceinline__ uint2 finish4(const float (&z)[4], const float (&up)[
     return make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
 }
 
+// What the epilogue reads: the residual of the lane's rows and columns, and its columns' terms.
+template <typename S>
+struct DenseExtra {
+    static constexpr int OUT = S::SWIGLU ? S::FB / 2 : S::FB;
+    uint2 residual[S::FA][OUT];
+    float sx[S::FA];
+    float scale[OUT][4], bias[OUT][4], up_scale[S::SWIGLU ? OUT : 1][4], up_bias[S::SWIGLU ? OUT : 1][4];
+
+    __device__ __forceinline__ void load_columns(const LinearArgs& p, int64_t col0) {
+        static_for<OUT>([&](auto j_c) {
+            constexpr int j = decltype(j_c)::value;
+            const int64_t col = min(col0 + j * 16, p.n - 4);
+            column_terms<S::FP8>(p, col, scale[j], bias[j]);
+            if constexpr (S::SWIGLU) column_terms<S::FP8>(p, p.n + col, up_scale[j], up_bias[j]);
+        });
+    }
+    // Row fragment i, whose row of x the lane has.
+    template <int I>
+    __device__ __forceinline__ void load_row(const LinearArgs& p, int64_t row, int64_t col0) {
+        const bool ok = row < p.tokens;
+        sx[I] = S::FP8 && ok ? p.x_scales[row] : 1.0f;
+        static_for<OUT>([&](auto j_c) {
+            constexpr int j = decltype(j_c)::value;
+            const int64_t col = col0 + j * 16;
+            residual[I][j] = make_uint2(0, 0);
+            if (p.residual != nullptr && ok && col < p.n)
+                residual[I][j] = *reinterpret_cast<const uint2*>(p.residual + row * p.n + col);
+        });
+    }
+};
+
 __device__ __forceinline__ void to_vgpr(floatx4& v) { asm volatile("" : "+v"(v)); }
 
-// One tile. Its prologue has been issued; `wait_all`: stores of the tile before may be in flight (they share the
+// One tile. Its prologue has been issued (`CHAIN`; else it goes out here, behind the epilogue's operands, whose
+// latency then hides behind the product); `wait_all`: stores of the tile before may be in flight (they share the
 // loads' counter). With `chain` the last windows load the first stages of the next tile (resources
 // `next`), otherwise its whole prologue goes out in `hook`, once every wave is done with the ring.
 template <typename S, typename Hook>
@@ -305,6 +339,22 @@ __device__ __forceinline__ void dense_tile(const LinearArgs& p, const LinearPlan
         for (int j = 0; j < FB; ++j)
 #pragma unroll
             for (int r = 0; r < 4; ++r) acc[i][j][r] = 0.0f;
+
+    const int lane_row = lane >> 4;
+    const int col4 = 4 * lane_row;
+    const int64_t first_row = t.row0 + wm * S::WTM + (lane & 15);
+    const int64_t first_col = t.col0 + wn * (SWIGLU ? S::WTN / 2 : S::WTN);
+    DenseExtra<S> extra;
+    if constexpr (!S::CHAIN) {
+        if (plan.splits == 1) {
+            extra.load_columns(p, first_col + col4);
+            static_for<FA>([&](auto i_c) {
+                constexpr int i = decltype(i_c)::value;
+                extra.template load_row<i>(p, first_row + i * 16, first_col + col4);
+            });
+        }
+        ops.prologue(t.steps, ends, 0, 0, false);
+    }
 
     using Frag = DenseFrag<FP8>;
     // Fragment idx of the step whose (first) address is va[sub] or vb[sub] plus the slot's offset.
@@ -413,8 +463,10 @@ __device__ __forceinline__ void dense_tile(const LinearArgs& p, const LinearPlan
         }
     };
     int u = 0;
-    // Refills of this tile's whole stages, without selects; then the last windows in full.
-    for (; u < steps - SB - 1; ++u) {
+    // Refills of this tile's whole stages, without selects; then the last windows in full. (A workgroup of one small
+    // tile is bound by LDS and latency, not by the scalar unit, and its code is fetched anew by each launch: one
+    // loop.)
+    for (; S::CHAIN && u < steps - SB - 1; ++u) {
         const int na = sa + 1 == SA ? 0 : sa + 1, nb = sb + 1 == SB ? 0 : sb + 1;
         window(Refill{u + SA, sa, u + SB, sb, ops.ra, ops.rb, false, false}, na, nb);
         sa = na;
@@ -422,7 +474,7 @@ __device__ __forceinline__ void dense_tile(const LinearArgs& p, const LinearPlan
     }
     for (; u + 1 < steps; ++u) {
         const int na = sa + 1 == SA ? 0 : sa + 1, nb = sb + 1 == SB ? 0 : sb + 1;
-        const bool a_next = chain && u + SA >= steps, b_next = chain && u + SB >= steps;
+        const bool a_next = S::CHAIN && chain && u + SA >= steps, b_next = S::CHAIN && chain && u + SB >= steps;
         const int kt_a = a_next ? u + SA - steps : min(u + SA, steps - 1);
         const int kt_b = b_next ? u + SB - steps : min(u + SB, steps - 1);
         window(Refill{kt_a, sa, kt_b, sb, a_next ? next.a : ops.ra, b_next ? next.b : ops.rb,
@@ -433,22 +485,22 @@ __device__ __forceinline__ void dense_tile(const LinearArgs& p, const LinearPlan
         sb = nb;
     }
     second_half(0u, 0u, C0{}, std::true_type{}, NoLoads{}, none);
+    // Also without a next tile: no load may land in this LDS once the workgroup has ended.
     wait_vm_lgkm<0>();
-    ring_barrier();
-    hook();
+    if constexpr (S::CHAIN) {
+        ring_barrier();
+        hook();
+    }
 
     // Lane l holds, of each 16 x 16 block, row l % 16 and columns 4 (l / 16) + 0..3. The empty asm moves a row of
     // accumulators to plain registers before the epilogue's pairs could shape their assignment in the loop.
-    const int lane_row = lane >> 4;
-    const int col4 = 4 * lane_row;
     const int col8 = 8 * (((lane_row & 1) << 1) | (lane_row >> 1));
-    constexpr int OUT = SWIGLU ? FB / 2 : FB;
-    const int64_t first_col = t.col0 + wn * (SWIGLU ? S::WTN / 2 : S::WTN);
+    constexpr int OUT = DenseExtra<S>::OUT;
     if (plan.splits > 1) {
         // Partial sums of weight rows, as they are.
         static_for<FA>([&](auto i_c) {
             constexpr int i = decltype(i_c)::value;
-            const int64_t row = t.row0 + wm * S::WTM + i * 16 + (lane & 15);
+            const int64_t row = first_row + i * 16;
             float* to = plan.partial + (t.split * p.tokens + row) * p.rows;
             static_for<FB>([&](auto j_c) {
                 constexpr int j = decltype(j_c)::value;
@@ -460,34 +512,26 @@ __device__ __forceinline__ void dense_tile(const LinearArgs& p, const LinearPlan
         });
         return;
     }
-    float scale[OUT][4], bias[OUT][4], up_scale[OUT][4], up_bias[OUT][4];
-    static_for<OUT>([&](auto j_c) {
-        constexpr int j = decltype(j_c)::value;
-        const int64_t col = min(first_col + j * 16 + col4, p.n - 4);
-        column_terms<FP8>(p, col, scale[j], bias[j]);
-        if constexpr (SWIGLU) column_terms<FP8>(p, p.n + col, up_scale[j], up_bias[j]);
-    });
+    if constexpr (S::CHAIN) extra.load_columns(p, first_col + col4);
     static_for<FA>([&](auto i_c) {
         constexpr int i = decltype(i_c)::value;
         static_for<FB>([&](auto j_c) { to_vgpr(acc[i][decltype(j_c)::value]); });
-        const int64_t row = t.row0 + wm * S::WTM + i * 16 + (lane & 15);
+        const int64_t row = first_row + i * 16;
         const bool row_ok = row < p.tokens;
         const int64_t at = (row_ok ? row : t.row0) * p.n;
-        const float sx = FP8 && row_ok ? p.x_scales[row] : 1.0f;
+        if constexpr (S::CHAIN) extra.template load_row<i>(p, row, first_col + col4);
         uint2 out[OUT];
         static_for<OUT>([&](auto j_c) {
             constexpr int j = decltype(j_c)::value;
-            const int64_t col = first_col + j * 16 + col4;
-            uint2 residual = make_uint2(0, 0);
-            if (p.residual != nullptr && row_ok && col < p.n)
-                residual = *reinterpret_cast<const uint2*>(p.residual + at + col);
+            constexpr int up = SWIGLU ? j + OUT : j, ju = SWIGLU ? j : 0;
             float z[4], v[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 z[r] = acc[i][j][r];
-                v[r] = SWIGLU ? acc[i][SWIGLU ? j + OUT : j][r] : 0.0f;
+                v[r] = acc[i][up][r];
             }
-            out[j] = finish4<FP8, S::ACT>(z, v, sx, scale[j], bias[j], up_scale[j], up_bias[j], p.activation, residual);
+            out[j] = finish4<FP8, S::ACT>(z, v, extra.sx[i], extra.scale[j], extra.bias[j], extra.up_scale[ju],
+                                          extra.up_bias[ju], p.activation, extra.residual[i][j]);
         });
         // Lanes 16 apart trade halves of two neighbouring blocks: 16-byte stores of 8 columns.
         static_for<OUT / 2>([&](auto h_c) {
@@ -503,6 +547,24 @@ __device__ __forceinline__ void dense_tile(const LinearArgs& p, const LinearPlan
             if (row_ok && col < p.n) *reinterpret_cast<uint2*>(p.output + at + col) = out[OUT - 1];
         }
     });
+}
+
+// A workgroup a tile. XCD i % 8 has a contiguous share of the tiles, as below.
+template <typename S>
+__global__ __launch_bounds__(256) void dense_tile_kernel(LinearArgs p, LinearPlan plan) {
+    __shared__ __attribute__((aligned(1024))) char lds[S::LDS];
+    const int tiles = plan.row_tiles * plan.col_tiles * plan.splits;
+    const int per = (tiles + kNumXcd - 1) / kNumXcd;
+    const int index = static_cast<int>(blockIdx.x) % kNumXcd * per + static_cast<int>(blockIdx.x) / kNumXcd;
+    if (index >= tiles) return;
+    const int column = index / plan.row_tiles;
+    LinearTile t{};
+    t.split = column / plan.col_tiles;
+    t.row0 = (index - column * plan.row_tiles) * S::TM;
+    t.col0 = (column - t.split * plan.col_tiles) * S::COLS;
+    t.step0 = t.split * plan.split_steps;
+    t.steps = min(plan.split_steps, plan.steps - t.step0);
+    dense_tile<S>(p, plan, lds, t, false, 0, 0, false, {}, false, 0, [] {});
 }
 
 // Persistent: workgroups on XCD i % 8 take a contiguous share of the tiles, in order, so that the CUs of one L2
@@ -576,17 +638,24 @@ void linear_instance(const LinearArgs& a, F&& f) {
         by_type(std::integral_constant<LinearAct, kActElement>{});
 }
 
-// The shape's kernel for these operands.
-template <int TM, int BN, uint32_t LDS, int WC>
+// The shape's kernel for these operands: `grid` persistent workgroups, or one for each tile.
+template <int TM, int BN, uint32_t LDS, bool CHAIN>
 void run_dense(const LinearArgs& a, const LinearPlan& plan, int grid, hipStream_t stream) {
     linear_instance(a, [&](auto act, auto fp8) {
-        using S = DenseShape<TM, BN, decltype(act)::value, decltype(fp8)::value, LDS, WC>;
-        dense_ring_kernel<S><<<grid, 256, 0, stream>>>(a, plan);
+        using S = DenseShape<TM, BN, decltype(act)::value, decltype(fp8)::value, LDS, CHAIN>;
+        if constexpr (CHAIN) {
+            dense_ring_kernel<S><<<grid, 256, 0, stream>>>(a, plan);
+        } else {
+            const int tiles = plan.row_tiles * plan.col_tiles * plan.splits;
+            dense_tile_kernel<S><<<(tiles + kNumXcd - 1) / kNumXcd * kNumXcd, 256, 0, stream>>>(a, plan);
+        }
     });
 }
 
-extern template void run_dense<256, 256, 160 * 1024, 2>(const LinearArgs&, const LinearPlan&, int, hipStream_t);
-extern template void run_dense<128, 128, 80 * 1024, 2>(const LinearArgs&, const LinearPlan&, int, hipStream_t);
-extern template void run_dense<64, 64, 53 * 1024, 2>(const LinearArgs&, const LinearPlan&, int, hipStream_t);
+extern template void run_dense<256, 256, 160 * 1024, true>(const LinearArgs&, const LinearPlan&, int, hipStream_t);
+extern template void run_dense<128, 128, 160 * 1024, false>(const LinearArgs&, const LinearPlan&, int, hipStream_t);
+extern template void run_dense<128, 128, 80 * 1024, false>(const LinearArgs&, const LinearPlan&, int, hipStream_t);
+extern template void run_dense<64, 128, 80 * 1024, false>(const LinearArgs&, const LinearPlan&, int, hipStream_t);
+extern template void run_dense<64, 64, 80 * 1024, false>(const LinearArgs&, const LinearPlan&, int, hipStream_t);
 
 }  // namespace moe

@@ -2,5 +2,6 @@
 #include "linear_ring.h"
 
 namespace moe {
-template void run_dense<128, 128, 80 * 1024, 2>(const LinearArgs&, const LinearPlan&, int, hipStream_t);
+template void run_dense<128, 128, 160 * 1024, false>(const LinearArgs&, const LinearPlan&, int, hipStream_t);
+template void run_dense<128, 128, 80 * 1024, false>(const LinearArgs&, const LinearPlan&, int, hipStream_t);
 }  // namespace moe

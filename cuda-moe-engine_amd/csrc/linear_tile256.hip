@@ -2,5 +2,5 @@
 #include "linear_ring.h"
 
 namespace moe {
-template void run_dense<256, 256, 160 * 1024, 2>(const LinearArgs&, const LinearPlan&, int, hipStream_t);
+template void run_dense<256, 256, 160 * 1024, true>(const LinearArgs&, const LinearPlan&, int, hipStream_t);
 }  // namespace moe
