@@ -114,7 +114,7 @@ __global__ __launch_bounds__(WAVES * 64) void linear_few_kernel(LinearArgs p, in
         const int64_t at = row * p.n + col;
         uint2 residual = make_uint2(0, 0);
         if (p.residual != nullptr) residual = *reinterpret_cast<const uint2*>(p.residual + at);
-        *reinterpret_cast<uint2*>(p.output + at) = finish4<FP8, ACT>(
+        *reinterpret_cast<uint2*>(p.output + at) = finish4<FP8, ACT, false>(
             z, up, FP8 ? p.x_scales[row] : 1.0f, scale, bias, up_scale, up_bias, p.activation, residual);
     }
 }
@@ -145,7 +145,7 @@ __global__ __launch_bounds__(256) void linear_join_kernel(LinearArgs p, const fl
     const int64_t at = row * p.n + col;
     uint2 residual = make_uint2(0, 0);
     if (p.residual != nullptr) residual = *reinterpret_cast<const uint2*>(p.residual + at);
-    *reinterpret_cast<uint2*>(p.output + at) = finish4<FP8, ACT>(
+    *reinterpret_cast<uint2*>(p.output + at) = finish4<FP8, ACT, false>(
         z, up, FP8 ? p.x_scales[row] : 1.0f, scale, bias, up_scale, up_bias, p.activation, residual);
 }
 
@@ -166,8 +166,8 @@ struct TileShape {
     int cycles;    // a stage
     int overhead;  // first loads and epilogue
 };
-enum Kernel { kTile64, kTile64x128, kTile128, kTile256, kFew };
-constexpr TileShape kShapes[] = {{64, 64, 470, 2500}, {64, 128, 700, 3200}, {128, 128, 950, 4500}, {256, 256, 2150, 8000}};
+enum Kernel { kTile64, kTile64x128, kTile96x128, kTile128, kTile256, kFew };
+constexpr TileShape kShapes[] = {{64, 64, 470, 2500}, {64, 128, 700, 3200}, {96, 128, 830, 3900}, {128, 128, 950, 4500}, {256, 256, 2150, 8000}};
 
 struct Choice {
     Kernel kernel;
@@ -238,6 +238,7 @@ int launch_linear(const LinearArgs& a, void* scratch, hipStream_t stream) {
         case kFew: run_few(a, stream); break;
         case kTile64: run_dense<64, 64, 80 * 1024, false>(a, c.plan, c.grid, stream); break;
         case kTile64x128: run_dense<64, 128, 80 * 1024, false>(a, c.plan, c.grid, stream); break;
+        case kTile96x128: run_dense<96, 128, 80 * 1024, false>(a, c.plan, c.grid, stream); break;
         case kTile128:
             if (c.deep)
                 run_dense<128, 128, 160 * 1024, false>(a, c.plan, c.grid, stream);
