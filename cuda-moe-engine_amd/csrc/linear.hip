@@ -92,31 +92,33 @@ __global__ __launch_bounds__(WAVES * 64) void linear_few_kernel(LinearArgs p, in
         for (int j = 0; j < WF; ++j) sums[wave][i * WF + j][lane] = acc[i][j];
     __syncthreads();
     // A wave an output block.
-    constexpr int BLOCKS = SWIGLU ? XF : XF * WF;
-    for (int b = wave; b < BLOCKS; b += WAVES) {
-        const int i = SWIGLU ? b : b / WF, j = SWIGLU ? 0 : b % WF;
-        float z[4] = {}, up[4] = {};
-        for (int w = 0; w < WAVES; ++w) {
-            const floatx4 v = sums[w][i * WF + j][lane];
+    with_activation<ACT>(p.activation, [&](auto act_c) {
+        constexpr int BLOCKS = SWIGLU ? XF : XF * WF;
+        for (int b = wave; b < BLOCKS; b += WAVES) {
+            const int i = SWIGLU ? b : b / WF, j = SWIGLU ? 0 : b % WF;
+            float z[4] = {}, up[4] = {};
+            for (int w = 0; w < WAVES; ++w) {
+                const floatx4 v = sums[w][i * WF + j][lane];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) z[r] += v[r];
-            if constexpr (SWIGLU) {
-                const floatx4 g = sums[w][i * WF + 1][lane];
+                for (int r = 0; r < 4; ++r) z[r] += v[r];
+                if constexpr (SWIGLU) {
+                    const floatx4 g = sums[w][i * WF + 1][lane];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) up[r] += g[r];
+                    for (int r = 0; r < 4; ++r) up[r] += g[r];
+                }
             }
+            const int64_t row = i * 16 + (lane & 15), col = col0 + j * 16 + 4 * (lane >> 4);
+            if (row >= p.tokens || col >= p.n) continue;
+            float scale[4], bias[4], up_scale[4] = {}, up_bias[4] = {};
+            column_terms<FP8>(p, col, scale, bias);
+            if constexpr (SWIGLU) column_terms<FP8>(p, p.n + col, up_scale, up_bias);
+            const int64_t at = row * p.n + col;
+            uint2 residual = make_uint2(0, 0);
+            if (p.residual != nullptr) residual = *reinterpret_cast<const uint2*>(p.residual + at);
+            *reinterpret_cast<uint2*>(p.output + at) = finish4<FP8, decltype(act_c)::value, false>(
+                z, up, FP8 ? p.x_scales[row] : 1.0f, scale, bias, up_scale, up_bias, residual);
         }
-        const int64_t row = i * 16 + (lane & 15), col = col0 + j * 16 + 4 * (lane >> 4);
-        if (row >= p.tokens || col >= p.n) continue;
-        float scale[4], bias[4], up_scale[4] = {}, up_bias[4] = {};
-        column_terms<FP8>(p, col, scale, bias);
-        if constexpr (SWIGLU) column_terms<FP8>(p, p.n + col, up_scale, up_bias);
-        const int64_t at = row * p.n + col;
-        uint2 residual = make_uint2(0, 0);
-        if (p.residual != nullptr) residual = *reinterpret_cast<const uint2*>(p.residual + at);
-        *reinterpret_cast<uint2*>(p.output + at) = finish4<FP8, ACT, false>(
-            z, up, FP8 ? p.x_scales[row] : 1.0f, scale, bias, up_scale, up_bias, p.activation, residual);
-    }
+    });
 }
 
 // Joins the partial sums of k's parts, in order: four columns a thread.
@@ -145,8 +147,10 @@ __global__ __launch_bounds__(256) void linear_join_kernel(LinearArgs p, const fl
     const int64_t at = row * p.n + col;
     uint2 residual = make_uint2(0, 0);
     if (p.residual != nullptr) residual = *reinterpret_cast<const uint2*>(p.residual + at);
-    *reinterpret_cast<uint2*>(p.output + at) = finish4<FP8, ACT, false>(
-        z, up, FP8 ? p.x_scales[row] : 1.0f, scale, bias, up_scale, up_bias, p.activation, residual);
+    with_activation<ACT>(p.activation, [&](auto act_c) {
+        *reinterpret_cast<uint2*>(p.output + at) = finish4<FP8, decltype(act_c)::value, false>(
+            z, up, FP8 ? p.x_scales[row] : 1.0f, scale, bias, up_scale, up_bias, residual);
+    });
 }
 
 void run_few(const LinearArgs& a, hipStream_t stream) {

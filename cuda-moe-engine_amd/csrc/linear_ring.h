@@ -136,7 +136,10 @@ struct DenseLoads {
               static_cast<uint32_t>(kt) * kStageBytes);
     }
     __device__ __forceinline__ uint32_t offset(uint32_t off, int kt, int g, bool last) const {
-        return last && !in_tail[g & 1] ? 0xfffffff0u - static_cast<uint32_t>(kt) * kStageBytes : off;
+        // (Both places by name: with an odd number of loads a wave the parity is the wave's, and an index into two
+        // flags would put them in memory.)
+        const bool in = g & 1 ? in_tail[1] : in_tail[0];
+        return last && !in ? 0xfffffff0u - static_cast<uint32_t>(kt) * kStageBytes : off;
     }
     // The loads of the windows before stage 0, in the loop's order (only the last window's when
     // `chained`: the others went out in the tile before). Stages past the end load the last one again,
@@ -202,21 +205,34 @@ __device__ __forceinline__ float gelu_erf(float z) {
     return z < 0.0f ? z * q : z - z * q;
 }
 
-__device__ __forceinline__ void linear_activate(float (&y)[4], int act) {
-    if (act == MOE_ACT_RELU) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) y[r] = y[r] < 0.0f ? 0.0f : y[r];  // NaN stays
-    } else if (act == MOE_ACT_GELU) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) y[r] = gelu_erf(y[r]);
+template <int ACT>
+__device__ __forceinline__ float activated(float z) {
+    if constexpr (ACT == MOE_ACT_RELU) return z < 0.0f ? 0.0f : z;  // NaN stays
+    if constexpr (ACT == MOE_ACT_SILU) return sigmoid_times(z, z);
+    if constexpr (ACT == MOE_ACT_GELU) return gelu_erf(z);
+    // z / 2 (1 + tanh u) = z / (1 + e^-2u)
+    if constexpr (ACT == MOE_ACT_GELU_TANH) return sigmoid_times(z, 1.5957691216057308f * (z + 0.044715f * z * z * z));
+    return z;
+}
+
+// f(constant<activation>) of a kernel whose kind of activation is KIND. The choice is made here, outside of an
+// epilogue's loops: made for each value, the code of 256 x 256 values and four activations does not stay in the
+// instruction cache (12995 x 448 x 13232 e4m3 with silu 315 -> SILU_US us).
+template <LinearAct KIND, typename F>
+__device__ __forceinline__ void with_activation(int act, const F& f) {
+    if constexpr (KIND == kActElement) {
+        if (act == MOE_ACT_RELU)
+            f(std::integral_constant<int, MOE_ACT_RELU>{});
+        else if (act == MOE_ACT_SILU)
+            f(std::integral_constant<int, MOE_ACT_SILU>{});
+        else if (act == MOE_ACT_GELU)
+            f(std::integral_constant<int, MOE_ACT_GELU>{});
+        else
+            f(std::integral_constant<int, MOE_ACT_GELU_TANH>{});
+    } else if constexpr (KIND == kActSwiglu) {
+        f(std::integral_constant<int, MOE_ACT_SWIGLU>{});
     } else {
-        // silu, or z / 2 (1 + tanh u) = z / (1 + e^-2u)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const float z = y[r];
-            const float u = act == MOE_ACT_SILU ? z : 1.5957691216057308f * (z + 0.044715f * z * z * z);
-            y[r] = sigmoid_times(z, u);
-        }
+        f(std::integral_constant<int, MOE_ACT_NONE>{});
     }
 }
 
@@ -248,24 +264,23 @@ __device__ __forceinline__ void column_terms(const LinearArgs& p, int64_t row, f
 
 // Four columns of one row of x: sums to bf16, with bias and the residual's four values. Without them (PLAIN) neither
 // is added: an epilogue of 256 x 256 is 128 or 256 values a lane, a tenth of a tile of 32 stages.
-template <bool FP8, LinearAct ACT, bool PLAIN>
+template <bool FP8, int ACT, bool PLAIN>
 __device__ __forceinline__ uint2 finish4(const float (&z)[4], const float (&up)[4], float sx, const float (&scale)[4],
                                          const float (&bias)[4], const float (&up_scale)[4], const float (&up_bias)[4],
-                                         int act, uint2 residual) {
+                                         uint2 residual) {
     float y[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
         float v = FP8 ? z[r] * (sx * scale[r]) : z[r];
         if constexpr (!PLAIN) v += bias[r];
-        if constexpr (ACT == kActSwiglu) {
+        if constexpr (ACT == MOE_ACT_SWIGLU) {
             float u = FP8 ? up[r] * (sx * up_scale[r]) : up[r];
             if constexpr (!PLAIN) u += up_bias[r];
             y[r] = sigmoid_times(v, v) * u;
         } else {
-            y[r] = v;
+            y[r] = activated<ACT>(v);
         }
     }
-    if constexpr (ACT == kActElement) linear_activate(y, act);
     if constexpr (!PLAIN) {
         y[0] += __uint_as_float(residual.x << 16);
         y[1] += __uint_as_float(residual.x & 0xffff0000u);
@@ -279,7 +294,7 @@ __device__ __forceinline__ uint2 finish4(const float (&z)[4], const float (&up)[
 template <typename S>
 struct DenseExtra {
     static constexpr int OUT = S::SWIGLU ? S::FB / 2 : S::FB;
-    uint2 residual[S::FA][OUT];
+    uint32_t residual[S::FA * OUT * 2];
     float sx[S::FA];
     float scale[OUT][4], bias[OUT][4], up_scale[S::SWIGLU ? OUT : 1][4], up_bias[S::SWIGLU ? OUT : 1][4];
 
@@ -299,9 +314,10 @@ struct DenseExtra {
         static_for<OUT>([&](auto j_c) {
             constexpr int j = decltype(j_c)::value;
             const int64_t col = col0 + j * 16;
-            residual[I][j] = make_uint2(0, 0);
-            if (p.residual != nullptr && ok && col < p.n)
-                residual[I][j] = *reinterpret_cast<const uint2*>(p.residual + row * p.n + col);
+            uint2 v = make_uint2(0, 0);
+            if (p.residual != nullptr && ok && col < p.n) v = *reinterpret_cast<const uint2*>(p.residual + row * p.n + col);
+            residual[(I * OUT + j) * 2] = v.x;
+            residual[(I * OUT + j) * 2 + 1] = v.y;
         });
     }
 };
@@ -523,7 +539,8 @@ __device__ __forceinline__ void dense_tile(const LinearArgs& p, const LinearPlan
         return;
     }
     if constexpr (S::CHAIN) extra.load_columns(p, first_col + col4);
-    auto finish = [&](auto plain_c) {
+    auto finish = [&](auto act_c, auto plain_c) {
+        constexpr int ACT = decltype(act_c)::value;
         constexpr bool PLAIN = decltype(plain_c)::value;
         static_for<FA>([&](auto i_c) {
             constexpr int i = decltype(i_c)::value;
@@ -542,8 +559,8 @@ __device__ __forceinline__ void dense_tile(const LinearArgs& p, const LinearPlan
                     z[r] = acc[i][j][r];
                     v[r] = acc[i][up][r];
                 }
-                out[j] = finish4<FP8, S::ACT, PLAIN>(z, v, extra.sx[i], extra.scale[j], extra.bias[j], extra.up_scale[ju],
-                                              extra.up_bias[ju], p.activation, extra.residual[i][j]);
+                out[j] = finish4<FP8, ACT, PLAIN>(z, v, extra.sx[i], extra.scale[j], extra.bias[j], extra.up_scale[ju],
+                                              extra.up_bias[ju], make_uint2(extra.residual[(i * OUT + j) * 2], extra.residual[(i * OUT + j) * 2 + 1]));
             });
             // Lanes 16 apart trade halves of two neighbouring blocks: 16-byte stores of 8 columns.
             static_for<OUT / 2>([&](auto h_c) {
@@ -560,11 +577,12 @@ __device__ __forceinline__ void dense_tile(const LinearArgs& p, const LinearPlan
             }
         });
     };
-    // Small tiles keep one copy of this code: they are short, and a launch fetches it anew.
-    if (S::CHAIN && p.bias == nullptr && p.residual == nullptr)
-        finish(std::true_type{});
-    else
-        finish(std::false_type{});
+    with_activation<S::ACT>(p.activation, [&](auto act_c) {
+        if constexpr (S::CHAIN) {
+            if (p.bias == nullptr && p.residual == nullptr) return finish(act_c, std::true_type{});
+        }
+        finish(act_c, std::false_type{});
+    });
 }
 
 // A workgroup a tile. XCD i % 8 has a contiguous share of the tiles, as below.
