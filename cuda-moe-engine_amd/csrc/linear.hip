@@ -171,7 +171,7 @@ struct TileShape {
     int overhead;  // first loads and epilogue
 };
 enum Kernel { kTile64, kTile64x128, kTile96x128, kTile128, kTile256, kFew };
-constexpr TileShape kShapes[] = {{64, 64, 470, 2500}, {64, 128, 700, 3200}, {96, 128, 830, 3900}, {128, 128, 950, 4500}, {256, 256, 2150, 8000}};
+constexpr TileShape kShapes[] = {{64, 64, 470, 2500}, {64, 128, 700, 3200}, {96, 128, 830, 3900}, {128, 128, 950, 4500}, {256, 256, 2150, 13000}};
 
 struct Choice {
     Kernel kernel;
@@ -182,6 +182,7 @@ struct Choice {
 };
 
 constexpr int kCus = 256;
+constexpr int64_t kMostTiles = 1 << 22;
 constexpr int kJoinCycles = 6000;   // the second launch of a split product
 constexpr int kJoinBytes = 1800;    // of partial sums a cycle, written and read
 
@@ -205,8 +206,8 @@ Choice choose(const LinearArgs& a) {
         const int cols = a.activation == MOE_ACT_SWIGLU ? s.bn / 2 : s.bn;
         const int64_t row_tiles = (a.tokens + s.tm - 1) / s.tm, col_tiles = (a.n + cols - 1) / cols;
         const int64_t tiles = row_tiles * col_tiles;
-        // An elementwise activation takes about as long again as the rest of the epilogue.
-        const int overhead = element ? 7 * s.overhead / 4 : s.overhead;
+        if (k != kTile256 && tiles > kMostTiles) continue;  // a workgroup each: a grid's threads stay below 2^32
+        const int overhead = element ? 5 * s.overhead / 4 : s.overhead;  // an elementwise activation's part
         for (int splits = 1; splits <= 16 && 8 * splits <= std::max(steps, 8); ++splits) {
             if (splits > 1 && tiles * splits > 2 * kCus) break;
             const int part = (steps + splits - 1) / splits;
@@ -221,7 +222,8 @@ Choice choose(const LinearArgs& a) {
             best.plan.split_steps = part;
             best.plan.splits = (steps + part - 1) / part;
             best.deep = tiles * best.plan.splits <= kCus && part >= 32;
-            best.grid = static_cast<int>(std::min<int64_t>((tiles + kNumXcd - 1) / kNumXcd * kNumXcd, kCus));
+            best.grid = static_cast<int>(
+                std::min<int64_t>((tiles * best.plan.splits + kNumXcd - 1) / kNumXcd * kNumXcd, kCus));
         }
     }
     return best;
