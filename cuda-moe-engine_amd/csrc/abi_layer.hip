@@ -17,12 +17,11 @@ int check_struct(const Args* args) {
     return MOE_OK;
 }
 
-int check_rows(int64_t tokens, int64_t hidden, int64_t dtype) {
+int check_rows(int64_t tokens, int64_t hidden, int64_t dtype, int64_t most = kMaxNormWidth) {
     MOE_REQUIRE(valid_dtype(dtype), MOE_ERR_INVALID_ARGUMENT, "only FP32, FP16 and BF16 are supported");
     MOE_REQUIRE(tokens >= 0, MOE_ERR_INVALID_ARGUMENT, "tokens must be >= 0");
     MOE_REQUIRE(tokens <= kMaxLayerTokens, MOE_ERR_CAPACITY, "takes up to %lld tokens", (long long)kMaxLayerTokens);
-    MOE_REQUIRE(hidden >= 1 && hidden <= kMaxNormWidth, MOE_ERR_UNSUPPORTED, "rows have 1..%lld elements",
-                (long long)kMaxNormWidth);
+    MOE_REQUIRE(hidden >= 1 && hidden <= most, MOE_ERR_UNSUPPORTED, "rows have 1..%lld elements", (long long)most);
     return MOE_OK;
 }
 
@@ -79,7 +78,7 @@ int moe_rms_norm(const moe_rms_norm_args* p, void* stream) {
 
 int moe_quantize_rows(const void* x, int dtype, void* values, float* scales, int64_t tokens, int64_t hidden,
                       void* stream) {
-    const int rc = check_rows(tokens, hidden, dtype);
+    const int rc = check_rows(tokens, hidden, dtype, kMaxQuantizeWidth);
     if (rc != MOE_OK || tokens == 0) return rc;
     MOE_REQUIRE(x && values && scales, MOE_ERR_INVALID_ARGUMENT, "null pointer");
     MOE_REQUIRE(aligned_to(x, dtype_size(dtype)) && aligned_to(scales, 4), MOE_ERR_INVALID_ARGUMENT,

@@ -184,13 +184,18 @@ __global__ __launch_bounds__(WAVES < 4 ? 256 : WAVES * 64) void rms_norm_kernel(
     }
 }
 
-template <int DT, int NV, int WAVES>
-void run_norm(const NormArgs& a, bool norm, hipStream_t stream) {
+// As many workgroups as the chip holds at 32 waves a CU, an equal number of rows each.
+template <int WAVES>
+unsigned norm_grid(const NormArgs& a) {
     constexpr int ROWS = WAVES < 4 ? 4 / WAVES : 1;
-    // As many workgroups as the chip holds at 32 waves a CU, an equal number of rows each.
     const int64_t blocks = (a.tokens + ROWS - 1) / ROWS, most = 256 * (WAVES < 4 ? 8 : 32 / WAVES);
     const int64_t turns = (blocks + most - 1) / most;
-    const dim3 grid(static_cast<unsigned>((blocks + turns - 1) / turns)), block(WAVES < 4 ? 256 : WAVES * 64);
+    return static_cast<unsigned>((blocks + turns - 1) / turns);
+}
+
+template <int DT, int NV, int WAVES>
+void run_norm(const NormArgs& a, bool norm, hipStream_t stream) {
+    const dim3 grid(norm_grid<WAVES>(a)), block(WAVES < 4 ? 256 : WAVES * 64);
     if (!norm)
         rms_norm_kernel<DT, NV, WAVES, true, false><<<grid, block, 0, stream>>>(a);
     else if (a.scales != nullptr)
@@ -210,8 +215,13 @@ void norm_by_width(const NormArgs& a, bool norm, hipStream_t stream) {
     if (vectors <= 256) return run_norm<DT, 1, 4>(a, norm, stream);
     if (vectors <= 512) return run_norm<DT, 1, 8>(a, norm, stream);
     if (vectors <= 1024) return run_norm<DT, 1, 16>(a, norm, stream);
-    if (DT != MOE_DTYPE_F32 || vectors <= 2048) return run_norm<DT, 2, 16>(a, norm, stream);
-    run_norm<DT, DT == MOE_DTYPE_F32 ? 4 : 2, 16>(a, norm, stream);
+    if (vectors <= 2048) return run_norm<DT, 2, 16>(a, norm, stream);
+    if (norm) {
+        if constexpr (DT == MOE_DTYPE_F32) run_norm<DT, 4, 16>(a, norm, stream);
+        return;
+    }
+    // Rows that are only quantized may be twice as wide.
+    rms_norm_kernel<DT, DT == MOE_DTYPE_F32 ? 8 : 4, 16, true, false><<<norm_grid<16>(a), 1024, 0, stream>>>(a);
 }
 
 }  // namespace

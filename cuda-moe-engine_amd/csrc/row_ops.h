@@ -9,6 +9,7 @@
 namespace moe {
 
 constexpr int64_t kMaxNormWidth = 16384;      // a row stays in a workgroup's registers
+constexpr int64_t kMaxQuantizeWidth = 32768;
 constexpr int64_t kMaxLayerTokens = 1 << 21;  // grids of up to 1024 threads a token stay below 2^32
 constexpr int kMaxScoredExperts = 512;        // sixteen scores a lane, one wave
 constexpr float kE4m3Most = 448.0f;           // largest finite e4m3 value

@@ -22,6 +22,7 @@ from ._lib import RMS_NORM_ARGS
 from .training import _ptr, on_device, refuse_autograd, require_gpu, require_tensor, shape_of
 
 MAX_HIDDEN = 16384
+MAX_QUANTIZED = 32768  # of quantize_rows
 MAX_TOKENS = 2**21
 E4M3 = torch.float8_e4m3fn
 
@@ -46,14 +47,14 @@ class Normed(NamedTuple):
     rstd: torch.Tensor | None
 
 
-def _check_rows(x):
+def _check_rows(x, most=MAX_HIDDEN):
     tokens, hidden = shape_of(x, "x", 2)
     if x.dtype not in DTYPE_CODES:
         raise TypeError(f"x must be float32, float16 or bfloat16, got {x.dtype}")
     if not x.is_contiguous():
         raise ValueError("x must be contiguous")
-    if not 1 <= hidden <= MAX_HIDDEN:
-        raise ValueError("rows must have 1..16384 elements")
+    if not 1 <= hidden <= most:
+        raise ValueError(f"rows must have 1..{most} elements")
     if tokens > MAX_TOKENS:
         raise ValueError("takes up to 2^21 rows")
     return tokens, hidden
@@ -107,8 +108,8 @@ def rms_norm(x, weight=None, *, residual=None, eps=1e-6, quantize=False, return_
 
 
 def quantize_rows(x):
-    """Rows x [T, H] (fp32, fp16 or bf16) as ``QuantizedRows``, with ``rms_norm``'s scales."""
-    tokens, hidden = _check_rows(x)
+    """Rows x [T, H] (fp32, fp16 or bf16, H up to 32768) as ``QuantizedRows``, with ``rms_norm``'s scales."""
+    tokens, hidden = _check_rows(x, MAX_QUANTIZED)
     require_gpu(x)
     refuse_autograd(x)
     device = x.device

@@ -575,7 +575,7 @@ typedef struct moe_rms_norm_args {
 int moe_rms_norm(const moe_rms_norm_args* args, void* stream);
 
 /* Rows in e4m3 with a scale each, as moe_rms_norm writes its y = x: activations between two 8-bit
- * products, and weights (rows: output columns) when they are loaded. */
+ * products, and weights (rows: output columns) when they are loaded. H up to 32768. */
 int moe_quantize_rows(const void* x, int dtype, void* values, float* scales, int64_t tokens, int64_t hidden,
                       void* stream);
 

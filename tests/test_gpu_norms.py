@@ -89,6 +89,13 @@ def test_norm_against_the_formula(tokens, hidden, dtype):
         _check_quantized(quantize_rows(x), x.double(), "rows", steps=4)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hidden", [16385, 20000, 32767, 32768])
+def test_wide_rows_in_8_bits(hidden, dtype):
+    x = _case(5, hidden, dtype, None, False, seed=hidden)[0]
+    _check_quantized(quantize_rows(x), x.double(), "wide", steps=4)
+
+
 def test_rows_of_zeros_tiny_values_and_no_rows():
     x = torch.zeros(5, 96, device="cuda")
     x[1] = 1e-35  # below the least scale

@@ -49,8 +49,9 @@ def test_rms_norm_refuses_bad_tensors():
             rms_norm(x, w, eps=eps)
     with pytest.raises(ValueError, match="16384"):
         rms_norm(torch.zeros(1, 16385, dtype=BF16))
-    with pytest.raises(ValueError, match="16384"):
-        quantize_rows(torch.zeros(1, 0, dtype=BF16))
+    for hidden in (0, 32769):
+        with pytest.raises(ValueError, match="32768"):
+            quantize_rows(torch.zeros(1, hidden, dtype=BF16))
     with pytest.raises(ValueError, match="2\\^21"):
         rms_norm(torch.zeros(2**21 + 1, 1, dtype=BF16))
     rstd = torch.ones(4)
