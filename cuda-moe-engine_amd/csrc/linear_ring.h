@@ -202,7 +202,7 @@ __device__ __forceinline__ float gelu_erf(float z) {
     p = p * t + 0.2824094757421122f;
     p = p * t + 0.2820844776905523f;
     const float q = 0.5f * t * p * __builtin_amdgcn_exp2f(a * a * -1.4426950408889634f);
-    return z < 0.0f ? z * q : z - z * q;
+    return z * (z < 0.0f ? q : 1.0f - q);  // of infinity 1, and no difference of two infinities
 }
 
 template <int ACT>
@@ -271,10 +271,10 @@ __device__ __forceinline__ uint2 finish4(const float (&z)[4], const float (&up)[
     float y[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-        float v = FP8 ? z[r] * (sx * scale[r]) : z[r];
+        float v = FP8 ? z[r] * sx * scale[r] : z[r];  // (the product of the scales alone may leave fp32)
         if constexpr (!PLAIN) v += bias[r];
         if constexpr (ACT == MOE_ACT_SWIGLU) {
-            float u = FP8 ? up[r] * (sx * up_scale[r]) : up[r];
+            float u = FP8 ? up[r] * sx * up_scale[r] : up[r];
             if constexpr (!PLAIN) u += up_bias[r];
             y[r] = sigmoid_times(v, v) * u;
         } else {
@@ -554,7 +554,7 @@ __device__ __forceinline__ void dense_tile(const LinearArgs& p, const LinearPlan
                 constexpr int j = decltype(j_c)::value;
                 constexpr int up = SWIGLU ? j + OUT : j, ju = SWIGLU ? j : 0;
                 float z[4], v[4];
-    #pragma unroll
+#pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     z[r] = acc[i][j][r];
                     v[r] = acc[i][up][r];

@@ -99,7 +99,7 @@ def linear(x, weight, bias=None, *, activation=None, residual=None, output=None)
                                                                 None if same else residual)):
             raise ValueError("output may be residual itself, but must not overlap another operand")
     require_gpu(x)
-    refuse_autograd(x, weight, bias, residual, output)
+    refuse_autograd(x, weight, x_scales, w_scales, bias, residual, output)
     lib = get_extension().lib
     with on_device(device):
         if output is None:

@@ -182,6 +182,57 @@ def test_activations_over_their_range(activation):
     _check(linear(x, w, activation=activation), x, w, None, None, activation, activation)
 
 
+@pytest.mark.parametrize("activation", ACTS)
+@pytest.mark.parametrize("tokens", [2, 40])
+def test_activations_of_infinities(tokens, activation):
+    inf = float("inf")
+    x = torch.zeros(tokens, 8, device="cuda", dtype=torch.bfloat16)
+    values = torch.tensor([inf, -inf, float("nan"), 3e38, -3e38, 2e19, -2e19, 0.0], device="cuda")
+    bias = values if activation != "swiglu" else torch.cat([values, torch.full((8,), 0.5, device="cuda")])
+    w = torch.zeros(bias.numel(), 8, device="cuda", dtype=torch.bfloat16)
+    got = linear(x, w, bias, activation=activation)
+    f = torch.nn.functional
+    # Halves of fp32 values: what the activations do to them needs no rounding but bf16's.
+    want = {None: lambda z: z, "relu": torch.relu, "silu": f.silu, "gelu": f.gelu,
+            "gelu_tanh": lambda z: f.gelu(z, approximate="tanh"), "swiglu": lambda z: f.silu(z) * 0.5}[activation]
+    want = want(values.double().cpu()).bfloat16().expand(tokens, 8)
+    assert torch.equal(got.cpu().nan_to_num(7.0), want.nan_to_num(7.0))
+    assert torch.equal(got.cpu().isnan(), want.isnan())
+
+
+@pytest.mark.parametrize("tokens", [2, 40])
+@pytest.mark.parametrize("part,factor", [(256, 1e13), (65536, 1e16)])
+def test_scales_whose_product_nears_or_leaves_fp32(tokens, part, factor):
+    """Results past bf16's range are infinite: from (2 - 2^-8) 2^127 on the nearest value is."""
+    x, w, _, _ = _case(tokens, 64, 264, True, seed=9)
+    x = x._replace(values=(x.values.float() / part).to(x.values.dtype), scales=x.scales * 1e30)
+    w = w._replace(values=(w.values.float() / part).to(w.values.dtype), scales=w.scales * factor)
+    got, (want, off) = linear(x, w), _formula(x, w, None, None, None)
+    past = want.abs() >= (2 - HALF) * 2.0**127
+    assert torch.equal(got[past].double(), want[past].sign() * float("inf"))
+    bad = ~past & ~((got.double() - want).abs() <= want.abs() * HALF * 1.001 + off * 1.01)
+    assert not bool(bad.any())
+
+
+def test_operands_that_record_gradients_are_refused():
+    x, w, b, r = _case(3, 64, 24, False, bias=torch.float32, residual=True)
+    for t in (x, w, b, r):
+        with pytest.raises(ValueError, match="autograd"):
+            t.requires_grad_()
+            try:
+                linear(x, w, b, residual=r)
+            finally:
+                t.requires_grad_(False)
+    x, w, _, _ = _case(3, 64, 24, True)
+    for t in (x.scales, w.scales):
+        t.requires_grad_()
+        with pytest.raises(ValueError, match="autograd"):
+            linear(x, w)
+        with torch.no_grad():
+            linear(x, w)
+        t.requires_grad_(False)
+
+
 def test_graph_replays_and_streams_share_nothing():
     """Two captured graphs and eager work in between: each call's scratch is its own."""
     x, w, b, r = _case(3, 4096, 1408, True, "swiglu", torch.float32, False)
