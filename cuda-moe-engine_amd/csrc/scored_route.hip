@@ -246,7 +246,7 @@ __device__ __forceinline__ bool choose_fast(const ScoreArgs& a, const Place& p, 
 #pragma unroll
             for (int i = 0; i < V; ++i) s[i] *= inverse;
         }
-        // Magnitudes as integers: of numbers they order alike, and a NaN's or infinity's are the largest.
+        // Magnitudes as integers: of numbers they order alike, and an infinity's or NaN's are the largest.
         uint32_t largest = 0;
         float first = minus, second = minus;
 #pragma unroll
@@ -261,8 +261,8 @@ __device__ __forceinline__ bool choose_fast(const ScoreArgs& a, const Place& p, 
         }
         largest = lanes_max<LANES>(largest);
         near = 2.0f * error * __uint_as_float(largest);
-        // A key that is no number or infinite: the other path sorts that out.
-        unsure = largest >= 0x7f800000u;
+        // A key that is no number, infinite, or so large that a sum of two is: the other path sorts that out.
+        unsure = largest >= 0x7e800000u;
         if (a.groups > 1) {
             best_two<LANES>(first, second, p.group_lanes);
             const float group = a.group_best == 2 && second > minus ? first + second : first;

@@ -129,6 +129,14 @@ def test_a_bias_that_drowns_scores():
             assert torch.equal(route_scored(logits, 6, **options)[0], _reference(logits, 6, **options)[0])
 
 
+def test_groups_whose_sums_leave_fp32():
+    bias = torch.tensor([3.3e38, 1e38, 2.5e38, 2.4e38], device="cuda")
+    logits = _logits(70, 4, 12)
+    for scoring in ("softmax", "sigmoid"):
+        ids, _ = route_scored(logits, 2, scoring=scoring, bias=bias, groups=2, top_groups=1)
+        assert ids.tolist() == [[2, 3]] * 70
+
+
 @pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("with_bias", [False, True])
 def test_experts_that_are_out(scoring, with_bias):
