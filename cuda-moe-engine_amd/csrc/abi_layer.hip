@@ -222,6 +222,8 @@ int moe_clip_gradients(const moe_clip_args* p, void* stream) {
 
 int moe_clip_overlap(const void* const* grads, const void* const* outputs, const int64_t* elements,
                      const int64_t* dtypes, uint64_t* room, int64_t tensors) {
+    if (tensors <= 0) return 0;
+    MOE_REQUIRE(grads && outputs && elements && dtypes && room, MOE_ERR_INVALID_ARGUMENT, "null pointer");
     struct Range {
         uint64_t from, to;
     };

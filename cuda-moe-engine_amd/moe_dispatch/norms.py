@@ -76,7 +76,8 @@ def rms_norm(x, weight=None, *, residual=None, eps=1e-6, quantize=False, return_
     of x's type (None: 0). Statistics and products are fp32, from the unrounded sum; ``output``
     is rounded once to x's type, or with ``quantize`` to e4m3 with
     ``scales[t] = max(max_j |y_tj|, 2^-100) / 448``. A NaN stays one; a row that holds an
-    infinity has no finite scale. H is at most 16384.
+    infinity has no finite scale. H is at most 16384, and values are below 1e17 (their squares' sum
+    is fp32).
     """
     tokens, hidden = _check_rows(x)
     weight_code = _check_weight(weight, x)

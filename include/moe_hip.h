@@ -554,7 +554,7 @@ int moe_low_rank_backward(const void* grad_output, const void* x, const void* do
  * itself). scales fp32 [T]: output is e4m3 (OCP, one byte),
  *   scales[t] = max(max_j |y_j|, 2^-100) / 448,  output = round_e4m3(y / scales[t]).
  * A NaN stays NaN; an infinite y makes its row's scale infinite, so that nothing finite stands
- * for it. fp32 rows have finite squares. Limits: 1 <= H <= 16384, T <= 2^21, eps >= 0.
+ * for it. The squares' sum is fp32: rows keep it finite (values below 1e17 do). Limits: 1 <= H <= 16384, T <= 2^21, eps >= 0.
  */
 typedef struct moe_rms_norm_args {
     int64_t struct_bytes;
@@ -702,7 +702,7 @@ int64_t moe_clip_scratch_bytes(void);
  * before the call returns; tensors are contiguous, aligned to their element, and outputs[i]
  * is grads[i] (in place) or of its type and overlaps nothing else. Sums are 64 bits, in an
  * order that the sizes fix. A norm that is infinite or NaN leaves the values as they are. norm: one fp32 on the
- * device. Limits: 2^16 tensors, 2^40 elements.
+ * device (one past its range is written as infinite, the values are scaled all the same). Limits: 2^16 tensors, 2^40 elements.
  */
 typedef struct moe_clip_args {
     int64_t struct_bytes;
@@ -721,7 +721,7 @@ int moe_clip_gradients(const moe_clip_args* args, void* stream);
 
 /* Whether any two of the tensors share memory (1) or none do (0), an output that is its own
  * gradient aside: the check that moe_clip_gradients leaves to its caller. Host work alone; room: 4 * tensors
- * uint64_t of host memory. */
+ * uint64_t of host memory. A null pointer is MOE_ERR_INVALID_ARGUMENT. */
 int moe_clip_overlap(const void* const* grads, const void* const* outputs, const int64_t* elements,
                      const int64_t* dtypes, uint64_t* room, int64_t tensors);
 

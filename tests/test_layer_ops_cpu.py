@@ -246,3 +246,9 @@ def test_entry_points_check_their_arguments_without_launching():
     assert clip(norm=0) == invalid and clip(most=0.0) == invalid and clip(most=float("nan")) == invalid
     assert clip(nbytes=8) == workspace and clip(tensors=-1) == capacity and clip(tensors=2**16 + 1) == capacity
     assert clip(grads=0, tensors=1) == invalid
+
+
+def test_overlap_check_takes_no_null_pointers():
+    lib = _lib.load_library()
+    assert lib.moe_clip_overlap(None, None, None, None, None, 0) == 0
+    assert lib.moe_clip_overlap(None, None, None, None, None, 2) == 1  # MOE_ERR_INVALID_ARGUMENT
