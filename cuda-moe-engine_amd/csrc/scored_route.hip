@@ -8,11 +8,15 @@
 //
 // A token is a segment of LANES lanes of a wave, V experts a lane, every group in lanes of
 // its own. A lane sorts its keys once; each choice is then a maximum over the segment of the lanes' first
-// keys, which the owner removes. The choice is by exact value: keys are fp32 first, and a token whose
-// order hangs on a difference within their rounding (or on a tie, or that has no K experts left) is decided
-// again by its wave in 64 bits, so that the ids are the definition's and do not depend on how exp rounds.
-// About one token in a thousand at 256 experts. Bound by instructions, not bytes: see the figures at the
-// launcher.
+// keys, which the owner removes. The choice is by exact value, so that the ids are the definition's and do not
+// depend on how exp rounds: keys are fp32 first, and where the order hangs on a difference within their
+// rounding, or on a tie, the few experts or the groups that it concerns are compared in 64 bits (about one
+// token in a thousand at 256 experts; all of such a token's experts, in straight code, took 16384 of them from
+// 14 to 19 us: a wave that comes last waits for code that is in no cache). A token without K experts, with
+// infinite keys, NaN, or more than kCandidates of like keys is chosen in 64 bits as a whole.
+//
+// Bound by instructions, not bytes: 16384 tokens of 256 experts, top-8 in 4 of 8 groups, are 17.6 MB (3.5 us)
+// and 14.3 us; one token 4.2.
 #include "row_ops.h"
 
 namespace moe {
@@ -210,18 +214,76 @@ __device__ __forceinline__ void sort_keys(uint32_t (&key)[V], int (&place)[V]) {
                     }
 }
 
-// Chooses by fp32 keys into picked[0..topk); true where fp32 does not decide it. `scores`: the token's
-// room for a score a group.
+// Candidates whose order is worked out in 64 bits, a lane each.
+constexpr int kCandidates = 16;
+
+// Softmax's sum in 64 bits, relative to the token's largest logit. (Loops of few instructions, here and below: what
+// only a token in a thousand comes to is not in the instruction cache.)
+template <int LANES>
+__device__ __forceinline__ double exact_total(const ScoreArgs& a, const Place& p, const float* row, float top) {
+    double total = 0.0;
+    if (a.sigmoid) return 1.0;
+#pragma unroll 1
+    for (int i = 0; i < p.count; ++i) total += exp(static_cast<double>(row[p.first + i]) - static_cast<double>(top));
+#pragma unroll 1
+    for (int d = 1; d < LANES; d <<= 1) total += lane_xor(total, d);
+    return total;
+}
+
+// Expert id's score and bias in 64 bits.
+__device__ __forceinline__ double exact_key(const ScoreArgs& a, const float* row, int id, float top, double total) {
+    const double x = static_cast<double>(row[id]);
+    const double e = exp(a.sigmoid ? -x : x - static_cast<double>(top));
+    return (a.sigmoid ? 1.0 / (1.0 + e) : e / total) + (a.bias != nullptr ? static_cast<double>(a.bias[id]) : 0.0);
+}
+
+// Whether the lane's group takes part, by its exact score.
+template <int LANES>
+__device__ __forceinline__ bool exact_open(const ScoreArgs& a, const Place& p, const float* row, float top) {
+    const double minus = -__builtin_inf();
+    const double total = exact_total<LANES>(a, p, row, top);
+    double first = minus, second = minus;
+#pragma unroll 1
+    for (int i = 0; i < p.count; ++i) {
+        if (!(row[p.first + i] > -__builtin_inff())) continue;
+        const double key = exact_key(a, row, p.first + i, top, total);
+        second = most(second, key < first ? key : first);
+        first = most(first, key);
+    }
+#pragma unroll 1
+    for (int d = 1; d < p.group_lanes; d <<= 1) {
+        const double f = lane_xor(first, d), s = lane_xor(second, d);
+        second = most(most(second, s), f < first ? f : first);
+        first = most(first, f);
+    }
+    const double group = a.group_best == 2 && second > minus ? first + second : first;
+    const int mine = p.lane / p.group_lanes;
+    int before = 0;
+#pragma unroll 1
+    for (int o = p.group_lanes; o < LANES; o += p.group_lanes) {
+        const double other = lane_xor(group, o);
+        const int index = (p.lane ^ o) / p.group_lanes;
+        before += index < a.groups && (other > group || (other == group && index < mine));
+    }
+    return mine < a.groups && before < a.top_groups;
+}
+
+// Chooses by fp32 keys into picked[0..topk); true where that does not decide it. Where groups are too near each
+// other to tell which take part, their scores are worked out in 64 bits; where keys are (or equal), among the chosen ones and
+// those next to them, these candidates alone are ordered in 64 bits. `row`: the token's logits;
+// `scores`: its room for a score a group; `exact`: for a key a candidate.
 template <int LANES, int V>
-__device__ __forceinline__ bool choose_fast(const ScoreArgs& a, const Place& p, const float (&l)[V], const float (&b)[V],
-                                            int* picked, float* scores) {
+__device__ __forceinline__ bool choose_fast(const ScoreArgs& a, const Place& p, const float* row, const float (&l)[V],
+                                            const float (&b)[V], int* picked, float* scores, double* exact) {
     const bool has_bias = a.bias != nullptr;
     const float minus = -__builtin_inff();
     bool unsure = false;
     uint32_t key[V];
-    float near = 0.0f;
+    float near = 0.0f, largest_logit = minus;
+    if (!has_bias) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) key[i] = l[i] > minus ? ordered(l[i]) : 0u;
+        for (int i = 0; i < V; ++i) key[i] = l[i] > minus ? ordered(l[i]) : 0u;
+    }
     if (has_bias || a.groups > 1) {
         float s[V];
         // A score's roundings: sigmoid 6 of 2^-24 (argument, exp, sum, reciprocal), softmax up to V + 16 (its sum
@@ -236,6 +298,7 @@ __device__ __forceinline__ bool choose_fast(const ScoreArgs& a, const Place& p, 
 #pragma unroll
             for (int i = 1; i < V; ++i) top = fmaxf(top, l[i]);
             top = lanes_reduce<MaxOp, LANES>(top);
+            largest_logit = top;
             float total = 0.0f;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
@@ -270,7 +333,11 @@ __device__ __forceinline__ bool choose_fast(const ScoreArgs& a, const Place& p, 
             // Lanes past the last group bring -inf, which is before and close to none.
             if (p.lane % p.group_lanes == 0) scores[mine] = group;
             wave_fence();
-            int before = 0, close = 0;
+            // Groups that are certainly before this one, and those that may be (itself among them). The two sums
+            // here and a group's own are three more roundings of up to twice the largest key: 2.25 near, of which 2
+            // are the keys' own.
+            const float low = group - 2.25f * near, high = group + 2.25f * near;
+            int before = 0, maybe = 0;
             const int places = LANES / p.group_lanes;  // a power of two
             for (int g = 0; g < places; g += 4) {
                 float other[4];
@@ -278,13 +345,20 @@ __device__ __forceinline__ bool choose_fast(const ScoreArgs& a, const Place& p, 
                 for (int j = 0; j < 4; ++j) other[j] = j < 2 || places > 2 ? scores[g + j] : minus;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    before += other[j] > group;
-                    close += fabsf(other[j] - group) <= 2.0f * near;  // itself among them
+                    before += other[j] > high;
+                    maybe += other[j] >= low;
                 }
             }
             const bool real = mine < a.groups;
-            unsure |= real && close > 1;
-            if (!real || before >= a.top_groups) {
+            // Only whether it is among the best counts; of groups without an expert left there is nothing to choose.
+            bool open = real && before < a.top_groups;
+            const bool cut = open && group > minus && maybe > a.top_groups;
+            if constexpr (LANES < kCandidates) {
+                unsure |= cut;
+            } else if (__ballot(cut) != 0) {
+                open = exact_open<LANES>(a, p, row, largest_logit);
+            }
+            if (!open) {
 #pragma unroll
                 for (int i = 0; i < V; ++i) key[i] = 0u;
             }
@@ -297,8 +371,13 @@ __device__ __forceinline__ bool choose_fast(const ScoreArgs& a, const Place& p, 
     const uint32_t lane = threadIdx.x & 63;
     const uint64_t segment = (LANES == 64 ? ~0ull : ((1ull << (LANES & 63)) - 1)) << (lane / LANES * LANES);
     const uint64_t lower = segment & ((1ull << lane) - 1);
+    if (!has_bias) near = 0.0f;  // keys are the logits themselves
     float previous = __builtin_inff();
-    for (int k = 0; k < a.topk; ++k) {
+    bool close = false;
+    // (Unrolled: after k + 1 choices at most kMaxTopk - k + 1 of a lane's keys are still looked at.)
+#pragma unroll
+    for (int k = 0; k < kMaxTopk; ++k) {
+        if (k == a.topk) break;
         const uint32_t top = lanes_max<LANES>(key[0]);
         const uint64_t with = __ballot(key[0] == top);
         // The lowest lane that has it.
@@ -307,27 +386,75 @@ __device__ __forceinline__ bool choose_fast(const ScoreArgs& a, const Place& p, 
         if (owner) {
             picked[k] = place[0];
 #pragma unroll
-            for (int i = 0; i + 1 < V; ++i) {
-                key[i] = key[i + 1];
-                place[i] = place[i + 1];
+            for (int i = 0; i < V && i <= kMaxTopk - k; ++i) {
+                key[i] = i + 1 < V ? key[i + 1] : 0u;
+                place[i] = i + 1 < V ? place[i + 1] : 0;
             }
-            key[V - 1] = 0u;
         }
-        // Neighbours in the order that are too near (equal ones included), no expert left, or no numbers.
         const float value = unordered(top);
-        unsure |= !(previous - value > near) || top == 0u;
+        close |= !(previous - value > near);  // neighbours in the order, equal ones included
+        unsure |= top == 0u;                  // no expert left
         previous = value;
     }
-    // The first one left out.
-    const uint32_t next = lanes_max<LANES>(key[0]);
-    return unsure || (next != 0u && !(previous - unordered(next) > near));
+    // Those left out that are as near to the last one chosen.
+    auto next_near = [&](uint32_t next) { return next != 0u && !(previous - unordered(next) > near); };
+    uint32_t next = lanes_max<LANES>(key[0]);
+    close |= next_near(next);
+    if constexpr (LANES < kCandidates) {
+        return unsure || close;
+    } else {
+        bool part = close && (__ballot(unsure) & segment) == 0;  // of the token's lanes alike
+        if (__ballot(part) == 0) return unsure;
+        constexpr uint32_t kUnknown = ~0u;  // a second key of the lane's behind its last choice: not kept
+        int count = a.topk;
+        for (bool more = part;;) {
+            more = more && next_near(next);
+            if (more && (next == kUnknown || count == kCandidates)) {
+                unsure = true;
+                more = part = false;
+            }
+            const uint64_t with = __ballot(more && key[0] == next);
+            if (with == 0) break;
+            if (more && key[0] == next && (with & lower) == 0) {
+                picked[count] = place[0];
+                key[0] = key[1];
+                place[0] = place[1];
+                key[1] = kUnknown;
+            }
+            count += more;
+            next = lanes_max<LANES>(key[0]);
+        }
+        const double total = has_bias ? exact_total<LANES>(a, p, row, largest_logit) : 1.0;
+        wave_fence();
+        part = part && p.lane < count;
+        int id = 0, rank = 0;
+        double mine = 0.0;
+        if (part) {
+            id = picked[p.lane];
+            mine = has_bias ? exact_key(a, row, id, largest_logit, total) : static_cast<double>(row[id]);
+            exact[p.lane] = mine;
+        }
+        wave_fence();
+        for (int c = 0; c < kCandidates; c += 4) {
+#pragma unroll
+            for (int j = c; j < c + 4; ++j) {
+                const double other = exact[j];
+                rank += j < count && (other > mine || (other == mine && picked[j] < id));
+            }
+        }
+        wave_fence();
+        if (part && rank < a.topk) picked[rank] = id;
+        return unsure;
+    }
 }
 
 template <int LANES, int V>
 __global__ __launch_bounds__(256) void route_scored_kernel(ScoreArgs a) {
     constexpr int TOKENS = 256 / LANES;
     constexpr int GROUPS = LANES < 64 ? LANES : 64;  // a lane each at least
-    __shared__ int picked[TOKENS][kMaxTopk];
+    constexpr int ROOM = LANES < kCandidates ? kMaxTopk : kCandidates;
+    __shared__ int picked[TOKENS][ROOM];
+    __shared__ double exact[TOKENS][LANES < kCandidates ? 1 : kCandidates];
     __shared__ float scores[TOKENS][GROUPS];
     const int lane = threadIdx.x & 63;
     const int slot = threadIdx.x / LANES;  // the token's place in the workgroup: one wave's
@@ -356,7 +483,7 @@ __global__ __launch_bounds__(256) void route_scored_kernel(ScoreArgs a) {
     for (int i = 0; i < V; ++i) number &= l[i] == l[i];
     const uint64_t segment = (LANES == 64 ? ~0ull : ((1ull << (LANES & 63)) - 1)) << (lane / LANES * LANES);
     number = (__ballot(!number) & segment) == 0;
-    const bool unsure = choose_fast<LANES, V>(a, p, l, b, picked[slot], scores[slot]) || !number;
+    const bool unsure = choose_fast<LANES, V>(a, p, row, l, b, picked[slot], scores[slot], exact[slot]) || !number;
     if (__ballot(unsure && live) != 0) {
         int rank[V];
         choose<LANES, V>(a, p, l, b, rank);
@@ -455,9 +582,10 @@ int lanes_of(const ScoreArgs& a, int v) {
 
 int launch_route_scored(const ScoreArgs& a, hipStream_t stream) {
     // Four experts a lane where that fits a wave, else eight or sixteen. Eight as well for large batches of more than
-    // 64 experts, where instructions count and not the length of a lane's chain: two tokens share a wave's
-    // choices. Four against eight, 16384 tokens, top-8: 256 experts in 8 groups (sigmoid, bias) 21.2 and 19.8 us,
-    // 128 experts 7.7 and 6.2; 8192 of 64 in 8 groups 7.7 and 9.7; one token of 256 4.4 and 4.9.
+    // 64 experts, where instructions count and not the length of a lane's chain: more tokens share a wave's
+    // choices. Four against eight, top-8 by sigmoid and bias: 16384 tokens of 256 experts in 8 groups 17.5 and
+    // 14.3 us, of 128 experts 9.4 and 8.4; 8192 of 64 in 8 groups 6.1 and 10.5; one of 256 4.2 and 4.7; 2048 of 128
+    // in 8 groups 4.7 and 6.5.
     const bool large = a.tokens >= 4096 && a.experts > 64 && lanes_of(a, 8) <= kWave;
     if (!large && lanes_of(a, 4) <= kWave)
         by_lanes<4>(a, lanes_of(a, 4), stream);

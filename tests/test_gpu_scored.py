@@ -119,6 +119,55 @@ def test_choices_that_fp32_cannot_tell_apart():
         assert ids.tolist() == [[0, 1, 2, 3]] * 5 and torch.equal(weights, torch.full_like(weights, 0.25))
 
 
+@pytest.mark.parametrize("experts,topk,groups,top_groups", [(64, 8, 1, 1), (256, 8, 8, 4), (256, 6, 1, 1), (512, 8, 16, 4),
+                                                            (160, 6, 8, 3), (510, 5, 2, 1)])
+@pytest.mark.parametrize("scoring,with_bias", [("sigmoid", True), ("softmax", True), ("softmax", False), ("sigmoid", False)])
+def test_clusters_of_near_and_equal_keys(experts, topk, groups, top_groups, scoring, with_bias):
+    """Two to forty keys within an fp32 rounding or equal, above, across and below the last choice, spread over the
+    experts or side by side."""
+    g = torch.Generator(device="cuda").manual_seed(experts + topk)
+    logits = torch.randn(600, experts, device="cuda", generator=g)
+    for t in range(600):
+        size, at = 2 + t % 39, t % 12
+        row = logits[t]
+        order = torch.argsort(row, descending=True)
+        where = order[at:at + size] if t % 3 else (torch.arange(size, device="cuda") + t) % experts
+        value = row[order[at]]
+        step = torch.arange(size, device="cuda") * (0.0 if t % 2 else 1.2e-7) * value.abs()
+        row[where] = value + step
+    bias = torch.full((experts,), 0.25, device="cuda") if with_bias else None
+    options = dict(scoring=scoring, bias=bias, groups=groups, top_groups=top_groups)
+    ids, weights = route_scored(logits, topk, **options)
+    want_ids, want = _reference(logits, topk, **options)
+    assert torch.equal(ids, want_ids)
+    _weights_near(weights, want, logits, options)
+
+
+@pytest.mark.parametrize("experts,groups,top_groups", [(256, 8, 4), (160, 8, 3), (510, 34, 5), (512, 16, 4), (64, 4, 2)])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_groups_that_are_near_or_equal_at_the_cut(experts, groups, top_groups, scoring):
+    """The last group in and the first one out hold the same logits, in another order, or one that is an ulp more."""
+    g = torch.Generator(device="cuda").manual_seed(groups)
+    size = experts // groups
+    logits = torch.randn(300, experts, device="cuda", generator=g)
+    for best in (1, 2):
+        options = dict(scoring=scoring, bias=None, groups=groups, top_groups=top_groups, group_best=best)
+        inside = logits.view(300, groups, size)
+        order = torch.argsort(torch.sort(inside, -1, descending=True).values[..., :best].exp().sum(-1), -1, descending=True)
+        tokens = torch.arange(300, device="cuda")
+        last, out = order[:, top_groups - 1], order[:, top_groups]
+        near = inside.clone()
+        near[tokens, out] = inside[tokens, last].flip(-1)
+        top = near[tokens, out].argmax(-1)
+        more = near[tokens, out, top]
+        near[tokens[::2], out[::2], top[::2]] = torch.nextafter(more, more + 1)[::2]
+        near = near.view(300, experts)
+        ids, weights = route_scored(near, 6, **options)
+        want_ids, want = _reference(near, 6, **options)
+        assert torch.equal(ids, want_ids), best
+        _weights_near(weights, want, near, options)
+
+
 def test_a_bias_that_drowns_scores():
     """Keys of a bias so large that fp32 keys would lose the scores' differences."""
     logits = _logits(400, 64, 2)
