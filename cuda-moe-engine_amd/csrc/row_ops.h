@@ -9,7 +9,7 @@
 namespace moe {
 
 constexpr int64_t kMaxNormWidth = 16384;      // a row stays in a workgroup's registers
-constexpr int64_t kMaxQuantizeWidth = 32768;
+constexpr int64_t kMaxQuantizeWidth = 32768;  // without a weight's registers
 constexpr int64_t kMaxLayerTokens = 1 << 21;  // grids of up to 1024 threads a token stay below 2^32
 constexpr int kMaxScoredExperts = 512;        // sixteen scores a lane, one wave
 constexpr float kE4m3Most = 448.0f;           // largest finite e4m3 value
@@ -149,8 +149,7 @@ __device__ __forceinline__ void load_row(const typename Elem<DT>::T* row, int at
 }
 
 template <int DT, int N>
-__device__ __forceinline__ void store_row(typename Elem<DT>::T* row, int at, int n, const float (&in)[N],
-                                          bool stream = false) {
+__device__ __forceinline__ void store_row(typename Elem<DT>::T* row, int at, int n, const float (&in)[N]) {
     using T = typename Elem<DT>::T;
     constexpr int STEP = N * sizeof(T) > 16 ? 16 / sizeof(T) : N;
 #pragma unroll

@@ -1,8 +1,9 @@
 """The training operators as differentiable functions, for ``loss.backward()``.
 
 ``route``, ``dispatch``, ``combine``, ``low_rank_add``, ``rms_norm`` and ``route_scored`` run
-the forward kernels and record the gradients of ``training``, ``adapters``, ``norms`` and ``scored``. Each returns new tensors, so that
-several layers and micro-batches may be in flight; none keeps a buffer for the next call.
+the forward kernels and record the gradients of ``training``, ``adapters``, ``norms`` and
+``scored``. Each returns new tensors, so that several layers and micro-batches may be in
+flight; none keeps a buffer for the next call.
 Gradients are first order (a second differentiation raises).
 
 They are eager: under graph capture they raise, since a backward pass recorded beside a

@@ -3,8 +3,8 @@
 ``MoEBlock`` and ``autograd.route`` choose by the logits and weigh by the softmax of the
 chosen ones. ``route_scored`` is for the other routers of mixture models: it takes logits
 (``router_fused_out``'s, or any other product's, of up to 512 experts), and its ids and
-weights go to ``dispatch`` and ``combine`` like theirs; ``route_scored_backward`` gives the
-logits' gradient. No counterpart in the reference.
+weights go to ``dispatch`` and ``combine`` like theirs (which take up to 64 experts);
+``route_scored_backward`` gives the logits' gradient. No counterpart in the reference.
 
 Checks, streams and errors are those of ``moe_dispatch.training``.
 """

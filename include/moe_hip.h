@@ -664,8 +664,8 @@ int moe_route_scored_backward(const moe_route_scored_backward_args* args, void* 
  * scaled by the two). bias [R] is bias_dtype, MOE_DTYPE_F32 or MOE_DTYPE_BF16 (NULL: 0), residual [T, N]
  * bf16 (NULL: 0; it may be output itself), output [T, N] bf16. Sums, bias and activation are
  * fp32; of e4m3 the matrix instruction first adds eight neighbouring products to 2^-13 of the
- * largest, which is far below what 8 bits keep of each operand. Rows are multiples of 16 bytes and 16-byte aligned, N is a multiple of 8. Limits: T <=
- * 2^21, K and N <= 2^20, weight below 4 GiB. scratch: moe_linear_scratch_bytes bytes, for this
+ * largest, which is far below what 8 bits keep of each operand. Rows are multiples of 16 bytes
+ * and 16-byte aligned, N is a multiple of 8. Limits: T <= 2^21, K and N <= 2^20, weight below 4 GiB. scratch: moe_linear_scratch_bytes bytes, for this
  * call alone (NULL when that is 0), 16-byte aligned.
  */
 typedef struct moe_linear_args {
