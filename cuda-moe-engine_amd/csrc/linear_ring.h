@@ -74,9 +74,13 @@ struct DenseShape {
     // stage u + SB are issued in each window.
     static constexpr int VM_STEADY = (SB > SA ? B_LOADS : 0) + (SA - 2) * LOADS;
     static constexpr int VM_FIRST = (SB > SA ? B_LOADS : 0) + (SA - 1) * LOADS;
+    // 16-byte stores of a tile's epilogue, none of them behind a branch: as many operations at least are younger than
+    // the next tile's first loads, which go out before them.
+    static constexpr int STORES = CHAIN ? FA * (SWIGLU ? FB / 2 : FB) / 2 : 0;
     static_assert(A_LOADS >= 1 && B_LOADS >= 1 && FA >= 1 && FB >= 2 && FB % 2 == 0, "tile shape");
     static_assert(SA >= 2 && SB >= SA && SA * A_STAGE + SB * B_STAGE <= LDS, "ring does not fit");
-    static_assert(VM_FIRST < 64, "loads in flight fit the counter");
+    static_assert(VM_FIRST + STORES < 64, "loads in flight fit the counter");
+    static_assert(!CHAIN || FB % 4 == 0, "stores in pairs of blocks");
 };
 
 template <typename S>
@@ -290,11 +294,15 @@ __device__ __forceinline__ uint2 finish4(const float (&z)[4], const float (&up)[
     return make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
 }
 
-// What the epilogue reads: the residual of the lane's rows and columns, and its columns' terms.
+// What the epilogue reads: the scales of the lane's rows, its columns' terms, and the residual (of two rows at a time
+// where tiles are chained). Rows past the end and columns past it (kPastColumns) read as zero through the
+// resource's range.
+constexpr uint32_t kPastColumns = 0xd0000000u;  // past every range, and a row's offset (below 2^29) added to it as well
 template <typename S>
 struct DenseExtra {
     static constexpr int OUT = S::SWIGLU ? S::FB / 2 : S::FB;
-    uint32_t residual[S::FA * OUT * 2];
+    static constexpr int KEPT = S::CHAIN ? 2 : S::FA;
+    uint32_t residual[KEPT * OUT * 2];
     float sx[S::FA];
     float scale[OUT][4], bias[OUT][4], up_scale[S::SWIGLU ? OUT : 1][4], up_bias[S::SWIGLU ? OUT : 1][4];
 
@@ -306,31 +314,47 @@ struct DenseExtra {
             if constexpr (S::SWIGLU) column_terms<S::FP8>(p, p.n + col, up_scale[j], up_bias[j]);
         });
     }
-    // Row fragment i, whose row of x the lane has.
+    __device__ __forceinline__ void load_scales(const LinearArgs& p, const LinearTile& t, int row) {
+        if constexpr (S::FP8) {
+            const auto r = make_rsrc(p.x_scales + t.row0, static_cast<uint32_t>(min<int64_t>(p.tokens - t.row0, S::TM) * 4));
+#pragma unroll
+            for (int i = 0; i < S::FA; ++i)
+                sx[i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, (row + i * 16) * 4, 0, 0));
+        } else {
+#pragma unroll
+            for (int i = 0; i < S::FA; ++i) sx[i] = 1.0f;
+        }
+    }
+    // Row fragment I at byte `at` of the tile's rows, columns from col on.
     template <int I>
-    __device__ __forceinline__ void load_row(const LinearArgs& p, int64_t row, int64_t col0) {
-        const bool ok = row < p.tokens;
-        sx[I] = S::FP8 && ok ? p.x_scales[row] : 1.0f;
+    __device__ __forceinline__ void load_row(const LinearArgs& p, __amdgpu_buffer_rsrc_t r, uint32_t at, int col) {
         static_for<OUT>([&](auto j_c) {
             constexpr int j = decltype(j_c)::value;
-            const int64_t col = col0 + j * 16;
-            uint2 v = make_uint2(0, 0);
-            if (p.residual != nullptr && ok && col < p.n) v = *reinterpret_cast<const uint2*>(p.residual + row * p.n + col);
-            residual[(I * OUT + j) * 2] = v.x;
-            residual[(I * OUT + j) * 2 + 1] = v.y;
+            const uint32_t c = col + j * 16 < p.n ? static_cast<uint32_t>(col + j * 16) * 2 : kPastColumns;
+            const auto v = __builtin_amdgcn_raw_buffer_load_b64(r, at + c, 0, 0);
+            residual[(I % KEPT * OUT + j) * 2] = v[0];
+            residual[(I % KEPT * OUT + j) * 2 + 1] = v[1];
         });
     }
 };
+// A tile's rows of the residual or the output; none where there is no residual.
+template <typename S>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rows(const LinearArgs& p, const LinearTile& t, const uint16_t* of) {
+    const int64_t rows = min<int64_t>(p.tokens - t.row0, S::TM);
+    return make_rsrc(of + t.row0 * p.n, of != nullptr ? static_cast<uint32_t>(rows * p.n * 2) : 0u);
+}
 
 __device__ __forceinline__ void to_vgpr(floatx4& v) { asm volatile("" : "+v"(v)); }
 
 // One tile. Its prologue has been issued (`CHAIN`; else it goes out here, behind the epilogue's operands, whose
-// latency then hides behind the product); `wait_all`: stores of the tile before may be in flight (they share the
-// loads' counter). With `chain` the last windows load the first stages of the next tile (resources
+// latency then hides behind the product); `after`: the stores of the tile before may be in flight (they share the
+// loads' counter, and were issued after these, so that a wait may leave them out: this and a tile's row
+// scales in one load instead of eight, each behind the row's stores before it, took 4096 x 4096 x 28672 e4m3 with SwiGLU from
+// 370 to 355 us in one session). With `chain` the last windows load the first stages of the next tile (resources
 // `next`), otherwise its whole prologue goes out in `hook`, once every wave is done with the ring.
 template <typename S, typename Hook>
 __device__ __forceinline__ void dense_tile(const LinearArgs& p, const LinearPlan& plan, char* lds, const LinearTile& t,
-                                           bool wait_all, int sa0, int sb0, bool chain,
+                                           bool after, int sa0, int sb0, bool chain,
                                            typename DenseLoads<S>::Rsrc next, bool next_ends, int next_steps,
                                            const Hook& hook) {
     constexpr bool FP8 = S::FP8, SWIGLU = S::SWIGLU;
@@ -363,15 +387,18 @@ __device__ __forceinline__ void dense_tile(const LinearArgs& p, const LinearPlan
 
     const int lane_row = lane >> 4;
     const int col4 = 4 * lane_row;
-    const int64_t first_row = t.row0 + wm * S::WTM + (lane & 15);
-    const int64_t first_col = t.col0 + wn * (SWIGLU ? S::WTN / 2 : S::WTN);
+    const int tile_row = wm * S::WTM + (lane & 15);
+    const int first_col = t.col0 + wn * (SWIGLU ? S::WTN / 2 : S::WTN);
+    const uint32_t row_bytes = static_cast<uint32_t>(p.n) * 2;
     DenseExtra<S> extra;
     if constexpr (!S::CHAIN) {
         if (plan.splits == 1) {
             extra.load_columns(p, first_col + col4);
+            extra.load_scales(p, t, tile_row);
+            const auto r = tile_rows<S>(p, t, p.residual);
             static_for<FA>([&](auto i_c) {
                 constexpr int i = decltype(i_c)::value;
-                extra.template load_row<i>(p, first_row + i * 16, first_col + col4);
+                extra.template load_row<i>(p, r, (tile_row + i * 16) * row_bytes, first_col + col4);
             });
         }
         ops.prologue(t.steps, ends, 0, 0, false);
@@ -456,7 +483,10 @@ __device__ __forceinline__ void dense_tile(const LinearArgs& p, const LinearPlan
     using More = std::false_type;
     const Refill none{0, 0, 0, 0, ops.ra, ops.rb, false, false};
     const int steps = t.steps;
-    if (wait_all)
+    const bool stores = S::CHAIN && after && plan.splits == 1;
+    if (stores)
+        wait_vm_lgkm<S::VM_FIRST + S::STORES>();
+    else if (after)
         wait_vm_lgkm<0>();
     else
         wait_vm_lgkm<S::VM_FIRST>();
@@ -475,10 +505,13 @@ __device__ __forceinline__ void dense_tile(const LinearArgs& p, const LinearPlan
         }
     }
     int sa = sa0, sb = sb0;  // slots of the stage whose last half is pending
-    auto window = [&](const Refill& rf, int na, int nb) {
+    auto window = [&](const Refill& rf, int na, int nb, bool behind) {
         const uint32_t a0 = na * S::A_STAGE, b0 = nb * S::B_STAGE;
         fence();
-        wait_vm_lgkm<S::VM_STEADY>();
+        if (behind)
+            wait_vm_lgkm<S::VM_STEADY + S::STORES>();
+        else
+            wait_vm_lgkm<S::VM_STEADY>();
         ring_barrier();
         fence();
         second_half(a0, b0, C0{}, More{}, C0{}, rf);
@@ -494,7 +527,7 @@ __device__ __forceinline__ void dense_tile(const LinearArgs& p, const LinearPlan
     // loop.)
     for (; S::CHAIN && u < steps - SB - 1; ++u) {
         const int na = sa + 1 == SA ? 0 : sa + 1, nb = sb + 1 == SB ? 0 : sb + 1;
-        window(Refill{u + SA, sa, u + SB, sb, ops.ra, ops.rb, false, false}, na, nb);
+        window(Refill{u + SA, sa, u + SB, sb, ops.ra, ops.rb, false, false}, na, nb, stores && u == 0);
         sa = na;
         sb = nb;
     }
@@ -506,9 +539,16 @@ __device__ __forceinline__ void dense_tile(const LinearArgs& p, const LinearPlan
         window(Refill{kt_a, sa, kt_b, sb, a_next ? next.a : ops.ra, b_next ? next.b : ops.rb,
                       a_next ? next_ends && kt_a == next_steps - 1 : ends && kt_a == steps - 1,
                       b_next ? next_ends && kt_b == next_steps - 1 : ends && kt_b == steps - 1},
-               na, nb);
+               na, nb, stores && u == 0);
         sa = na;
         sb = nb;
+    }
+    if constexpr (S::CHAIN) {
+        if (plan.splits == 1) {
+            extra.load_columns(p, first_col + col4);
+            extra.load_scales(p, t, tile_row);
+        }
+        fence();
     }
     second_half(0u, 0u, C0{}, std::true_type{}, NoLoads{}, none);
     // Also without a next tile: no load may land in this LDS once the workgroup has ended.
@@ -526,29 +566,30 @@ __device__ __forceinline__ void dense_tile(const LinearArgs& p, const LinearPlan
         // Partial sums of weight rows, as they are.
         static_for<FA>([&](auto i_c) {
             constexpr int i = decltype(i_c)::value;
-            const int64_t row = first_row + i * 16;
+            const int64_t row = t.row0 + tile_row + i * 16;
             float* to = plan.partial + (t.split * p.tokens + row) * p.rows;
             static_for<FB>([&](auto j_c) {
                 constexpr int j = decltype(j_c)::value;
                 to_vgpr(acc[i][j]);
                 constexpr bool up = SWIGLU && j >= OUT;
-                const int64_t col = first_col + (up ? j - OUT : j) * 16 + col4;
+                const int col = first_col + (up ? j - OUT : j) * 16 + col4;
                 if (row < p.tokens && col < p.n) *reinterpret_cast<floatx4*>(to + (up ? p.n : 0) + col) = acc[i][j];
             });
         });
         return;
     }
-    if constexpr (S::CHAIN) extra.load_columns(p, first_col + col4);
+    const auto out_rows = tile_rows<S>(p, t, p.output), residual_rows = tile_rows<S>(p, t, p.residual);
     auto finish = [&](auto act_c, auto plain_c) {
         constexpr int ACT = decltype(act_c)::value;
         constexpr bool PLAIN = decltype(plain_c)::value;
+        if constexpr (S::CHAIN && !PLAIN) extra.template load_row<0>(p, residual_rows, tile_row * row_bytes, first_col + col4);
         static_for<FA>([&](auto i_c) {
             constexpr int i = decltype(i_c)::value;
             static_for<FB>([&](auto j_c) { to_vgpr(acc[i][decltype(j_c)::value]); });
-            const int64_t row = first_row + i * 16;
-            const bool row_ok = row < p.tokens;
-            const int64_t at = (row_ok ? row : t.row0) * p.n;
-            if constexpr (S::CHAIN) extra.template load_row<i>(p, row, first_col + col4);
+            const uint32_t at = (tile_row + i * 16) * row_bytes;
+            // The next row's residual is in flight while this one is worked out.
+            if constexpr (S::CHAIN && !PLAIN && i + 1 < FA)
+                extra.template load_row<i + 1>(p, residual_rows, at + 16 * row_bytes, first_col + col4);
             uint2 out[OUT];
             static_for<OUT>([&](auto j_c) {
                 constexpr int j = decltype(j_c)::value;
@@ -559,22 +600,27 @@ __device__ __forceinline__ void dense_tile(const LinearArgs& p, const LinearPlan
                     z[r] = acc[i][j][r];
                     v[r] = acc[i][up][r];
                 }
+                const uint32_t* kept = extra.residual + (i % DenseExtra<S>::KEPT * OUT + j) * 2;
                 out[j] = finish4<FP8, ACT, PLAIN>(z, v, extra.sx[i], extra.scale[j], extra.bias[j], extra.up_scale[ju],
-                                              extra.up_bias[ju],
-                                              make_uint2(extra.residual[(i * OUT + j) * 2], extra.residual[(i * OUT + j) * 2 + 1]));
+                                                  extra.up_bias[ju], PLAIN ? make_uint2(0, 0) : make_uint2(kept[0], kept[1]));
             });
             // Lanes 16 apart trade halves of two neighbouring blocks: 16-byte stores of 8 columns.
             static_for<OUT / 2>([&](auto h_c) {
                 constexpr int j = 2 * decltype(h_c)::value;
                 const auto s0 = __builtin_amdgcn_permlane16_swap(out[j].x, out[j + 1].x, false, false);
                 const auto s1 = __builtin_amdgcn_permlane16_swap(out[j].y, out[j + 1].y, false, false);
-                const int64_t col = first_col + j * 16 + col8;
-                if (row_ok && col < p.n)
-                    *reinterpret_cast<uint4*>(p.output + at + col) = make_uint4(s0[0], s1[0], s0[1], s1[1]);
+                const int col = first_col + j * 16 + col8;
+                const uint32_t c = col < p.n ? static_cast<uint32_t>(col) * 2 : kPastColumns;
+                const intx4 v = {static_cast<int>(s0[0]), static_cast<int>(s1[0]), static_cast<int>(s0[1]),
+                                 static_cast<int>(s1[1])};
+                __builtin_amdgcn_raw_buffer_store_b128(v, out_rows, at + c, 0, 0);
             });
             if constexpr (OUT % 2 == 1) {
-                const int64_t col = first_col + (OUT - 1) * 16 + col4;
-                if (row_ok && col < p.n) *reinterpret_cast<uint2*>(p.output + at + col) = out[OUT - 1];
+                const int col = first_col + (OUT - 1) * 16 + col4;
+                const uint32_t c = col < p.n ? static_cast<uint32_t>(col) * 2 : kPastColumns;
+                typedef int intx2 __attribute__((ext_vector_type(2)));
+                const intx2 v = {static_cast<int>(out[OUT - 1].x), static_cast<int>(out[OUT - 1].y)};
+                __builtin_amdgcn_raw_buffer_store_b64(v, out_rows, at + c, 0, 0);
             }
         });
     };
