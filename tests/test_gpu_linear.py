@@ -117,6 +117,18 @@ def test_larger_products(tokens, hidden, width, activation, eight):
     _check(linear(x, w, b, activation=activation, residual=r), x, w, b, r, activation, "larger")
 
 
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("hidden", [112, 208, 336, 544, 1040])
+@pytest.mark.parametrize("activation,extras", [(None, False), (None, True), ("gelu", True), ("swiglu", False), ("swiglu", True)])
+def test_rounds_of_chained_tiles(hidden, eight, activation, extras):
+    """More of the largest tiles than CUs, of one stage to seventeen: stores of one tile beside loads of the next."""
+    x, w, b, r = _case(4200, hidden, 5000, eight, activation, torch.float32 if extras else None, extras, seed=hidden)
+    first = linear(x, w, b, activation=activation, residual=r)
+    _check(first, x, w, b, r, activation, (hidden, activation, extras))
+    for _ in range(3):
+        assert torch.equal(linear(x, w, b, activation=activation, residual=r), first)
+
+
 def test_no_rows():
     x, w, _, _ = _case(0, 64, 16, False)
     assert linear(x, w).shape == (0, 16)
@@ -263,6 +275,25 @@ def test_graph_replays_and_streams_share_nothing():
         torch.cuda.synchronize()
         for got in (*outs, eager):
             assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("tokens", [3, 20, 260, 700])
+def test_widest_output_and_longest_rows(tokens, eight):
+    """2^20 columns (a tile's rows span half a GiB) and 2^20 deep."""
+    x, w, b, r = _case(tokens, 16, 2**20, eight, bias=torch.float32, residual=True)
+    around = torch.full((tokens + 1, 2**20), 7.0, device="cuda", dtype=torch.bfloat16)
+    got = linear(x, w, b, residual=r, output=around[:tokens])
+    for part in (slice(0, 512), slice(2**19 - 256, 2**19 + 256), slice(2**20 - 512, 2**20)):
+        few = QuantizedRows(w.values[part], w.scales[part]) if eight else w[part]
+        _check(got[:, part], x, few, b[part], r[:, part], None, (tokens, part))
+    assert bool((around[tokens] == 7).all())
+    del around, got, r
+    x, w, _, _ = _case(tokens, 2**20, 8, False)
+    if eight:  # (longer than quantize_rows takes)
+        x, w = (QuantizedRows((t.float() * s).to(torch.float8_e4m3fn), torch.full((len(t),), 1 / s, device="cuda"))
+                for t, s in ((x, 64.0), (w, 2.0**16)))
+    _check(linear(x, w), x, w, None, None, None, (tokens, "deep"))
 
 
 def test_weights_past_two_gib():
