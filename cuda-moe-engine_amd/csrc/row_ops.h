@@ -215,6 +215,8 @@ struct ScoreArgs {
     bool sigmoid;
     bool renormalize;
     float scale;
+    int group_size;  // set by the launcher: experts of a group,
+    int lane_shift;  // log2 of its lanes
 };
 
 struct ScoreGradArgs {

@@ -39,7 +39,8 @@ struct Place {
     int first;   // the lane's first expert
     int count;   // its experts (0: none)
     int lane;    // lane of the token's segment
-    int group_lanes;
+    int group;   // its group, past the last one without experts
+    int group_lanes;  // a power of two
 };
 
 // Chooses the token's experts in 64 bits, ties to the lower index: rank[i] = the slot
@@ -97,11 +98,11 @@ __device__ __forceinline__ void choose(const ScoreArgs& a, const Place& p, const
         double group = first;
         if (a.group_best == 2 && second > -__builtin_inf()) group += second;
         // Its place among the groups, ties to the lower one; lanes without a group are last.
-        const int mine = p.lane / p.group_lanes;
+        const int mine = p.group;
         const bool real = mine < a.groups;
         int before = 0;
-        for (int o = 1; o < LANES / p.group_lanes; ++o) {
-            const double other = lane_xor(group, o * p.group_lanes);
+        for (int o = 1; o << a.lane_shift < LANES; ++o) {
+            const double other = lane_xor(group, o << a.lane_shift);
             const int index = mine ^ o;
             if (index < a.groups && (other > group || (other == group && index < mine))) ++before;
         }
@@ -257,12 +258,12 @@ __device__ __forceinline__ bool exact_open(const ScoreArgs& a, const Place& p, c
         first = most(first, f);
     }
     const double group = a.group_best == 2 && second > minus ? first + second : first;
-    const int mine = p.lane / p.group_lanes;
+    const int mine = p.group;
     int before = 0;
 #pragma unroll 1
     for (int o = p.group_lanes; o < LANES; o += p.group_lanes) {
         const double other = lane_xor(group, o);
-        const int index = (p.lane ^ o) / p.group_lanes;
+        const int index = (p.lane ^ o) >> a.lane_shift;
         before += index < a.groups && (other > group || (other == group && index < mine));
     }
     return mine < a.groups && before < a.top_groups;
@@ -329,16 +330,16 @@ __device__ __forceinline__ bool choose_fast(const ScoreArgs& a, const Place& p, 
         if (a.groups > 1) {
             best_two<LANES>(first, second, p.group_lanes);
             const float group = a.group_best == 2 && second > minus ? first + second : first;
-            const int mine = p.lane / p.group_lanes;
+            const int mine = p.group;
             // Lanes past the last group bring -inf, which is before and close to none.
-            if (p.lane % p.group_lanes == 0) scores[mine] = group;
+            if ((p.lane & (p.group_lanes - 1)) == 0) scores[mine] = group;
             wave_fence();
             // Groups that are certainly before this one, and those that may be (itself among them). The two sums
             // here and a group's own are three more roundings of up to twice the largest key: 2.25 near, of which 2
             // are the keys' own.
             const float low = group - 2.25f * near, high = group + 2.25f * near;
             int before = 0, maybe = 0;
-            const int places = LANES / p.group_lanes;  // a power of two
+            const int places = LANES >> a.lane_shift;
             for (int g = 0; g < places; g += 4) {
                 float other[4];
 #pragma unroll
@@ -461,12 +462,11 @@ __global__ __launch_bounds__(256) void route_scored_kernel(ScoreArgs a) {
     const int64_t token = static_cast<int64_t>(blockIdx.x) * TOKENS + slot;
     Place p;
     p.lane = lane % LANES;
-    const int size = a.experts / a.groups;
-    const int per = (size + V - 1) / V;
-    p.group_lanes = per <= 1 ? 1 : 1 << (32 - __builtin_clz(per - 1));
-    const int group = p.lane / p.group_lanes, part = p.lane % p.group_lanes;
-    p.first = group * size + part * V;
-    p.count = group < a.groups ? max(0, min(V, size - part * V)) : 0;
+    p.group_lanes = 1 << a.lane_shift;
+    p.group = p.lane >> a.lane_shift;
+    const int part = p.lane & (p.group_lanes - 1);
+    p.first = p.group * a.group_size + part * V;
+    p.count = p.group < a.groups ? max(0, min(V, a.group_size - part * V)) : 0;
     const bool live = token < a.tokens;
     if (!live) p.count = 0;  // these lanes take part in the reductions only
     float l[V], b[V];
@@ -548,7 +548,11 @@ __global__ __launch_bounds__(256) void route_scored_kernel(ScoreArgs a) {
 }
 
 template <int LANES, int V>
-void run(const ScoreArgs& a, hipStream_t stream) {
+void run(ScoreArgs a, hipStream_t stream) {
+    // (Divisions are the host's.)
+    a.group_size = a.experts / a.groups;
+    a.lane_shift = 0;
+    while (V << a.lane_shift < a.group_size) ++a.lane_shift;
     const int64_t threads = a.tokens * LANES;
     route_scored_kernel<LANES, V><<<static_cast<unsigned>((threads + 255) / 256), 256, 0, stream>>>(a);
 }
