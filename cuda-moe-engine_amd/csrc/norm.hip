@@ -381,10 +381,10 @@ __global__ __launch_bounds__(1024) void column_sum_kernel(const float* __restric
     }
     lds[slice][col] = sum;
     __syncthreads();
-    if (slice == 0 && j < n) {
-        for (int s = 1; s < SLICES; ++s) sum += lds[s][col];
-        out[j] = sum;
-    }
+    // Half a wave a column, a lane a slice.
+    const int at = blockIdx.x * 32 + slice;
+    sum = lanes_reduce<SumOp, SLICES>(lds[col][slice]);
+    if (col == 0 && at < n) out[at] = sum;
 }
 
 // Waves a row of the gradient kernel.

@@ -60,12 +60,12 @@ def _check_rows(x, most=MAX_HIDDEN):
     return tokens, hidden
 
 
-def _check_weight(weight, x):
+def _check_weight(weight, x, hidden):
     if weight is None:
         return DTYPE_CODES[x.dtype]
     if weight.dtype is not x.dtype and weight.dtype is not torch.float32:
         raise TypeError(f"weight must be {x.dtype} or float32, got {weight.dtype}")
-    require_tensor(weight, "weight", x.shape[1:], weight.dtype, x.device)
+    require_tensor(weight, "weight", (hidden,), weight.dtype, x.device)
     return DTYPE_CODES[weight.dtype]
 
 
@@ -80,7 +80,7 @@ def rms_norm(x, weight=None, *, residual=None, eps=1e-6, quantize=False, return_
     is fp32).
     """
     tokens, hidden = _check_rows(x)
-    weight_code = _check_weight(weight, x)
+    weight_code = _check_weight(weight, x, hidden)
     if residual is not None:
         require_tensor(residual, "residual", x.shape, x.dtype, x.device)
     if not 0 <= eps < 1e30:
@@ -138,7 +138,7 @@ def rms_norm_backward(grad_output, x, weight, rstd, *, grad_x=None, gradients=(T
     is None and is not computed.
     """
     tokens, hidden = _check_rows(x)
-    weight_code = _check_weight(weight, x)
+    weight_code = _check_weight(weight, x, hidden)
     require_tensor(grad_output, "grad_output", x.shape, x.dtype, x.device)
     require_tensor(rstd, "rstd", (tokens,), torch.float32, x.device)
     if grad_x is not None:
