@@ -8,8 +8,8 @@
 // instructions (linear_ring.h); between them k is split over workgroups, so that every CU has
 // a part, and the partial sums are joined by a second launch with the epilogue.
 //
-// One row of 4096 e4m3 by 2 x 14336 weight rows (SwiGLU) 22.9 us, 5.1 TB/s; 4096 rows of it 352 us, 2734 TFLOP/s;
-// 4096 x 14336 x 4096 bf16 with a residual 335 us, 1437 TFLOP/s (a large library product: 1536 bf16, 3090 e4m3; all
+// One row of 4096 e4m3 by 2 x 14336 weight rows (SwiGLU) 22.9 us, 5.1 TB/s; 4096 rows of it 345 us, 2787 TFLOP/s;
+// 4096 x 14336 x 4096 bf16 with a residual 328 us, 1465 TFLOP/s (a large library product: 1536 bf16, 3090 e4m3; all
 // of these within 5% from one card to another, by its power).
 #include <algorithm>
 
