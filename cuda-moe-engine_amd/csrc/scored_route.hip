@@ -10,10 +10,11 @@
 // its own. A lane sorts its keys once; each choice is then a maximum over the segment of the lanes' first
 // keys, which the owner removes. The choice is by exact value, so that the ids are the definition's and do not
 // depend on how exp rounds: keys are fp32 first, and where the order hangs on a difference within their
-// rounding, or on a tie, the few experts or the groups that it concerns are compared in 64 bits (about one
-// token in a thousand at 256 experts; all of such a token's experts, in straight code, took 16384 of them from
-// 14 to 19 us: a wave that comes last waits for code that is in no cache). A token without K experts, with
-// infinite keys, NaN, or more than kCandidates of like keys is chosen in 64 bits as a whole.
+// rounding, or on a tie, the few experts or the groups that it concerns are compared in 64 bits. That is about one
+// token in a thousand at 256 experts; choosing such a token in 64 bits as a whole made 16384 tokens 19 us instead of
+// 14, since the wave that does it waits for code that is in no cache. Chosen as a whole are tokens without K
+// experts, with infinite keys, NaN, or more than kCandidates like keys, and near ties where a token has
+// fewer lanes than that.
 //
 // Bound by instructions, not bytes: 16384 tokens of 256 experts, top-8 in 4 of 8 groups, are 17.6 MB (3.5 us)
 // and 13.8 us; one token 4.2.

@@ -87,6 +87,8 @@ def linear(x, weight, bias=None, *, activation=None, residual=None, output=None)
         require_tensor(x_scales, "x.scales", (tokens,), torch.float32, device)
         require_tensor(w_scales, "weight.scales", (rows,), torch.float32, device)
     if bias is not None:
+        if not isinstance(bias, torch.Tensor):
+            raise TypeError("bias must be a tensor")
         if bias.dtype not in (torch.float32, torch.bfloat16):
             raise TypeError(f"bias must be float32 or bfloat16, got {bias.dtype}")
         require_tensor(bias, "bias", (rows,), bias.dtype, device)

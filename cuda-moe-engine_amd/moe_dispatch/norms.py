@@ -63,6 +63,8 @@ def _check_rows(x, most=MAX_HIDDEN):
 def _check_weight(weight, x, hidden):
     if weight is None:
         return DTYPE_CODES[x.dtype]
+    if not isinstance(weight, torch.Tensor):
+        raise TypeError("weight must be a tensor")
     if weight.dtype is not x.dtype and weight.dtype is not torch.float32:
         raise TypeError(f"weight must be {x.dtype} or float32, got {weight.dtype}")
     require_tensor(weight, "weight", (hidden,), weight.dtype, x.device)

@@ -252,3 +252,13 @@ def test_overlap_check_takes_no_null_pointers():
     lib = _lib.load_library()
     assert lib.moe_clip_overlap(None, None, None, None, None, 0) == 0
     assert lib.moe_clip_overlap(None, None, None, None, None, 2) == 1  # MOE_ERR_INVALID_ARGUMENT
+
+
+def test_operands_that_are_no_tensors():
+    x = torch.zeros(2, 16, dtype=BF16)
+    for call in (lambda: rms_norm([1.0]), lambda: rms_norm(x, [1.0] * 16), lambda: rms_norm(x, residual=[0.0]),
+                 lambda: linear(x, [[0.0] * 16]), lambda: linear(x, x.new_zeros(8, 16), [0.0] * 8),
+                 lambda: linear(x, x.new_zeros(8, 16), residual=0), lambda: quantize_rows(3), lambda: route_scored([1.0], 1),
+                 lambda: clip_gradients([x, None], 1.0)):
+        with pytest.raises(TypeError, match="tensor"):
+            call()
