@@ -163,8 +163,8 @@ __device__ __forceinline__ void load_some(const float* row, int first, int count
     }
 }
 
-// e^x and 1 / (1 + e^-x) by hardware exp2 and reciprocal. For scores that only order: within 2^-24 |x| for the
-// argument and 2^-23 for each of the two.
+// e^x by hardware exp2: within 1.224 |x| 2^-24 for the argument and 2^-23 of its own, of scores that order (which
+// choose_fast counts), of weights and of gradients alike; 0 below 2^-126.
 __device__ __forceinline__ float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
 
 // A token's lanes are one wave, whose LDS accesses are in order: only the compiler has to keep it.
@@ -288,14 +288,29 @@ __device__ __forceinline__ bool choose_fast(const ScoreArgs& a, const Place& p, 
     }
     if (has_bias || a.groups > 1) {
         float s[V];
-        // A score's roundings: sigmoid 6 of 2^-24 (argument, exp, sum, reciprocal), softmax up to V + 16 (its sum
-        // besides), one more for the bias, of the largest key or bias.
-        float error = 0x1p-21f;
+        // How far the token's keys may be off, in units of u = 2^-24: `reach` from the scores, `weight` times the largest
+        // bias. log2 e's own rounding and the product's put e^x's argument off by 1.224 |x| u (softmax's difference adds
+        // |x| u), exp2 and a reciprocal are within 2 u.
+        //  * sigmoid: s is off by s ((1 - s) (1.224 |l| + 2) + 3) u < s (4.01 + 1.5 L) u, L = max(-l, 0): what the
+        //    argument's rounding does grows with the logit's size while s vanishes. A key adds (s + |b|) u. So two keys
+        //    are off by 2 (s (5.01 + 1.5 L) + |b|), and two sums of two keys, with their roundings and the comparison's,
+        //    by s (26.1 + 6 L) + 10 |b|: below 2 and 4.6 times max(s (8 + 2 L), 8 |b|). s (8 + 2 L) rises with l, so
+        //    the token's largest logit has the most.
+        //  * softmax: V + 5 for the sum's roundings, 11 for its terms (the mean of |x| weighted by e^x is below 4 with up to
+        //    512 terms), 5 for exp, reciprocal and product, and 2.224 |x| e^x < 0.9 of the largest score: (V + 22) of that
+        //    one. With key and sums as above below 2 and 4.6 times (V + 24) max(s, |b|).
+        // Scores below the normal range are 0: off by 2^-126.
+        float reach, weight;
         if (a.sigmoid) {
+            float top = l[0];
 #pragma unroll
-            for (int i = 0; i < V; ++i) s[i] = __builtin_amdgcn_rcpf(1.0f + fast_exp(-l[i]));
+            for (int i = 0; i < V; ++i) {
+                s[i] = __builtin_amdgcn_rcpf(1.0f + fast_exp(-l[i]));
+                top = fmaxf(top, l[i]);
+            }
+            weight = 8.0f;
+            reach = __builtin_amdgcn_rcpf(1.0f + fast_exp(-top)) * (8.0f + 2.0f * fminf(fmaxf(-top, 0.0f), 128.0f));
         } else {
-            error = (V + 20) * 0x1p-24f;
             float top = l[0];
 #pragma unroll
             for (int i = 1; i < V; ++i) top = fmaxf(top, l[i]);
@@ -310,24 +325,25 @@ __device__ __forceinline__ bool choose_fast(const ScoreArgs& a, const Place& p, 
             const float inverse = __builtin_amdgcn_rcpf(lanes_reduce<SumOp, LANES>(total));
 #pragma unroll
             for (int i = 0; i < V; ++i) s[i] *= inverse;
+            weight = V + 24;
+            reach = weight * inverse;
         }
         // Magnitudes as integers: of numbers they order alike, and an infinity's or NaN's are the largest.
-        uint32_t largest = 0;
+        uint32_t drawn = 0;
         float first = minus, second = minus;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             const bool in = l[i] > minus;
             const float k = in ? s[i] + b[i] : minus;
-            const uint32_t size = max(__float_as_uint(k) & 0x7fffffffu, __float_as_uint(b[i]) & 0x7fffffffu);
-            largest = max(largest, in ? size : 0u);
+            drawn = max(drawn, __float_as_uint(b[i]) & 0x7fffffffu);
             second = fmaxf(second, fminf(first, k));
             first = fmaxf(first, k);
             if (has_bias) key[i] = in ? ordered(k) : 0u;
         }
-        largest = lanes_max<LANES>(largest);
-        near = 2.0f * error * __uint_as_float(largest);
+        const uint32_t size = lanes_max<LANES>(max(__float_as_uint(reach), __float_as_uint(weight * __uint_as_float(drawn))));
+        near = 0x1p-23f * __uint_as_float(size) + 0x1p-124f;
         // A key that is no number, infinite, or so large that a sum of two is: the other path sorts that out.
-        unsure = largest >= 0x7e800000u;
+        unsure = size >= 0x7e800000u;
         if (a.groups > 1) {
             best_two<LANES>(first, second, p.group_lanes);
             const float group = a.group_best == 2 && second > minus ? first + second : first;
@@ -335,10 +351,8 @@ __device__ __forceinline__ bool choose_fast(const ScoreArgs& a, const Place& p, 
             // Lanes past the last group bring -inf, which is before and close to none.
             if ((p.lane & (p.group_lanes - 1)) == 0) scores[mine] = group;
             wave_fence();
-            // Groups that are certainly before this one, and those that may be (itself among them). The two sums
-            // here and a group's own are three more roundings of up to twice the largest key: 2.25 near, of which 2
-            // are the keys' own.
-            const float low = group - 2.25f * near, high = group + 2.25f * near;
+            // Groups that are certainly before this one, and those that may be (itself among them).
+            const float low = group - 2.3f * near, high = group + 2.3f * near;
             int before = 0, maybe = 0;
             const int places = LANES >> a.lane_shift;
             for (int g = 0; g < places; g += 4) {

@@ -1,0 +1,66 @@
+"""Scored routing where fp32 scores do not tell which groups or experts are ahead, against 64 bits."""
+
+import pytest
+import torch
+
+from moe_dispatch import route_scored
+from tests._helpers import gpu
+from tests.test_gpu_scored import _reference
+
+pytestmark = gpu
+
+
+def _near_groups(tokens, experts, groups, best, shift, seed):
+    """Logits around `shift` whose groups' best one or two sum to nearly the same: 1e-8 to 1e-5 apart, either way."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    logits = (torch.randn(tokens, experts, device="cuda", generator=g) * 0.5).double()
+    inside = logits.view(tokens, groups, -1)
+
+    def size(group):
+        s = torch.sigmoid(group + shift)
+        return torch.topk(s, min(best, s.shape[-1]), -1).values.sum(-1)
+
+    want = size(inside[:, 0])
+    for j in range(1, groups):
+        apart = 10 ** (-8 + 3 * torch.rand(tokens, device="cuda", generator=g, dtype=torch.float64))
+        apart *= torch.randint(0, 2, (tokens,), device="cuda", generator=g) * 2 - 1
+        for _ in range(3):  # of a sigmoid, by Newton's steps in the logits
+            now = size(inside[:, j])
+            s = torch.sigmoid(inside[:, j] + shift)
+            slope = (1 - torch.topk(s, 1, -1).values[:, 0]).clamp(min=1e-3)
+            inside[:, j] += ((torch.log(want / now) + apart) / slope).unsqueeze(-1)
+    return (logits + shift).float()
+
+
+SHAPES = [(256, 8, 4), (64, 4, 2), (64, 8, 4), (24, 2, 1), (12, 3, 2), (510, 34, 5), (512, 16, 4)]
+
+
+@pytest.mark.parametrize("experts,groups,top_groups", SHAPES)
+@pytest.mark.parametrize("shift", [4.0, 0.0, -4.0, -12.0, -16.0, -24.0, -30.0, -45.0, -60.0, -80.0, -87.0, -88.0, -95.0])
+def test_near_groups_of_sigmoid_scores_at_any_size(experts, groups, top_groups, shift):
+    for best in (1, 2):
+        logits = _near_groups(1500, experts, groups, best, shift, groups + best)
+        middle = float(torch.sigmoid(logits.double()).mean())
+        for bias in (None, 0.0, -0.25, -0.5 * middle, -middle):
+            b = None if bias is None else torch.full((experts,), bias, device="cuda")
+            options = dict(scoring="sigmoid", bias=b, groups=groups, top_groups=top_groups, group_best=best)
+            ids, _ = route_scored(logits, 4, **options)
+            want, _ = _reference(logits, 4, **options)
+            wrong = int((ids != want).any(-1).sum())
+            assert wrong == 0, (best, bias, wrong)
+
+
+@pytest.mark.parametrize("shift", [0.0, -5.0, -16.0, -45.0, -87.5, -100.0])
+@pytest.mark.parametrize("experts", [8, 64, 256, 512])
+def test_near_keys_under_a_bias_that_cancels_scores(experts, shift):
+    """Keys s + b with b near -s, and zero: their order is that of scores whose roundings are those of s."""
+    g = torch.Generator(device="cuda").manual_seed(experts)
+    logits = shift + 1e-6 * abs(shift) * torch.randn(1000, experts, device="cuda", generator=g) + 1e-3 * torch.randn(
+        1000, 1, device="cuda", generator=g)
+    for scoring in ("sigmoid", "softmax"):
+        s = torch.sigmoid(logits.double()) if scoring == "sigmoid" else torch.softmax(logits.double(), -1)
+        for part in (0.0, -0.5, -1.0):
+            bias = (part * s.mean(0)).float()
+            options = dict(scoring=scoring, bias=bias)
+            want, _ = _reference(logits, 6, **options)
+            assert torch.equal(route_scored(logits, 6, **options)[0], want), (scoring, part)
