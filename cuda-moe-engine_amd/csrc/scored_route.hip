@@ -63,7 +63,10 @@ __device__ __forceinline__ void choose(const ScoreArgs& a, const Place& p, const
             double total = 0;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                score[i] = l[i] == -__builtin_inff() ? 0.0 : exp(static_cast<double>(l[i]) - top);
+                // NaN is out as -inf is and has no part in the others' scores. Logits of +inf (each equal to `top`, where a
+                // difference would be NaN) share the whole sum.
+                const double x = static_cast<double>(l[i]);
+                score[i] = !(l[i] > -__builtin_inff()) ? 0.0 : x == top ? 1.0 : exp(x - top);
                 total += score[i];
             }
 #pragma unroll

@@ -63,8 +63,8 @@ def route_scored(logits, topk, *, scoring="softmax", bias=None, groups=1, top_gr
     * weights are ``scale * s``, with ``renormalize`` divided by the sum of the chosen s.
 
     A logit of -inf takes an expert out: it is chosen, with weight 0, only where the token's
-    groups have nothing else left. A NaN logit is out too and makes its token's weights NaN, as
-    +inf does under softmax.
+    groups have nothing else left. A NaN logit is out too and makes its token's weights NaN. So does
+    +inf under softmax, where in the choice the experts with +inf have equal scores and the others 0.
     """
     tokens, experts = _check_logits(logits, topk, scoring)
     _check_choice(experts, topk, groups, top_groups, group_best)

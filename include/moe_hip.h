@@ -606,8 +606,8 @@ int moe_rms_norm_backward(const void* grad_output, const void* x, int dtype, con
  * how fp32 rounds a score (values that are nearer than 64 bits tell apart count as ties).
  * A logit of -inf takes an expert out: it counts in no group's score and is chosen, with
  * weight 0, only when its groups have nothing else left, lowest index first. A NaN logit is
- * out as well and makes the token's weights NaN; so does +inf under softmax. ids are always K
- * different experts. Limits: 1 <= E <= 512, 1 <= K <= 8, K <= top_groups * E / groups,
+ * out as well, and makes the token's weights NaN. So does +inf under softmax, where in the
+ * choice the experts with +inf have equal scores and the others 0. ids are always K different experts. Limits: 1 <= E <= 512, 1 <= K <= 8, K <= top_groups * E / groups,
  * groups <= 64, T <= 2^21.
  */
 typedef struct moe_route_scored_args {

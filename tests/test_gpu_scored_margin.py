@@ -64,3 +64,30 @@ def test_near_keys_under_a_bias_that_cancels_scores(experts, shift):
             options = dict(scoring=scoring, bias=bias)
             want, _ = _reference(logits, 6, **options)
             assert torch.equal(route_scored(logits, 6, **options)[0], want), (scoring, part)
+
+
+@pytest.mark.parametrize("experts,groups,top_groups", [(64, 1, 1), (64, 8, 4), (12, 3, 2), (256, 8, 4), (510, 34, 5)])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("with_bias", [True, False])
+def test_values_that_are_no_numbers_leave_the_others_their_order(experts, groups, top_groups, scoring, with_bias):
+    """NaN is out: the choice is that of the row with -inf in its place. +inf outweighs the rest: of the row with a
+    logit so large that all others' scores are 0 beside it (sigmoid: 1)."""
+    g = torch.Generator(device="cuda").manual_seed(experts)
+    logits = torch.randn(60, experts, device="cuda", generator=g)
+    bias = 0.01 * torch.randn(experts, device="cuda", generator=g) if with_bias else None
+    for best in (1, 2):
+        options = dict(scoring=scoring, bias=bias, groups=groups, top_groups=top_groups, group_best=best)
+        clean, _ = route_scored(logits, 4, **options)
+        rows = torch.arange(60, device="cuda")
+        for place in ("first", "chosen", "last", "several"):
+            where = torch.zeros(60, experts, dtype=torch.bool, device="cuda")
+            if place == "chosen":
+                where[rows, clean[:, 1].long()] = True
+            else:
+                where[:, {"first": [0], "last": [experts - 1], "several": [0, 1, 2, experts // 2]}[place]] = True
+            for value, stand_in in ((float("nan"), float("-inf")), (float("inf"), 2e4)):
+                ids, weights = route_scored(logits.masked_fill(where, value), 4, **options)
+                want, _ = _reference(logits.masked_fill(where, stand_in), 4, **options)
+                assert torch.equal(ids, want), (best, place, value)
+                if value != value:
+                    assert torch.isnan(weights).all()
