@@ -1,9 +1,11 @@
 """Values of the operators around the experts where a rounding or a range decides them."""
 
+import math
+
 import pytest
 import torch
 
-from moe_dispatch import quantize_rows, rms_norm
+from moe_dispatch import clip_gradients, quantize_rows, rms_norm
 from tests._helpers import gpu
 
 pytestmark = gpu
@@ -37,3 +39,25 @@ def test_eight_bit_rows_are_the_quotients(tokens, hidden, dtype):
         weight = 1 + 0.2 * torch.randn(hidden, device="cuda", generator=g)
         x = x.float()
         _same_rows(rms_norm(x, weight, quantize=True).output, rms_norm(x, weight).output)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("value,most", [(1e30, 1e-12), (1e36, 1e-6), (3e38, 1.0), (2e38, 0.5), (1e38, 1e-7), (1e30, 1e3), (1e20, 1e-30)])
+def test_clip_factors_below_the_normal_range_of_fp32(value, most, dtype):
+    """Large gradients and a small norm to reach, and norms past fp32 (written as infinite, the values scaled all the
+    same): a factor within half a step of fp32's normal numbers, whatever its size."""
+    grads = [torch.full((1000,), value, device="cuda", dtype=dtype), torch.full((333,), -value / 3, device="cuda", dtype=dtype)]
+    kept = [t.double() for t in grads]
+    exact = math.sqrt(math.fsum(float(t.square().sum()) for t in kept))
+    outputs = [torch.empty_like(t) for t in grads]
+    norm = clip_gradients(grads, most, outputs=outputs)
+    assert float(norm) == (pytest.approx(exact, rel=1e-6) if exact < 3.4e38 else math.inf)
+    for got, g in zip(outputs, kept):
+        y = g * (most / (exact + 1e-6))
+        half = torch.finfo(dtype).eps / 2
+        # The factor and the product in fp32, half a step of a narrower type, and a step of the subnormals.
+        steps = (half * 1.001 if dtype is not torch.float32 else 0.0) + 2.01 * 2.0**-24
+        off = (got.double() - y).abs() - (y.abs() * steps + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps)
+        assert float(off.max()) <= 0, float(((got.double() - y) / y).abs().max())
+    clip_gradients(grads, most)
+    assert all(torch.equal(a, b) for a, b in zip(grads, outputs))
