@@ -66,8 +66,10 @@ def clip_gradients(grads, max_norm, *, outputs=None):
     ``grads`` is a list of contiguous fp32, fp16 or bf16 tensors of any shapes on one GPU, no
     two of which share memory; with ``outputs`` (a tensor of the same type and size for each, the
     gradient itself or apart from all others) they are read only and the results go there. Sums are 64
-    bits, in an order that the sizes fix; a result is rounded once. A norm that is infinite
-    or NaN leaves the values as they are, so that a program can look at the norm and skip the step.
+    bits, in an order that the sizes fix; the factor and its products are fp32, rounded once to a
+    narrower type. Gradients that hold an infinity or NaN stay as they are, so that a program can
+    look at the norm and skip the step. The norm of finite gradients may pass fp32 (3.4e38): it is
+    returned as infinite, and the values are scaled by what it is.
     """
     grads = list(grads)
     if not grads:

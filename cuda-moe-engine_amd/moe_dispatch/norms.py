@@ -77,9 +77,11 @@ def rms_norm(x, weight=None, *, residual=None, eps=1e-6, quantize=False, return_
     x [T, H] is fp32, fp16 or bf16, weight [H] of x's type or fp32 (None: 1), residual [T, H]
     of x's type (None: 0). Statistics and products are fp32, from the unrounded sum; ``output``
     is rounded once to x's type, or with ``quantize`` to e4m3 with
-    ``scales[t] = max(max_j |y_tj|, 2^-100) / 448``. A NaN stays one; a row that holds an
-    infinity has no finite scale. H is at most 16384, and values are below 1e17 (their squares' sum
-    is fp32).
+    ``scales[t] = max(max_j |y_tj|, 2^-100) / 448``. A NaN makes its whole row NaN (with
+    ``quantize`` the scale is then the least one). An infinity makes rstd 0: its own y is NaN, the
+    row's others 0, and the scale the least one as well. H is at most 16384, and values are below 1e17 (their
+    squares' sum is fp32); with an eps below 1e-30 a row's largest value is above 1e-16, or all of it 0
+    (of ``eps=0`` y is NaN there).
     """
     tokens, hidden = _check_rows(x)
     weight_code = _check_weight(weight, x, hidden)
@@ -111,7 +113,11 @@ def rms_norm(x, weight=None, *, residual=None, eps=1e-6, quantize=False, return_
 
 
 def quantize_rows(x):
-    """Rows x [T, H] (fp32, fp16 or bf16, H up to 32768) as ``QuantizedRows``, with ``rms_norm``'s scales."""
+    """Rows x [T, H] (fp32, fp16 or bf16, H up to 32768) as ``QuantizedRows``, with ``rms_norm``'s scales.
+
+    A NaN stays one and has no part in the scale; a row that holds an infinity has an infinite scale,
+    and all of it stands for NaN.
+    """
     tokens, hidden = _check_rows(x, MAX_QUANTIZED)
     require_gpu(x)
     refuse_autograd(x)

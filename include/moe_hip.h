@@ -553,8 +553,10 @@ int moe_low_rank_backward(const void* grad_output, const void* x, const void* do
  * MOE_DTYPE_F32 (NULL: 1). scales NULL: output = round(y) in dtype (it may be x or residual
  * itself). scales fp32 [T]: output is e4m3 (OCP, one byte),
  *   scales[t] = max(max_j |y_j|, 2^-100) / 448,  output = round_e4m3(y / scales[t]).
- * A NaN stays NaN; an infinite y makes its row's scale infinite, so that nothing finite stands
- * for it. The squares' sum is fp32: rows keep it finite (values below 1e17 do). Limits: 1 <= H <= 16384, T <= 2^21, eps >= 0.
+ * A NaN stays NaN and has no part in its row's scale; an infinite y makes the scale infinite, so that
+ * nothing finite stands for it. An infinite h makes rstd 0: y is NaN there and 0 elsewhere, of the least
+ * scale in 8 bits. The squares' sum is fp32: rows keep it finite (values below 1e17 do), and with an
+ * eps below 1e-30 in the normal range (a row's largest value above 1e-16, or all of it 0). Limits: 1 <= H <= 16384, T <= 2^21, eps >= 0.
  */
 typedef struct moe_rms_norm_args {
     int64_t struct_bytes;
@@ -586,8 +588,8 @@ int64_t moe_rms_norm_backward_scratch_bytes(int64_t tokens, int64_t hidden, int 
  * Gradients of y = x * rstd * weight, x the normed rows (total, with a residual), rstd as
  * moe_rms_norm wrote it: with u = x * rstd and g = grad_output,
  *   grad_x = round(grad_x_base + rstd * (g * weight - u * mean_j(g_j weight_j u_j)))  (base NULL: 0, or grad_x)
- *   grad_weight = sum_t g * u  (fp32 [H], in a fixed order; 0 for no rows)
- * Either may be NULL; scratch is needed for grad_weight. grad_x may be grad_output or x itself.
+ *   grad_weight = sum_t g * u  (fp32 [H], in a fixed order)
+ * Either may be NULL; scratch is needed for grad_weight. grad_x may be grad_output or x itself. T >= 1.
  */
 int moe_rms_norm_backward(const void* grad_output, const void* x, int dtype, const void* weight, int weight_dtype,
                           const float* rstd, const void* grad_x_base, void* grad_x, float* grad_weight, void* scratch,
@@ -701,8 +703,10 @@ int64_t moe_clip_scratch_bytes(void);
  * grads, outputs, elements and dtypes (MOE_DTYPE_*) are host arrays of `tensors` entries, read
  * before the call returns; tensors are contiguous, aligned to their element, and outputs[i]
  * is grads[i] (in place) or of its type and overlaps nothing else. Sums are 64 bits, in an
- * order that the sizes fix. A norm that is infinite or NaN leaves the values as they are. norm: one fp32 on the
- * device (one past its range is written as infinite, the values are scaled all the same). Limits: 2^16 tensors, 2^40 elements.
+ * order that the sizes fix; the factor is fp32, below fp32's normal range 64 bits. Gradients that hold
+ * an infinity or NaN stay as they are. norm: one fp32 on the device; that of finite gradients may
+ * pass fp32's range: it is written as infinite, the values are scaled by what it is all the same.
+ * Limits: 2^16 tensors, 2^40 elements.
  */
 typedef struct moe_clip_args {
     int64_t struct_bytes;

@@ -61,3 +61,42 @@ def test_clip_factors_below_the_normal_range_of_fp32(value, most, dtype):
         assert float(off.max()) <= 0, float(((got.double() - y) / y).abs().max())
     clip_gradients(grads, most)
     assert all(torch.equal(a, b) for a, b in zip(grads, outputs))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_scales_of_rows_that_are_no_numbers(dtype):
+    """As documented: what a NaN and an infinity leave of their row and its scale, in the norm and alone."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    least = float(torch.tensor(2.0**-100) / torch.tensor(448.0))
+    for hidden in (5, 200, 4096):
+        x = torch.randn(4, hidden, device="cuda", generator=g).to(dtype)
+        x[1, 2], x[2, 4] = float("nan"), float("-inf")
+        rows = rms_norm(x, quantize=True).output
+        assert rows.scales[1:3].tolist() == [least, least] and bool(torch.isfinite(rows.scales).all())
+        back = rows.dequantize()
+        assert torch.isnan(back[1]).all() and torch.isnan(back[2, 4])
+        rest = torch.arange(hidden, device="cuda") != 4
+        assert not back[2][rest].any() and bool(torch.isfinite(back[0]).all())
+        rows = quantize_rows(x)
+        back = rows.dequantize()
+        assert math.isinf(float(rows.scales[2])) and torch.isnan(back[2]).all()
+        rest = torch.arange(hidden, device="cuda") != 2
+        assert torch.isnan(back[1, 2]) and bool(torch.isfinite(back[1][rest]).all())
+        assert float(rows.scales[1]) == float((x[1].float()[rest].abs().amax().cpu() / torch.tensor(448.0)))
+
+
+@pytest.mark.parametrize("hidden", [1, 65, 2048, 16384])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_norm_of_tiny_rows_without_eps(hidden, dtype):
+    """eps 0 at the end of the documented range: squares below it vanish beside the row's largest."""
+    x = torch.zeros(3, hidden, device="cuda")
+    x[0, 0] = 1.01e-16
+    x[1] = 2e-16 * torch.linspace(-1, 1, hidden, device="cuda") if hidden > 1 else 2e-16
+    x[2, -1], x[2, 0] = 1e-16 if hidden > 1 else 0.0, 3e-16
+    x = x.to(dtype)
+    y = rms_norm(x, eps=0.0).output.double()
+    want = x.double() / x.double().square().mean(-1, keepdim=True).sqrt()
+    # 70 roundings of fp32 as in the norm's own tests, squares lost below 2^-126 (16384 of them against 1e-32), half a step.
+    half = torch.finfo(dtype).eps / 2 if dtype is not torch.float32 else 0.0
+    lost = 16384 * 2.0**-126 / 1e-32
+    assert bool(((y - want).abs() <= want.abs() * (half * 1.001 + 70 * 2.0**-24 + lost)).all())
