@@ -246,7 +246,7 @@ def route_scored(logits, topk, *, scoring="softmax", bias=None, groups=1, top_gr
                  renormalize=True, scale=1.0):
     """``scored.route_scored`` with the weights' gradient to the logits: ``(ids, weights)``."""
     _eager_only()
-    if bias is not None and bias.requires_grad:
+    if isinstance(bias, torch.Tensor) and bias.requires_grad:
         raise ValueError("the selection bias gets no gradient; detach it")
     return _RouteScored.apply(logits, topk, {"scoring": scoring, "renormalize": renormalize, "scale": scale},
                               {"bias": bias, "groups": groups, "top_groups": top_groups, "group_best": group_best})

@@ -9,6 +9,8 @@ weights go to ``dispatch`` and ``combine`` like theirs (which take up to 64 expe
 Checks, streams and errors are those of ``moe_dispatch.training``.
 """
 
+from numbers import Real
+
 import torch
 
 from ._extension import current_stream_handle, get_extension
@@ -22,7 +24,7 @@ MAX_TOKENS = 2**21
 SCORINGS = ("softmax", "sigmoid")
 
 
-def _check_logits(logits, topk, scoring):
+def _check_logits(logits, topk, scoring, scale):
     tokens, experts = shape_of(logits, "logits", 2)
     require_tensor(logits, "logits", logits.shape, torch.float32, logits.device)
     if not 1 <= experts <= MAX_SCORED_EXPERTS:
@@ -33,6 +35,8 @@ def _check_logits(logits, topk, scoring):
         raise ValueError("topk must be in 1..8")
     if scoring not in SCORINGS:
         raise ValueError("scoring must be softmax or sigmoid")
+    if not isinstance(scale, Real):
+        raise TypeError("scale must be a number")
     return tokens, experts
 
 
@@ -43,7 +47,7 @@ def _check_choice(experts, topk, groups, top_groups, group_best):
         raise ValueError("top_groups must be in 1..groups")
     if topk > top_groups * (experts // groups):
         raise ValueError("topk exceeds the experts of top_groups groups")
-    if group_best not in (1, 2):
+    if not isinstance(group_best, int) or group_best not in (1, 2):
         raise ValueError("group_best must be 1 or 2")
 
 
@@ -66,7 +70,7 @@ def route_scored(logits, topk, *, scoring="softmax", bias=None, groups=1, top_gr
     groups have nothing else left. A NaN logit is out too and makes its token's weights NaN. So does
     +inf under softmax, where in the choice the experts with +inf have equal scores and the others 0.
     """
-    tokens, experts = _check_logits(logits, topk, scoring)
+    tokens, experts = _check_logits(logits, topk, scoring, scale)
     _check_choice(experts, topk, groups, top_groups, group_best)
     device = logits.device
     if bias is not None:
@@ -92,7 +96,7 @@ def route_scored_backward(grad_weights, logits, ids, *, scoring="softmax", renor
     ``renormalize`` and ``scale``; the choice itself, and so the bias, has no gradient.
     """
     tokens, topk = shape_of(ids, "ids", 2)
-    _, experts = _check_logits(logits, topk, scoring)
+    _, experts = _check_logits(logits, topk, scoring, scale)
     device = logits.device
     require_tensor(ids, "ids", (logits.shape[0], topk), torch.int32, device)
     require_tensor(grad_weights, "grad_weights", ids.shape, torch.float32, device)
