@@ -158,6 +158,8 @@ __global__ __launch_bounds__(kThreads) void clip_scale_kernel(ClipTable t, const
         each_chunk(static_cast<float>(factor));
 }
 
+// A launch's share of the partial sums bounds its workgroups, in the second pass as well: lists of thousands of tensors
+// leave CUs idle (554 M bf16 in 200 tensors 668 us in place, in 2000 1822, in 6000 5810).
 int blocks_of(int chunks, int launches) {
     const int most = static_cast<int>(kClipPartials) / launches;
     return chunks < most ? (chunks < 1 ? 1 : chunks) : most;

@@ -4,12 +4,13 @@
 //   swiglu: W holds n gate rows, then n up rows; y = silu(z_gate) z_up + residual
 //
 // Products accumulate in fp32 on MFMA and everything behind them stays in fp32: one rounding
-// to bf16. Few rows of x are bound by the weight's bytes (linear_few_kernel), many by the matrix
+// to bf16. Up to 16 rows of x are bound by the weight's bytes (linear_few_kernel: a workgroup for 16 columns, so
+// outputs of fewer than 4096 columns leave CUs idle: 14336 to 1024 18.7 us, 1.6 TB/s), many by the matrix
 // instructions (linear_ring.h); between them k is split over workgroups, so that every CU has
 // a part, and the partial sums are joined by a second launch with the epilogue.
 //
-// One row of 4096 e4m3 by 2 x 14336 weight rows (SwiGLU) 22.9 us, 5.1 TB/s; 4096 rows of it 345 us, 2787 TFLOP/s;
-// 4096 x 14336 x 4096 bf16 with a residual 328 us, 1465 TFLOP/s (a large library product: 1536 bf16, 3090 e4m3; all
+// One row of 4096 e4m3 by 2 x 14336 weight rows (SwiGLU) 22.9 us, 5.1 TB/s; 4096 rows of it 340 us, 2830 TFLOP/s;
+// 4096 x 14336 x 4096 bf16 with a residual 320 us, 1500 TFLOP/s (a large library product: 1536 bf16, 3090 e4m3; all
 // of these within 5% from one card to another, by its power).
 #include <algorithm>
 

@@ -221,7 +221,7 @@ __device__ __forceinline__ float activated(float z) {
 
 // f(constant<activation>) of a kernel whose kind of activation is KIND. The choice is made here, outside of an
 // epilogue's loops: made for each value, the code of 256 x 256 values and four activations does not stay in the
-// instruction cache (12995 x 448 x 13232 e4m3 with silu in one part of k 315 -> 220 us).
+// instruction cache (12995 rows, k 448, 13232 columns, e4m3 with silu: 315 -> 220 us).
 template <LinearAct KIND, typename F>
 __device__ __forceinline__ void with_activation(int act, const F& f) {
     if constexpr (KIND == kActElement) {

@@ -6,8 +6,8 @@
 //
 // A row is read once: it waits in registers between its sum of squares, its largest value
 // and its output (the norm is taken of the fp32 sum of x and residual, not of its rounded
-// copy, so y is rounded once). Bound by the bytes: 8192 x 4096 bf16 with residual to 8 bits 41 us, 5.7 TB/s (a
-// copy of 1 GiB 5.1); 4096 x 2048 bf16 forward 8.9 us and gradients 12.2 + 4.5 (the partial rows' sum), 3.5 TB/s in all;
+// copy, so y is rounded once). Bound by the bytes: 8192 x 4096 bf16 with residual to 8 bits 46 us, 5.1 TB/s (as a
+// copy of 1 GiB), rows alone to 8 bits 28672 x 4096 67.6 us, 5.2 TB/s; 4096 x 2048 bf16 forward 8.9 us and gradients 12.2 + 4.5 (the partial rows' sum), 3.5 TB/s in all;
 // one row 3.1 us, of which two are any launch's.
 #include <algorithm>
 

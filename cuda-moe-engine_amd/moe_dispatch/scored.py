@@ -35,7 +35,7 @@ def _check_logits(logits, topk, scoring, scale):
         raise ValueError("topk must be in 1..8")
     if scoring not in SCORINGS:
         raise ValueError("scoring must be softmax or sigmoid")
-    if not isinstance(scale, Real):
+    if scale.__class__ is not float and not isinstance(scale, Real):
         raise TypeError("scale must be a number")
     return tokens, experts
 
@@ -64,7 +64,8 @@ def route_scored(logits, topk, *, scoring="softmax", bias=None, groups=1, top_gr
       ``top_groups`` highest groups alone are chosen;
     * ids are the K highest keys, highest first, ties to the lower index. The choice is that of
       the exact keys, however fp32 rounds them;
-    * weights are ``scale * s``, with ``renormalize`` divided by the sum of the chosen s.
+    * weights are ``scale * s``, with ``renormalize`` divided by the sum of the chosen s: fp32, within about
+      40 + 2 |l - l_top| roundings of 2^-24 (|l| for sigmoid without ``renormalize``), 0 below 2^-126.
 
     A logit of -inf takes an expert out: it is chosen, with weight 0, only where the token's
     groups have nothing else left. A NaN logit is out too and makes its token's weights NaN. So does

@@ -91,3 +91,20 @@ def test_values_that_are_no_numbers_leave_the_others_their_order(experts, groups
                 assert torch.equal(ids, want), (best, place, value)
                 if value != value:
                     assert torch.isnan(weights).all()
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_logits_of_the_lowest_value(scoring):
+    """fp32's lowest value masks as -inf does, but stays an expert: of score 0, ahead of those that are out."""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    lowest = torch.finfo(torch.float32).min
+    for experts, groups, top_groups in ((64, 1, 1), (256, 8, 4), (12, 3, 2), (510, 34, 5)):
+        logits = torch.randn(200, experts, device="cuda", generator=g)
+        for share in (0.5, 0.98, 1.0):
+            logits[torch.rand(200, experts, device="cuda", generator=g) < share] = lowest
+            logits[:50][torch.rand(50, experts, device="cuda", generator=g) < 0.5] = float("-inf")
+            for bias in (None, 0.01 * torch.randn(experts, device="cuda", generator=g)):
+                options = dict(scoring=scoring, bias=bias, groups=groups, top_groups=top_groups)
+                ids, weights = route_scored(logits, 4, **options)
+                want, _ = _reference(logits, 4, **options)
+                assert torch.equal(ids, want) and not bool(torch.isnan(weights).any())
