@@ -9,8 +9,6 @@ weights go to ``dispatch`` and ``combine`` like theirs (which take up to 64 expe
 Checks, streams and errors are those of ``moe_dispatch.training``.
 """
 
-from numbers import Real
-
 import torch
 
 from ._extension import current_stream_handle, get_extension
@@ -35,7 +33,7 @@ def _check_logits(logits, topk, scoring, scale):
         raise ValueError("topk must be in 1..8")
     if scoring not in SCORINGS:
         raise ValueError("scoring must be softmax or sigmoid")
-    if scale.__class__ is not float and not isinstance(scale, Real):
+    if not (hasattr(scale, "__float__") or hasattr(scale, "__index__")):
         raise TypeError("scale must be a number")
     return tokens, experts
 
@@ -47,7 +45,7 @@ def _check_choice(experts, topk, groups, top_groups, group_best):
         raise ValueError("top_groups must be in 1..groups")
     if topk > top_groups * (experts // groups):
         raise ValueError("topk exceeds the experts of top_groups groups")
-    if not isinstance(group_best, int) or group_best not in (1, 2):
+    if not hasattr(group_best, "__index__") or group_best not in (1, 2):
         raise ValueError("group_best must be 1 or 2")
 
 
